@@ -427,6 +427,68 @@ mlk_status mlk_mamba3_siso_step(const float* projected, int64_t streams, int64_t
                                 double a_floor, float* ssm_state, float* k_state, float* v_state,
                                 double* angle_state, int started, float* out, mlk_stream_t stream);
 
+/* --------------------------------------- streaming over a 4-bit cache -- */
+
+/* The operators of a streamed attention layer; the reference has none of them (its KV cache,
+ * python/montlok/rdt/reference/Model/layers/mla.py, is outside its fast path). Activations are fp32 or bf16 (`dtype`, an
+ * mlk_dtype), every sum is held in fp32 or more and results are rounded once.
+ *
+ * Four-bit values are OCP MX: codes of four bits (sign, e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32 consecutive ones under a
+ * scale byte that stands for 2^(byte - 127); 255 makes the group NaN. Byte j of a row of codes holds elements 2 j (low
+ * four bits) and 2 j + 1.
+ *
+ * `positions` [batch, length] gives every token its place in its sequence; a negative one is padding. `page_table`
+ * [batch, table_width] names a sequence's pages; entries of pages that no token needs are not read. Both are contiguous
+ * int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes, 16-byte aligned, page_size a
+ * multiple of 16 up to 1024, head_dim 32, 64, 128 or 256. A (page, head) holds key codes [page_size][head_dim / 2], value
+ * codes [head_dim / 2][page_size], key scales [page_size][head_dim / 32], value scales [head_dim / 32][page_size].
+ * Strides are {sequence, token, head} in elements, head_dim dense. */
+
+/* RMSNorm over head_dim of every head of q [batch, length, heads, head_dim] and k [.., kv_heads, ..], each with its fp32
+ * weight [head_dim], then the rotation (rotate_half, as mlk_mla_rope_qk) of the last rope_dim lanes by the tables' row
+ * [table_rows, rope_dim] of the token's position. Double arithmetic, one rounding. Tokens at negative positions give
+ * zeros, tokens past the tables NaN. q_out, k_out: contiguous. head_dim up to 1024. */
+mlk_status mlk_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int32_t dtype,
+                            const float* q_weight, const float* k_weight, double eps, const float* cosine,
+                            const float* sine, int64_t table_rows, int64_t rope_dim, const int32_t* positions,
+                            int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t head_dim, void* q_out,
+                            void* k_out, mlk_stream_t stream);
+
+/* Keys and values [batch, length, kv_heads, head_dim] into the cache: each group of 32 is scaled by the smallest power of
+ * two whose six-fold reaches its largest magnitude (bytes 3 to 252; a group with an infinity or a NaN becomes NaN) and
+ * rounded to nearest, ties to the even code. Tokens at negative positions, past the page table or on a page outside
+ * [0, pages) are dropped. The places of one call's tokens must be distinct. */
+mlk_status mlk_kv4_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int32_t dtype,
+                          int64_t batch, int64_t length, int64_t kv_heads, int64_t head_dim, uint8_t* cache,
+                          int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                          const int32_t* positions, mlk_stream_t stream);
+
+/* The keys and values that the cache holds at `positions`, exactly, into contiguous k and v [batch, length, kv_heads,
+ * head_dim]. Negative positions give zeros, places that the page table does not name NaN. */
+mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, const int32_t* page_table,
+                        int64_t table_width, const int32_t* positions, int64_t batch, int64_t length, int64_t kv_heads,
+                        int64_t head_dim, int32_t dtype, void* k, void* v, mlk_stream_t stream);
+
+/* softmax(q k^T * scale) v of q [batch, length, heads, head_dim] over the cached keys 0 .. position of each token (heads
+ * a multiple of kv_heads: query head h reads key head h * kv_heads / heads). out: contiguous, 16-byte aligned. A token at
+ * a negative position sees no key and gives zeros; one past the page table, or that sees a key on a page outside
+ * [0, pages), gives NaN. What the cache holds behind a token's position does not reach it. fp32 q runs with fp32
+ * accuracy, bf16 q with the softmax weights rounded to bf16 for the value product. The workspace is 16-byte aligned and
+ * private to the call until it has run. */
+size_t mlk_kv4_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         int64_t page_size, int64_t table_width);
+mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dtype, int64_t batch, int64_t length,
+                             int64_t heads, int64_t kv_heads, int64_t head_dim, const uint8_t* cache, int64_t pages,
+                             int64_t page_size, const int32_t* page_table, int64_t table_width, const int32_t* positions,
+                             double scale, void* out, void* workspace, size_t workspace_bytes, mlk_stream_t stream);
+
+/* y [rows, out_features] = x W^T + bias with four-bit weights: codes [out_features, in_features / 2] (16-byte aligned),
+ * scales [out_features, in_features / 32], bias fp32 or NULL. x rows `x_stride` elements apart; y contiguous, of x's
+ * dtype. in_features must be a multiple of 32. */
+mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int64_t x_stride, int32_t dtype,
+                          const uint8_t* codes, const uint8_t* scales, const float* bias, int64_t out_features, void* out,
+                          mlk_stream_t stream);
+
 /* --------------------------------------------------------- diagnostics -- */
 
 /* Evaluates the kernels' device math helpers on x[count] (float64):

@@ -10,6 +10,7 @@
 // selects it here as it does for ctypes.
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/utils/pybind.h>
@@ -76,7 +77,8 @@ using OptTensor = std::optional<Tensor>;
     X(mlk_last_error) X(mlk_rms_norm) X(mlk_add_rms_norm) X(mlk_layer_norm) X(mlk_swiglu) X(mlk_linear)            \
     X(mlk_linear_residual) X(mlk_rms_norm_linear) X(mlk_linear_swiglu) X(mlk_mhc_prepare) X(mlk_mhc_combine) X(mlk_mhc_combine_prepare) \
     X(mlk_mamba3_workspace_bytes) X(mlk_mamba3_siso_forward) X(mlk_mamba3_siso_step)                               \
-    X(mlk_rms_norm_mamba3_forward) X(mlk_mla_rope_qk) X(mlk_attention)
+    X(mlk_rms_norm_mamba3_forward) X(mlk_mla_rope_qk) X(mlk_attention) X(mlk_qk_norm_rope) X(mlk_kv4_append)       \
+    X(mlk_kv4_read) X(mlk_kv4_attention_workspace_bytes) X(mlk_kv4_attention) X(mlk_linear_fp4)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -568,6 +570,157 @@ Tensor attention(const OptTensor& q_, const OptTensor& k_, const OptTensor& v_, 
     return out;
 }
 
+// ------------------------------------------------------------------ streaming over a 4-bit cache
+
+// A float32 or bfloat16 activation, dense along its last dimension.
+const Tensor& activation(const OptTensor& t, const char* name, int64_t dims) {
+    const std::string n(name);
+    REQUIRE(t.has_value() && t->defined(), n + " must be defined");
+    REQUIRE(t->is_cuda(), n + " must be on the GPU");
+    REQUIRE(t->scalar_type() == at::kFloat || t->scalar_type() == at::kBFloat16, n + " must be float32 or bfloat16");
+    REQUIRE(dims <= 0 || t->dim() == dims, n + " must have " + std::to_string(dims) + " dimensions");
+    REQUIRE(t->dim() >= 1 && (t->stride(-1) == 1 || t->size(-1) <= 1), n + " must be dense along its last dimension");
+    return *t;
+}
+
+const Tensor& typed(const OptTensor& t, const char* name, at::ScalarType type, const char* type_name, const Tensor& like) {
+    const std::string n(name);
+    REQUIRE(t.has_value() && t->defined(), n + " must be defined");
+    REQUIRE(t->is_cuda() && t->device() == like.device(), n + " must be on the same GPU as the others");
+    REQUIRE(t->scalar_type() == type, n + " must be " + type_name);
+    return *t;
+}
+
+Tensor index_of(const OptTensor& t, const char* name, const Tensor& like) {
+    REQUIRE(typed(t, name, at::kInt, "int32", like).dim() == 2, std::string(name) + " must have 2 dimensions");
+    return t->contiguous();
+}
+
+Tensor positions_of(const OptTensor& positions, const Tensor& like, int64_t batch, int64_t length) {
+    const Tensor p = index_of(positions, "positions", like);
+    REQUIRE(p.size(0) == batch && p.size(1) == length, "positions must be [batch, length]");
+    return p;
+}
+
+struct Strides {
+    int64_t s[3];
+    operator const int64_t*() const { return s; }
+};
+Strides strides_of(const Tensor& t) { return {{t.stride(0), t.stride(1), t.stride(2)}}; }
+
+struct CacheView {
+    Tensor pages, table;
+    int64_t count, page_size, width;
+};
+CacheView cache_of(const OptTensor& cache_, const OptTensor& table, const Tensor& like, int64_t batch, int64_t kv_heads,
+                   int64_t head_dim) {
+    const Tensor& cache = typed(cache_, "cache", at::kByte, "uint8", like);
+    REQUIRE(cache.dim() == 3 && cache.is_contiguous(), "cache must be contiguous [pages, kv_heads, bytes]");
+    REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 32, 64, 128 or 256");
+    REQUIRE(cache.size(1) == kv_heads, "cache holds " + std::to_string(cache.size(1)) + " key heads, expected " + std::to_string(kv_heads));
+    const int64_t token = head_dim + head_dim / 16;
+    REQUIRE(cache.size(2) % token == 0, "cache records must be page_size * (head_dim + head_dim / 16) bytes");
+    CacheView v{cache, index_of(table, "page_table", like), cache.size(0), cache.size(2) / token, 0};
+    REQUIRE(v.table.size(0) == batch, "page_table must have a row for each sequence");
+    v.width = v.table.size(1);
+    return v;
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const OptTensor& q_, const OptTensor& k_, const OptTensor& q_weight, const OptTensor& k_weight,
+                                        Real eps, const OptTensor& cos_, const OptTensor& sin_, const OptTensor& positions) {
+    const Tensor &q = activation(q_, "q", 4), &k = activation(k_, "k", 4);
+    const c10::DeviceGuard guard(q.device());
+    typed(k_, "k", q.scalar_type(), "of q's dtype", q);
+    const int64_t batch = q.size(0), length = q.size(1), heads = q.size(2), dim = q.size(3), kv_heads = k.size(2);
+    REQUIRE(k.size(0) == batch && k.size(1) == length && k.size(3) == dim, "k must be [batch, length, kv_heads, head_dim] as q");
+    const Tensor qw = typed(q_weight, "q_weight", at::kFloat, "float32", q).contiguous();
+    const Tensor kw = typed(k_weight, "k_weight", at::kFloat, "float32", q).contiguous();
+    REQUIRE(qw.numel() == dim && kw.numel() == dim, "q_weight and k_weight must have head_dim elements");
+    const Tensor cos = typed(cos_, "cos", at::kFloat, "float32", q).contiguous(), sin = typed(sin_, "sin", at::kFloat, "float32", q).contiguous();
+    REQUIRE(cos.dim() == 2 && sin.sizes() == cos.sizes(), "cos and sin must be [positions, rope_dim]");
+    REQUIRE(cos.size(1) % 2 == 0 && cos.size(1) <= dim, "rope_dim must be even and at most head_dim");
+    const Tensor at = positions_of(positions, q, batch, length);
+    const Tensor q_out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    const Tensor k_out = at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous));
+    done(lib.mlk_qk_norm_rope(q.const_data_ptr(), strides_of(q), k.const_data_ptr(), strides_of(k), dtype_of(q), data(qw), data(kw), eps,
+                              data(cos), data(sin), cos.size(0), cos.size(1), at.const_data_ptr<int32_t>(), batch, length, heads,
+                              kv_heads, dim, q_out.data_ptr(), k_out.data_ptr(), stream()));
+    return {q_out, k_out};
+}
+
+void kv4_append(const OptTensor& k_, const OptTensor& v_, const OptTensor& cache, const OptTensor& page_table, const OptTensor& positions) {
+    const Tensor &k = activation(k_, "k", 4), &v = activation(v_, "v", 4);
+    const c10::DeviceGuard guard(k.device());
+    typed(v_, "v", k.scalar_type(), "of k's dtype", k);
+    REQUIRE(v.sizes() == k.sizes(), "k and v must be [batch, length, kv_heads, head_dim]");
+    const int64_t batch = k.size(0), length = k.size(1), kv_heads = k.size(2), dim = k.size(3);
+    const CacheView c = cache_of(cache, page_table, k, batch, kv_heads, dim);
+    const Tensor at = positions_of(positions, k, batch, length);
+    done(lib.mlk_kv4_append(k.const_data_ptr(), strides_of(k), v.const_data_ptr(), strides_of(v), dtype_of(k), batch, length, kv_heads, dim,
+                            static_cast<uint8_t*>(c.pages.data_ptr()), c.count, c.page_size, c.table.const_data_ptr<int32_t>(), c.width,
+                            at.const_data_ptr<int32_t>(), stream()));
+}
+
+std::tuple<Tensor, Tensor> kv4_read(const OptTensor& cache, const OptTensor& page_table, const OptTensor& positions, Count head_dim,
+                                    bool bf16) {
+    REQUIRE(cache.has_value() && cache->defined(), "cache must be defined");
+    REQUIRE(cache->is_cuda(), "cache must be on the GPU");
+    REQUIRE(cache->dim() == 3, "cache must be contiguous [pages, kv_heads, bytes]");
+    const c10::DeviceGuard guard(cache->device());
+    const Tensor at = index_of(positions, "positions", *cache);
+    const int64_t batch = at.size(0), length = at.size(1), kv_heads = cache->size(1);
+    const CacheView c = cache_of(cache, page_table, *cache, batch, kv_heads, head_dim);
+    const auto options = at::TensorOptions().dtype(bf16 ? at::kBFloat16 : at::kFloat).device(cache->device());
+    const Tensor k = at::empty({batch, length, kv_heads, head_dim}, options), v = at::empty({batch, length, kv_heads, head_dim}, options);
+    done(lib.mlk_kv4_read(static_cast<const uint8_t*>(c.pages.const_data_ptr()), c.count, c.page_size, c.table.const_data_ptr<int32_t>(),
+                          c.width, at.const_data_ptr<int32_t>(), batch, length, kv_heads, head_dim, dtype_of(k), k.data_ptr(), v.data_ptr(),
+                          stream()));
+    return {k, v};
+}
+
+Tensor kv4_attention(const OptTensor& q_, const OptTensor& cache, const OptTensor& page_table, const OptTensor& positions, Real scale) {
+    const Tensor& q = activation(q_, "q", 4);
+    const c10::DeviceGuard guard(q.device());
+    const int64_t batch = q.size(0), length = q.size(1), heads = q.size(2), dim = q.size(3);
+    REQUIRE(cache.has_value() && cache->defined() && cache->dim() == 3, "cache must be contiguous [pages, kv_heads, bytes]");
+    const int64_t kv_heads = cache->size(1);
+    REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "q's heads must be a multiple of the cache's");
+    const CacheView c = cache_of(cache, page_table, q, batch, kv_heads, dim);
+    const Tensor at = positions_of(positions, q, batch, length);
+    const Tensor out = at::empty({batch, length, heads, dim}, q.options().memory_format(at::MemoryFormat::Contiguous));
+    const size_t bytes = lib.mlk_kv4_attention_workspace_bytes(batch, length, heads, kv_heads, dim, c.page_size, c.width);
+    const Tensor ws = bytes == 0 ? Tensor() : at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+    done(lib.mlk_kv4_attention(q.const_data_ptr(), strides_of(q), dtype_of(q), batch, length, heads, kv_heads, dim,
+                               static_cast<const uint8_t*>(c.pages.const_data_ptr()), c.count, c.page_size,
+                               c.table.const_data_ptr<int32_t>(), c.width, at.const_data_ptr<int32_t>(), scale, out.data_ptr(),
+                               bytes == 0 ? nullptr : ws.data_ptr(), bytes, stream()));
+    return out;
+}
+
+Tensor linear_fp4(const OptTensor& input, const OptTensor& codes_, const OptTensor& scales_, const OptTensor& bias_) {
+    REQUIRE(input.has_value() && input->defined(), "input must be defined");
+    REQUIRE(input->is_cuda(), "input must be on the GPU");
+    REQUIRE(input->scalar_type() == at::kFloat || input->scalar_type() == at::kBFloat16, "input must be float32 or bfloat16");
+    const Tensor& x = *input;
+    const c10::DeviceGuard guard(x.device());
+    const Tensor codes = typed(codes_, "codes", at::kByte, "uint8", x).contiguous(), scales = typed(scales_, "scales", at::kByte, "uint8", x).contiguous();
+    REQUIRE(codes.dim() == 2 && codes.size(0) > 0 && codes.size(1) > 0 && codes.size(1) % 16 == 0, "codes must be [out_features, in_features / 2], in_features a multiple of 32");
+    const int64_t n = codes.size(0), k = 2 * codes.size(1);
+    REQUIRE(scales.dim() == 2 && scales.size(0) == n && scales.size(1) == k / 32, "scales must be [out_features, in_features / 32]");
+    REQUIRE(x.dim() >= 1 && x.size(-1) == k, "input must end in in_features=" + std::to_string(k));
+    Tensor bias;
+    if (bias_.has_value() && bias_->defined() && bias_->numel() > 0) {
+        bias = typed(bias_, "bias", at::kFloat, "float32", x).contiguous();
+        REQUIRE(bias.numel() == n, "bias must have " + std::to_string(n) + " elements, got " + std::to_string(bias.numel()));
+    }
+    const Rows r = rows_of(x, k);
+    const Tensor out = at::empty(with_last(x, n), x.options().memory_format(at::MemoryFormat::Contiguous));
+    done(lib.mlk_linear_fp4(r.t.const_data_ptr(), r.count, k, r.stride, dtype_of(x), static_cast<const uint8_t*>(codes.const_data_ptr()),
+                            static_cast<const uint8_t*>(scales.const_data_ptr()), bias.defined() ? data(bias) : nullptr, n, out.data_ptr(),
+                            stream()));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -592,5 +745,10 @@ PYBIND11_MODULE(_torch_ops, m) {
     OPERATOR(rms_norm_mamba3_forward);
     OPERATOR(mla_rope_qk);
     OPERATOR(attention);
+    OPERATOR(qk_norm_rope);
+    OPERATOR(kv4_append);
+    OPERATOR(kv4_read);
+    OPERATOR(kv4_attention);
+    OPERATOR(linear_fp4);
 #undef OPERATOR
 }

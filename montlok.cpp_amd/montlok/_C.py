@@ -65,6 +65,13 @@ def _load():
         "mlk_mhc_prepare": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _dbl, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
                             _vp, _dbl, _vp, _vp, _vp, _vp, _vp],
         "mlk_mhc_combine": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+        "mlk_qk_norm_rope": [_vp, _vp, _vp, _vp, C.c_int32, _vp, _vp, _dbl, _vp, _vp, _i64, _i64, _vp] + [_i64] * 5 +
+                            [_vp, _vp, _vp],
+        "mlk_kv4_append": [_vp, _vp, _vp, _vp, C.c_int32] + [_i64] * 4 + [_vp, _i64, _i64, _vp, _i64, _vp, _vp],
+        "mlk_kv4_read": [_vp, _i64, _i64, _vp, _i64, _vp] + [_i64] * 4 + [C.c_int32, _vp, _vp, _vp],
+        "mlk_kv4_attention": [_vp, _vp, C.c_int32] + [_i64] * 5 + [_vp, _i64, _i64, _vp, _i64, _vp, _dbl, _vp, _vp,
+                                                                   C.c_size_t, _vp],
+        "mlk_linear_fp4": [_vp, _i64, _i64, _i64, C.c_int32, _vp, _vp, _vp, _i64, _vp, _vp],
         "mlk_math_check": [_vp, _i64, _vp, _vp],
         "mlk_mamba3_siso_recurrent": [_vp, _vp] * 7 + [_vp] + [_i64] * 5 + [_vp, _vp, C.c_size_t, _vp],
         "mlk_mamba3_siso_recurrent_noalloc": [_vp, _vp] * 7 + [_vp] + [_i64] * 5 + [_vp, _vp],
@@ -83,6 +90,8 @@ def _load():
         fn.restype = C.c_int
     lib.mlk_mamba3_workspace_bytes.argtypes = [_i64] * 5
     lib.mlk_mamba3_workspace_bytes.restype = C.c_size_t
+    lib.mlk_kv4_attention_workspace_bytes.argtypes = [_i64] * 7
+    lib.mlk_kv4_attention_workspace_bytes.restype = C.c_size_t
     lib.mlk_mla_packed_elems.argtypes = [_i64] * 5
     lib.mlk_mla_packed_elems.restype = C.c_int64
     _lib = lib
@@ -576,6 +585,71 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: int, scal
     return (_native or _ops()).attention(q, k, v, mask, scale, precision == torch.bfloat16)
 
 
+# ------------------------------------------------------------------ streaming over a 4-bit cache
+#
+# No counterparts in the reference. Four-bit values are OCP MX: codes (sign, e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32
+# consecutive ones under a scale byte for 2^(byte - 127), 255 for NaN. ``positions`` [batch, length] (int32) is each
+# token's place in its sequence, negative for padding; ``page_table`` [batch, n] (int32) names a sequence's pages.
+# Activations are float32 or bfloat16; the tensors of a call are on one GPU, whose current stream it uses.
+
+
+def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device=None) -> torch.Tensor:
+    """An empty cache of ``pages`` pages: uint8 [pages, kv_heads, page_size * (head_dim + head_dim / 16)], a token's
+    key and value in 4.25 bits an element. ``page_size`` is a multiple of 16 up to 1024, ``head_dim`` 32, 64, 128 or
+    256. The layout of a page is described in ``include/mlk_hip.h``."""
+    _check(head_dim in (32, 64, 128, 256), "head_dim must be 32, 64, 128 or 256")
+    _check(0 < page_size <= 1024 and page_size % 16 == 0, "page_size must be a multiple of 16, at most 1024")
+    _check(pages > 0 and kv_heads > 0, "pages and kv_heads must be positive")
+    return torch.zeros(pages, kv_heads, page_size * (head_dim + head_dim // 16), dtype=torch.uint8,
+                       device="cuda" if device is None else device)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                 cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head of q [B, L, H, D] and k [B, L, Hkv, D] (float32 weights [D]), then rotate_half of the last
+    R lanes by row ``positions[b, l]`` of cos and sin [P, R]; float64 arithmetic, one rounding, new tensors.
+
+    A negative position gives zeros, one past the tables NaN."""
+    return (_native or _ops()).qk_norm_rope(q, k, q_weight, k_weight, eps, cos, sin, positions)
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
+               positions: torch.Tensor) -> None:
+    """k and v [B, L, Hkv, D] into the cache, in place: each group of 32 under the smallest power of two whose six-fold
+    reaches its largest magnitude, rounded to nearest with ties to the even code; a group with an infinity or a NaN
+    becomes NaN. Tokens at negative positions or on pages that the table does not name are dropped.
+
+    The places of one call's tokens must be distinct: which token stays at a shared one is not defined."""
+    (_native or _ops()).kv4_append(k, v, cache, page_table, positions)
+
+
+def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, head_dim: int,
+             dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [B, L, Hkv, D] that the cache holds at ``positions`` [B, L], exactly. Negative positions
+    give zeros, places on pages that the table does not name NaN."""
+    _check(dtype in (torch.float32, torch.bfloat16), "dtype must be float32 or bfloat16")
+    return (_native or _ops()).kv4_read(cache, page_table, positions, head_dim, dtype == torch.bfloat16)
+
+
+def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
+                  scale: float) -> torch.Tensor:
+    """softmax(q k^T * scale) v of q [B, L, H, D] over the cached tokens 0 .. ``positions[b, l]`` -> [B, L, H, D].
+
+    H is a multiple of the cache's key heads; query head h reads key head h // (H / Hkv). One new token a sequence, a
+    chunk of a prompt and padded batches are the same call: a token at a negative position sees no key and gives zeros.
+    A token past the page table, or that sees a key on a page that the table does not name, gives NaN; what the cache
+    holds behind a token's position does not reach it. float32 q runs with float32 accuracy."""
+    return (_native or _ops()).kv4_attention(q, cache, page_table, positions, scale)
+
+
+def linear_fp4(input: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+               bias: torch.Tensor | None = None) -> torch.Tensor:
+    """input [..., K] @ W^T + bias with W in four bits: codes uint8 [N, K / 2] (element 2 j in the low bits of byte j),
+    scales uint8 [N, K / 32], bias float32 [N]. The result has the input's dtype; sums are in float32 and the products
+    exact, for float32 input too."""
+    return (_native or _ops()).linear_fp4(input, codes, scales, bias)
+
+
 def mla_forward(x, in_proj_weight, q_weight, kv_norm_weight, kv_norm_bias, kv_norm_eps, kv_up_weight, out_weight,
                 cosine, sine, n_heads, head_dim, nope_dim, kv_lora_rank, n_last, causal, scale):
     """montlok.cpp:1159-1211: projection, latent LayerNorm, kv_up, RoPE, attention and output projection.
@@ -898,7 +972,9 @@ def exported_symbols() -> list[str]:
             "mlk_mamba3_siso_recurrent_noalloc", "mlk_mamba3_siso_forward", "mlk_rms_norm_mamba3_forward",
             "mlk_mamba3_siso_step", "mlk_linear", "mlk_linear_residual", "mlk_rms_norm_linear", "mlk_linear_swiglu",
             "mlk_layer_norm_bf16", "mlk_mla_rope_qk", "mlk_attention", "mlk_mla_attend", "mlk_mla_attend_normed",
-            "mlk_mla_forward", "mlk_mla_packed_elems", "mlk_mla_pack_weights", "mlk_mla_forward_packed"]
+            "mlk_mla_forward", "mlk_mla_packed_elems", "mlk_mla_pack_weights", "mlk_mla_forward_packed",
+            "mlk_qk_norm_rope", "mlk_kv4_append", "mlk_kv4_read", "mlk_kv4_attention_workspace_bytes",
+            "mlk_kv4_attention", "mlk_linear_fp4"]
 
 
 def empty_kernel(blocks: int, threads: int, dynamic_lds_bytes: int = 0) -> None:

@@ -1,0 +1,157 @@
+"""The linear with 4-bit weights against float64."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kv4_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _weights(g, n, k, low=120, high=124):
+    return (torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8),
+            torch.randint(low, high, (n, k // 32), generator=g, dtype=torch.uint8))
+
+
+def _check(got, x, codes, scales, bias, dtype):
+    """Products are exact; the sum of a float32 row has three parts a product, each addition u = 2^-24 of what is summed,
+    the bias one more; bf16 rounds the result (2^-8)."""
+    w = ref.value_of(codes, scales)
+    rows = x.double().reshape(-1, x.shape[-1])
+    out, size = rows @ w.t(), rows.abs() @ w.abs().t()
+    if bias is not None:
+        out, size = out + bias.double(), size + bias.double().abs()
+    bound = (3 * x.shape[-1] + 8) * 2.0 ** -24 * size + 1e-37
+    if dtype == BF16:
+        bound = bound + 2.0 ** -8 * out.abs() * 1.01
+    got = got.double().cpu().reshape(out.shape)
+    off = float(((got - out).abs() / bound).max())
+    assert off <= 1.0, f"{off:.3g} of the bound"
+    # What sums of many terms are off by in earnest: far below the bound above.
+    assert float((got - out).norm() / out.norm()) <= (3e-3 if dtype == BF16 else 2e-6)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 2, 5, 15, 16, 17, 33, 64, 65, 100, 129, 300])
+@pytest.mark.parametrize("k,n", [(32, 16), (64, 1), (96, 17), (128, 64), (160, 130), (512, 100), (1056, 257), (4096, 48)])
+def test_against_float64(dev, dtype, rows, k, n):
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(rows * 7 + k + n)
+    codes, scales = _weights(g, n, k)
+    x = torch.randn(rows, k, generator=g).to(dtype)
+    bias = torch.randn(n, generator=g) if (rows + n) % 2 else None
+    got = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), None if bias is None else bias.to(dev))
+    assert got.shape == (rows, n) and got.dtype == dtype
+    _check(got, x, codes, scales, bias, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,k,n", [(1, 8192, 4096), (3, 2048, 9000), (24, 4096, 4100), (200, 1024, 2051), (520, 512, 1000)])
+def test_larger_shapes(dev, dtype, rows, k, n):
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(n)
+    codes, scales = _weights(g, n, k)
+    x, bias = torch.randn(rows, k, generator=g).to(dtype), torch.randn(n, generator=g)
+    _check(_C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), bias.to(dev)), x, codes, scales, bias, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_views_and_leading_dimensions(dev, dtype):
+    """Row strides, alignments and shapes of x: the same bits as a contiguous copy."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(3)
+    codes, scales = (t.to(dev) for t in _weights(g, 70, 96))
+    wide = torch.randn(2, 5, 7, 131, generator=g).to(dtype).to(dev)
+    for x in (wide[..., 1:97], wide[..., 3:99], wide[:, 1:4, ::2, 8:104], wide[0, 0, :, 2:98].t().contiguous().t(), wide[0, 0, 0, 5:101],
+              wide[:0, 0, 0, :96]):
+        got = _C.linear_fp4(x, codes, scales)
+        assert got.shape == (*x.shape[:-1], 70)
+        assert torch.equal(got, _C.linear_fp4(x.contiguous(), codes, scales))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_range_of_values(dev, rows):
+    """The largest and smallest scales and inputs: every product that float32 holds."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(5)
+    for low, high, size in ((3, 4, 2.0 ** 90), (240, 252, 2.0 ** -100), (100, 150, 2.0 ** -20), (127, 128, 2.0 ** 120), (200, 210, 2.0 ** -80)):
+        codes, scales = _weights(g, 33, 64, low, high)
+        x = torch.randn(rows, 64, generator=g) * size
+        _check(_C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)), x, codes, scales, None, F32)
+    codes, scales = _weights(g, 33, 64, 100, 110)
+    x = torch.full((rows, 64), 3.4028234663852886e38)  # no part of a value overflows
+    x[:, ::2] *= -1
+    _check(_C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)), x, codes, scales, None, F32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_infinities_and_nan(dev, dtype, rows):
+    """Rows and groups that hold them, as IEEE sums have them; the other rows and columns keep their bits."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(7)
+    codes, scales = _weights(g, 40, 160)
+    codes |= 0x11  # no weight is zero: an infinity gives an infinity
+    x = torch.randn(rows, 160, generator=g).to(dtype)
+    clean = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    x[0, 3], x[1, 100], x[2, 159] = torch.inf, -torch.inf, torch.nan
+    scales[9, 2] = 255
+    got = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    expect = x.double() @ ref.value_of(codes, scales).t()
+    assert torch.equal(torch.isnan(got), torch.isnan(expect)) and torch.equal(torch.isinf(got), torch.isinf(expect))
+    assert torch.equal(torch.sign(got[:2, :9].double()), torch.sign(expect[:2, :9]))
+    keep = torch.ones(40, dtype=torch.bool)
+    keep[9] = False
+    assert torch.equal(got[3:][:, keep], clean[3:][:, keep])
+
+
+def test_refusals(dev):
+    from montlok import _C
+
+    x, codes, scales = torch.zeros(2, 64, device=dev), torch.zeros(8, 32, dtype=torch.uint8, device=dev), torch.zeros(8, 2, dtype=torch.uint8, device=dev)
+    for call, text in ((lambda: _C.linear_fp4(x.half(), codes, scales), "input must be float32 or bfloat16"),
+                       (lambda: _C.linear_fp4(x[:, :32], codes, scales), "input must end in in_features=64"),
+                       (lambda: _C.linear_fp4(x, codes.int(), scales), "codes must be uint8"),
+                       (lambda: _C.linear_fp4(x, codes[:, :24], scales), "codes must be"),
+                       (lambda: _C.linear_fp4(x, codes[:0], scales), "codes must be"),
+                       (lambda: _C.linear_fp4(x, codes, scales[:, :1]), "scales must be"),
+                       (lambda: _C.linear_fp4(x, codes, scales.float()), "scales must be uint8"),
+                       (lambda: _C.linear_fp4(x, codes, scales, torch.zeros(7, device=dev)), "bias must have 8 elements, got 7"),
+                       (lambda: _C.linear_fp4(x, codes, scales, torch.zeros(8, device=dev).bfloat16()), "bias must be float32"),
+                       (lambda: _C.linear_fp4(x, codes.cpu(), scales), "codes must be on the same GPU"),
+                       (lambda: _C.linear_fp4(x, None, scales), "codes must be defined")):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+def test_graph_replays(dev):
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(9)
+    codes, scales = (t.to(dev) for t in _weights(g, 1000, 512))
+    for rows in (1, 100):
+        x = torch.randn(rows, 512, generator=g).to(dev)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _C.linear_fp4(x, codes, scales)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _C.linear_fp4(x, codes, scales)
+        for replay in range(4):
+            x.copy_(torch.randn(x.shape, generator=g))
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, _C.linear_fp4(x, codes, scales)), f"replay {replay}"

@@ -1,0 +1,138 @@
+"""Refusals of the 4-bit cache's operators that need no GPU: of the C ABI before any launch, and of montlok._C."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from montlok import _C
+
+    return _C.library()
+
+
+def _cache(lib, name, head_dim=64, page_size=64, pages=4, width=2, kv_heads=2, batch=1, length=1, dtype=1, heads=4, scale=1.0):
+    """One call with null tensors: the geometry is checked before the pointers."""
+    if name == "append":
+        status = lib.mlk_kv4_append(None, None, None, None, dtype, batch, length, kv_heads, head_dim, None, pages, page_size, None,
+                                    width, None, None)
+    elif name == "read":
+        status = lib.mlk_kv4_read(None, pages, page_size, None, width, None, batch, length, kv_heads, head_dim, dtype, None, None, None)
+    else:
+        status = lib.mlk_kv4_attention(None, None, dtype, batch, length, heads, kv_heads, head_dim, None, pages, page_size, None, width,
+                                       None, scale, None, None, 0, None)
+    return status, lib.mlk_last_error().decode()
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attention"])
+@pytest.mark.parametrize("change,text", [
+    (dict(head_dim=48), "head_dim must be"), (dict(head_dim=0), "head_dim must be"), (dict(head_dim=512), "head_dim must be"),
+    (dict(page_size=0), "page_size must be"), (dict(page_size=24), "page_size must be"), (dict(page_size=1040), "page_size must be"),
+    (dict(page_size=-16), "page_size must be"),
+    (dict(pages=0), "between 1 and"), (dict(pages=2 ** 31), "between 1 and"),
+    (dict(width=0), "page_table must hold"), (dict(width=2 ** 24 + 1), "page_table must hold"),
+    (dict(kv_heads=0), "invalid cache geometry"), (dict(batch=-1), "invalid cache geometry"), (dict(length=-1), "invalid cache geometry"),
+    (dict(dtype=2), "dtype must be"), (dict(), "null tensor pointer"),
+])
+def test_cache_geometry_is_refused_before_a_launch(lib, name, change, text):
+    status, message = _cache(lib, name, **change)
+    assert status == 1 and text in message
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(heads=3), "multiple of kv_heads"), (dict(heads=0), "multiple of kv_heads"), (dict(heads=-2), "multiple of kv_heads"),
+    (dict(length=2 ** 30), "too many tokens"),
+])
+def test_attention_geometry_is_refused_before_a_launch(lib, change, text):
+    status, message = _cache(lib, "attention", **change)
+    assert status == 1 and text in message
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attention"])
+@pytest.mark.parametrize("change", [dict(batch=0), dict(length=0)])
+def test_calls_without_tokens_do_nothing(lib, name, change):
+    assert _cache(lib, name, **change)[0] == 0
+
+
+def test_workspace_is_bounded_and_zero_for_what_is_refused(lib):
+    size = lib.mlk_kv4_attention_workspace_bytes
+    assert size(1, 1, 32, 8, 128, 64, 2048) > 0  # one long stream is split
+    assert size(1024, 1, 32, 8, 128, 64, 2048) == 0  # many streams are not
+    assert size(1, 1, 32, 8, 128, 64, 1) == 0
+    for bad in ((0, 1, 32, 8, 128, 64, 64), (1, 1, 31, 8, 128, 64, 64), (1, 1, 32, 8, 48, 64, 64), (1, 1, 32, 8, 128, 0, 64),
+                (1, 1, 32, 8, 128, 64, 0), (1, 1, 32, 8, 128, 64, 2 ** 40), (1, 0, 32, 8, 128, 64, 64), (1, 1, 32, 0, 128, 64, 64)):
+        assert size(*bad) == 0
+    for batch in (1, 3, 64):
+        for length in (1, 7, 500):
+            assert size(batch, length, 32, 8, 256, 16, 2 ** 26) <= 2 ** 28
+
+
+def _norm(lib, dtype=0, rows=8, rope=4, batch=1, length=1, heads=2, kv_heads=1, dim=8):
+    status = lib.mlk_qk_norm_rope(None, None, None, None, dtype, None, None, 1e-5, None, None, rows, rope, None, batch, length, heads,
+                                  kv_heads, dim, None, None, None)
+    return status, lib.mlk_last_error().decode()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(rope=3), "rope_dim must be"), (dict(rope=10), "rope_dim must be"), (dict(rope=-2), "rope_dim must be"),
+    (dict(dim=0), "head_dim must be"), (dict(dim=1025), "head_dim must be"), (dict(heads=0), "invalid norm geometry"),
+    (dict(kv_heads=0), "invalid norm geometry"), (dict(rows=-1), "invalid norm geometry"), (dict(dtype=7), "dtype must be"),
+    (dict(length=2 ** 34), "too many"), (dict(), "null tensor pointer"),
+])
+def test_norm_geometry_is_refused_before_a_launch(lib, change, text):
+    status, message = _norm(lib, **change)
+    assert status == 1 and text in message
+
+
+def _linear(lib, rows=1, k=64, n=8, dtype=0, codes=None):
+    status = lib.mlk_linear_fp4(None, rows, k, k, dtype, codes, None, None, n, None, None)
+    return status, lib.mlk_last_error().decode()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(k=0), "multiple of 32"), (dict(k=48), "multiple of 32"), (dict(n=0), "invalid linear"), (dict(rows=-1), "invalid linear"),
+    (dict(dtype=3), "dtype must be"), (dict(rows=2 ** 31), "too many"), (dict(), "null tensor pointer"),
+])
+def test_linear_geometry_is_refused_before_a_launch(lib, change, text):
+    status, message = _linear(lib, **change)
+    assert status == 1 and text in message
+
+
+def test_calls_without_rows_do_nothing(lib):
+    assert _linear(lib, rows=0)[0] == 0
+    assert _norm(lib, batch=0)[0] == 0 and _norm(lib, length=0)[0] == 0
+
+
+def test_operators_refuse_host_tensors():
+    from montlok import _C
+
+    x, c, i = torch.ones(1, 1, 2, 32), torch.zeros(1, 2, 16 * 34, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.int32)
+    for call, text in ((lambda: _C.qk_norm_rope(x, x, x, x, 1e-5, x, x, i), "q must be on the GPU"),
+                       (lambda: _C.kv4_append(x, x, c, i, i), "k must be on the GPU"),
+                       (lambda: _C.kv4_append(None, x, c, i, i), "k must be defined"),
+                       (lambda: _C.kv4_read(c, i, i, 32), "cache must be on the GPU"),
+                       (lambda: _C.kv4_read(c, i, i, 32, torch.float16), "dtype must be float32 or bfloat16"),
+                       (lambda: _C.kv4_attention(x, c, i, i, 1.0), "q must be on the GPU"),
+                       (lambda: _C.linear_fp4(x, c, c), "input must be on the GPU"),
+                       (lambda: _C.linear_fp4(None, c, c), "input must be defined")):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+@pytest.mark.parametrize("args", [(4, 2, 64, 48), (4, 2, 24, 64), (4, 2, 0, 64), (0, 2, 64, 64), (4, 0, 64, 64), (4, 2, 2048, 64)])
+def test_cache_allocation_is_refused(args):
+    from montlok import _C
+
+    with pytest.raises(RuntimeError):
+        _C.kv4_cache(*args, device="cpu")
+
+
+def test_cache_allocation():
+    from montlok import _C
+
+    cache = _C.kv4_cache(3, 2, 48, 64, device="cpu")
+    assert cache.shape == (3, 2, 48 * 68) and cache.dtype == torch.uint8 and not cache.any()
