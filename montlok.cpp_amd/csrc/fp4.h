@@ -53,15 +53,17 @@ __device__ __forceinline__ uint32_t scale_byte(float most) {
 }
 
 // An fp32 value as the sum of three bf16 values, exactly: its leading 8 significant bits, the next 8, the rest
-// (each cut off, so that none of them overflows). Infinite and NaN values have no rest.
+// (each cut off, so that none of them overflows). An infinity or a NaN stays alone with CAREFUL, and makes the rest NaN
+// without: half the instructions, for callers that look at their result.
 struct Parts3 {
     float a, b, c;
 };
+template <bool CAREFUL>
 __device__ __forceinline__ Parts3 parts_of(float x) {
     const uint32_t bits = __float_as_uint(x);
     Parts3 p;
-    p.a = __uint_as_float((x != x ? bits | 0x400000u : bits) & 0xFFFF0000u);
-    const float rest = (bits & 0x7F800000u) == 0x7F800000u ? 0.0f : x - p.a;
+    p.a = __uint_as_float((CAREFUL && x != x ? bits | 0x400000u : bits) & 0xFFFF0000u);
+    const float rest = CAREFUL && (bits & 0x7F800000u) == 0x7F800000u ? 0.0f : x - p.a;
     p.b = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
     p.c = rest - p.b;
     return p;
@@ -72,11 +74,12 @@ __device__ __forceinline__ uint32_t pack_upper(float lo, float hi) {
 }
 
 // Eight fp32 values as three bf16 operands.
+template <bool CAREFUL>
 __device__ __forceinline__ void planes_of(const float (&x)[8], bf16x8 (&plane)[3]) {
     u32x4 v[3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const Parts3 lo = parts_of(x[2 * i]), hi = parts_of(x[2 * i + 1]);
+        const Parts3 lo = parts_of<CAREFUL>(x[2 * i]), hi = parts_of<CAREFUL>(x[2 * i + 1]);
         v[0][i] = pack_upper(lo.a, hi.a);
         v[1][i] = pack_upper(lo.b, hi.b);
         v[2][i] = pack_upper(lo.c, hi.c);

@@ -234,7 +234,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_attention_kernel(AttentionArg
             for (int i = 0; i < 8; ++i) x[i] = Element<F32>::get(p.q, from + 8 * s + i);
             if constexpr (F32) {
                 bf16x8 plane[3];
-                planes_of(x, plane);
+                planes_of<true>(x, plane);
 #pragma unroll
                 for (int i = 0; i < 3; ++i) q[m][i][s] = plane[i];
             } else {
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_attention_kernel(AttentionArg
                 for (int i = 0; i < 8; ++i) w[i] = x[8 * h + i];
                 if constexpr (F32) {
                     bf16x8 plane[3];
-                    planes_of(w, plane);
+                    planes_of<false>(w, plane);  // of finite values, or NaN
 #pragma unroll
                     for (int i = 0; i < 3; ++i) weight[m][i][h] = plane[i];
                 } else {

@@ -2,6 +2,9 @@
 // the bf16 matrix cores with fp32 accumulation. Every weight is exact in bf16,
 // a bf16 x is too, and an fp32 x is the exact sum of three bf16 values, so the
 // only rounding is that of the sums.
+#include <algorithm>
+#include <type_traits>
+
 #include "fp4.h"
 
 namespace mlk {
@@ -17,53 +20,443 @@ struct Fp4LinearArgs {
     int32_t rows, K, N;
 };
 
-constexpr int kStep = 128;  // k of one 16-byte load of a wave's four lane groups
-constexpr int kWaves = 4;
+// Sixteen bytes at any element's alignment.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// Block: 16 columns of y (rows of W) by 16 rows, its waves' share of K interleaved. Lane (g, l) holds group
-// 4 step + g of row l of W (16 bytes) and the same 32 elements of row l of x: the products sum over k in an order of
-// their own, the same for both operands.
+// Four results side by side; `first` a multiple of 4 from an aligned base.
 template <bool F32>
-__global__ __launch_bounds__(kWaves * 64) void linear_fp4_kernel(Fp4LinearArgs p) {
-    constexpr int P = F32 ? 3 : 1;
-    __shared__ float part[kWaves][16][17];
+__device__ __forceinline__ void put4(void* out, int64_t first, const float (&y)[4]) {
+    if constexpr (F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(out) + first) = f32x4{y[0], y[1], y[2], y[3]};
+    } else {
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + first) =
+            u32x2{float_to_bf16(y[0]) | float_to_bf16(y[1]) << 16, float_to_bf16(y[2]) | float_to_bf16(y[3]) << 16};
+    }
+}
+
+// Few rows: a block takes 16 columns of y (rows of W) by 16 rows, its KW waves interleaved blocks of 512 k. A wave loads
+// its block of W whole rows at a time (256 bytes of 4 rows an instruction; the order of the matrix instruction, lane
+// (g, l) = group of row l, straight from memory costs a cache access a lane and bounded this kernel) and turns it in
+// its own piece of LDS. x comes the same way (TURN), or, for the first FEW rows, straight to the lanes whose row exists.
+// Past K a lane's x is zero (its W is that of the last group, which counts anyway). An infinity or a NaN in fp32 x makes
+// the quick planes NaN; a wave that sees one in its sums forms them again.
+// Blocks of 16 columns are held to the registers of two blocks a CU: with 146 the 257th block waited for a round of its
+// own (fp32, 4100 x 4096, 16 rows: 14.2 us).
+constexpr int kFew = 4;
+template <bool F32, bool TURN, int KW, int NT, int U>
+__global__ __launch_bounds__(KW * 64, NT == 1 ? 4 : 1) void linear_fp4_stream_kernel(Fp4LinearArgs p) {
+    constexpr int P = F32 ? 3 : 1, kPieces = F32 ? 8 : 4;  // 16-byte pieces of 32 elements of x
+    constexpr int kRow = 4 * U;                            // groups of a row that an iteration takes, 4 a matrix instruction
+    constexpr int kTurn = 16 * kRow * NT + (TURN ? 16 * 4 * kPieces : 0), kPart = (16 * (16 * NT + 1) + 3) / 4;
+    __shared__ u32x4 lds[KW][kTurn > kPart ? kTurn : kPart];
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-    const int64_t n = min(n0 + l, p.N - 1), m = min(m0 + l, p.rows - 1);
-    f32x4 acc = {0, 0, 0, 0};
-    for (int step = wave; step * kStep < p.K; step += kWaves) {
-        const int k0 = step * kStep + kGroup * g;
-        const bool live = k0 < p.K;
-        const int k = live ? k0 : 0;
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p.codes + n * (p.K / 2) + k / 2);
-        const float scale = scale_of(p.scales[n * (p.K / kGroup) + k / kGroup]);
+    const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * 16, groups = p.K / kGroup;
+    const uint8_t* const codes = p.codes + static_cast<int64_t>(n0) * (p.K / 2);
+    const uint8_t* const scales = p.scales + static_cast<int64_t>(n0) * groups;
+    const char* const xs = static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * p.x_stride * (F32 ? 4 : 2);
+    u32x4* const turn_w = lds[wave];
+    u32x4* const turn_x = lds[wave] + 16 * kRow * NT;
+    f32x4 acc[NT];
+    auto sum = [&](auto careful) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[8];
-            bf16x8 xs[P];
+        for (int n = 0; n < NT; ++n) acc[n] = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+        for (int group0 = kRow * wave; group0 < groups; group0 += kRow * KW) {
+            u32x4 w[NT][U];
+            uint32_t byte[NT][U];
+            u32x4 x[U][kPieces];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = live ? Element<F32>::get(p.x, m * p.x_stride + k + 8 * i + j) : 0.0f;
-            if constexpr (F32) {
-                planes_of(v, xs);
-            } else {
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) xs[0][j] = static_cast<__bf16>(v[j]);
+                for (int t = 0; t < U; ++t) {
+                    const int row = min(16 * n + t * (64 / kRow) + lane / kRow, p.N - 1 - n0), group = min(group0 + lane % kRow, groups - 1);
+                    w[n][t] = *reinterpret_cast<const u32x4*>(codes + static_cast<int64_t>(row) * (p.K / 2) + 16 * group);
+                }
+                const uint8_t* const from = scales + static_cast<int64_t>(min(16 * n + l, p.N - 1 - n0)) * groups;
+                if (group0 + kRow <= groups) {
+                    typedef uint32_t Scales __attribute__((ext_vector_type(U), aligned(1)));
+                    const Scales v = *reinterpret_cast<const Scales*>(from + group0);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) byte[n][u] = v[u] >> (8 * g);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) byte[n][u] = from[min(group0 + 4 * u + g, groups - 1)];
+                }
             }
-            const bf16x8 ws = fp4_octet(live ? w[i] : 0, live ? scale : 1.0f);
 #pragma unroll
-            for (int j = P - 1; j >= 0; --j) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ws, xs[j], acc, 0, 0, 0);
+            for (int u = 0; u < U; ++u) {
+                if constexpr (TURN) {
+                    // 4 kPieces pieces of a row side by side; past K the last of the row, zeroed below.
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int at = 64 * i + lane, row = min(at / (4 * kPieces), p.rows - 1 - m0);
+                        const int piece = min((group0 + 4 * u) * kPieces + at % (4 * kPieces), groups * kPieces - 1);
+                        x[u][i] = *reinterpret_cast<const u32x4_any*>(xs + static_cast<int64_t>(row) * p.x_stride * (F32 ? 4 : 2) + 16 * piece);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) x[u][i] = u32x4{0, 0, 0, 0};
+                    if (group0 + 4 * u + g < groups && m0 + l < p.rows) {
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i)
+                            x[u][i] = reinterpret_cast<const u32x4_any*>(xs + static_cast<int64_t>(l) * p.x_stride * (F32 ? 4 : 2) +
+                                                                         16 * kPieces * (group0 + 4 * u + g))[i];
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);  // every load of the iteration in flight before the first wait
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int t = 0; t < U; ++t) {
+                    const int row = t * (64 / kRow) + lane / kRow;
+                    turn_w[(16 * n + row) * kRow + ((lane % kRow) ^ (row % kRow))] = w[n][t];
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (TURN) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int at = 64 * i + lane, row = at / (4 * kPieces), piece = at % (4 * kPieces);
+                        const bool inside = (group0 + 4 * u) * kPieces + piece < groups * kPieces;
+                        turn_x[row * (4 * kPieces) + (piece ^ row)] = inside ? x[u][i] : u32x4{0, 0, 0, 0};
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                u32x4 ws[NT];
+                float scale[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    ws[n] = turn_w[(16 * n + l) * kRow + ((4 * u + g) ^ (l % kRow))];
+                    scale[n] = scale_of(byte[n][u] & 0xFF);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u32x4 piece[F32 ? 2 : 1];
+#pragma unroll
+                    for (int j = 0; j < (F32 ? 2 : 1); ++j) {
+                        const int at = (F32 ? 2 * i : i) + j;
+                        piece[j] = TURN ? turn_x[l * (4 * kPieces) + ((kPieces * g + at) ^ l)] : x[u][at];
+                    }
+                    bf16x8 xv[P];
+                    if constexpr (F32) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(piece[j / 4][j % 4]);
+                        planes_of<decltype(careful)::value>(v, xv);
+                    } else {
+                        xv[0] = __builtin_bit_cast(bf16x8, piece[0]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const bf16x8 wv = fp4_octet(ws[n][i], scale[n]);
+#pragma unroll
+                        for (int j = P - 1; j >= 0; --j) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[j], acc[n], 0, 0, 0);
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    };
+    sum(std::false_type{});
+    if constexpr (F32) {
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) odd = odd || acc[n][r] != acc[n][r];
+        if (__ballot(odd) != 0) sum(std::true_type{});
+    }
+    __syncthreads();
+    float* const part = reinterpret_cast<float*>(lds);  // [KW][16][16 NT + 1]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) part[(wave * 16 + l) * (16 * NT + 1) + 16 * n + 4 * g + r] = acc[n][r];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * NT; at += KW * 64) {
+        const int row = at / (16 * NT), col = at % (16 * NT);
+        if (m0 + row >= p.rows || n0 + col >= p.N) continue;
+        float y = part[row * (16 * NT + 1) + col];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) y += part[(w * 16 + row) * (16 * NT + 1) + col];
+        if (p.bias != nullptr) y += p.bias[n0 + col];
+        Element<F32>::put(p.out, static_cast<int64_t>(m0 + row) * p.N + n0 + col, y);
+    }
+}
+
+// More rows: a block of WN KW waves takes 16 NT WN columns of y by 16 MT rows. WN waves share the columns and KW the k of
+// a step, 64 each, so that a wave's products need MT P LDS reads for NT MT P matrix instructions and every weight is
+// converted once, between the products of the k before it. Codes, scales and x are staged in LDS a step ahead, x as
+// bf16 (three planes for fp32): loaded in rows, 8 lanes to 128 bytes, read in operand order. Unit u (8 consecutive k) of
+// row m of x lies at u * rows + (m ^ (u & 7)), piece c (32 codes) of row n of W at n * pieces + (c ^ (n & 7)): what
+// 8 lanes write, or read, together lies in different banks. The KW partial sums meet in LDS.
+template <bool F32, int WN, int KW, int NT, int MT, int BUFFERS>
+struct TileShape {
+    static constexpr int P = F32 ? 3 : 1, kRows = 16 * MT, kCols = 16 * NT * WN, kThreads = 64 * WN * KW;
+    static constexpr int kK = 64 * KW, kUnits = kK / 8, kPieces = kK / kGroup;
+    static constexpr int kX = P * kUnits * kRows, kW = kCols * kPieces, kScales = kCols * kPieces / 16;  // 16-byte units a buffer
+    static constexpr int kBuffer = kX + kW + kScales;
+    // A wave's partial sums of the tiles t = n MT + m that others finish (t mod KW is the wave that does).
+    static constexpr int kParts = NT * MT - NT * MT / KW;
+    static constexpr __device__ int part_of(int kw, int tile) { return tile - tile / KW - (tile % KW > kw ? 1 : 0); }
+    static constexpr size_t kLds = std::max(size_t{BUFFERS} * kBuffer * 16, size_t{WN} * KW * kParts * 1024);
+};
+template <bool F32, int WN, int KW, int NT, int MT, int DEPTH, int BUFFERS>
+__global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4LinearArgs p, int n_tiles, int m_tiles) {
+    using T = TileShape<F32, WN, KW, NT, MT, BUFFERS>;
+    constexpr int P = T::P, kBytes = F32 ? 4 : 2;
+    constexpr int kXLoads = T::kRows * T::kUnits / T::kThreads, kWLoads = (T::kW + T::kThreads - 1) / T::kThreads;
+    static_assert(kXLoads * T::kThreads == T::kRows * T::kUnits && T::kThreads % T::kUnits == 0 && T::kPieces % 8 == 0);
+    extern __shared__ u32x4 lds[];
+    // Blocks of the same columns side by side on one XCD: W comes from memory once, then from that L2.
+    const int xcd = blockIdx.x & 7, index = blockIdx.x >> 3;
+    const int n_tile = xcd + 8 * (index / m_tiles), m_tile = index % m_tiles;
+    if (n_tile >= n_tiles) return;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+    const int wn = wave % WN, kw = wave / WN;
+    const int n0 = n_tile * T::kCols, m0 = m_tile * T::kRows;
+
+    // Offsets from the block's first rows in 32 bits: the rows' once, the step's added.
+    const int groups = p.K / kGroup;
+    const uint8_t* const codes = p.codes + static_cast<int64_t>(n0) * (p.K / 2);
+    const uint8_t* const scales = p.scales + static_cast<int64_t>(n0) * groups;
+    const char* const xs = static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * p.x_stride * kBytes;
+    const int unit = threadIdx.x % T::kUnits;  // of x, the same in every load
+    const int x_first = static_cast<int>(threadIdx.x) / T::kUnits, x_rows = T::kThreads / T::kUnits;
+
+    struct Ahead {  // what a thread has loaded of a step
+        u32x4 w[kWLoads], scale_bytes, x[kXLoads][F32 ? 2 : 1];
+    } ahead[DEPTH];
+    auto load = [&](int step, Ahead& to) {
+        // Past K: the last group's, x is zeroed when it is staged, and that group counts anyway.
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i) {
+            const int at = i * T::kThreads + static_cast<int>(threadIdx.x), row = at / T::kPieces, piece = at % T::kPieces;
+            if (T::kW % T::kThreads != 0 && at >= T::kW) break;
+            const uint32_t offset = static_cast<uint32_t>(min(row, p.N - 1 - n0)) * static_cast<uint32_t>(groups) +
+                                    static_cast<uint32_t>(min(step * T::kPieces + piece, groups - 1));
+            to.w[i] = *reinterpret_cast<const u32x4*>(codes + 16 * static_cast<uint64_t>(offset));
+        }
+        if (static_cast<int>(threadIdx.x) < T::kCols) {
+            const uint8_t* const from = scales + static_cast<int64_t>(min(static_cast<int>(threadIdx.x), p.N - 1 - n0)) * groups;
+            const int first = step * T::kPieces;
+            if constexpr (T::kPieces == 8) {
+                typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+                if (first + 8 <= groups) {
+                    const u32x2 v = *reinterpret_cast<const u32x2_any*>(from + first);
+                    to.scale_bytes[0] = v[0];
+                    to.scale_bytes[1] = v[1];
+                }
+            } else {
+                static_assert(T::kPieces == 16);
+                typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
+                if (first + 16 <= groups) to.scale_bytes = *reinterpret_cast<const u32x4_byte*>(from + first);
+            }
+            if (first + T::kPieces > groups) {
+#pragma unroll
+                for (int i = 0; i < T::kPieces / 4; ++i) {
+                    to.scale_bytes[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) to.scale_bytes[i] |= static_cast<uint32_t>(from[min(first + 4 * i + j, groups - 1)]) << (8 * j);
+                }
+            }
+        }
+        const int kx = min(step * T::kK + 8 * unit, p.K - 8) * kBytes;
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) {
+            const char* const from = xs + (static_cast<uint32_t>(min(x_first + i * x_rows, p.rows - 1 - m0)) * static_cast<uint32_t>(p.x_stride * kBytes) + kx);
+#pragma unroll
+            for (int j = 0; j < (F32 ? 2 : 1); ++j) to.x[i][j] = reinterpret_cast<const u32x4_any*>(from)[j];
+        }
+    };
+    auto stage = [&](int step, int buffer, Ahead& from) {
+        u32x4* const to_x = lds + buffer * T::kBuffer;
+        u32x4* const to_w = to_x + T::kX;
+        const bool inside = step * T::kK + 8 * unit < p.K;
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) {
+            const int row = x_first + i * x_rows;
+#pragma unroll
+            for (int j = 0; j < (F32 ? 2 : 1); ++j) from.x[i][j] = inside ? from.x[i][j] : u32x4{0, 0, 0, 0};
+            u32x4* const to = to_x + unit * T::kRows + (row ^ (unit & 7));
+            if constexpr (F32) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(from.x[i][j / 4][j % 4]);
+                bf16x8 planes[3];
+                planes_of<true>(v, planes);
+#pragma unroll
+                for (int j = 0; j < 3; ++j) to[j * (T::kUnits * T::kRows)] = __builtin_bit_cast(u32x4, planes[j]);
+            } else {
+                to[0] = from.x[i][0];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i) {
+            const int at = i * T::kThreads + static_cast<int>(threadIdx.x), row = at / T::kPieces, piece = at % T::kPieces;
+            if (T::kW % T::kThreads != 0 && at >= T::kW) break;
+            to_w[row * T::kPieces + (piece ^ (row & 7))] = from.w[i];
+        }
+        if (static_cast<int>(threadIdx.x) < T::kCols) {
+            uint32_t* const to = reinterpret_cast<uint32_t*>(to_w + T::kW) + threadIdx.x * (T::kPieces / 4);
+#pragma unroll
+            for (int i = 0; i < T::kPieces / 4; ++i) to[i] = from.scale_bytes[i];
+        }
+    };
+
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0, 0, 0, 0};
+    // Each column tile starts elsewhere in K. All blocks of an XCD read the same x, a step of it in rows that lie a
+    // multiple of 4 KB apart as often as not: in step they would all meet in the one or two channels of L2 that hold it.
+    const int steps = (p.K + T::kK - 1) / T::kK, start = (n_tile >> 3) % steps;
+    auto turned = [&](int step) { return start + step < steps ? start + step : start + step - steps; };
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+        if (i < steps) load(turned(i), ahead[i]);
+    stage(turned(0), 0, ahead[0]);
+    // A lane's 16 elements of the wave's 64 are k = 64 kw + 16 g ..: half (g & 1) of piece 2 kw + g / 2, units 8 kw + 2 g
+    // and the next.
+    const int piece = 2 * kw + (g >> 1);
+    auto advance = [&](int step, auto place) {  // place: step modulo DEPTH
+        constexpr int kPlace = decltype(place)::value;
+        const u32x4* const from_x = lds + kPlace % BUFFERS * T::kBuffer;
+        const u32x4* const from_w = from_x + T::kX;
+        __syncthreads();
+        if (step + DEPTH < steps) load(turned(step + DEPTH), ahead[kPlace]);
+        bf16x8 xv[2][MT][P];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int u = 8 * kw + 2 * g + i;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < P; ++j)
+                    xv[i][m][j] = __builtin_bit_cast(bf16x8, from_x[j * (T::kUnits * T::kRows) + u * T::kRows + 16 * m + (l ^ (u & 7))]);
+        }
+        u32x2 codes_of[NT];
+        float scale[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = 16 * (NT * wn + n) + l;
+            codes_of[n] = reinterpret_cast<const u32x2*>(from_w + row * T::kPieces + (piece ^ (row & 7)))[g & 1];
+            scale[n] = scale_of(reinterpret_cast<const uint8_t*>(from_w + T::kW)[row * T::kPieces + piece]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const bf16x8 wv = fp4_octet(codes_of[n][i], scale[n]);
+#pragma unroll
+                for (int j = P - 1; j >= 0; --j)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[i][m][j], acc[n][m], 0, 0, 0);
+            }
+        if (BUFFERS == 1) __syncthreads();
+        if (step + 1 < steps) stage(turned(step + 1), (kPlace + 1) % BUFFERS, ahead[(kPlace + 1) % DEPTH]);
+    };
+    static_assert(DEPTH == 2 || DEPTH == 4, "the place of a step gives its buffer");
+    for (int step = 0; step < steps; step += DEPTH) {
+        advance(step, std::integral_constant<int, 0>{});
+        if (step + 1 < steps) advance(step + 1, std::integral_constant<int, 1>{});
+        if constexpr (DEPTH == 4) {
+            if (step + 2 < steps) advance(step + 2, std::integral_constant<int, 2>{});
+            if (step + 3 < steps) advance(step + 3, std::integral_constant<int, 3>{});
         }
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) part[wave][l][4 * g + r] = acc[r];
+
     __syncthreads();
-    const int row = threadIdx.x / 16, col = threadIdx.x % 16;
-    if (m0 + row >= p.rows || n0 + col >= p.N) return;
-    float y = part[0][row][col];
+    float* const part = reinterpret_cast<float*>(lds) + wn * KW * T::kParts * 256 + lane;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) y += part[w][row][col];
-    if (p.bias != nullptr) y += p.bias[n0 + col];
-    Element<F32>::put(p.out, static_cast<int64_t>(m0 + row) * p.N + n0 + col, y);
+    for (int t = 0; t < NT * MT; ++t)
+        if (t % KW != kw)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[(kw * T::kParts + T::part_of(kw, t)) * 256 + r * 64] = acc[t / MT][t % MT][r];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int col = n0 + 16 * (NT * wn + n) + 4 * g;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int row = m0 + 16 * m + l, t = n * MT + m;
+            if (t % KW != kw) continue;
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = acc[n][m][r];
+#pragma unroll
+            for (int other = 0; other < KW; ++other)
+                if (other != t % KW)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] += part[(other * T::kParts + T::part_of(other, t)) * 256 + r * 64];
+            if (row >= p.rows || col >= p.N) continue;
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] += p.bias[min(col + r, p.N - 1)];
+            }
+            const int64_t to = static_cast<int64_t>(row) * p.N + col;
+            if (p.N % 4 == 0) {
+                put4<F32>(p.out, to, y);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (col + r < p.N) Element<F32>::put(p.out, to + r, y[r]);
+            }
+        }
+    }
+}
+
+template <bool F32, int WN, int KW, int NT, int MT, int DEPTH, int BUFFERS>
+void launch_tile(const Fp4LinearArgs& p, hipStream_t s) {
+    using T = TileShape<F32, WN, KW, NT, MT, BUFFERS>;
+    static_assert(T::kLds <= 160 * 1024);
+    const int64_t n_tiles = ceil_div(p.N, T::kCols), m_tiles = ceil_div(p.rows, T::kRows);
+    hipLaunchKernelGGL((linear_fp4_tile_kernel<F32, WN, KW, NT, MT, DEPTH, BUFFERS>), dim3(static_cast<unsigned>(8 * ceil_div(n_tiles, 8) * m_tiles)),
+                       dim3(T::kThreads), T::kLds, s, p, static_cast<int>(n_tiles), static_cast<int>(m_tiles));
+}
+template <bool F32, int NT>
+void launch_stream(const Fp4LinearArgs& p, hipStream_t s) {
+    constexpr int KW = 8, U = 2;
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 16 * NT)), static_cast<unsigned>(ceil_div(p.rows, 16)));
+    if (p.rows <= kFew) {
+        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, false, KW, NT, U>), grid, dim3(KW * 64), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, true, KW, NT, U>), grid, dim3(KW * 64), 0, s, p);
+    }
+}
+
+// The forms' times go as the rounds of blocks on 256 CUs. Measured for K = 4096 in bf16 (us, launch included):
+//
+//   N      rows  stream  64-column tiles  128-column tiles
+//   4096    64     9.2        17.8             24
+//   4096   128    15.6        18.4             24
+//   4096   256    31          19.2             24
+//   12288   32    17.0        22.3             29
+//   12288   64    25.5        22.5             29
+//   12288  128    45          41               29
+//
+// that is 3.5 us for 256 stream blocks of 32 columns and 16 rows (fractions of a round count, blocks are many to a CU),
+// 17 and 24 for a round of tiles by 64 rows. fp32: 12 for 256 stream blocks of 64 columns, 34 for a round of 128-column
+// tiles by 32 rows. Stream blocks take more columns, and share what x costs, where enough blocks are left: 12288 x 16 rows
+// 14.8 us with 16 columns and 11.2 with 32, but 4096 x 16 rows 6.0 and 6.9; fp32 12288 x 1 row 16.9, 18.2 and with 64
+// columns 14.5.
+template <bool F32>
+void launch(const Fp4LinearArgs& p, hipStream_t s) {
+    const double tiles16 = static_cast<double>(ceil_div(p.rows, 16));
+    auto rounds = [&](int64_t cols, int64_t rows) { return static_cast<double>(ceil_div(ceil_div(p.N, cols) * ceil_div(p.rows, rows), 256)); };
+    const bool offsets_fit = p.x_stride < (int64_t{1} << 24);  // a tile's rows of x are addressed in 32 bits
+    if constexpr (F32) {
+        if (offsets_fit && 34 * rounds(128, 32) < 12 * std::max(1.0, static_cast<double>(ceil_div(p.N, 64)) * tiles16 / 256)) return launch_tile<true, 2, 4, 4, 2, 2, 2>(p, s);
+        if (static_cast<double>(ceil_div(p.N, 64)) * tiles16 >= 192) return launch_stream<true, 4>(p, s);
+    } else {
+        const double stream = 3.5 * std::max(1.0, static_cast<double>(ceil_div(p.N, 32)) * tiles16 / 256), narrow = 17 * rounds(64, 64), wide = 24 * rounds(128, 64);
+        if (offsets_fit && std::min(narrow, wide) < stream) return narrow < wide ? launch_tile<false, 2, 4, 2, 4, 2, 2>(p, s) : launch_tile<false, 2, 4, 4, 4, 2, 2>(p, s);
+    }
+    if (static_cast<double>(ceil_div(p.N, 32)) * tiles16 >= 256) return launch_stream<F32, 2>(p, s);
+    launch_stream<F32, 1>(p, s);
 }
 
 }  // namespace
@@ -77,17 +470,17 @@ extern "C" mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_fea
     MLK_CHECK(dtype == MLK_DTYPE_F32 || dtype == MLK_DTYPE_BF16, "dtype must be f32 or bf16");
     MLK_CHECK(rows >= 0 && out_features > 0, "invalid linear geometry");
     MLK_CHECK(in_features > 0 && in_features % kGroup == 0, "in_features must be a positive multiple of 32");
-    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 31) && out_features < (int64_t{1} << 31) - 16, "too many rows or features");
+    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 24) && out_features < (int64_t{1} << 31) - 16, "too many rows or features");
     if (rows == 0) return MLK_OK;
     MLK_CHECK(x && codes && scales && out, "null tensor pointer");
-    MLK_CHECK((reinterpret_cast<uintptr_t>(codes) & 15) == 0, "codes must be 16-byte aligned");
+    MLK_CHECK((reinterpret_cast<uintptr_t>(codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
+              "codes and out must be 16-byte aligned");
     Fp4LinearArgs p{x, x_stride, codes, scales, bias, out, static_cast<int32_t>(rows), static_cast<int32_t>(in_features), static_cast<int32_t>(out_features)};
-    const dim3 grid(static_cast<unsigned>(ceil_div(out_features, 16)), static_cast<unsigned>(ceil_div(rows, 16)));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (dtype == MLK_DTYPE_F32) {
-        hipLaunchKernelGGL(linear_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, s, p);
+        launch<true>(p, s);
     } else {
-        hipLaunchKernelGGL(linear_fp4_kernel<false>, grid, dim3(kWaves * 64), 0, s, p);
+        launch<false>(p, s);
     }
     return launch_status("linear fp4");
 }
