@@ -40,11 +40,9 @@ __device__ __forceinline__ void put4(void* out, int64_t first, const float (&y)[
 // its own piece of LDS. x comes the same way (TURN), or, for the first FEW rows, straight to the lanes whose row exists.
 // Past K a lane's x is zero (its W is that of the last group, which counts anyway). An infinity or a NaN in fp32 x makes
 // the quick planes NaN; a wave that sees one in its sums forms them again.
-// Blocks of 16 columns are held to the registers of two blocks a CU: with 146 the 257th block waited for a round of its
-// own (fp32, 4100 x 4096, 16 rows: 14.2 us).
 constexpr int kFew = 4;
 template <bool F32, bool TURN, int KW, int NT, int U>
-__global__ __launch_bounds__(KW * 64, NT == 1 ? 4 : 1) void linear_fp4_stream_kernel(Fp4LinearArgs p) {
+__global__ __launch_bounds__(KW * 64) void linear_fp4_stream_kernel(Fp4LinearArgs p) {
     constexpr int P = F32 ? 3 : 1, kPieces = F32 ? 8 : 4;  // 16-byte pieces of 32 elements of x
     constexpr int kRow = 4 * U;                            // groups of a row that an iteration takes, 4 a matrix instruction
     constexpr int kTurn = 16 * kRow * NT + (TURN ? 16 * 4 * kPieces : 0), kPart = (16 * (16 * NT + 1) + 3) / 4;
@@ -440,23 +438,27 @@ void launch_stream(const Fp4LinearArgs& p, hipStream_t s) {
 //
 // that is 3.5 us for 256 stream blocks of 32 columns and 16 rows (fractions of a round count, blocks are many to a CU),
 // 17 and 24 for a round of tiles by 64 rows. fp32: 12 for 256 stream blocks of 64 columns, 34 for a round of 128-column
-// tiles by 32 rows. Stream blocks take more columns, and share what x costs, where enough blocks are left: 12288 x 16 rows
-// 14.8 us with 16 columns and 11.2 with 32, but 4096 x 16 rows 6.0 and 6.9; fp32 12288 x 1 row 16.9, 18.2 and with 64
-// columns 14.5.
+// tiles by 32 rows. A stream block that takes more columns shares what its x costs among them, and leaves CUs idle where
+// there are few: the round of 256 blocks of 16, 32 and 64 columns takes 4.0 and 4.9 us in bf16 (2.9 and 3.8 with 4 rows
+// and less), 6.7, 8.1 and 11.6 in fp32 (5.2, 6.8 and 9.5). 12288 x 16 rows in bf16: 14.8 us with 16 columns, 11.2 with
+// 32; 4096 x 16 rows 6.0 and 6.9; fp32 12288 x 1 row 16.9, 18.2 and 14.5; 4100 x 16 rows 14.2 (257 blocks) and 10.0.
 template <bool F32>
 void launch(const Fp4LinearArgs& p, hipStream_t s) {
-    const double tiles16 = static_cast<double>(ceil_div(p.rows, 16));
+    const int64_t tiles16 = ceil_div(p.rows, 16);
     auto rounds = [&](int64_t cols, int64_t rows) { return static_cast<double>(ceil_div(ceil_div(p.N, cols) * ceil_div(p.rows, rows), 256)); };
+    auto full = [&](int64_t cols) { return std::max(1.0, static_cast<double>(ceil_div(p.N, cols) * tiles16) / 256); };
     const bool offsets_fit = p.x_stride < (int64_t{1} << 24);  // a tile's rows of x are addressed in 32 bits
+    const bool few = p.rows <= kFew;
     if constexpr (F32) {
-        if (offsets_fit && 34 * rounds(128, 32) < 12 * std::max(1.0, static_cast<double>(ceil_div(p.N, 64)) * tiles16 / 256)) return launch_tile<true, 2, 4, 4, 2, 2, 2>(p, s);
-        if (static_cast<double>(ceil_div(p.N, 64)) * tiles16 >= 192) return launch_stream<true, 4>(p, s);
+        if (offsets_fit && 34 * rounds(128, 32) < 12 * full(64)) return launch_tile<true, 2, 4, 4, 2, 2, 2>(p, s);
+        const double by16 = (few ? 5.2 : 6.7) * rounds(16, 16), by32 = (few ? 6.8 : 8.1) * rounds(32, 16), by64 = (few ? 9.5 : 11.6) * rounds(64, 16);
+        if (by64 < std::min(by16, by32)) return launch_stream<true, 4>(p, s);
+        by16 <= by32 ? launch_stream<true, 1>(p, s) : launch_stream<true, 2>(p, s);
     } else {
-        const double stream = 3.5 * std::max(1.0, static_cast<double>(ceil_div(p.N, 32)) * tiles16 / 256), narrow = 17 * rounds(64, 64), wide = 24 * rounds(128, 64);
+        const double stream = 3.5 * full(32), narrow = 17 * rounds(64, 64), wide = 24 * rounds(128, 64);
         if (offsets_fit && std::min(narrow, wide) < stream) return narrow < wide ? launch_tile<false, 2, 4, 2, 4, 2, 2>(p, s) : launch_tile<false, 2, 4, 4, 4, 2, 2>(p, s);
+        (few ? 2.9 : 4.0) * rounds(16, 16) <= (few ? 3.8 : 4.9) * rounds(32, 16) ? launch_stream<false, 1>(p, s) : launch_stream<false, 2>(p, s);
     }
-    if (static_cast<double>(ceil_div(p.N, 32)) * tiles16 >= 256) return launch_stream<F32, 2>(p, s);
-    launch_stream<F32, 1>(p, s);
 }
 
 }  // namespace
