@@ -438,8 +438,8 @@ mlk_status mlk_mamba3_siso_step(const float* projected, int64_t streams, int64_t
  * four bits) and 2 j + 1.
  *
  * `positions` [batch, length] gives every token its place in its sequence; a negative one is padding. `page_table`
- * [batch, table_width] names a sequence's pages; entries of pages that no token needs are not read. Both are contiguous
- * int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes, 16-byte aligned, page_size a
+ * [batch, table_width] names a sequence's pages, 2^28 tokens at most; entries of pages that no token needs may be
+ * anything. Both are contiguous int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes, 16-byte aligned, page_size a
  * multiple of 16 up to 1024, head_dim 32, 64, 128 or 256. A (page, head) holds key codes [page_size][head_dim / 2], value
  * codes [head_dim / 2][page_size], key scales [page_size][head_dim / 32], value scales [head_dim / 32][page_size].
  * Strides are {sequence, token, head} in elements, head_dim dense. */

@@ -27,10 +27,12 @@ constexpr int kGroup = 32;  // values under one scale
 // The float whose exponent bits are the scale byte: what the conversions take as scale.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Byte `i` of a dword as that float.
+// Byte `i` of a dword as a scale: shifted to the exponent's place. The neighbouring bits that come along as sign and
+// significand do not count (all bytes and codes, 64 patterns of them each, convert alike).
 template <int i>
 __device__ __forceinline__ float scale_at(uint32_t dword) {
-    return __uint_as_float(((dword >> (8 * i)) & 0xFF) << 23);
+    if constexpr (i == 3) return __uint_as_float(dword >> 1);
+    return __uint_as_float(dword << ((23 - 8 * i) & 31));
 }
 
 template <int byte>

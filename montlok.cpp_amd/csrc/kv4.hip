@@ -24,14 +24,14 @@ namespace {
 
 constexpr int kRun = 16;     // tokens of a page that one lane takes: page sizes are multiples of it
 constexpr int kTile = 64;    // keys a wave takes at a time
-constexpr int kWaves = 4;    // of an attention block
+constexpr int W = 8;         // waves of an attention block
 
 struct Cache {
     uint8_t* bytes;
     int64_t record;  // bytes of a (page, head)
     int32_t pages, kv_heads, page_size;
     int32_t runs;     // page_size / kRun
-    uint32_t magic;   // ceil(2^32 / runs); runs = 1: 0
+    uint32_t magic;   // ceil(2^31 / runs)
     const int32_t* table;
     int32_t width;
     const int32_t* positions;
@@ -40,19 +40,19 @@ struct Cache {
     int64_t value_codes(int dim) const { return static_cast<int64_t>(page_size) * (dim / 2); }
 };
 
-// Page index of a run of 16 tokens and the run's place in it. run < 2^26, runs <= 64: the product with the
-// rounded-up reciprocal is exact.
+// Page index of a run of 16 tokens and the run's place in it. run < 2^24, runs <= 64: the product of twice the run with
+// the rounded-up reciprocal of twice the runs is exact (its error is below 2^25 * 127 / 2^32 of a page's 128th).
 __device__ __forceinline__ void split_run(const Cache& c, uint32_t run, uint32_t& page, uint32_t& token) {
-    page = c.magic == 0 ? run : __umulhi(run, c.magic);
+    page = __umulhi(2 * run, c.magic);
     token = (run - page * static_cast<uint32_t>(c.runs)) * kRun;
 }
 
 // The record of token `at` of sequence b, and its place in the page; null where the table has no such page.
 __device__ __forceinline__ uint8_t* record_of(const Cache& c, int b, int at, int head, int& offset) {
+    if (at >= c.width * c.page_size) return nullptr;
     uint32_t page, first;
     split_run(c, static_cast<uint32_t>(at) / kRun, page, first);
     offset = static_cast<int>(first) + at % kRun;
-    if (page >= static_cast<uint32_t>(c.width)) return nullptr;
     const int id = c.table[static_cast<int64_t>(b) * c.width + page];
     if (id < 0 || id >= c.pages) return nullptr;
     return c.bytes + (static_cast<int64_t>(id) * c.kv_heads + head) * c.record;
@@ -183,6 +183,21 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// Eight elements of a row at any alignment.
+template <bool F32>
+__device__ __forceinline__ void load8(const void* p, int64_t first, float (&x)[8]) {
+    typedef uint32_t Four __attribute__((ext_vector_type(4), aligned(2)));
+    if constexpr (F32) {
+        const Four* const from = reinterpret_cast<const Four*>(static_cast<const float*>(p) + first);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(from[i / 4][i % 4]);
+    } else {
+        const Four v = *reinterpret_cast<const Four*>(static_cast<const uint16_t*>(p) + first);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i % 2 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
+    }
+}
+
 // Eight results of a lane: elements first .. first + 7 of an output row.
 template <bool F32>
 __device__ __forceinline__ void put8(void* out, int64_t first, const float (&v)[8]) {
@@ -198,208 +213,318 @@ __device__ __forceinline__ void put8(void* out, int64_t first, const float (&v)[
     }
 }
 
-template <int D, bool F32, int MT>
-__global__ __launch_bounds__(kWaves * 64) void kv4_attention_kernel(AttentionArgs p) {
-    constexpr int S = D / 32;          // k steps of a score product, and groups of a token
-    constexpr int P = F32 ? 3 : 1;     // bf16 operands that make up a query or a weight
-    constexpr int kScales = D == 256 ? 2 : 1;  // scales that a lane's part of a key row meets
-    __shared__ float exchange[2][2 * S * 4 * MT][64];
-    __shared__ float stats[kWaves][2][16 * MT];
+// What a wave holds in LDS of its tile of 64 keys: their codes, then, once they are in registers, the values'.
+template <int S>
+struct TileLds {
+    u32x4 codes[64 * S];        // keys: row l of key tile a, 16-byte piece c at (16 a + l) S + (c ^ turn(l)); values: row j,
+                                // piece c at 4 j + (c ^ (j / 2 & 3))
+    uint8_t key_scale[64 * S];  // of row l of key tile a at (4 l + a) S
+    uint8_t value_scale[64 * S];  // [S][64]
+    // Eight lanes that read, or write, together meet in different banks.
+    static __device__ __forceinline__ int turn(int l) { return S == 8 ? l & 7 : S == 4 ? l >> 1 & 3 : S == 2 ? l >> 2 & 1 : 0; }
+};
+
+// N bytes of a lane.
+template <int N>
+struct Bytes;
+template <>
+struct Bytes<1> {
+    using type = uint8_t;
+};
+template <>
+struct Bytes<2> {
+    using type = uint16_t;
+};
+template <>
+struct Bytes<4> {
+    using type = uint32_t;
+};
+template <>
+struct Bytes<8> {
+    using type = uint64_t;
+};
+
+// A block takes 16 rows of a (sequence, key head) and every p.splits-th group of W tiles of 64 keys, a tile a wave.
+//
+// Scores are key tile x q^T, so that lane (g, l) holds row l's scores of 16 tokens, in the registers from which the
+// product with the values takes its weights: nothing moves between lanes but the maximum (a column's sum is formed at
+// the end). Key tile a, row 4 g' + r is token 16 g' + 4 a + r of the 64, so that a lane's scores (rows 4 g .. 4 g + 3 of
+// every tile) are its 16 tokens 16 g .. 16 g + 15 of the value product.
+// WHOLE: pages of whole tiles. A tile then has one page, looked up by the scalar unit.
+template <int D, bool F32, bool WHOLE>
+__global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void kv4_attention_kernel(AttentionArgs p) {
+    constexpr int S = D / 32;       // k steps of a score product, groups of a token, 1 KB loads of a tile's keys (or values)
+    constexpr int P = F32 ? 3 : 1;  // bf16 operands that make up a query or a weight
+    constexpr bool kShared = F32 || S == 8;  // q in LDS: its registers would cost the second wave a SIMD
+    using Scales = typename Bytes<S>::type;
+    struct Exchange {
+        f32x4 acc[W][2 * S][64];
+        float stats[W][2][16];
+    };
+    __shared__ union {
+        TileLds<S> tile[W];
+        Exchange end;
+    } lds;
+    __shared__ bf16x8 shared_q[kShared ? P * S : 1][64];
     const Cache& c = p.c;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
     unsigned id = blockIdx.x;
     const int split = id % p.splits;
     id /= p.splits;
-    const int row0 = static_cast<int>(id % p.row_tiles) * (16 * MT);
+    const int row0 = static_cast<int>(id % p.row_tiles) * 16;
     id /= p.row_tiles;
     const int head = id % c.kv_heads, b = id / c.kv_heads;
     const int capacity = c.width * c.page_size;
+    const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2), page_stride = c.kv_heads * c.record;
+    const int32_t* const table = c.table + static_cast<int64_t>(b) * c.width;
+    const uint8_t* const records = c.bytes + head * c.record;
+    TileLds<S>& mine = lds.tile[wave];
 
-    // Rows, their positions, and q as operands.
-    int position[MT];
-    bf16x8 q[MT][P][S];
-    int last = -1, least = 0x7FFFFFFF;
+    // Loads take 16 bytes a lane of whole stretches of memory (in operand order every lane would be a cache access of its
+    // own); a tile is 4 runs of 16 tokens, each on a page of its own for all that is known. Keys: load t is bytes 1024 t ..
+    // of [64][D / 2]; values: rows 16 t .. of [D / 2][64], run lane & 3; scales: S bytes a lane of [64][S] and [S][64].
+    // A run on no page is read from page 0 and its keys made NaN, which only rows that see them take.
+    struct Ids {
+        int32_t by_group, by_piece;  // pages of runs g and lane & 3; the tile's page
+    };
+    auto lookup = [&](int tile) {
+        auto page_of = [&](int run) {
+            uint32_t page, token;
+            split_run(c, 4 * tile + run, page, token);
+            return page < static_cast<uint32_t>(c.width) ? table[page] : -1;
+        };
+        if constexpr (WHOLE) return Ids{page_of(0), 0};
+        return Ids{page_of(g), page_of(lane & 3)};
+    };
+    u32x4 key_ahead[S], value_ahead[S];
+    Scales key_scale_ahead, value_scale_ahead;
+    auto load_whole = [&](int tile, const Ids& ids) {
+        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
+        uint32_t page, token;
+        split_run(c, 4 * tile, page, token);
+        const uint8_t* const record = records + (bad ? 0 : ids.by_group) * page_stride;
+        const uint8_t* const keys = record + token * (D / 2);
+        const uint8_t* const values = record + half + token;
+        const uint8_t* const scales = record + 2 * half;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = row0 + 16 * m + l, clamped = min(row, p.rows - 1), token = clamped / p.group;
-        const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
-        position[m] = row < p.rows && at < capacity ? at : -1;
-        last = max(last, position[m]);
-        least = min(least, position[m] < 0 ? 0x7FFFFFFF : position[m]);
-        const int64_t from = b * p.q_bs + token * p.q_ts + (head * p.group + clamped % p.group) * p.q_hs + (D / 4) * g;
+        for (int t = 0; t < S; ++t) key_ahead[t] = *reinterpret_cast<const u32x4*>(keys + static_cast<uint32_t>(1024 * t + 16 * lane));
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float x[8];
+        for (int t = 0; t < S; ++t)
+            value_ahead[t] = *reinterpret_cast<const u32x4*>(values + static_cast<uint32_t>((16 * t + (lane >> 2)) * c.page_size + 16 * (lane & 3)));
+        key_scale_ahead = *reinterpret_cast<const Scales*>(scales + token * S + static_cast<uint32_t>(lane * S));
+        if (bad) key_scale_ahead = static_cast<Scales>(~uint64_t{0});
+        value_scale_ahead = *reinterpret_cast<const Scales*>(scales + S * c.page_size + token +
+                                                             static_cast<uint32_t>(lane * S / 64 * c.page_size + lane * S % 64));
+    };
+    auto load = [&](int tile, const Ids& ids) {
+        if constexpr (WHOLE) return load_whole(tile, ids);
+        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
+        const int group_id = bad ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
+        uint32_t page, token;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = Element<F32>::get(p.q, from + 8 * s + i);
-            if constexpr (F32) {
-                bf16x8 plane[3];
-                planes_of<true>(x, plane);
+        for (int t = 0; t < S; ++t) {
+            const int run = S == 8 ? t / 2 : S == 4 ? t : S == 2 ? 2 * t + (lane >> 5) : g;
+            const int key_id = S >= 4 ? __builtin_amdgcn_readlane(group_id, 16 * run) : S == 2 ? __shfl(group_id, 16 * run, kWave) : group_id;
+            split_run(c, 4 * tile + run, page, token);
+            key_ahead[t] = *reinterpret_cast<const u32x4*>(records + key_id * page_stride + (token * (D / 2) + 1024 * t + 16 * lane - run * (8 * D)));
+        }
+        split_run(c, 4 * tile + (lane & 3), page, token);
+        const uint8_t* const value = records + piece_id * page_stride + half + ((lane >> 2) * c.page_size + static_cast<int>(token));
 #pragma unroll
-                for (int i = 0; i < 3; ++i) q[m][i][s] = plane[i];
+        for (int t = 0; t < S; ++t) value_ahead[t] = *reinterpret_cast<const u32x4*>(value + 16 * t * c.page_size);
+        split_run(c, 4 * tile + g, page, token);
+        key_scale_ahead = *reinterpret_cast<const Scales*>(records + group_id * page_stride + 2 * half + (static_cast<int>(token) + l) * S);
+        if (bad) key_scale_ahead = static_cast<Scales>(~uint64_t{0});
+        const int at = lane * S % 64, run = at / 16;  // token of the lane's value scales
+        split_run(c, 4 * tile + run, page, token);
+        value_scale_ahead = *reinterpret_cast<const Scales*>(records + (S == 1 ? group_id : __shfl(group_id, 16 * run, kWave)) * page_stride + 2 * half +
+                                                             ((S + lane * S / 64) * c.page_size + static_cast<int>(token) + at % 16));
+    };
+    // The first tile is on its way before the rows are known.
+    const int stride = W * p.splits, first_tile = split * W + wave;
+    Ids ids = lookup(first_tile);
+    load(first_tile, ids);
+    ids = lookup(first_tile + stride);
+
+    // Rows, their positions, and q as operands, times the sign of the scale: the largest score is then the one of the
+    // largest weight.
+    const float factor = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
+    const float scale = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
+    const int row = row0 + l, token = min(row, p.rows - 1) / p.group, of_group = min(row, p.rows - 1) - token * p.group;
+    const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
+    const int position = row < p.rows && at < capacity ? at : -1;
+    bf16x8 q[P][kShared ? 1 : S];
+    const int64_t q_from = b * p.q_bs + token * p.q_ts + (head * p.group + of_group) * p.q_hs + (D / 4) * g;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        if (kShared && s % W != wave) continue;
+        float x[8];
+        load8<F32>(p.q, q_from + 8 * s, x);
+        bf16x8 operand[P];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= factor;
+        if constexpr (F32) {
+            planes_of<true>(x, operand);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) operand[0][i] = static_cast<__bf16>(x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if constexpr (kShared) {
+                shared_q[s * P + i][lane] = operand[i];
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[m][0][s][i] = static_cast<__bf16>(x[i]);
+                q[i][s] = operand[i];
             }
         }
     }
+    int last = position, least = position < 0 ? 0x7FFFFFFF : position;
 #pragma unroll
     for (int i = 1; i < 16; i *= 2) {
         last = max(last, __shfl_xor(last, i, kWave));
         least = min(least, __shfl_xor(least, i, kWave));
     }
-    const int tiles = (last + kTile) / kTile;  // 0 where no row has a key
-    const int begin = static_cast<int>(static_cast<int64_t>(tiles) * split / p.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / p.splits);
+    if constexpr (kShared) __syncthreads();
 
-    float top[MT], sum[MT];
-    f32x4 acc[MT][S][2];
+    float top = -INFINITY, sum = 0.0f;  // the largest score so far, and the lane's part of the sum of 2^(scale (score - top))
+    f32x4 acc[S][2];                    // elements 32 s + 8 g + 2 r and the next, of row l
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        top[m] = -INFINITY;
-        sum[m] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S; ++s) acc[m][s][0] = acc[m][s][1] = f32x4{0, 0, 0, 0};
-    }
+    for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = f32x4{0, 0, 0, 0};
 
-    const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2);
-    const int32_t* const table = c.table + static_cast<int64_t>(b) * c.width;
-    for (int tile = begin + wave; tile < end; tile += kWaves) {
+    for (int tile = first_tile; tile * kTile <= last; tile += stride) {
         const int first = tile * kTile;
-        // Key tile a, row 4 g' + r is token 16 g' + 4 a + r of the 64, so that a lane's scores (rows 4 g .. 4 g + 3
-        // of every tile) are its 16 tokens 16 g .. 16 g + 15 of the value product.
-        uint32_t page, run;
-        split_run(c, (first >> 4) + (l >> 2), page, run);
-        bool held = first + 16 * (l >> 2) <= last;
-        int id_k = held ? table[page] : 0;
-        const bool bad = id_k < 0 || id_k >= c.pages;
-        if (bad) id_k = 0;
-        const uint8_t* const key = c.bytes + (static_cast<int64_t>(id_k) * c.kv_heads + head) * c.record;
+#pragma unroll
+        for (int t = 0; t < S; ++t) {
+            const int at = 64 * t + lane, token = at / S, row = token >> 4 << 2 | (token & 3), a = token >> 2 & 3;
+            mine.codes[(16 * a + row) * S + (at % S ^ mine.turn(row))] = key_ahead[t];
+        }
+        reinterpret_cast<Scales*>(mine.key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = key_scale_ahead;  // token 16 g + l
+        reinterpret_cast<Scales*>(mine.value_scale)[lane] = value_scale_ahead;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         uint32_t kc[4][S], ks[4];
+        // The scales of a lane's part of a key row: byte g of four (S = 4), g / 2 of two, the only one, or 2 g and 2 g + 1.
+        const uint8_t* const key_scales = mine.key_scale + 4 * l * S;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const int token = run + 4 * a + (l & 3);
-            const uint8_t* const from = key + token * (D / 2) + (D / 8) * g;
-            const uint8_t* const scale = key + 2 * half + token * S;
+            const uint8_t* const row = reinterpret_cast<const uint8_t*>(mine.codes + (16 * a + l) * S);
             if constexpr (S == 1) {
-                kc[a][0] = *reinterpret_cast<const uint32_t*>(from);
-                ks[a] = scale[0];
-            } else if constexpr (S == 2) {
-                const u32x2 v = *reinterpret_cast<const u32x2*>(from);
+                kc[a][0] = reinterpret_cast<const uint32_t*>(row)[g];
+                ks[a] = key_scales[a];
+            }
+            if constexpr (S == 2) {
+                const u32x2 v = reinterpret_cast<const u32x2*>(row + 16 * (g >> 1 ^ mine.turn(l)))[g & 1];
                 kc[a][0] = v[0], kc[a][1] = v[1];
-                ks[a] = scale[g >> 1];
-            } else {
+                ks[a] = key_scales[2 * a + (g >> 1)];
+            }
+            if constexpr (S >= 4) {
 #pragma unroll
                 for (int i = 0; i < S / 4; ++i) {
-                    const u32x4 v = reinterpret_cast<const u32x4*>(from)[i];
+                    const u32x4 v = reinterpret_cast<const u32x4*>(row)[(S / 4 * g + i) ^ mine.turn(l)];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) kc[a][4 * i + j] = v[j];
                 }
-                ks[a] = S == 4 ? scale[g] : reinterpret_cast<const uint16_t*>(scale)[g];
+                ks[a] = S == 4 ? key_scales[4 * a + g] : reinterpret_cast<const uint16_t*>(key_scales)[4 * a + g];
             }
-            if (bad) ks[a] = 0xFFFF;
         }
-        split_run(c, (first >> 4) + g, page, run);
-        held = first + 16 * g <= last;
-        int id_v = held ? table[page] : 0;
-        if (id_v < 0 || id_v >= c.pages) id_v = 0;
-        const uint8_t* const value = c.bytes + (static_cast<int64_t>(id_v) * c.kv_heads + head) * c.record;
-        u32x4 vc[S], vs[S];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int t = 0; t < S; ++t) {
+            const int j = 16 * t + (lane >> 2);
+            mine.codes[4 * j + ((lane & 3) ^ (j >> 1 & 3))] = value_ahead[t];
+        }
+        if ((tile + stride) * kTile <= last) {
+            load(tile + stride, ids);
+            ids = lookup(tile + 2 * stride);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+
+        f32x4 score[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) score[a] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            vc[s] = *reinterpret_cast<const u32x4*>(value + half + static_cast<int64_t>(16 * s + l) * c.page_size + run);
-            vs[s] = *reinterpret_cast<const u32x4*>(value + 2 * half + static_cast<int64_t>(S + s) * c.page_size + run);
-        }
-
-        f32x4 score[MT][4];
+            bf16x8 qs[P];
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
+            for (int i = 0; i < P; ++i) {
+                if constexpr (kShared) {
+                    qs[i] = shared_q[s * P + i][lane];
+                } else {
+                    qs[i] = q[i][s];
+                }
+            }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) score[m][a] = f32x4{0, 0, 0, 0};
+            for (int a = 0; a < 4; ++a) {
+                const bf16x8 k = fp4_octet(kc[a][s], s < 4 ? scale_at<0>(ks[a]) : scale_at<1>(ks[a]));
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const bf16x8 k = fp4_octet(kc[a][s], kScales == 1 ? scale_at<0>(ks[a]) : (s < 4 ? scale_at<0>(ks[a]) : scale_at<1>(ks[a])));
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = P - 1; i >= 0; --i) score[m][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[m][i][s], score[m][a], 0, 0, 0);
+                for (int i = P - 1; i >= 0; --i) score[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qs[i], score[a], 0, 0, 0);
             }
         }
 
         const bool masked = first + kTile - 1 > least;  // some row does not see the whole tile
-        uint32_t poison[MT];
-        if (masked) {
-            // A value that no row may see must not reach a sum as 0 * NaN: its NaN scale goes, and the rows that do
-            // see it are made NaN below.
+        float most = -INFINITY;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) poison[m] = 0;
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if ((vs[s][i / 4] >> (8 * (i % 4)) & 0xFF) == 0xFF) {
-                        vs[s][i / 4] &= ~(0xFFu << (8 * (i % 4)));
-#pragma unroll
-                        for (int m = 0; m < MT; ++m)
-                            if (first + 16 * g + i <= position[m]) poison[m] |= 1u << s;
-                    }
+        for (int i = 0; i < 16; ++i) {
+            if (masked && first + 16 * g + i > position) score[i / 4][i % 4] = -INFINITY;
+            most = fmaxf(most, score[i / 4][i % 4]);
         }
-
-        bf16x8 weight[MT][P][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float x[16];
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = score[m][i / 4][i % 4] * p.scale_log2;
-                if (masked && first + 16 * g + i > position[m]) x[i] = -INFINITY;
-                most = fmaxf(most, x[i]);
-            }
-            const float before = top[m];
-            top[m] = fmaxf(before, max_over_groups(most));
-            const float base = finite_or_zero(top[m]), shrink = __builtin_amdgcn_exp2f(before - base);
-            float part = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(x[i] - base);
-                part += x[i];
-            }
-            sum[m] = fmaf(sum[m], shrink, part);
+        const float now = fmaxf(top, max_over_groups(most));
+        if (__ballot(now != top) != 0) {  // seldom after the first tiles
+            const float shrink = __builtin_amdgcn_exp2f(fmaf(top, scale, -finite_or_zero(now) * scale));
+            top = now;
+            sum *= shrink;
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                acc[m][s][0] *= shrink;
-                acc[m][s][1] *= shrink;
+                acc[s][0] *= shrink;
+                acc[s][1] *= shrink;
             }
+        }
+        bf16x8 weight[P][2];
+        const float base = finite_or_zero(top) * scale;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float w[8];
+        for (int h = 0; h < 2; ++h) {
+            float w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = x[8 * h + i];
-                if constexpr (F32) {
-                    bf16x8 plane[3];
-                    planes_of<false>(w, plane);  // of finite values, or NaN
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(score[2 * h + i / 4][i % 4], scale, -base));
+                sum += w[i];
+            }
+            if constexpr (F32) {
+                bf16x8 plane[3];
+                planes_of<false>(w, plane);  // of finite values, or NaN
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) weight[m][i][h] = plane[i];
-                } else {
+                for (int i = 0; i < 3; ++i) weight[i][h] = plane[i];
+            } else {
+                // Rounded to nearest: 2^-9 of a weight, which a mean over many keys loses; the sum is of the unrounded.
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) weight[m][0][h][i] = static_cast<__bf16>(w[i]);
-                }
+                for (int i = 0; i < 8; ++i) weight[0][h][i] = static_cast<__bf16>(w[i]);
             }
         }
 
+        uint32_t poison = 0;
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+        for (int s = 0; s < S; ++s) {
+            u32x4 vs = reinterpret_cast<const u32x4*>(mine.value_scale)[4 * s + g];
+            if (masked) {
+                // A value that no row may see must not reach a sum as 0 * NaN: its NaN scale goes, and the rows that do see
+                // it are made NaN below.
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if ((vs[i / 4] >> (8 * (i % 4)) & 0xFF) == 0xFF) {
+                        vs[i / 4] &= ~(0xFFu << (8 * (i % 4)));
+                        if (first + 16 * g + i <= position) poison |= 1u << s;
+                    }
+            }
+            const u32x4 codes = mine.codes[4 * (16 * s + l) + (g ^ (l >> 1 & 3))];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t pair[8];  // elements 2 j and 2 j + 1 of a token
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const uint32_t codes = vc[s][2 * h + w], scales = vs[s][2 * h + w];
-                    pair[4 * w] = fp4_pair<0>(codes, scale_at<0>(scales));
-                    pair[4 * w + 1] = fp4_pair<1>(codes, scale_at<1>(scales));
-                    pair[4 * w + 2] = fp4_pair<2>(codes, scale_at<2>(scales));
-                    pair[4 * w + 3] = fp4_pair<3>(codes, scale_at<3>(scales));
+                    const uint32_t code = codes[2 * h + w], scales = vs[2 * h + w];
+                    pair[4 * w] = fp4_pair<0>(code, scale_at<0>(scales));
+                    pair[4 * w + 1] = fp4_pair<1>(code, scale_at<1>(scales));
+                    pair[4 * w + 2] = fp4_pair<2>(code, scale_at<2>(scales));
+                    pair[4 * w + 3] = fp4_pair<3>(code, scale_at<3>(scales));
                 }
                 u32x4 even, odd;
 #pragma unroll
@@ -408,134 +533,118 @@ __global__ __launch_bounds__(kWaves * 64) void kv4_attention_kernel(AttentionArg
                     odd[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i], 0x07060302u);
                 }
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = P - 1; i >= 0; --i) {
-                        acc[m][s][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), weight[m][i][h], acc[m][s][0], 0, 0, 0);
-                        acc[m][s][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), weight[m][i][h], acc[m][s][1], 0, 0, 0);
-                    }
-            }
-        if (masked) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (__ballot(poison[m] != 0) == 0) continue;
-                uint32_t any = poison[m];
-                any |= __shfl_xor(any, 16, kWave);
-                any |= __shfl_xor(any, 32, kWave);
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-                    if (any >> s & 1) acc[m][s][0] = acc[m][s][1] = f32x4{NAN, NAN, NAN, NAN};
+                for (int i = P - 1; i >= 0; --i) {
+                    acc[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), weight[i][h], acc[s][0], 0, 0, 0);
+                    acc[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), weight[i][h], acc[s][1], 0, 0, 0);
+                }
             }
         }
+        if (masked && __ballot(poison != 0) != 0) {
+            poison |= __shfl_xor(poison, 16, kWave);
+            poison |= __shfl_xor(poison, 32, kWave);
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (poison >> s & 1) acc[s][0] = acc[s][1] = f32x4{NAN, NAN, NAN, NAN};
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 
-    // The four waves' parts joined.
+    // The waves' parts joined: each writes its own, wave s adds up elements 32 s .. 32 s + 31 of the rows.
+    __syncthreads();
+    auto& stats = lds.end.stats;
+    sum = sum_over_groups(sum);
+    if (g == 0) {
+        stats[wave][0][l] = top;
+        stats[wave][1][l] = sum;
+    }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        sum[m] = sum_over_groups(sum[m]);
-        if (g == 0) {
-            stats[wave][0][16 * m + l] = top[m];
-            stats[wave][1][16 * m + l] = sum[m];
-        }
+    for (int s = 0; s < S; ++s) {
+        lds.end.acc[wave][2 * s][lane] = acc[s][0];
+        lds.end.acc[wave][2 * s + 1][lane] = acc[s][1];
     }
     __syncthreads();
-    float all_top[MT], all_sum[MT];
+    static_assert(W >= S);
+    if (wave >= S || row >= p.rows) return;
+    float all_top = -INFINITY, all_sum = 0.0f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        all_top[m] = -INFINITY;
+    for (int w = 0; w < W; ++w) all_top = fmaxf(all_top, stats[w][0][l]);
+    const float base = finite_or_zero(all_top) * scale;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) all_top[m] = fmaxf(all_top[m], stats[w][0][16 * m + l]);
-        const float base = finite_or_zero(all_top[m]);
-        all_sum[m] = 0.0f;
+    for (int w = 0; w < W; ++w) {
+        const float by = __builtin_amdgcn_exp2f(fmaf(stats[w][0][l], scale, -base));
+        all_sum = fmaf(stats[w][1][l], by, all_sum);
+        const f32x4 even = lds.end.acc[w][2 * wave][lane], odd = lds.end.acc[w][2 * wave + 1][lane];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) all_sum[m] = fmaf(stats[w][1][16 * m + l], __builtin_amdgcn_exp2f(stats[w][0][16 * m + l] - base), all_sum[m]);
-        const float shrink = __builtin_amdgcn_exp2f(top[m] - base);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            acc[m][s][0] *= shrink;
-            acc[m][s][1] *= shrink;
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = fmaf(even[i], by, v[2 * i]);
+            v[2 * i + 1] = fmaf(odd[i], by, v[2 * i + 1]);
         }
     }
-#pragma unroll
-    for (int other = 2; other > 0; other /= 2) {
-        if (wave >= other && wave < 2 * other) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) exchange[wave - other][(m * S + s) * 8 + i][lane] = acc[m][s][i / 4][i % 4];
-        }
-        __syncthreads();
-        if (wave < other) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[m][s][i / 4][i % 4] += exchange[wave][(m * S + s) * 8 + i][lane];
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = row0 + 16 * m + l;
-        if (row >= p.rows) continue;
+    const int first = 32 * wave + 8 * g;
+    if (p.splits > 1) {
         const int64_t part = ((static_cast<int64_t>(b) * c.kv_heads + head) * p.rows + row) * p.splits + split;
-        const int token = row / p.group;
-        const int64_t to = ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + row % p.group) * D;
-        const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
-        const float by = 1.0f / all_sum[m];
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[m][s][i % 2][i / 2];
-            if (p.splits > 1) {
-                put8<true>(p.part, part * D + 32 * s + 8 * g, v);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = at < 0 ? 0.0f : (at >= capacity ? NAN : v[i] * by);
-                put8<F32>(p.out, to + 32 * s + 8 * g, v);
-            }
-        }
-        if (p.splits > 1 && g == 0) {
+        put8<true>(p.part, part * D + first, v);
+        if (wave == 0 && g == 0) {
             float* const st = p.part + p.part_rows * D + 2 * part;
-            st[0] = all_top[m];
-            st[1] = all_sum[m];
+            st[0] = all_top * scale;
+            st[1] = all_sum;
         }
+        return;
     }
+    const float by = 1.0f / all_sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at < 0 ? 0.0f : (at >= capacity ? NAN : v[i] * by);
+    put8<F32>(p.out, ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + of_group) * D + first, v);
 }
 
-// The splits of a row joined: D / 8 lanes a row.
+// The splits of a row joined: a block a row, D / 8 lanes across it and 2048 / D splits at a time.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
-    constexpr int kLanes = D / 8;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;  // (sequence, key head, row)
-    const int lane = threadIdx.x % kLanes;
+    constexpr int kLanes = D / 8, kTeams = 256 / kLanes;
+    __shared__ float joined[kTeams][D + 4];  // a team's part, then its maximum and sum
+    const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
     const Cache& c = p.c;
-    if (idx >= static_cast<int64_t>(c.batch) * c.kv_heads * p.rows) return;
+    const int64_t idx = blockIdx.x;  // (sequence, key head, row)
     const int64_t bh = idx / p.rows;
     const int row = static_cast<int>(idx - bh * p.rows), head = static_cast<int>(bh % c.kv_heads), b = static_cast<int>(bh / c.kv_heads);
-    const int token = row / p.group;
+    const int token = row / p.group, at = c.positions[static_cast<int64_t>(b) * c.length + token];
     const float* const st = p.part + p.part_rows * D + 2 * idx * p.splits;
-    float top = -INFINITY;
-    for (int i = 0; i < p.splits; ++i) top = fmaxf(top, st[2 * i]);
-    const float base = finite_or_zero(top);
-    float sum = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int i = 0; i < p.splits; ++i) {
-        const float by = __builtin_amdgcn_exp2f(st[2 * i] - base);
+    float top = -INFINITY, sum = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int i = team; i < p.splits; i += kTeams) {
         const float* const from = p.part + (idx * p.splits + i) * D + 8 * lane;
         const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
-        sum = fmaf(st[2 * i + 1], by, sum);
+        const float its = st[2 * i], before = top;
+        top = fmaxf(top, its);
+        const float base = finite_or_zero(top), shrink = __builtin_amdgcn_exp2f(before - base), by = __builtin_amdgcn_exp2f(its - base);
+        sum = fmaf(st[2 * i + 1], by, sum * shrink);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            v[j] = fmaf(lo[j], by, v[j]);
-            v[4 + j] = fmaf(hi[j], by, v[4 + j]);
+            v[j] = fmaf(lo[j], by, v[j] * shrink);
+            v[4 + j] = fmaf(hi[j], by, v[4 + j] * shrink);
         }
     }
-    const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) joined[team][8 * lane + j] = v[j];
+    if (lane == 0) {
+        joined[team][D] = top;
+        joined[team][D + 1] = sum;
+    }
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll
+    for (int i = 0; i < kTeams; ++i) top = fmaxf(top, joined[i][D]);
+    const float base = finite_or_zero(top);
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTeams; ++i) {
+        const float by = __builtin_amdgcn_exp2f(joined[i][D] - base);
+        sum = fmaf(joined[i][D + 1], by, sum);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(joined[i][8 * lane + j], by, v[j]);
+    }
     const float by = 1.0f / sum;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = at < 0 ? 0.0f : (at >= c.width * c.page_size ? NAN : v[j] * by);
@@ -552,7 +661,7 @@ mlk_status cache_of(Cache& c, uint8_t* bytes, int64_t pages, int64_t page_size, 
     MLK_CHECK(dim_ok(dim), "head_dim must be 32, 64, 128 or 256");
     MLK_CHECK(page_size > 0 && page_size % kRun == 0 && page_size <= 1024, "page_size must be a multiple of 16, at most 1024");
     MLK_CHECK(pages > 0 && pages < (int64_t{1} << 31), "the cache must have between 1 and 2^31 - 1 pages");
-    MLK_CHECK(width > 0 && width <= (int64_t{1} << 30) / page_size, "page_table must hold between 1 and 2^30 / page_size pages a sequence");
+    MLK_CHECK(width > 0 && width <= (int64_t{1} << 28) / page_size, "page_table must hold between 1 and 2^28 / page_size pages a sequence");
     MLK_CHECK(kv_heads < (int64_t{1} << 20) && batch < (int64_t{1} << 31) && length < (int64_t{1} << 31) && batch * length < (int64_t{1} << 36),
               "too many heads, sequences or tokens");
     c = Cache{};
@@ -562,7 +671,7 @@ mlk_status cache_of(Cache& c, uint8_t* bytes, int64_t pages, int64_t page_size, 
     c.kv_heads = static_cast<int32_t>(kv_heads);
     c.page_size = static_cast<int32_t>(page_size);
     c.runs = static_cast<int32_t>(page_size / kRun);
-    c.magic = c.runs == 1 ? 0 : static_cast<uint32_t>(((int64_t{1} << 32) + c.runs - 1) / c.runs);
+    c.magic = static_cast<uint32_t>(((int64_t{1} << 31) + c.runs - 1) / c.runs);
     c.table = table;
     c.width = static_cast<int32_t>(width);
     c.positions = positions;
@@ -583,17 +692,19 @@ bool rows_fit(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads) {
 }
 
 struct Plan {
-    int mt;
     int64_t row_tiles, splits, rows, part_rows;
     size_t bytes;
 };
+#ifndef SP_
+#define SP_ 2
+#endif
 Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t dim, int64_t capacity) {
     Plan t{};
     t.rows = length * (heads / kv_heads);
-    t.mt = 1;
-    t.row_tiles = ceil_div(t.rows, 16 * t.mt);
+    t.row_tiles = ceil_div(t.rows, 16);
     const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * t.row_tiles), tiles = ceil_div(capacity, kTile);
-    t.splits = std::max<int64_t>(1, std::min(ceil_div(1024, blocks), tiles / (2 * kWaves)));
+    const int64_t resident = dim <= 64 ? 512 : 256;
+    t.splits = tiles <= SP_ * W ? 1 : std::max<int64_t>(1, std::min(resident / blocks, tiles / W));
     t.part_rows = batch * kv_heads * t.rows * t.splits;
     t.bytes = t.splits > 1 ? static_cast<size_t>(t.part_rows) * (dim + 2) * sizeof(float) : 0;
     return t;
@@ -602,11 +713,12 @@ Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int
 template <int D, bool F32>
 void launch_attention(const AttentionArgs& p, const Plan& t, hipStream_t s) {
     const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * t.row_tiles * t.splits;
-    hipLaunchKernelGGL((kv4_attention_kernel<D, F32, 1>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64), 0, s, p);
-    if (t.splits > 1) {
-        const int64_t rows = int64_t{p.c.batch} * p.c.kv_heads * p.rows;
-        hipLaunchKernelGGL((kv4_join_kernel<D, F32>), dim3(static_cast<unsigned>(ceil_div(rows, 256 / (D / 8)))), dim3(256), 0, s, p);
+    if (p.c.runs % 4 == 0) {
+        hipLaunchKernelGGL((kv4_attention_kernel<D, F32, true>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((kv4_attention_kernel<D, F32, false>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     }
+    if (t.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, F32>), dim3(static_cast<unsigned>(t.part_rows / t.splits)), dim3(256), 0, s, p);
 }
 
 template <bool F32>
@@ -668,7 +780,7 @@ extern "C" mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t 
 extern "C" size_t mlk_kv4_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                     int64_t page_size, int64_t table_width) {
     if (batch <= 0 || length <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || !dim_ok(head_dim) || page_size <= 0 ||
-        page_size > 1024 || !rows_fit(batch, length, heads, kv_heads) || table_width <= 0 || table_width > (int64_t{1} << 30) / page_size)
+        page_size > 1024 || !rows_fit(batch, length, heads, kv_heads) || table_width <= 0 || table_width > (int64_t{1} << 28) / page_size)
         return 0;
     return plan_of(batch, length, heads, kv_heads, head_dim, page_size * table_width).bytes;
 }
