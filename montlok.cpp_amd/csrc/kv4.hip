@@ -16,6 +16,7 @@
 // stores, once a token; the attention reads every byte of it for every token
 // that follows.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp4.h"
 
@@ -65,124 +66,6 @@ struct Rows3 {
     int64_t bs, ts, hs;  // element strides of a sequence, a token, a head
 };
 
-// One thread a group of 32.
-template <bool F32>
-__global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, Rows3 k, Rows3 v, int dim) {
-    const int groups = dim / kGroup;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = idx / groups;  // (token, head)
-    const int group = static_cast<int>(idx - row * groups);
-    const int64_t token = row / c.kv_heads;
-    if (token >= static_cast<int64_t>(c.batch) * c.length) return;
-    const int head = static_cast<int>(row - token * c.kv_heads), b = static_cast<int>(token / c.length);
-    const int at = c.positions[token];
-    if (at < 0) return;
-    int offset;
-    uint8_t* const record = record_of(c, b, at, head, offset);
-    if (record == nullptr) return;
-    const bool values = blockIdx.y != 0;
-    const Rows3& r = values ? v : k;
-    const int64_t from = b * r.bs + (token - static_cast<int64_t>(b) * c.length) * r.ts + head * r.hs + group * kGroup;
-    float x[kGroup];
-    float most = 0.0f;
-    bool fine = true;
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-        x[i] = Element<F32>::get(r.p, from + i);
-        most = fmaxf(most, fabsf(x[i]));
-        fine = fine && (__float_as_uint(x[i]) & 0x7F800000u) != 0x7F800000u;
-    }
-    const uint32_t byte = fine ? scale_byte(most) : 255;
-    const float scale = scale_of(byte);
-    u32x4 codes = {0, 0, 0, 0};
-    if (fine) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w = 0;
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i], x[8 * i + 1], scale, 0);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 2], x[8 * i + 3], scale, 1);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 4], x[8 * i + 5], scale, 2);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 6], x[8 * i + 7], scale, 3);
-            codes[i] = w;
-        }
-    }
-    const int64_t half = static_cast<int64_t>(c.page_size) * (dim / 2), scales = static_cast<int64_t>(c.page_size) * groups;
-    if (!values) {
-        *reinterpret_cast<u32x4*>(record + static_cast<int64_t>(offset) * (dim / 2) + 16 * group) = codes;
-        record[2 * half + static_cast<int64_t>(offset) * groups + group] = static_cast<uint8_t>(byte);
-    } else {
-        uint8_t* const to = record + half + static_cast<int64_t>(16 * group) * c.page_size + offset;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) to[static_cast<int64_t>(j) * c.page_size] = static_cast<uint8_t>(codes[j / 4] >> (8 * (j % 4)));
-        record[2 * half + scales + static_cast<int64_t>(group) * c.page_size + offset] = static_cast<uint8_t>(byte);
-    }
-}
-
-template <bool F32>
-__global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, void* k, void* v, int dim) {
-    const int groups = dim / kGroup;
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = idx / groups;
-    const int group = static_cast<int>(idx - row * groups);
-    const int64_t token = row / c.kv_heads;
-    if (token >= static_cast<int64_t>(c.batch) * c.length) return;
-    const int head = static_cast<int>(row - token * c.kv_heads), b = static_cast<int>(token / c.length);
-    const bool values = blockIdx.y != 0;
-    void* const out = values ? v : k;
-    const int64_t to = row * dim + group * kGroup;
-    const int at = c.positions[token];
-    uint32_t byte = 3;
-    u32x4 codes = {0, 0, 0, 0};
-    if (at >= 0) {
-        int offset;
-        const uint8_t* const record = record_of(c, b, at, head, offset);
-        const int64_t half = static_cast<int64_t>(c.page_size) * (dim / 2), scales = static_cast<int64_t>(c.page_size) * groups;
-        if (record == nullptr) {
-            byte = 255;
-        } else if (!values) {
-            codes = *reinterpret_cast<const u32x4*>(record + static_cast<int64_t>(offset) * (dim / 2) + 16 * group);
-            byte = record[2 * half + static_cast<int64_t>(offset) * groups + group];
-        } else {
-            const uint8_t* const from = record + half + static_cast<int64_t>(16 * group) * c.page_size + offset;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) codes[j / 4] |= static_cast<uint32_t>(from[static_cast<int64_t>(j) * c.page_size]) << (8 * (j % 4));
-            byte = record[2 * half + scales + static_cast<int64_t>(group) * c.page_size + offset];
-        }
-    }
-    const float scale = scale_of(byte);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bf16x8 x = fp4_octet(codes[i], scale);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) Element<F32>::put(out, to + 8 * i + j, static_cast<float>(x[j]));
-    }
-}
-
-// ------------------------------------------------------------- attention
-
-struct AttentionArgs {
-    Cache c;
-    const void* q;
-    int64_t q_bs, q_ts, q_hs;
-    int32_t heads, group;  // query heads; query heads to a key head
-    int32_t rows;          // of a (sequence, key head): length * group; row r = token r / group, head r % group
-    int32_t row_tiles, splits;
-    float scale_log2;
-    void* out;    // [batch, length, heads, D]
-    float* part;  // [batch, kv_heads, rows, splits][D], then [...][2] (maximum, sum)
-    int64_t part_rows;
-};
-
-__device__ __forceinline__ float max_over_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, kWave));
-    return fmaxf(v, __shfl_xor(v, 32, kWave));
-}
-__device__ __forceinline__ float sum_over_groups(float v) {
-    v += __shfl_xor(v, 16, kWave);
-    return v + __shfl_xor(v, 32, kWave);
-}
-__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
-
 // Eight elements of a row at any alignment.
 template <bool F32>
 __device__ __forceinline__ void load8(const void* p, int64_t first, float (&x)[8]) {
@@ -213,17 +96,6 @@ __device__ __forceinline__ void put8(void* out, int64_t first, const float (&v)[
     }
 }
 
-// What a wave holds in LDS of its tile of 64 keys: their codes, then, once they are in registers, the values'.
-template <int S>
-struct TileLds {
-    u32x4 codes[64 * S];        // keys: row l of key tile a, 16-byte piece c at (16 a + l) S + (c ^ turn(l)); values: row j,
-                                // piece c at 4 j + (c ^ (j / 2 & 3))
-    uint8_t key_scale[64 * S];  // of row l of key tile a at (4 l + a) S
-    uint8_t value_scale[64 * S];  // [S][64]
-    // Eight lanes that read, or write, together meet in different banks.
-    static __device__ __forceinline__ int turn(int l) { return S == 8 ? l & 7 : S == 4 ? l >> 1 & 3 : S == 2 ? l >> 2 & 1 : 0; }
-};
-
 // N bytes of a lane.
 template <int N>
 struct Bytes;
@@ -242,6 +114,205 @@ struct Bytes<4> {
 template <>
 struct Bytes<8> {
     using type = uint64_t;
+};
+
+// A wave moves the keys, or the values, of 16 consecutive tokens of the call and one head: lane 4 t + q the eight elements
+// 32 s + 8 q .. of token t for each group s, a dword of codes. A value dword is four rows of one token, where the cache
+// holds rows of tokens: four lanes that hold a run of four tokens turn their 4 x 4 bytes, so that a lane moves one row's
+// four tokens. Tokens that are no such run are moved byte by byte.
+
+// Byte k of the lane whose token is i of its four against byte i of the one whose token is k; its own inverse.
+__device__ __forceinline__ uint32_t turn4(uint32_t v, int i) {
+    const uint32_t a = __shfl_xor(v, 4, kWave);
+    v = i & 1 ? __builtin_amdgcn_perm(v, a, 0x07030501u) : __builtin_amdgcn_perm(a, v, 0x06020400u);
+    const uint32_t c = __shfl_xor(v, 8, kWave);
+    return i & 2 ? __builtin_amdgcn_perm(v, c, 0x07060302u) : __builtin_amdgcn_perm(c, v, 0x05040100u);
+}
+
+// Where a lane's token lies: its record (null: nowhere), its place in the page, and whether the lane's four tokens are
+// four places side by side from a multiple of four.
+struct Place {
+    uint8_t* record;
+    int offset;
+    bool run;
+};
+__device__ __forceinline__ Place place_of(const Cache& c, int64_t token, int head) {
+    Place p{nullptr, 0, false};
+    const int i = (threadIdx.x >> 2) & 3;
+    if (token < static_cast<int64_t>(c.batch) * c.length) {
+        const int at = c.positions[token];
+        if (at >= 0) p.record = record_of(c, static_cast<int>(token / c.length), at, head, p.offset);
+    }
+    bool same = p.record != nullptr && (p.offset & 3) == i;
+#pragma unroll
+    for (int m = 4; m <= 8; m += 4) {
+        const uint64_t bits = reinterpret_cast<uint64_t>(p.record) + static_cast<uint64_t>(p.offset & ~3);
+        const uint32_t low = __shfl_xor(static_cast<uint32_t>(bits), m, kWave), high = __shfl_xor(static_cast<uint32_t>(bits >> 32), m, kWave);
+        same = same && (static_cast<uint64_t>(high) << 32 | low) == bits;
+        const int other = __shfl_xor(static_cast<int>(same), m, kWave);
+        same = same && other != 0;
+    }
+    p.run = same;
+    return p;
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, Rows3 k, Rows3 v, int64_t waves) {
+    constexpr int S = D / 32;
+    using Scales = typename Bytes<S>::type;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (id >= waves) return;
+    const bool values = id & 1;
+    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) % c.kv_heads);
+    const int64_t token = (id >> 1) / c.kv_heads * 16 + (lane >> 2), all = static_cast<int64_t>(c.batch) * c.length, held = min(token, all - 1);
+    const Rows3& r = values ? v : k;
+    const int64_t b = held / c.length, from = b * r.bs + (held - b * c.length) * r.ts + head * r.hs + 8 * q;
+    float x[S][8];
+#pragma unroll
+    for (int s = 0; s < S; ++s) load8<F32>(r.p, from + 32 * s, x[s]);
+    const Place place = place_of(c, token, head);
+    uint32_t codes[S];
+    uint64_t bytes = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        // The largest magnitude's bits; those of an infinity or a NaN are larger than any number's.
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[s][e]) & 0x7FFFFFFFu);
+        most = max(most, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(most), 0xB1, 0xF, 0xF, false)));
+        most = max(most, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(most), 0x4E, 0xF, 0xF, false)));
+        const bool fine = most < 0x7F800000u;
+        const uint32_t byte = fine ? scale_byte(__uint_as_float(most)) : 255;
+        const float scale = scale_of(byte);
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[s][0], x[s][1], scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[s][2], x[s][3], scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[s][4], x[s][5], scale, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[s][6], x[s][7], scale, 3);
+        codes[s] = fine ? w : 0;
+        bytes |= static_cast<uint64_t>(byte) << (8 * s);
+    }
+    const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2);
+    if (!values) {
+        if (place.record == nullptr) return;
+        uint32_t* const to = reinterpret_cast<uint32_t*>(place.record + place.offset * (D / 2)) + q;
+#pragma unroll
+        for (int s = 0; s < S; ++s) to[4 * s] = codes[s];
+        if (q == 0) *reinterpret_cast<Scales*>(place.record + 2 * half + place.offset * S) = static_cast<Scales>(bytes);
+        return;
+    }
+    uint32_t turned[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) turned[s] = turn4(codes[s], i);
+    if (place.record == nullptr) return;
+    uint8_t* const to = place.record + half + 4 * q * c.page_size;
+    if (place.run) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) *reinterpret_cast<uint32_t*>(to + (16 * s + i) * c.page_size + (place.offset & ~3)) = turned[s];
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[(16 * s + e) * c.page_size + place.offset] = static_cast<uint8_t>(codes[s] >> (8 * e));
+    }
+    if (q == 0) {
+        uint8_t* const scales = place.record + 2 * half + S * c.page_size + place.offset;
+#pragma unroll
+        for (int s = 0; s < S; ++s) scales[s * c.page_size] = static_cast<uint8_t>(bytes >> (8 * s));
+    }
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, void* k, void* v, int64_t waves) {
+    constexpr int S = D / 32;
+    using Scales = typename Bytes<S>::type;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (id >= waves) return;
+    const bool values = id & 1;
+    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) % c.kv_heads);
+    const int64_t token = (id >> 1) / c.kv_heads * 16 + (lane >> 2), all = static_cast<int64_t>(c.batch) * c.length;
+    const Place place = place_of(c, token, head);
+    const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2);
+    uint32_t codes[S];
+    uint64_t bytes = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) codes[s] = 0;
+    if (place.record != nullptr) {
+        if (!values) {
+            const uint32_t* const from = reinterpret_cast<const uint32_t*>(place.record + place.offset * (D / 2)) + q;
+#pragma unroll
+            for (int s = 0; s < S; ++s) codes[s] = from[4 * s];
+            bytes = *reinterpret_cast<const Scales*>(place.record + 2 * half + place.offset * S);
+        } else {
+            const uint8_t* const from = place.record + half + 4 * q * c.page_size;
+            if (place.run) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) codes[s] = *reinterpret_cast<const uint32_t*>(from + (16 * s + i) * c.page_size + (place.offset & ~3));
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) codes[s] |= static_cast<uint32_t>(from[(16 * s + e) * c.page_size + place.offset]) << (8 * e);
+            }
+            const uint8_t* const scales = place.record + 2 * half + S * c.page_size + place.offset;
+#pragma unroll
+            for (int s = 0; s < S; ++s) bytes |= static_cast<uint64_t>(scales[s * c.page_size]) << (8 * s);
+        }
+    }
+    if (values) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const uint32_t turned = turn4(codes[s], i);
+            if (place.run) codes[s] = turned;
+        }
+    }
+    if (token >= all) return;
+    if (place.record == nullptr) bytes = c.positions[token] < 0 ? 0 : ~uint64_t{0};  // zero codes, or NaN
+    const int64_t to = (token * c.kv_heads + head) * D + 8 * q;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const bf16x8 x = fp4_octet(codes[s], scale_of(static_cast<uint32_t>(bytes >> (8 * s)) & 0xFF));
+        float out[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = static_cast<float>(x[e]);
+        put8<F32>(values ? v : k, to + 32 * s, out);
+    }
+}
+
+// ------------------------------------------------------------- attention
+
+struct AttentionArgs {
+    Cache c;
+    const void* q;
+    int64_t q_bs, q_ts, q_hs;
+    int32_t heads, group;  // query heads; query heads to a key head
+    int32_t rows;          // of a (sequence, key head): length * group; row r = token r / group, head r % group
+    int32_t row_tiles, splits;
+    float scale_log2;
+    void* out;    // [batch, length, heads, D]
+    float* part;  // [batch, kv_heads, rows, splits][D], then [...][2] (maximum, sum)
+    int64_t part_rows;
+};
+
+__device__ __forceinline__ float max_over_groups(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+    v += __shfl_xor(v, 16, kWave);
+    return v + __shfl_xor(v, 32, kWave);
+}
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// What a wave holds in LDS of its tile of 64 keys: their codes, then, once they are in registers, the values'.
+template <int S>
+struct TileLds {
+    u32x4 codes[64 * S];        // keys: row l of key tile a, 16-byte piece c at (16 a + l) S + (c ^ turn(l)); values: row j,
+                                // piece c at 4 j + (c ^ (j / 2 & 3))
+    uint8_t key_scale[64 * S];  // of row l of key tile a at (4 l + a) S
+    uint8_t value_scale[64 * S];  // [S][64]
+    // Eight lanes that read, or write, together meet in different banks.
+    static __device__ __forceinline__ int turn(int l) { return S == 8 ? l & 7 : S == 4 ? l >> 1 & 3 : S == 2 ? l >> 2 & 1 : 0; }
 };
 
 // A block takes 16 rows of a (sequence, key head) and every p.splits-th group of W tiles of 64 keys, a tile a wave.
@@ -655,6 +726,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
 
 bool dim_ok(int64_t dim) { return dim == 32 || dim == 64 || dim == 128 || dim == 256; }
 
+template <typename Body>
+void by_dim(int64_t dim, Body body) {
+    if (dim == 32) body(std::integral_constant<int, 32>{});
+    if (dim == 64) body(std::integral_constant<int, 64>{});
+    if (dim == 128) body(std::integral_constant<int, 128>{});
+    if (dim == 256) body(std::integral_constant<int, 256>{});
+}
+
 mlk_status cache_of(Cache& c, uint8_t* bytes, int64_t pages, int64_t page_size, int64_t kv_heads, int64_t dim, const int32_t* table,
                     int64_t width, const int32_t* positions, int64_t batch, int64_t length) {
     MLK_CHECK(batch >= 0 && length >= 0 && kv_heads > 0, "invalid cache geometry");
@@ -721,14 +800,6 @@ void launch_attention(const AttentionArgs& p, const Plan& t, hipStream_t s) {
     if (t.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, F32>), dim3(static_cast<unsigned>(t.part_rows / t.splits)), dim3(256), 0, s, p);
 }
 
-template <bool F32>
-void launch_attention(int64_t dim, const AttentionArgs& p, const Plan& t, hipStream_t s) {
-    if (dim == 32) launch_attention<32, F32>(p, t, s);
-    if (dim == 64) launch_attention<64, F32>(p, t, s);
-    if (dim == 128) launch_attention<128, F32>(p, t, s);
-    if (dim == 256) launch_attention<256, F32>(p, t, s);
-}
-
 }  // namespace
 }  // namespace mlk
 
@@ -743,16 +814,14 @@ extern "C" mlk_status mlk_kv4_append(const void* k, const int64_t* k_strides, co
     const mlk_status status = cache_of(c, cache, pages, page_size, kv_heads, head_dim, page_table, table_width, positions, batch, length);
     if (status != MLK_OK || batch == 0 || length == 0) return status;
     MLK_CHECK(k && k_strides && v && v_strides, "null tensor pointer");
-    const int64_t blocks = ceil_div(batch * length * kv_heads * (head_dim / kGroup), 256);
-    MLK_CHECK(blocks < (int64_t{1} << 31), "too many tokens for one launch");
+    const int64_t waves = ceil_div(batch * length, 16) * kv_heads * 2;
+    MLK_CHECK(waves < (int64_t{1} << 33), "too many tokens for one launch");
     const Rows3 kr{k, k_strides[0], k_strides[1], k_strides[2]}, vr{v, v_strides[0], v_strides[1], v_strides[2]};
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == MLK_DTYPE_F32) {
-        hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(256), 0, s, c, kr, vr, static_cast<int>(head_dim));
-    } else {
-        hipLaunchKernelGGL(kv4_append_kernel<false>, grid, dim3(256), 0, s, c, kr, vr, static_cast<int>(head_dim));
-    }
+    by_dim(head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_append_kernel<D, true> : kv4_append_kernel<D, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, kr, vr, waves);
+    });
     return launch_status("kv4 append");
 }
 
@@ -765,15 +834,14 @@ extern "C" mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t 
                                        positions, batch, length);
     if (status != MLK_OK || batch == 0 || length == 0) return status;
     MLK_CHECK(k && v, "null tensor pointer");
-    const int64_t blocks = ceil_div(batch * length * kv_heads * (head_dim / kGroup), 256);
-    MLK_CHECK(blocks < (int64_t{1} << 31), "too many tokens for one launch");
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == MLK_DTYPE_F32) {
-        hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(256), 0, s, c, k, v, static_cast<int>(head_dim));
-    } else {
-        hipLaunchKernelGGL(kv4_read_kernel<false>, grid, dim3(256), 0, s, c, k, v, static_cast<int>(head_dim));
-    }
+    MLK_CHECK((reinterpret_cast<uintptr_t>(k) & 15) == 0 && (reinterpret_cast<uintptr_t>(v) & 15) == 0, "k and v must be 16-byte aligned");
+    const int64_t waves = ceil_div(batch * length, 16) * kv_heads * 2;
+    MLK_CHECK(waves < (int64_t{1} << 33), "too many tokens for one launch");
+    by_dim(head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_read_kernel<D, true> : kv4_read_kernel<D, false>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, k, v, waves);
+    });
     return launch_status("kv4 read");
 }
 
@@ -816,10 +884,10 @@ extern "C" mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides,
     p.out = out;
     p.part = static_cast<float*>(workspace);
     p.part_rows = t.part_rows;
-    if (dtype == MLK_DTYPE_F32) {
-        launch_attention<true>(head_dim, p, t, reinterpret_cast<hipStream_t>(stream));
-    } else {
-        launch_attention<false>(head_dim, p, t, reinterpret_cast<hipStream_t>(stream));
-    }
+    by_dim(head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        dtype == MLK_DTYPE_F32 ? launch_attention<D, true>(p, t, reinterpret_cast<hipStream_t>(stream))
+                               : launch_attention<D, false>(p, t, reinterpret_cast<hipStream_t>(stream));
+    });
     return launch_status("kv4 attention");
 }
