@@ -532,12 +532,13 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         }
 
         const bool masked = first + kTile - 1 > least;  // some row does not see the whole tile
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) score[i / 4][i % 4] = first + 16 * g + i > position ? -INFINITY : score[i / 4][i % 4];
+        }
         float most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (masked && first + 16 * g + i > position) score[i / 4][i % 4] = -INFINITY;
-            most = fmaxf(most, score[i / 4][i % 4]);
-        }
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[i / 4][i % 4]);
         const float now = fmaxf(top, max_over_groups(most));
         if (__ballot(now != top) != 0) {  // seldom after the first tiles
             const float shrink = __builtin_amdgcn_exp2f(fmaf(top, scale, -finite_or_zero(now) * scale));
@@ -669,53 +670,385 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
     put8<F32>(p.out, ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + of_group) * D + first, v);
 }
 
-// The splits of a row joined: a block a row, D / 8 lanes across it and 2048 / D splits at a time.
-template <int D, bool F32>
-__global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
-    constexpr int kLanes = D / 8, kTeams = 256 / kLanes;
-    __shared__ float joined[kTeams][D + 4];  // a team's part, then its maximum and sum
-    const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
+// Heads of 128 only: with 64, what the lanes convert for themselves is half as much, and sharing it gained nothing.
+constexpr int kSharedDim = 128;
+// Tiles of 16 rows of a wave: what its queries, sums and scores leave of the registers of two waves a SIMD.
+template <bool F32>
+constexpr int kRowTiles = F32 ? 1 : 2;
+
+// Many rows: a block takes 16 MT rows a wave of a (sequence, key head), and its waves share each tile of 64 keys as bf16
+// operands in LDS. A wave of the kernel above spends most of its instructions on converting keys and values, for 16 rows
+// (512 tokens of two sequences over 8192 keys took 270 us so); here it converts an eighth of them, for 128 MT. A tile
+// passes through registers (three tiles ahead), LDS as it lies in memory (two ahead) and LDS as operands (one ahead).
+//
+// Operands: key tile a, k step s is unit a S + s; values of group s and half h of a lane's 16 tokens, their even and odd
+// elements, are unit 2 s + h.
+template <bool F32>
+__global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(AttentionArgs p) {
+    constexpr int D = kSharedDim, S = D / 32, P = F32 ? 3 : 1, MT = kRowTiles<F32>;
+    using Scales = typename Bytes<S>::type;
+    constexpr int kKeyUnits = 4 * S, kValueUnits = 2 * S;  // a value unit is two operands
+    static_assert(2 * S == W, "a wave loads 1 KB of keys or values, and converts two key units and a value unit");
+    struct Raw {
+        u32x4 key[64 * S], value[64 * S];  // as TileLds has them
+        uint8_t key_scale[64 * S], value_scale[64 * S];
+    };
+    __shared__ Raw raw[2];
+    __shared__ bf16x8 key_lds[2][kKeyUnits][64], value_lds[2][kValueUnits][2][64];
+    __shared__ int nan_tile[2];  // the last tile of the buffer that held a NaN value group, plus one
+    __shared__ int wave_last[W];
     const Cache& c = p.c;
-    const int64_t idx = blockIdx.x;  // (sequence, key head, row)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
+    unsigned id = blockIdx.x;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int block_row = static_cast<int>(id % p.row_tiles) * (W * 16 * MT), row0 = block_row + wave * (16 * MT);
+    id /= p.row_tiles;
+    const int head = id % c.kv_heads, b = id / c.kv_heads;
+    const int capacity = c.width * c.page_size;
+    const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2), page_stride = c.kv_heads * c.record;
+    const int32_t* const table = c.table + static_cast<int64_t>(b) * c.width;
+    const uint8_t* const records = c.bytes + head * c.record;
+    if (threadIdx.x < 2) nan_tile[threadIdx.x] = 0;
+
+    struct Ids {
+        int32_t by_group, by_piece;  // pages of runs g and lane & 3
+    };
+    auto lookup = [&](int tile) {
+        auto page_of = [&](int run) {
+            uint32_t page, token;
+            split_run(c, 4 * tile + run, page, token);
+            return page < static_cast<uint32_t>(c.width) ? table[page] : -1;
+        };
+        return Ids{page_of(g), page_of(lane & 3)};
+    };
+    u32x4 ahead;
+    Scales scale_ahead = 0;
+    auto load = [&](int tile, const Ids& ids) {
+        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
+        const int group_id = bad ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
+        uint32_t page, token;
+        if (wave < S) {
+            const int at = (64 * wave + lane) / S, run = at / 16;
+            const int key_id = __shfl(group_id, 16 * run, kWave);
+            split_run(c, 4 * tile + run, page, token);
+            ahead = *reinterpret_cast<const u32x4*>(records + key_id * page_stride + ((static_cast<int>(token) + at % 16) * (D / 2) + lane % S * 16));
+        } else {
+            split_run(c, 4 * tile + (lane & 3), page, token);
+            ahead = *reinterpret_cast<const u32x4*>(records + piece_id * page_stride + half + ((16 * (wave - S) + (lane >> 2)) * c.page_size + static_cast<int>(token)));
+        }
+        if (wave == W - 1) {
+            split_run(c, 4 * tile + g, page, token);
+            scale_ahead = *reinterpret_cast<const Scales*>(records + group_id * page_stride + 2 * half + (static_cast<int>(token) + l) * S);
+            if (bad) scale_ahead = static_cast<Scales>(~uint64_t{0});
+        }
+        if (wave == W - 2) {
+            const int at = lane * S % 64, run = at / 16;
+            const int value_id = __shfl(group_id, 16 * run, kWave);
+            split_run(c, 4 * tile + run, page, token);
+            scale_ahead = *reinterpret_cast<const Scales*>(records + value_id * page_stride + 2 * half + ((S + lane * S / 64) * c.page_size + static_cast<int>(token) + at % 16));
+        }
+    };
+    auto keep = [&](int buffer) {
+        if (wave < S) {
+            const int at = 64 * wave + lane, token = at / S, row = token >> 4 << 2 | (token & 3), a = token >> 2 & 3;
+            raw[buffer].key[(16 * a + row) * S + (at % S ^ TileLds<S>::turn(row))] = ahead;
+        } else {
+            const int j = 16 * (wave - S) + (lane >> 2);
+            raw[buffer].value[4 * j + ((lane & 3) ^ (j >> 1 & 3))] = ahead;
+        }
+        if (wave == W - 1) reinterpret_cast<Scales*>(raw[buffer].key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = scale_ahead;
+        if (wave == W - 2) reinterpret_cast<Scales*>(raw[buffer].value_scale)[lane] = scale_ahead;
+    };
+    auto convert = [&](int tile, int buffer) {
+        const Raw& from = raw[buffer];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int unit = W * i + wave, a = unit / S, step = unit % S;  // a lane's 8 elements: D / 4 g + 8 step ..
+            const int byte = D / 8 * g + 4 * step;
+            const uint32_t code = reinterpret_cast<const uint32_t*>(from.key + (16 * a + l) * S + (byte / 16 ^ TileLds<S>::turn(l)))[byte % 16 / 4];
+            key_lds[buffer][unit][lane] = fp4_octet(code, scale_of(from.key_scale[(4 * l + a) * S + byte / 16]));
+        }
+        bool nan = false;
+        const int s = wave / 2, h = wave % 2;
+        const u32x2 codes = reinterpret_cast<const u32x2*>(from.value + 4 * (16 * s + l) + (g ^ (l >> 1 & 3)))[h];
+        const u32x2 scales_of = reinterpret_cast<const u32x2*>(from.value_scale + 64 * s + 16 * g)[h];
+        uint32_t pair[8];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t code = codes[w];
+            uint32_t scales = scales_of[w];
+            // A NaN group must not meet the weight 0 of a row that does not see it: it counts as small here, and the
+            // rows that see it are made NaN by themselves.
+            if (((scales & 0x7F7F7F7Fu) + 0x01010101u) & scales & 0x80808080u) {
+                nan = true;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((scales >> (8 * e) & 0xFF) == 0xFF) scales &= ~(0xFFu << (8 * e));
+            }
+            pair[4 * w] = fp4_pair<0>(code, scale_at<0>(scales));
+            pair[4 * w + 1] = fp4_pair<1>(code, scale_at<1>(scales));
+            pair[4 * w + 2] = fp4_pair<2>(code, scale_at<2>(scales));
+            pair[4 * w + 3] = fp4_pair<3>(code, scale_at<3>(scales));
+        }
+        u32x4 even, odd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            even[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x05040100u);
+            odd[e] = __builtin_amdgcn_perm(pair[2 * e + 1], pair[2 * e], 0x07060302u);
+        }
+        value_lds[buffer][wave][0][lane] = __builtin_bit_cast(bf16x8, even);
+        value_lds[buffer][wave][1][lane] = __builtin_bit_cast(bf16x8, odd);
+        if (nan) nan_tile[buffer] = tile + 1;
+    };
+
+    const float factor = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
+    const float scale = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
+    int position[MT], least = 0x7FFFFFFF, last = -1;
+    bf16x8 q[MT][P][S];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = row0 + 16 * m + l, clamped = min(row, p.rows - 1), token = clamped / p.group;
+        const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
+        position[m] = row < p.rows && at < capacity ? at : -1;
+        last = max(last, position[m]);
+        least = min(least, position[m] < 0 ? 0x7FFFFFFF : position[m]);
+        const int64_t from = b * p.q_bs + token * p.q_ts + (head * p.group + clamped - token * p.group) * p.q_hs + (D / 4) * g;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float x[8];
+            load8<F32>(p.q, from + 8 * s, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= factor;
+            if constexpr (F32) {
+                bf16x8 plane[3];
+                planes_of<true>(x, plane);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) q[m][i][s] = plane[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[m][0][s][i] = static_cast<__bf16>(x[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 1; i < 16; i *= 2) {
+        last = max(last, __shfl_xor(last, i, kWave));
+        least = min(least, __shfl_xor(least, i, kWave));
+    }
+    // The block goes as far as its furthest row.
+    if (lane == 0) wave_last[wave] = last;
+    __syncthreads();
+    int block_last = -1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) block_last = max(block_last, wave_last[w]);
+
+    float top[MT], sum[MT];
+    f32x4 acc[MT][S][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        top[m] = -INFINITY;
+        sum[m] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) acc[m][s][0] = acc[m][s][1] = f32x4{0, 0, 0, 0};
+    }
+    const int stride = p.splits;
+    auto at_step = [&](int n) { return split + n * p.splits; };
+    load(split, lookup(split));
+    keep(0);
+    load(at_step(1), lookup(at_step(1)));
+    __syncthreads();
+    convert(split, 0);
+    keep(1);
+    load(at_step(2), lookup(at_step(2)));
+    Ids ids = lookup(at_step(3));
+    __syncthreads();
+    for (int step = 0, buffer = 0; at_step(step) * kTile <= block_last; ++step, buffer ^= 1) {
+        const int tile = at_step(step), first = tile * kTile;
+        if (at_step(step + 1) * kTile <= block_last) {
+            convert(at_step(step + 1), buffer ^ 1);
+            keep(buffer);
+            load(at_step(step + 3), ids);
+            ids = lookup(at_step(step + 4));
+        }
+        if (first <= last) {
+            f32x4 score[MT][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) score[m][a] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const bf16x8 k = key_lds[buffer][a * S + s][lane];
+#pragma unroll
+                    for (int i = P - 1; i >= 0; --i)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) score[m][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[m][i][s], score[m][a], 0, 0, 0);
+                }
+            const bool masked = first + kTile - 1 > least;
+            float now[MT];
+            bool moved = false;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) score[m][i / 4][i % 4] = first + 16 * g + i > position[m] ? -INFINITY : score[m][i / 4][i % 4];
+                }
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, score[m][i / 4][i % 4]);
+                now[m] = fmaxf(top[m], max_over_groups(most));
+                moved = moved || now[m] != top[m];
+            }
+            if (__ballot(moved) != 0) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const float shrink = __builtin_amdgcn_exp2f(fmaf(top[m], scale, -finite_or_zero(now[m]) * scale));
+                    top[m] = now[m];
+                    sum[m] *= shrink;
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        acc[m][s][0] *= shrink;
+                        acc[m][s][1] *= shrink;
+                    }
+                }
+            }
+            bf16x8 weight[MT][P][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const float base = finite_or_zero(top[m]) * scale;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(fmaf(score[m][2 * h + i / 4][i % 4], scale, -base));
+                        sum[m] += w[i];
+                    }
+                    if constexpr (F32) {
+                        bf16x8 plane[3];
+                        planes_of<false>(w, plane);
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) weight[m][i][h] = plane[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) weight[m][0][h][i] = static_cast<__bf16>(w[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 even = value_lds[buffer][2 * s + h][0][lane], odd = value_lds[buffer][2 * s + h][1][lane];
+#pragma unroll
+                    for (int i = P - 1; i >= 0; --i)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            acc[m][s][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weight[m][i][h], acc[m][s][0], 0, 0, 0);
+                            acc[m][s][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weight[m][i][h], acc[m][s][1], 0, 0, 0);
+                        }
+                }
+            if (nan_tile[buffer] == tile + 1) {  // rare: the scales again, from memory
+                uint32_t page, token;
+                split_run(c, 4 * tile + g, page, token);
+                const int32_t page_id = page < static_cast<uint32_t>(c.width) ? table[page] : -1;
+                const uint8_t* const scales = records + (page_id < 0 || page_id >= c.pages ? 0 : page_id) * page_stride + 2 * half;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        int poison = 0;
+                        for (int i = 0; i < 16; ++i)
+                            if (first + 16 * g + i <= position[m] && scales[(S + s) * c.page_size + static_cast<int>(token) + i] == 0xFF) poison = 1;
+                        poison |= __shfl_xor(poison, 16, kWave);
+                        poison |= __shfl_xor(poison, 32, kWave);
+                        if (poison) acc[m][s][0] = acc[m][s][1] = f32x4{NAN, NAN, NAN, NAN};
+                    }
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        sum[m] = sum_over_groups(sum[m]);
+        const int row = row0 + 16 * m + l;
+        if (row >= p.rows) continue;
+        const int token = row / p.group, at = c.positions[static_cast<int64_t>(b) * c.length + token];
+        const int64_t part = ((static_cast<int64_t>(b) * c.kv_heads + head) * p.rows + row) * p.splits + split;
+        const int64_t to = ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + row - token * p.group) * D;
+        const float by = 1.0f / sum[m];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = acc[m][s][i % 2][i / 2];
+            if (p.splits > 1) {
+                put8<true>(p.part, part * D + 32 * s + 8 * g, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = at < 0 ? 0.0f : (at >= capacity ? NAN : v[i] * by);
+                put8<F32>(p.out, to + 32 * s + 8 * g, v);
+            }
+        }
+        if (p.splits > 1 && g == 0) {
+            float* const st = p.part + p.part_rows * D + 2 * part;
+            st[0] = top[m] * scale;
+            st[1] = sum[m];
+        }
+    }
+}
+
+// The splits of a row joined: D / 8 lanes across it, and TEAMS such groups that take a split each at a time (many splits
+// of few rows: one group a row walked 64 of them for 20 us).
+template <int D, bool F32, int TEAMS>
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes / TEAMS;
+    __shared__ float joined[TEAMS > 1 ? kRows * TEAMS : 1][D + 4];  // a team's part, then its maximum and sum
+    const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes % TEAMS, in_block = threadIdx.x / kLanes / TEAMS;
+    const Cache& c = p.c;
+    const int64_t all = static_cast<int64_t>(c.batch) * c.kv_heads * p.rows, idx = min(static_cast<int64_t>(blockIdx.x) * kRows + in_block, all - 1);
     const int64_t bh = idx / p.rows;
     const int row = static_cast<int>(idx - bh * p.rows), head = static_cast<int>(bh % c.kv_heads), b = static_cast<int>(bh / c.kv_heads);
     const int token = row / p.group, at = c.positions[static_cast<int64_t>(b) * c.length + token];
     const float* const st = p.part + p.part_rows * D + 2 * idx * p.splits;
     float top = -INFINITY, sum = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int i = team; i < p.splits; i += kTeams) {
-        const float* const from = p.part + (idx * p.splits + i) * D + 8 * lane;
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
-        const float its = st[2 * i], before = top;
+    auto add = [&](float its, float its_sum, const float (&part)[8]) {
+        const float before = top;
         top = fmaxf(top, its);
         const float base = finite_or_zero(top), shrink = __builtin_amdgcn_exp2f(before - base), by = __builtin_amdgcn_exp2f(its - base);
-        sum = fmaf(st[2 * i + 1], by, sum * shrink);
+        sum = fmaf(its_sum, by, sum * shrink);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = fmaf(lo[j], by, v[j] * shrink);
-            v[4 + j] = fmaf(hi[j], by, v[4 + j] * shrink);
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(part[j], by, v[j] * shrink);
+    };
+#pragma unroll 4
+    for (int i = team; i < p.splits; i += TEAMS) {
+        float part[8];
+        load8<true>(p.part, (idx * p.splits + i) * D + 8 * lane, part);
+        add(st[2 * i], st[2 * i + 1], part);
+    }
+    if constexpr (TEAMS > 1) {
+        float* const mine = joined[in_block * TEAMS + team];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mine[8 * lane + j] = v[j];
+        if (lane == 0) {
+            mine[D] = top;
+            mine[D + 1] = sum;
+        }
+        __syncthreads();
+        if (team != 0) return;
+        for (int i = 1; i < TEAMS; ++i) {
+            const float* const other = joined[in_block * TEAMS + i];
+            float part[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) part[j] = other[8 * lane + j];
+            add(other[D], other[D + 1], part);
         }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) joined[team][8 * lane + j] = v[j];
-    if (lane == 0) {
-        joined[team][D] = top;
-        joined[team][D + 1] = sum;
-    }
-    __syncthreads();
-    if (team != 0) return;
-#pragma unroll
-    for (int i = 0; i < kTeams; ++i) top = fmaxf(top, joined[i][D]);
-    const float base = finite_or_zero(top);
-    sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kTeams; ++i) {
-        const float by = __builtin_amdgcn_exp2f(joined[i][D] - base);
-        sum = fmaf(joined[i][D + 1], by, sum);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(joined[i][8 * lane + j], by, v[j]);
-    }
+    if (static_cast<int64_t>(blockIdx.x) * kRows + in_block >= all) return;
     const float by = 1.0f / sum;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = at < 0 ? 0.0f : (at >= c.width * c.page_size ? NAN : v[j] * by);
@@ -771,33 +1104,58 @@ bool rows_fit(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads) {
 }
 
 struct Plan {
-    int64_t row_tiles, splits, rows, part_rows;
+    int64_t splits, rows, part_rows;
+    bool many;  // kv4_attention_rows_kernel
     size_t bytes;
 };
-#ifndef SP_
-#define SP_ 2
-#endif
+// Few blocks are split over the keys, as far as the chip takes them at once (256 blocks of eight waves, 512 with heads up to
+// 64; a second round of them cost more than uneven shares: 131072 keys, 8 key heads 67 us with 512 blocks, 39 with 256), a
+// tile a wave at least, and not for up to 16 tiles: joining the parts takes a launch of its own.
+//
+// The waves share the keys (kv4_attention_rows_kernel) from 2048 tiles of 256 rows by 64 keys on (us; heads of 128, 32 query
+// heads on 8 key heads):
+//
+//   sequences x tokens over keys   tiles   shared bf16  fp32   each wave its own bf16  fp32
+//   1 x 64 over 8192                1024       36                     31
+//   8 x 64 over 4000 (12 on 4)      2016       44        73          51                 68
+//   4 x 300 over 1000               2560       51        96          92                114
+//   1 x 512 over 8192               8192      115       202         180                229
+//   1 x 250 over 60000             30016      320                   558
 Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t dim, int64_t capacity) {
     Plan t{};
     t.rows = length * (heads / kv_heads);
-    t.row_tiles = ceil_div(t.rows, 16);
-    const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * t.row_tiles), tiles = ceil_div(capacity, kTile);
-    const int64_t resident = dim <= 64 ? 512 : 256;
-    t.splits = tiles <= SP_ * W ? 1 : std::max<int64_t>(1, std::min(resident / blocks, tiles / W));
+    const int64_t tiles = ceil_div(capacity, kTile), shared_blocks = batch * kv_heads * ceil_div(t.rows, 16 * W * 2);
+    t.many = dim == kSharedDim && t.rows >= 128 && shared_blocks * tiles >= 2048;
+    if (t.many) {
+        t.splits = std::max<int64_t>(1, std::min(256 / shared_blocks, tiles / 4));
+    } else {
+        const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * ceil_div(t.rows, 16)), resident = dim <= 64 ? 512 : 256;
+        t.splits = tiles <= 2 * W ? 1 : std::max<int64_t>(1, std::min(resident / blocks, tiles / W));
+    }
     t.part_rows = batch * kv_heads * t.rows * t.splits;
     t.bytes = t.splits > 1 ? static_cast<size_t>(t.part_rows) * (dim + 2) * sizeof(float) : 0;
     return t;
 }
 
 template <int D, bool F32>
-void launch_attention(const AttentionArgs& p, const Plan& t, hipStream_t s) {
-    const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * t.row_tiles * t.splits;
-    if (p.c.runs % 4 == 0) {
+void launch_attention(AttentionArgs p, const Plan& t, hipStream_t s) {
+    p.row_tiles = static_cast<int32_t>(ceil_div(t.rows, t.many ? 16 * W * kRowTiles<F32> : 16));
+    const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * p.row_tiles * t.splits;
+    if (t.many) {
+        if constexpr (D == kSharedDim) hipLaunchKernelGGL(kv4_attention_rows_kernel<F32>, dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
+    } else if (p.c.runs % 4 == 0) {
         hipLaunchKernelGGL((kv4_attention_kernel<D, F32, true>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     } else {
         hipLaunchKernelGGL((kv4_attention_kernel<D, F32, false>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     }
-    if (t.splits > 1) hipLaunchKernelGGL((kv4_join_kernel<D, F32>), dim3(static_cast<unsigned>(t.part_rows / t.splits)), dim3(256), 0, s, p);
+    if (t.splits == 1) return;
+    const int64_t rows = t.part_rows / t.splits;
+    constexpr int kAtOnce = 256 / (D / 8), kTeams = 8;
+    if (t.splits > 4) {
+        hipLaunchKernelGGL((kv4_join_kernel<D, F32, kTeams>), dim3(static_cast<unsigned>(ceil_div(rows, kAtOnce / kTeams))), dim3(256), 0, s, p);
+    } else {
+        hipLaunchKernelGGL((kv4_join_kernel<D, F32, 1>), dim3(static_cast<unsigned>(ceil_div(rows, kAtOnce))), dim3(256), 0, s, p);
+    }
 }
 
 }  // namespace
@@ -868,7 +1226,7 @@ extern "C" mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides,
     MLK_CHECK(q && q_strides && out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(out) & 15) == 0, "out must be 16-byte aligned");
     const Plan t = plan_of(batch, length, heads, kv_heads, head_dim, page_size * table_width);
-    MLK_CHECK(batch * kv_heads * t.row_tiles * t.splits < (int64_t{1} << 31), "too many tokens for one launch");
+    MLK_CHECK(batch * kv_heads * ceil_div(t.rows, 16) * t.splits < (int64_t{1} << 31), "too many tokens for one launch");
     MLK_CHECK(workspace_bytes >= t.bytes && (t.bytes == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)),
               "workspace must be 16-byte aligned and hold mlk_kv4_attention_workspace_bytes");
     p.q = q;
@@ -878,7 +1236,6 @@ extern "C" mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides,
     p.heads = static_cast<int32_t>(heads);
     p.group = static_cast<int32_t>(heads / kv_heads);
     p.rows = static_cast<int32_t>(t.rows);
-    p.row_tiles = static_cast<int32_t>(t.row_tiles);
     p.splits = static_cast<int32_t>(t.splits);
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     p.out = out;

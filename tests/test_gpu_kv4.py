@@ -428,3 +428,90 @@ def test_a_prompt_then_tokens_equals_the_sequence(dev):
         out, size, spread = ref.attention(q[b:b + 1, :n], keys, values, torch.zeros(1, 1, dtype=torch.int32), torch.arange(n)[None], D ** -0.5)
         _within(got[b:b + 1, :n], out, ref.attention_bound(size, spread, out, n, D, F32))
         assert not got[b, n:].any()
+
+
+# ------------------------------------------------------------------ many rows: waves that share the keys
+
+
+def _wide(table, width):
+    """The same table with more room than any sequence needs, as a server allots it."""
+    return torch.cat([table, torch.full((len(table), width - table.shape[1]), -1, dtype=torch.int32)], 1)
+
+
+def _shared_case(g, B, L, H, Hkv, page, room, dtype):
+    """A chunk of each of B sequences, causal, among them padding, rows in no order and a row at the start; the page table
+    of `room` tokens a sequence, most of it unused."""
+    positions = torch.stack([torch.arange(L) + 37 * b + (b % 3) * 130 for b in range(B)]).to(torch.int32)
+    positions[0] = positions[0][torch.randperm(L, generator=g)]
+    positions[B - 1, L // 2:] = -1
+    positions[0, 3] = 0
+    width = -(-(int(positions.max()) + 1) // page)
+    cache = ref.random_cache(g, B * width + 1, Hkv, page, 128)
+    table = ref.random_table(g, B, width, len(cache))
+    return torch.randn(B, L, H, 128, generator=g).to(dtype), cache, table, _wide(table, max(width, room // page)), positions
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,H,Hkv,page,room", [(2, 150, 6, 2, 48, 48 * 350), (2, 150, 6, 2, 64, 1 << 14), (1, 140, 1, 1, 16, 1 << 17),
+                                                 (3, 17, 40, 4, 1024, 1 << 14), (32, 33, 32, 8, 64, 1024), (2, 70, 16, 1, 32, 1 << 15)])
+def test_waves_that_share_the_keys(dev, dtype, B, L, H, Hkv, page, room):
+    g = torch.Generator().manual_seed(B * L + page)
+    q, cache, table, wide, positions = _shared_case(g, B, L, H, Hkv, page, room, dtype)
+    rows = L * H // Hkv
+    assert rows >= 128 and B * Hkv * -(-rows // 256) * (wide.shape[1] * page // 64) >= 2048  # what takes this form
+    got = _c().kv4_attention(q.to(dev), cache.to(dev), wide.to(dev), positions.to(dev), 0.09)
+    keys, values = ref.contents(cache, page, 128)
+    out, size, spread = ref.attention(q, keys, values, table, positions, 0.09)
+    _within(got, out, ref.attention_bound(size, spread, out, int(positions.max()) + 1, 128, dtype))
+    assert not got[B - 1, L // 2:].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_shared_keys_nan_and_missing_pages(dev, dtype):
+    """As for the other form: what lies behind a row's position does not reach it, NaN reaches the rows that see it and the
+    elements it belongs to, a missing page the rows that need it."""
+    g = torch.Generator().manual_seed(41)
+    page, D = 48, 128
+    q, cache, table, wide, positions = _shared_case(g, 2, 150, 6, 2, page, 48 * 350, dtype)
+    call = lambda c, t: _c().kv4_attention(q.to(dev), c.to(dev), t.to(dev), positions.to(dev), 0.09).cpu()
+    first = call(cache, wide)
+    dirty = cache.clone()
+    kc, vc, ks, vs = ref.parts(dirty, page, D)
+    used = torch.zeros(len(cache), page, dtype=torch.bool)
+    for b in range(2):
+        for t in range(int(positions[b].max()) + 1):
+            used[table[b, t // page].long(), t % page] = True
+    ks.copy_(torch.where(used[:, None, :, None], ks, torch.tensor(255, dtype=torch.uint8)))
+    vs.copy_(torch.where(used[:, None, None, :], vs, torch.tensor(255, dtype=torch.uint8)))
+    junk = wide.clone()
+    junk[:, table.shape[1]:] = torch.tensor([-3, 2 ** 30], dtype=torch.int32)[:, None]
+    assert torch.equal(call(dirty, junk), first)
+    place = lambda b, t: (table[b, t // page].long(), t % page)
+    p, o = place(0, 70)
+    ks[p, 0, o, 3] = 255
+    p, o = place(1, 180)
+    vs[p, 1, 1, o] = 255
+    got = call(dirty, wide)
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[0, :, :3] = (positions[0] >= 70)[:, None, None]
+    nan[1, :, 3:, 32:64] = (positions[1] >= 180)[:, None, None]
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], first[~nan])
+    gone = wide.clone()
+    gone[0, 2], gone[1, 3] = -1, len(cache)
+    got = call(cache, gone)
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[0] = (positions[0] >= 2 * page)[:, None, None]
+    nan[1] = (positions[1] >= 3 * page)[:, None, None]
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], first[~nan])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [3.0, 0.0, -0.2])
+def test_shared_keys_at_other_scales(dev, dtype, scale):
+    g = torch.Generator().manual_seed(43)
+    q, cache, table, wide, positions = _shared_case(g, 1, 140, 2, 1, 64, 1 << 16, dtype)
+    strided = torch.empty(1, 140, 2, 131, dtype=dtype)[..., 1:129].copy_(q)
+    got = _c().kv4_attention(strided.to(dev), cache.to(dev), wide.to(dev), positions.to(dev), scale)
+    keys, values = ref.contents(cache, 64, 128)
+    out, size, spread = ref.attention(q, keys, values, table, positions, scale)
+    _within(got, out, ref.attention_bound(size, spread, out, int(positions.max()) + 1, 128, dtype))
