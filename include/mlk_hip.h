@@ -484,7 +484,7 @@ mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dt
 
 /* y [rows, out_features] = x W^T + bias with four-bit weights: codes [out_features, in_features / 2] (16-byte aligned),
  * scales [out_features, in_features / 32], bias fp32 or NULL. x rows `x_stride` elements apart; y contiguous, of x's
- * dtype. in_features must be a multiple of 32. */
+ * dtype. in_features: a multiple of 32 below 2^24; out_features below 2^26. */
 mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int64_t x_stride, int32_t dtype,
                           const uint8_t* codes, const uint8_t* scales, const float* bias, int64_t out_features, void* out,
                           mlk_stream_t stream);

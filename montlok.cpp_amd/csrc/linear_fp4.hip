@@ -186,11 +186,11 @@ __global__ __launch_bounds__(KW * 64) void linear_fp4_stream_kernel(Fp4LinearArg
 
 // More rows: a block of WN KW waves takes 16 NT WN columns of y by 16 MT rows. WN waves share the columns and KW the k of
 // a step, 64 each, so that a wave's products need MT P LDS reads for NT MT P matrix instructions and every weight is
-// converted once, between the products of the k before it. Codes, scales and x are staged in LDS a step ahead, x as
+// converted once. Codes, scales and x are staged in LDS a step ahead, from registers loaded the step before that, x as
 // bf16 (three planes for fp32): loaded in rows, 8 lanes to 128 bytes, read in operand order. Unit u (8 consecutive k) of
 // row m of x lies at u * rows + (m ^ (u & 7)), piece c (32 codes) of row n of W at n * pieces + (c ^ (n & 7)): what
 // 8 lanes write, or read, together lies in different banks. The KW partial sums meet in LDS.
-template <bool F32, int WN, int KW, int NT, int MT, int BUFFERS>
+template <bool F32, int WN, int KW, int NT, int MT>
 struct TileShape {
     static constexpr int P = F32 ? 3 : 1, kRows = 16 * MT, kCols = 16 * NT * WN, kThreads = 64 * WN * KW;
     static constexpr int kK = 64 * KW, kUnits = kK / 8, kPieces = kK / kGroup;
@@ -199,11 +199,11 @@ struct TileShape {
     // A wave's partial sums of the tiles t = n MT + m that others finish (t mod KW is the wave that does).
     static constexpr int kParts = NT * MT - NT * MT / KW;
     static constexpr __device__ int part_of(int kw, int tile) { return tile - tile / KW - (tile % KW > kw ? 1 : 0); }
-    static constexpr size_t kLds = std::max(size_t{BUFFERS} * kBuffer * 16, size_t{WN} * KW * kParts * 1024);
+    static constexpr size_t kLds = std::max(size_t{2} * kBuffer * 16, size_t{WN} * KW * kParts * 1024);
 };
-template <bool F32, int WN, int KW, int NT, int MT, int DEPTH, int BUFFERS>
+template <bool F32, int WN, int KW, int NT, int MT>
 __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4LinearArgs p, int n_tiles, int m_tiles) {
-    using T = TileShape<F32, WN, KW, NT, MT, BUFFERS>;
+    using T = TileShape<F32, WN, KW, NT, MT>;
     constexpr int P = T::P, kBytes = F32 ? 4 : 2;
     constexpr int kXLoads = T::kRows * T::kUnits / T::kThreads, kWLoads = (T::kW + T::kThreads - 1) / T::kThreads;
     static_assert(kXLoads * T::kThreads == T::kRows * T::kUnits && T::kThreads % T::kUnits == 0 && T::kPieces % 8 == 0);
@@ -224,10 +224,10 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
     const int unit = threadIdx.x % T::kUnits;  // of x, the same in every load
     const int x_first = static_cast<int>(threadIdx.x) / T::kUnits, x_rows = T::kThreads / T::kUnits;
 
-    struct Ahead {  // what a thread has loaded of a step
+    struct {  // what a thread has loaded of the step that is staged next
         u32x4 w[kWLoads], scale_bytes, x[kXLoads][F32 ? 2 : 1];
-    } ahead[DEPTH];
-    auto load = [&](int step, Ahead& to) {
+    } ahead;
+    auto load = [&](int step) {
         // Past K: the last group's, x is zeroed when it is staged, and that group counts anyway.
 #pragma unroll
         for (int i = 0; i < kWLoads; ++i) {
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
             if (T::kW % T::kThreads != 0 && at >= T::kW) break;
             const uint32_t offset = static_cast<uint32_t>(min(row, p.N - 1 - n0)) * static_cast<uint32_t>(groups) +
                                     static_cast<uint32_t>(min(step * T::kPieces + piece, groups - 1));
-            to.w[i] = *reinterpret_cast<const u32x4*>(codes + 16 * static_cast<uint64_t>(offset));
+            ahead.w[i] = *reinterpret_cast<const u32x4*>(codes + 16 * static_cast<uint64_t>(offset));
         }
         if (static_cast<int>(threadIdx.x) < T::kCols) {
             const uint8_t* const from = scales + static_cast<int64_t>(min(static_cast<int>(threadIdx.x), p.N - 1 - n0)) * groups;
@@ -244,20 +244,20 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
                 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
                 if (first + 8 <= groups) {
                     const u32x2 v = *reinterpret_cast<const u32x2_any*>(from + first);
-                    to.scale_bytes[0] = v[0];
-                    to.scale_bytes[1] = v[1];
+                    ahead.scale_bytes[0] = v[0];
+                    ahead.scale_bytes[1] = v[1];
                 }
             } else {
                 static_assert(T::kPieces == 16);
                 typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
-                if (first + 16 <= groups) to.scale_bytes = *reinterpret_cast<const u32x4_byte*>(from + first);
+                if (first + 16 <= groups) ahead.scale_bytes = *reinterpret_cast<const u32x4_byte*>(from + first);
             }
             if (first + T::kPieces > groups) {
 #pragma unroll
                 for (int i = 0; i < T::kPieces / 4; ++i) {
-                    to.scale_bytes[i] = 0;
+                    ahead.scale_bytes[i] = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) to.scale_bytes[i] |= static_cast<uint32_t>(from[min(first + 4 * i + j, groups - 1)]) << (8 * j);
+                    for (int j = 0; j < 4; ++j) ahead.scale_bytes[i] |= static_cast<uint32_t>(from[min(first + 4 * i + j, groups - 1)]) << (8 * j);
                 }
             }
         }
@@ -266,41 +266,44 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
         for (int i = 0; i < kXLoads; ++i) {
             const char* const from = xs + (static_cast<uint32_t>(min(x_first + i * x_rows, p.rows - 1 - m0)) * static_cast<uint32_t>(p.x_stride * kBytes) + kx);
 #pragma unroll
-            for (int j = 0; j < (F32 ? 2 : 1); ++j) to.x[i][j] = reinterpret_cast<const u32x4_any*>(from)[j];
+            for (int j = 0; j < (F32 ? 2 : 1); ++j) ahead.x[i][j] = reinterpret_cast<const u32x4_any*>(from)[j];
         }
     };
-    auto stage = [&](int step, int buffer, Ahead& from) {
+    auto stage = [&](int step, int buffer) {
         u32x4* const to_x = lds + buffer * T::kBuffer;
         u32x4* const to_w = to_x + T::kX;
-        const bool inside = step * T::kK + 8 * unit < p.K;
+        if (step * T::kK + T::kK > p.K && step * T::kK + 8 * unit >= p.K) {
+#pragma unroll
+            for (int i = 0; i < kXLoads; ++i)
+#pragma unroll
+                for (int j = 0; j < (F32 ? 2 : 1); ++j) ahead.x[i][j] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < kXLoads; ++i) {
             const int row = x_first + i * x_rows;
-#pragma unroll
-            for (int j = 0; j < (F32 ? 2 : 1); ++j) from.x[i][j] = inside ? from.x[i][j] : u32x4{0, 0, 0, 0};
             u32x4* const to = to_x + unit * T::kRows + (row ^ (unit & 7));
             if constexpr (F32) {
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(from.x[i][j / 4][j % 4]);
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(ahead.x[i][j / 4][j % 4]);
                 bf16x8 planes[3];
                 planes_of<true>(v, planes);
 #pragma unroll
                 for (int j = 0; j < 3; ++j) to[j * (T::kUnits * T::kRows)] = __builtin_bit_cast(u32x4, planes[j]);
             } else {
-                to[0] = from.x[i][0];
+                to[0] = ahead.x[i][0];
             }
         }
 #pragma unroll
         for (int i = 0; i < kWLoads; ++i) {
             const int at = i * T::kThreads + static_cast<int>(threadIdx.x), row = at / T::kPieces, piece = at % T::kPieces;
             if (T::kW % T::kThreads != 0 && at >= T::kW) break;
-            to_w[row * T::kPieces + (piece ^ (row & 7))] = from.w[i];
+            to_w[row * T::kPieces + (piece ^ (row & 7))] = ahead.w[i];
         }
         if (static_cast<int>(threadIdx.x) < T::kCols) {
             uint32_t* const to = reinterpret_cast<uint32_t*>(to_w + T::kW) + threadIdx.x * (T::kPieces / 4);
 #pragma unroll
-            for (int i = 0; i < T::kPieces / 4; ++i) to[i] = from.scale_bytes[i];
+            for (int i = 0; i < T::kPieces / 4; ++i) to[i] = ahead.scale_bytes[i];
         }
     };
 
@@ -309,23 +312,21 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0, 0, 0, 0};
-    // Each column tile starts elsewhere in K. All blocks of an XCD read the same x, a step of it in rows that lie a
-    // multiple of 4 KB apart as often as not: in step they would all meet in the one or two channels of L2 that hold it.
-    const int steps = (p.K + T::kK - 1) / T::kK, start = (n_tile >> 3) % steps;
-    auto turned = [&](int step) { return start + step < steps ? start + step : start + step - steps; };
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i)
-        if (i < steps) load(turned(i), ahead[i]);
-    stage(turned(0), 0, ahead[0]);
+    const int steps = (p.K + T::kK - 1) / T::kK;
+    load(0);
+    stage(0, 0);
+    if (steps > 1) load(1);
     // A lane's 16 elements of the wave's 64 are k = 64 kw + 16 g ..: half (g & 1) of piece 2 kw + g / 2, units 8 kw + 2 g
     // and the next.
     const int piece = 2 * kw + (g >> 1);
-    auto advance = [&](int step, auto place) {  // place: step modulo DEPTH
+    auto advance = [&](int step, auto place) {  // place: step modulo 2
         constexpr int kPlace = decltype(place)::value;
-        const u32x4* const from_x = lds + kPlace % BUFFERS * T::kBuffer;
+        const u32x4* const from_x = lds + kPlace * T::kBuffer;
         const u32x4* const from_w = from_x + T::kX;
         __syncthreads();
-        if (step + DEPTH < steps) load(turned(step + DEPTH), ahead[kPlace]);
+        if (step + 1 < steps) stage(step + 1, 1 - kPlace);
+        if (step + 2 < steps) load(step + 2);
+        __builtin_amdgcn_sched_barrier(0);
         bf16x8 xv[2][MT][P];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -354,17 +355,10 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
 #pragma unroll
                     for (int m = 0; m < MT; ++m) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[i][m][j], acc[n][m], 0, 0, 0);
             }
-        if (BUFFERS == 1) __syncthreads();
-        if (step + 1 < steps) stage(turned(step + 1), (kPlace + 1) % BUFFERS, ahead[(kPlace + 1) % DEPTH]);
     };
-    static_assert(DEPTH == 2 || DEPTH == 4, "the place of a step gives its buffer");
-    for (int step = 0; step < steps; step += DEPTH) {
+    for (int step = 0; step < steps; step += 2) {
         advance(step, std::integral_constant<int, 0>{});
         if (step + 1 < steps) advance(step + 1, std::integral_constant<int, 1>{});
-        if constexpr (DEPTH == 4) {
-            if (step + 2 < steps) advance(step + 2, std::integral_constant<int, 2>{});
-            if (step + 3 < steps) advance(step + 3, std::integral_constant<int, 3>{});
-        }
     }
 
     __syncthreads();
@@ -407,12 +401,12 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
     }
 }
 
-template <bool F32, int WN, int KW, int NT, int MT, int DEPTH, int BUFFERS>
+template <bool F32, int WN, int KW, int NT, int MT>
 void launch_tile(const Fp4LinearArgs& p, hipStream_t s) {
-    using T = TileShape<F32, WN, KW, NT, MT, BUFFERS>;
+    using T = TileShape<F32, WN, KW, NT, MT>;
     static_assert(T::kLds <= 160 * 1024);
     const int64_t n_tiles = ceil_div(p.N, T::kCols), m_tiles = ceil_div(p.rows, T::kRows);
-    hipLaunchKernelGGL((linear_fp4_tile_kernel<F32, WN, KW, NT, MT, DEPTH, BUFFERS>), dim3(static_cast<unsigned>(8 * ceil_div(n_tiles, 8) * m_tiles)),
+    hipLaunchKernelGGL((linear_fp4_tile_kernel<F32, WN, KW, NT, MT>), dim3(static_cast<unsigned>(8 * ceil_div(n_tiles, 8) * m_tiles)),
                        dim3(T::kThreads), T::kLds, s, p, static_cast<int>(n_tiles), static_cast<int>(m_tiles));
 }
 template <bool F32, int NT>
@@ -429,15 +423,16 @@ void launch_stream(const Fp4LinearArgs& p, hipStream_t s) {
 // The forms' times go as the rounds of blocks on 256 CUs. Measured for K = 4096 in bf16 (us, launch included):
 //
 //   N      rows  stream  64-column tiles  128-column tiles
-//   4096    64     9.2        17.8             24
-//   4096   128    15.6        18.4             24
-//   4096   256    31          19.2             24
-//   12288   32    17.0        22.3             29
-//   12288   64    25.5        22.5             29
-//   12288  128    45          41               29
+//   4096    64     9.6        15.0             20.7
+//   4096   128    16.7        15.4             21.1
+//   4096   256    30.2        16.5             21.7
+//   12288   32    17.0        17.4             24.7
+//   12288   64    26.7        19.3             25.7
+//   12288  128    49          34               26.6
+//   12288  256    91          51               48.9
 //
-// that is 3.5 us for 256 stream blocks of 32 columns and 16 rows (fractions of a round count, blocks are many to a CU),
-// 17 and 24 for a round of tiles by 64 rows. fp32: 12 for 256 stream blocks of 64 columns, 34 for a round of 128-column
+// that is 3.7 us for 256 stream blocks of 32 columns and 16 rows (fractions of a round count, blocks are many to a CU),
+// 15.5 and 22 for a round of tiles by 64 rows. fp32: 12 for 256 stream blocks of 64 columns, 30 for a round of 128-column
 // tiles by 32 rows. A stream block that takes more columns shares what its x costs among them, and leaves CUs idle where
 // there are few: the round of 256 blocks of 16, 32 and 64 columns takes 4.0 and 4.9 us in bf16 (2.9 and 3.8 with 4 rows
 // and less), 6.7, 8.1 and 11.6 in fp32 (5.2, 6.8 and 9.5). 12288 x 16 rows in bf16: 14.8 us with 16 columns, 11.2 with
@@ -450,13 +445,13 @@ void launch(const Fp4LinearArgs& p, hipStream_t s) {
     const bool offsets_fit = p.x_stride < (int64_t{1} << 24);  // a tile's rows of x are addressed in 32 bits
     const bool few = p.rows <= kFew;
     if constexpr (F32) {
-        if (offsets_fit && 34 * rounds(128, 32) < 12 * full(64)) return launch_tile<true, 2, 4, 4, 2, 2, 2>(p, s);
+        if (offsets_fit && 30 * rounds(128, 32) < 12 * full(64)) return launch_tile<true, 2, 4, 4, 2>(p, s);
         const double by16 = (few ? 5.2 : 6.7) * rounds(16, 16), by32 = (few ? 6.8 : 8.1) * rounds(32, 16), by64 = (few ? 9.5 : 11.6) * rounds(64, 16);
         if (by64 < std::min(by16, by32)) return launch_stream<true, 4>(p, s);
         by16 <= by32 ? launch_stream<true, 1>(p, s) : launch_stream<true, 2>(p, s);
     } else {
-        const double stream = 3.5 * full(32), narrow = 17 * rounds(64, 64), wide = 24 * rounds(128, 64);
-        if (offsets_fit && std::min(narrow, wide) < stream) return narrow < wide ? launch_tile<false, 2, 4, 2, 4, 2, 2>(p, s) : launch_tile<false, 2, 4, 4, 4, 2, 2>(p, s);
+        const double stream = 3.7 * full(32), narrow = 15.5 * rounds(64, 64), wide = 22 * rounds(128, 64);
+        if (offsets_fit && std::min(narrow, wide) < stream) return narrow < wide ? launch_tile<false, 2, 4, 2, 4>(p, s) : launch_tile<false, 2, 4, 4, 4>(p, s);
         (few ? 2.9 : 4.0) * rounds(16, 16) <= (few ? 3.8 : 4.9) * rounds(32, 16) ? launch_stream<false, 1>(p, s) : launch_stream<false, 2>(p, s);
     }
 }
@@ -472,7 +467,8 @@ extern "C" mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_fea
     MLK_CHECK(dtype == MLK_DTYPE_F32 || dtype == MLK_DTYPE_BF16, "dtype must be f32 or bf16");
     MLK_CHECK(rows >= 0 && out_features > 0, "invalid linear geometry");
     MLK_CHECK(in_features > 0 && in_features % kGroup == 0, "in_features must be a positive multiple of 32");
-    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 24) && out_features < (int64_t{1} << 31) - 16, "too many rows or features");
+    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 24) && out_features < (int64_t{1} << 26), "too many rows or features");
+    MLK_CHECK(x_stride >= 0, "x_stride must not be negative");
     if (rows == 0) return MLK_OK;
     MLK_CHECK(x && codes && scales && out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
