@@ -724,9 +724,10 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
     };
     u32x4 ahead;
     Scales scale_ahead = 0;
+    bool missing = false;  // the page of scale_ahead: put in its place with keep, a select at the load would wait for it
     auto load = [&](int tile, const Ids& ids) {
-        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
-        const int group_id = bad ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
+        missing = ids.by_group < 0 || ids.by_group >= c.pages;
+        const int group_id = missing ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
         uint32_t page, token;
         if (wave < S) {
             const int at = (64 * wave + lane) / S, run = at / 16;
@@ -740,7 +741,6 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
         if (wave == W - 1) {
             split_run(c, 4 * tile + g, page, token);
             scale_ahead = *reinterpret_cast<const Scales*>(records + group_id * page_stride + 2 * half + (static_cast<int>(token) + l) * S);
-            if (bad) scale_ahead = static_cast<Scales>(~uint64_t{0});
         }
         if (wave == W - 2) {
             const int at = lane * S % 64, run = at / 16;
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
             const int j = 16 * (wave - S) + (lane >> 2);
             raw[buffer].value[4 * j + ((lane & 3) ^ (j >> 1 & 3))] = ahead;
         }
-        if (wave == W - 1) reinterpret_cast<Scales*>(raw[buffer].key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = scale_ahead;
+        if (wave == W - 1) reinterpret_cast<Scales*>(raw[buffer].key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = missing ? static_cast<Scales>(~uint64_t{0}) : scale_ahead;
         if (wave == W - 2) reinterpret_cast<Scales*>(raw[buffer].value_scale)[lane] = scale_ahead;
     };
     auto convert = [&](int tile, int buffer) {
@@ -852,7 +852,6 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
 #pragma unroll
         for (int s = 0; s < S; ++s) acc[m][s][0] = acc[m][s][1] = f32x4{0, 0, 0, 0};
     }
-    const int stride = p.splits;
     auto at_step = [&](int n) { return split + n * p.splits; };
     load(split, lookup(split));
     keep(0);
