@@ -369,11 +369,12 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
     };
     u32x4 key_ahead[S], value_ahead[S];
     Scales key_scale_ahead, value_scale_ahead;
+    bool missing = false;  // the page of key_scale_ahead: looked at when the tile is used, a select here would wait for the loads
     auto load_whole = [&](int tile, const Ids& ids) {
-        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
+        missing = ids.by_group < 0 || ids.by_group >= c.pages;
         uint32_t page, token;
         split_run(c, 4 * tile, page, token);
-        const uint8_t* const record = records + (bad ? 0 : ids.by_group) * page_stride;
+        const uint8_t* const record = records + (missing ? 0 : ids.by_group) * page_stride;
         const uint8_t* const keys = record + token * (D / 2);
         const uint8_t* const values = record + half + token;
         const uint8_t* const scales = record + 2 * half;
@@ -383,14 +384,13 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         for (int t = 0; t < S; ++t)
             value_ahead[t] = *reinterpret_cast<const u32x4*>(values + static_cast<uint32_t>((16 * t + (lane >> 2)) * c.page_size + 16 * (lane & 3)));
         key_scale_ahead = *reinterpret_cast<const Scales*>(scales + token * S + static_cast<uint32_t>(lane * S));
-        if (bad) key_scale_ahead = static_cast<Scales>(~uint64_t{0});
         value_scale_ahead = *reinterpret_cast<const Scales*>(scales + S * c.page_size + token +
                                                              static_cast<uint32_t>(lane * S / 64 * c.page_size + lane * S % 64));
     };
     auto load = [&](int tile, const Ids& ids) {
         if constexpr (WHOLE) return load_whole(tile, ids);
-        const bool bad = ids.by_group < 0 || ids.by_group >= c.pages;
-        const int group_id = bad ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
+        missing = ids.by_group < 0 || ids.by_group >= c.pages;
+        const int group_id = missing ? 0 : ids.by_group, piece_id = ids.by_piece < 0 || ids.by_piece >= c.pages ? 0 : ids.by_piece;
         uint32_t page, token;
 #pragma unroll
         for (int t = 0; t < S; ++t) {
@@ -405,7 +405,6 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         for (int t = 0; t < S; ++t) value_ahead[t] = *reinterpret_cast<const u32x4*>(value + 16 * t * c.page_size);
         split_run(c, 4 * tile + g, page, token);
         key_scale_ahead = *reinterpret_cast<const Scales*>(records + group_id * page_stride + 2 * half + (static_cast<int>(token) + l) * S);
-        if (bad) key_scale_ahead = static_cast<Scales>(~uint64_t{0});
         const int at = lane * S % 64, run = at / 16;  // token of the lane's value scales
         split_run(c, 4 * tile + run, page, token);
         value_scale_ahead = *reinterpret_cast<const Scales*>(records + (S == 1 ? group_id : __shfl(group_id, 16 * run, kWave)) * page_stride + 2 * half +
@@ -469,7 +468,8 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
             const int at = 64 * t + lane, token = at / S, row = token >> 4 << 2 | (token & 3), a = token >> 2 & 3;
             mine.codes[(16 * a + row) * S + (at % S ^ mine.turn(row))] = key_ahead[t];
         }
-        reinterpret_cast<Scales*>(mine.key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = key_scale_ahead;  // token 16 g + l
+        reinterpret_cast<Scales*>(mine.key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] =
+            missing ? static_cast<Scales>(~uint64_t{0}) : key_scale_ahead;  // token 16 g + l
         reinterpret_cast<Scales*>(mine.value_scale)[lane] = value_scale_ahead;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         uint32_t kc[4][S], ks[4];
