@@ -642,11 +642,31 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     return (_native or _ops()).kv4_attention(q, cache, page_table, positions, scale)
 
 
+def fp4_weights(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """weight [N, K] (K a multiple of 32) as the ``codes`` and ``scales`` of ``linear_fp4``, quantised as ``kv4_append``
+    quantises. Once for a weight, with tensor operations, on the weight's device."""
+    _check(weight.dim() == 2 and weight.size(0) > 0 and weight.size(1) > 0 and weight.size(1) % 32 == 0,
+           "weight must be [out_features, in_features], in_features a multiple of 32")
+    _check(weight.dtype in (torch.float32, torch.bfloat16), "weight must be float32 or bfloat16")
+    groups = weight.detach().float().unflatten(-1, (-1, 32))
+    fine = torch.isfinite(groups).all(-1, keepdim=True)
+    size = torch.where(fine, groups, 0.0).abs()
+    # most = m 2^e with m in [0.5, 1) and 6 = 0.75 * 2^3: the power is e - 3 up to 0.75 and e - 2 above.
+    m, e = torch.frexp(size.amax(-1, keepdim=True))
+    byte = torch.where(m == 0, 3, (e + 124 + (m > 0.75)).clamp(3, 252))
+    size = torch.ldexp(size, 127 - byte)
+    # Halves between two codes go to the even one.
+    code = ((size > 0.25).int() + (size >= 0.75) + (size > 1.25) + (size >= 1.75) + (size > 2.5) + (size >= 3.5) + (size > 5.0))
+    code = torch.where(fine, code + 8 * torch.signbit(groups), 0).to(torch.uint8).flatten(1)
+    scales = torch.where(fine, byte, 255).to(torch.uint8).flatten(1)
+    return code[:, ::2] | code[:, 1::2] << 4, scales
+
+
 def linear_fp4(input: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                bias: torch.Tensor | None = None) -> torch.Tensor:
-    """input [..., K] @ W^T + bias with W in four bits: codes uint8 [N, K / 2] (element 2 j in the low bits of byte j),
-    scales uint8 [N, K / 32], bias float32 [N]. The result has the input's dtype; sums are in float32 and the products
-    exact, for float32 input too."""
+    """input [..., K] @ W^T + bias with W in four bits, as ``fp4_weights`` gives it: codes uint8 [N, K / 2] (element 2 j in
+    the low bits of byte j), scales uint8 [N, K / 32], bias float32 [N]. The result has the input's dtype; sums are in
+    float32 and the products exact, for float32 input too."""
     return (_native or _ops()).linear_fp4(input, codes, scales, bias)
 
 

@@ -136,3 +136,34 @@ def test_cache_allocation():
 
     cache = _C.kv4_cache(3, 2, 48, 64, device="cpu")
     assert cache.shape == (3, 2, 48 * 68) and cache.dtype == torch.uint8 and not cache.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(1, 32), (7, 96), (33, 256)])
+def test_weights_in_four_bits(dtype, n, k):
+    """The nearest values of the format, by groups of every size, among them halves between codes, zeros, the smallest and
+    largest numbers, infinities and NaN."""
+    import kv4_reference as ref
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(n + k)
+    w = torch.randn(n, k, generator=g) * 2.0 ** torch.randint(-20, 20, (n, k // 32, 1), generator=g).expand(-1, -1, 32).flatten(1)
+    w[0, :32] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0] * 4) * torch.tensor([1.0, -1.0]).repeat(16)
+    if n > 1:
+        w[1, :32], w[2, :32], w[3, :32], w[4, 3], w[5, 40] = 0.0, 2.0 ** -140, 3e38, torch.inf, torch.nan
+        w[6, :32] = w[0, :32] * 2.0 ** -124
+    w = w.to(dtype)
+    codes, scales = _C.fp4_weights(w)
+    assert codes.shape == (n, k // 2) and scales.shape == (n, k // 32) and codes.dtype == scales.dtype == torch.uint8
+    assert codes.is_contiguous() and scales.is_contiguous()
+    assert torch.equal(ref.value_of(codes, scales).nan_to_num(nan=1e300), ref.nearest(w).nan_to_num(nan=1e300))
+    nan = ~torch.isfinite(w).unflatten(1, (-1, 32)).all(-1)
+    assert (scales[nan] == 255).all() and (scales[~nan] < 253).all()
+
+
+@pytest.mark.parametrize("w", [torch.ones(4), torch.ones(4, 48), torch.ones(4, 0), torch.ones(0, 32), torch.ones(4, 32, dtype=torch.float16)])
+def test_weights_that_do_not_fit_are_refused(w):
+    from montlok import _C
+
+    with pytest.raises(RuntimeError, match="weight must be"):
+        _C.fp4_weights(w)
