@@ -358,23 +358,31 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
     struct Ids {
         int32_t by_group, by_piece;  // pages of runs g and lane & 3; the tile's page
     };
+    uint32_t no_lane;
+    asm("v_mov_b32 %0, 0" : "=v"(no_lane));
     auto lookup = [&](int tile) {
         auto page_of = [&](int run) {
             uint32_t page, token;
             split_run(c, 4 * tile + run, page, token);
             return page < static_cast<uint32_t>(c.width) ? table[page] : -1;
         };
-        if constexpr (WHOLE) return Ids{page_of(0), 0};
+        if constexpr (WHOLE) {
+            // A vector load, waited for with the tile's: the scalar unit's would be waited for by the next read of LDS.
+            uint32_t page, token;
+            split_run(c, 4 * tile, page, token);
+            return Ids{page < static_cast<uint32_t>(c.width) ? table[page + no_lane] : -1, 0};
+        }
         return Ids{page_of(g), page_of(lane & 3)};
     };
     u32x4 key_ahead[S], value_ahead[S];
     Scales key_scale_ahead, value_scale_ahead;
     bool missing = false;  // the page of key_scale_ahead: looked at when the tile is used, a select here would wait for the loads
     auto load_whole = [&](int tile, const Ids& ids) {
-        missing = ids.by_group < 0 || ids.by_group >= c.pages;
+        const int id = __builtin_amdgcn_readfirstlane(ids.by_group);
+        missing = id < 0 || id >= c.pages;
         uint32_t page, token;
         split_run(c, 4 * tile, page, token);
-        const uint8_t* const record = records + (missing ? 0 : ids.by_group) * page_stride;
+        const uint8_t* const record = records + (missing ? 0 : id) * page_stride;
         const uint8_t* const keys = record + token * (D / 2);
         const uint8_t* const values = record + half + token;
         const uint8_t* const scales = record + 2 * half;
@@ -454,6 +462,8 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         last = max(last, __shfl_xor(last, i, kWave));
         least = min(least, __shfl_xor(least, i, kWave));
     }
+    last = __builtin_amdgcn_readfirstlane(last);  // of all lanes alike
+    least = __builtin_amdgcn_readfirstlane(least);
     if constexpr (kShared) __syncthreads();
 
     float top = -INFINITY, sum = 0.0f;  // the largest score so far, and the lane's part of the sum of 2^(scale (score - top))
