@@ -1011,19 +1011,21 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
     }
 }
 
-// The splits of a row joined: D / 8 lanes across it, and TEAMS such groups that take a split each at a time (many splits
-// of few rows: one group a row walked 64 of them for 20 us).
+// The splits of a row joined: D / 8 lanes across it, and TEAMS such groups that take a split each at a time (more than 16
+// splits: one group a row walked 64 of them for 20 us; up to 16 of them it saves 0.3 to 1.5 us).
 template <int D, bool F32, int TEAMS>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes / TEAMS;
     __shared__ float joined[TEAMS > 1 ? kRows * TEAMS : 1][D + 4];  // a team's part, then its maximum and sum
     const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes % TEAMS, in_block = threadIdx.x / kLanes / TEAMS;
     const Cache& c = p.c;
-    const int64_t all = static_cast<int64_t>(c.batch) * c.kv_heads * p.rows, idx = min(static_cast<int64_t>(blockIdx.x) * kRows + in_block, all - 1);
-    const int64_t bh = idx / p.rows;
-    const int row = static_cast<int>(idx - bh * p.rows), head = static_cast<int>(bh % c.kv_heads), b = static_cast<int>(bh / c.kv_heads);
-    const int token = row / p.group, at = c.positions[static_cast<int64_t>(b) * c.length + token];
-    const float* const st = p.part + p.part_rows * D + 2 * idx * p.splits;
+    const uint32_t all = static_cast<uint32_t>(c.batch * c.kv_heads) * static_cast<uint32_t>(p.rows);  // below 2^31
+    const uint32_t idx = min(blockIdx.x * kRows + in_block, all - 1);
+    const int bh = static_cast<int>(idx / static_cast<uint32_t>(p.rows)), row = static_cast<int>(idx - static_cast<uint32_t>(bh * p.rows));
+    const int b = bh / c.kv_heads, head = bh - b * c.kv_heads, token = row / p.group;
+    const int at = c.positions[static_cast<int64_t>(b) * c.length + token];
+    const int64_t first = static_cast<int64_t>(idx) * p.splits;
+    const float* const st = p.part + p.part_rows * D + 2 * first;
     float top = -INFINITY, sum = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     auto add = [&](float its, float its_sum, const float (&part)[8]) {
         const float before = top;
@@ -1036,7 +1038,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
 #pragma unroll 4
     for (int i = team; i < p.splits; i += TEAMS) {
         float part[8];
-        load8<true>(p.part, (idx * p.splits + i) * D + 8 * lane, part);
+        load8<true>(p.part, (first + i) * D + 8 * lane, part);
         add(st[2 * i], st[2 * i + 1], part);
     }
     if constexpr (TEAMS > 1) {
@@ -1057,11 +1059,11 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs p) {
             add(other[D], other[D + 1], part);
         }
     }
-    if (static_cast<int64_t>(blockIdx.x) * kRows + in_block >= all) return;
+    if (blockIdx.x * kRows + in_block >= all) return;
     const float by = 1.0f / sum;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = at < 0 ? 0.0f : (at >= c.width * c.page_size ? NAN : v[j] * by);
-    put8<F32>(p.out, ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + row % p.group) * D + 8 * lane, v);
+    put8<F32>(p.out, ((static_cast<int64_t>(b) * c.length + token) * p.heads + head * p.group + row - token * p.group) * D + 8 * lane, v);
 }
 
 // ------------------------------------------------------------- host
@@ -1139,7 +1141,8 @@ Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int
         t.splits = std::max<int64_t>(1, std::min(256 / shared_blocks, tiles / 4));
     } else {
         const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * ceil_div(t.rows, 16)), resident = dim <= 64 ? 512 : 256;
-        t.splits = tiles <= 2 * W ? 1 : std::max<int64_t>(1, std::min(resident / blocks, tiles / W));
+        const int64_t groups = ceil_div(tiles, W), most = std::max<int64_t>(1, std::min(resident / blocks, groups));
+        t.splits = tiles <= 2 * W ? 1 : ceil_div(groups, ceil_div(groups, most));
     }
     t.part_rows = batch * kv_heads * t.rows * t.splits;
     t.bytes = t.splits > 1 ? static_cast<size_t>(t.part_rows) * (dim + 2) * sizeof(float) : 0;
@@ -1160,7 +1163,7 @@ void launch_attention(AttentionArgs p, const Plan& t, hipStream_t s) {
     if (t.splits == 1) return;
     const int64_t rows = t.part_rows / t.splits;
     constexpr int kAtOnce = 256 / (D / 8), kTeams = 8;
-    if (t.splits > 4) {
+    if (t.splits > 16) {
         hipLaunchKernelGGL((kv4_join_kernel<D, F32, kTeams>), dim3(static_cast<unsigned>(ceil_div(rows, kAtOnce / kTeams))), dim3(256), 0, s, p);
     } else {
         hipLaunchKernelGGL((kv4_join_kernel<D, F32, 1>), dim3(static_cast<unsigned>(ceil_div(rows, kAtOnce))), dim3(256), 0, s, p);
