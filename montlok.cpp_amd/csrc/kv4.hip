@@ -8,13 +8,11 @@
 //   key scales   [page_size][D / 32]
 //   value scales [D / 32][page_size]
 //
-// Both products of attention then load their operands straight into the
-// registers that v_mfma_f32_16x16x32_bf16 takes them from (lane (g, l) = 16 g + l
-// holds row l of A, 8 consecutive k): a key row is contiguous in d, which the
-// score product sums over, and a value row in tokens, which the other one does.
-// A transposed value row in the cache costs the append 16-byte-apart byte
-// stores, once a token; the attention reads every byte of it for every token
-// that follows.
+// The operands of v_mfma_f32_16x16x32_bf16 are rows of eight consecutive k a
+// lane: a key row is contiguous in d, which the score product sums over, and a
+// value row in tokens, which the other one does. A transposed value row costs
+// the append a turn of 4 x 4 bytes between lanes, once a token; the attention
+// reads every byte of it for every token that follows.
 #include <algorithm>
 #include <type_traits>
 
@@ -41,8 +39,8 @@ struct Cache {
     int64_t value_codes(int dim) const { return static_cast<int64_t>(page_size) * (dim / 2); }
 };
 
-// Page index of a run of 16 tokens and the run's place in it. run < 2^24, runs <= 64: the product of twice the run with
-// the rounded-up reciprocal of twice the runs is exact (its error is below 2^25 * 127 / 2^32 of a page's 128th).
+// Page index of a run of 16 tokens and the run's place in it. run < 2^25 (a table's, and those looked up past its end),
+// runs <= 64: the quotient by the rounded-up reciprocal is above the true one by less than run / 2^31 < 1 / runs.
 __device__ __forceinline__ void split_run(const Cache& c, uint32_t run, uint32_t& page, uint32_t& token) {
     page = __umulhi(2 * run, c.magic);
     token = (run - page * static_cast<uint32_t>(c.runs)) * kRun;
@@ -119,7 +117,8 @@ struct Bytes<8> {
 // A wave moves the keys, or the values, of 16 consecutive tokens of the call and one head: lane 4 t + q the eight elements
 // 32 s + 8 q .. of token t for each group s, a dword of codes. A value dword is four rows of one token, where the cache
 // holds rows of tokens: four lanes that hold a run of four tokens turn their 4 x 4 bytes, so that a lane moves one row's
-// four tokens. Tokens that are no such run are moved byte by byte.
+// four tokens. Tokens that are no such run are moved byte by byte. Bound by memory: 4 x 2048 tokens of 8 heads of 128 in
+// fp32 are written in 14.4 us and read in 16.4 (5.3 and 4.7 TB/s).
 
 // Byte k of the lane whose token is i of its four against byte i of the one whose token is k; its own inverse.
 __device__ __forceinline__ uint32_t turn4(uint32_t v, int i) {
@@ -317,11 +316,16 @@ struct TileLds {
 
 // A block takes 16 rows of a (sequence, key head) and every p.splits-th group of W tiles of 64 keys, a tile a wave.
 //
+// Bound by memory with 8 waves of bf16 (64 sequences of 10000 keys, 8 key heads of 128: 132 us, 5.3 TB/s), by the issue of
+// some 500 vector instructions a tile in fp32 (182 us, 3.8 TB/s: three planes of each weight) and below 64 elements (4 a
+// key pair to convert, turn and scale); one tile a wave alone takes about 5 us, most of it waiting for memory.
+//
 // Scores are key tile x q^T, so that lane (g, l) holds row l's scores of 16 tokens, in the registers from which the
 // product with the values takes its weights: nothing moves between lanes but the maximum (a column's sum is formed at
 // the end). Key tile a, row 4 g' + r is token 16 g' + 4 a + r of the 64, so that a lane's scores (rows 4 g .. 4 g + 3 of
 // every tile) are its 16 tokens 16 g .. 16 g + 15 of the value product.
-// WHOLE: pages of whole tiles. A tile then has one page, looked up by the scalar unit.
+// WHOLE: pages of whole tiles. A tile then has one page, and its addresses are scalar. Not for D = 256, where the
+// registers that this takes are spilled (64 x 4000 keys of 8 heads, fp32: 161 against 138 us).
 template <int D, bool F32, bool WHOLE>
 __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void kv4_attention_kernel(AttentionArgs p) {
     constexpr int S = D / 32;       // k steps of a score product, groups of a token, 1 KB loads of a tile's keys (or values)
@@ -690,6 +694,9 @@ constexpr int kRowTiles = F32 ? 1 : 2;
 // operands in LDS. A wave of the kernel above spends most of its instructions on converting keys and values, for 16 rows
 // (512 tokens of two sequences over 8192 keys took 270 us so); here it converts an eighth of them, for 128 MT. A tile
 // passes through registers (three tiles ahead), LDS as it lies in memory (two ahead) and LDS as operands (one ahead).
+// 1 x 512 tokens over 8192 keys, 32 heads on 8: 111 us, 620 TFLOP/s; a SIMD's two waves issue vector instructions for 54%
+// of the time, products for 33%, and LDS hands out operands for 28%. Converting at the end of a tile in one of the two
+// waves, so that the other's products meet it, took 6% longer.
 //
 // Operands: key tile a, k step s is unit a S + s; values of group s and half h of a lane's 16 tokens, their even and odd
 // elements, are unit 2 s + h.
@@ -1121,17 +1128,21 @@ struct Plan {
 };
 // Few blocks are split over the keys, as far as the chip takes them at once (256 blocks of eight waves, 512 with heads up to
 // 64; a second round of them cost more than uneven shares: 131072 keys, 8 key heads 67 us with 512 blocks, 39 with 256), a
-// tile a wave at least, and not for up to 16 tiles: joining the parts takes a launch of its own.
+// tile a wave at least, in whole rounds of tiles (20 tiles in 3 blocks 9.8 us, in 2 11.0), and not for up to 16 tiles:
+// joining the parts takes a launch of its own (32 tiles: 14.5 us in one block, 10.5 in four).
 //
 // The waves share the keys (kv4_attention_rows_kernel) from 2048 tiles of 256 rows by 64 keys on (us; heads of 128, 32 query
 // heads on 8 key heads):
 //
 //   sequences x tokens over keys   tiles   shared bf16  fp32   each wave its own bf16  fp32
 //   1 x 64 over 8192                1024       36                     31
-//   8 x 64 over 4000 (12 on 4)      2016       44        73          51                 68
-//   4 x 300 over 1000               2560       51        96          92                114
-//   1 x 512 over 8192               8192      115       202         180                229
+//   8 x 64 over 4000 (12 on 4)      2016       44        73          48                 65
+//   4 x 300 over 1000               2560       49        93          92                114
+//   1 x 512 over 8192               8192      111       193         180                229
 //   1 x 250 over 60000             30016      320                   558
+//
+// One round of its blocks: two took 20 us more for sequences of one length and 15 less for two of which one is half as
+// long (2 x 512 over 8192).
 Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t dim, int64_t capacity) {
     Plan t{};
     t.rows = length * (heads / kv_heads);
@@ -1155,8 +1166,8 @@ void launch_attention(AttentionArgs p, const Plan& t, hipStream_t s) {
     const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * p.row_tiles * t.splits;
     if (t.many) {
         if constexpr (D == kSharedDim) hipLaunchKernelGGL(kv4_attention_rows_kernel<F32>, dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
-    } else if (p.c.runs % 4 == 0) {
-        hipLaunchKernelGGL((kv4_attention_kernel<D, F32, true>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
+    } else if (D < 256 && p.c.runs % 4 == 0) {
+        if constexpr (D < 256) hipLaunchKernelGGL((kv4_attention_kernel<D, F32, true>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     } else {
         hipLaunchKernelGGL((kv4_attention_kernel<D, F32, false>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     }
