@@ -118,7 +118,7 @@ struct Bytes<8> {
 // 32 s + 8 q .. of token t for each group s, a dword of codes. A value dword is four rows of one token, where the cache
 // holds rows of tokens: four lanes that hold a run of four tokens turn their 4 x 4 bytes, so that a lane moves one row's
 // four tokens. Tokens that are no such run are moved byte by byte. Bound by memory: 4 x 2048 tokens of 8 heads of 128 in
-// fp32 are written in 14.4 us and read in 16.4 (5.3 and 4.7 TB/s).
+// fp32 are written in 14.4 us and read in 16.4 (4.8 and 4.2 TB/s).
 
 // Byte k of the lane whose token is i of its four against byte i of the one whose token is k; its own inverse.
 __device__ __forceinline__ uint32_t turn4(uint32_t v, int i) {
@@ -419,7 +419,8 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         key_scale_ahead = *reinterpret_cast<const Scales*>(records + group_id * page_stride + 2 * half + (static_cast<int>(token) + l) * S);
         const int at = lane * S % 64, run = at / 16;  // token of the lane's value scales
         split_run(c, 4 * tile + run, page, token);
-        value_scale_ahead = *reinterpret_cast<const Scales*>(records + (S == 1 ? group_id : __shfl(group_id, 16 * run, kWave)) * page_stride + 2 * half +
+        const int value_id = S == 1 ? group_id : __shfl(group_id, 16 * run, kWave);
+        value_scale_ahead = *reinterpret_cast<const Scales*>(records + value_id * page_stride + 2 * half +
                                                              ((S + lane * S / 64) * c.page_size + static_cast<int>(token) + at % 16));
     };
     // The first tile is on its way before the rows are known.
@@ -753,7 +754,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
             ahead = *reinterpret_cast<const u32x4*>(records + key_id * page_stride + ((static_cast<int>(token) + at % 16) * (D / 2) + lane % S * 16));
         } else {
             split_run(c, 4 * tile + (lane & 3), page, token);
-            ahead = *reinterpret_cast<const u32x4*>(records + piece_id * page_stride + half + ((16 * (wave - S) + (lane >> 2)) * c.page_size + static_cast<int>(token)));
+            const int at = (16 * (wave - S) + (lane >> 2)) * c.page_size + static_cast<int>(token);
+            ahead = *reinterpret_cast<const u32x4*>(records + piece_id * page_stride + half + at);
         }
         if (wave == W - 1) {
             split_run(c, 4 * tile + g, page, token);
@@ -763,7 +765,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
             const int at = lane * S % 64, run = at / 16;
             const int value_id = __shfl(group_id, 16 * run, kWave);
             split_run(c, 4 * tile + run, page, token);
-            scale_ahead = *reinterpret_cast<const Scales*>(records + value_id * page_stride + 2 * half + ((S + lane * S / 64) * c.page_size + static_cast<int>(token) + at % 16));
+            const int place = (S + lane * S / 64) * c.page_size + static_cast<int>(token) + at % 16;
+            scale_ahead = *reinterpret_cast<const Scales*>(records + value_id * page_stride + 2 * half + place);
         }
     };
     auto keep = [&](int buffer) {
@@ -774,7 +777,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
             const int j = 16 * (wave - S) + (lane >> 2);
             raw[buffer].value[4 * j + ((lane & 3) ^ (j >> 1 & 3))] = ahead;
         }
-        if (wave == W - 1) reinterpret_cast<Scales*>(raw[buffer].key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = missing ? static_cast<Scales>(~uint64_t{0}) : scale_ahead;
+        if (wave == W - 1)
+            reinterpret_cast<Scales*>(raw[buffer].key_scale)[4 * (4 * g + (l & 3)) + (l >> 2)] = missing ? static_cast<Scales>(~uint64_t{0}) : scale_ahead;
         if (wave == W - 2) reinterpret_cast<Scales*>(raw[buffer].value_scale)[lane] = scale_ahead;
     };
     auto convert = [&](int tile, int buffer) {
@@ -1135,11 +1139,11 @@ struct Plan {
 // heads on 8 key heads):
 //
 //   sequences x tokens over keys   tiles   shared bf16  fp32   each wave its own bf16  fp32
-//   1 x 64 over 8192                1024       36                     31
-//   8 x 64 over 4000 (12 on 4)      2016       44        73          48                 65
-//   4 x 300 over 1000               2560       49        93          92                114
-//   1 x 512 over 8192               8192      111       193         180                229
-//   1 x 250 over 60000             30016      320                   558
+//   1 x 64 over 8192                1024       36                     28
+//   8 x 64 over 4000 (12 on 4)      2016       44        73          47                 65
+//   4 x 300 over 1000               2560       49        93          90                112
+//   1 x 512 over 8192               8192      111       193         170                224
+//   1 x 250 over 60000             30016      320                   490
 //
 // One round of its blocks: two took 20 us more for sequences of one length and 15 less for two of which one is half as
 // long (2 x 512 over 8192).
@@ -1201,7 +1205,8 @@ extern "C" mlk_status mlk_kv4_append(const void* k, const int64_t* k_strides, co
     by_dim(head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_append_kernel<D, true> : kv4_append_kernel<D, false>;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, kr, vr, waves);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0,
+                           reinterpret_cast<hipStream_t>(stream), c, kr, vr, waves);
     });
     return launch_status("kv4 append");
 }
@@ -1221,7 +1226,8 @@ extern "C" mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t 
     by_dim(head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_read_kernel<D, true> : kv4_read_kernel<D, false>;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, k, v, waves);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0,
+                           reinterpret_cast<hipStream_t>(stream), c, k, v, waves);
     });
     return launch_status("kv4 read");
 }

@@ -34,15 +34,19 @@ __device__ __forceinline__ void put4(void* out, int64_t first, const float (&y)[
     }
 }
 
-// Few rows: a block takes 16 columns of y (rows of W) by 16 rows, its KW waves interleaved blocks of 512 k. A wave loads
-// its block of W whole rows at a time (256 bytes of 4 rows an instruction; the order of the matrix instruction, lane
-// (g, l) = group of row l, straight from memory costs a cache access a lane and bounded this kernel) and turns it in
-// its own piece of LDS. x comes the same way (TURN), or, for the first FEW rows, straight to the lanes whose row exists.
-// Past K a lane's x is zero (its W is that of the last group, which counts anyway). An infinity or a NaN in fp32 x makes
-// the quick planes NaN; a wave that sees one in its sums forms them again.
-constexpr int kFew = 4;
-template <bool F32, bool TURN, int KW, int NT, int U>
-__global__ __launch_bounds__(KW * 64) void linear_fp4_stream_kernel(Fp4LinearArgs p) {
+// Few rows: a block takes 16 NT columns of y (rows of W) by 16 rows, its kWaves waves interleaved blocks of 256 k. A wave
+// loads its block of W whole lines at a time (128 bytes of 8 rows an instruction; the order of the matrix instruction, lane
+// (g, l) = group of row l, straight from memory costs a cache access a lane and bounded this kernel: 31 us where it takes
+// 8 now) and turns it in its own piece of LDS. x comes the same way (TURN), or, for up to kFew rows, straight to the lanes
+// whose row exists. Past K a lane's x is zero (its W is that of the last group, which counts anyway). An infinity or a NaN
+// in fp32 x makes the quick planes NaN; a wave that sees one in its sums forms them again.
+//
+// One bf16 row is bound by the reading of W (12288 x 4096: 7.4 us, 3.6 TB/s); 16 rows of fp32 by what a block does for
+// each of its columns' x, which it reads whole from L2 and takes apart (4100 x 4096: 9.5 us, 0.9 TB/s).
+constexpr int kFew = 4, kWaves = 8, kSteps = 2;
+template <bool F32, bool TURN, int NT>
+__global__ __launch_bounds__(kWaves * 64) void linear_fp4_stream_kernel(Fp4LinearArgs p) {
+    constexpr int KW = kWaves, U = kSteps;
     constexpr int P = F32 ? 3 : 1, kPieces = F32 ? 8 : 4;  // 16-byte pieces of 32 elements of x
     constexpr int kRow = 4 * U;                            // groups of a row that an iteration takes, 4 a matrix instruction
     constexpr int kTurn = 16 * kRow * NT + (TURN ? 16 * 4 * kPieces : 0), kPart = (16 * (16 * NT + 1) + 3) / 4;
@@ -184,14 +188,19 @@ __global__ __launch_bounds__(KW * 64) void linear_fp4_stream_kernel(Fp4LinearArg
     }
 }
 
-// More rows: a block of WN KW waves takes 16 NT WN columns of y by 16 MT rows. WN waves share the columns and KW the k of
+// More rows: a block of WN KW waves (two by four) takes 16 NT WN columns of y by 16 MT rows. WN waves share the columns and KW the k of
 // a step, 64 each, so that a wave's products need MT P LDS reads for NT MT P matrix instructions and every weight is
 // converted once. Codes, scales and x are staged in LDS a step ahead, from registers loaded the step before that, x as
 // bf16 (three planes for fp32): loaded in rows, 8 lanes to 128 bytes, read in operand order. Unit u (8 consecutive k) of
 // row m of x lies at u * rows + (m ^ (u & 7)), piece c (32 codes) of row n of W at n * pieces + (c ^ (n & 7)): what
 // 8 lanes write, or read, together lies in different banks. The KW partial sums meet in LDS.
-template <bool F32, int WN, int KW, int NT, int MT>
+//
+// 256 rows of bf16, 8192 x 8192: 40 us, 860 TFLOP/s, two thirds of what a large library product reaches. Of a wave's
+// cycles the matrix cores are busy for 37%, vector instructions 31%, LDS 38%, and one block a CU leaves little to overlap
+// them with; a step staged after its products, or two steps in registers, took 2 to 6 us longer.
+template <bool F32, int NT, int MT>
 struct TileShape {
+    static constexpr int WN = 2, KW = 4;
     static constexpr int P = F32 ? 3 : 1, kRows = 16 * MT, kCols = 16 * NT * WN, kThreads = 64 * WN * KW;
     static constexpr int kK = 64 * KW, kUnits = kK / 8, kPieces = kK / kGroup;
     static constexpr int kX = P * kUnits * kRows, kW = kCols * kPieces, kScales = kCols * kPieces / 16;  // 16-byte units a buffer
@@ -201,12 +210,12 @@ struct TileShape {
     static constexpr __device__ int part_of(int kw, int tile) { return tile - tile / KW - (tile % KW > kw ? 1 : 0); }
     static constexpr size_t kLds = std::max(size_t{2} * kBuffer * 16, size_t{WN} * KW * kParts * 1024);
 };
-template <bool F32, int WN, int KW, int NT, int MT>
-__global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4LinearArgs p, int n_tiles, int m_tiles) {
-    using T = TileShape<F32, WN, KW, NT, MT>;
-    constexpr int P = T::P, kBytes = F32 ? 4 : 2;
+template <bool F32, int NT, int MT>
+__global__ __launch_bounds__((TileShape<F32, NT, MT>::kThreads)) void linear_fp4_tile_kernel(Fp4LinearArgs p, int n_tiles, int m_tiles) {
+    using T = TileShape<F32, NT, MT>;
+    constexpr int WN = T::WN, KW = T::KW, P = T::P, kBytes = F32 ? 4 : 2;
     constexpr int kXLoads = T::kRows * T::kUnits / T::kThreads, kWLoads = (T::kW + T::kThreads - 1) / T::kThreads;
-    static_assert(kXLoads * T::kThreads == T::kRows * T::kUnits && T::kThreads % T::kUnits == 0 && T::kPieces % 8 == 0);
+    static_assert(kXLoads * T::kThreads == T::kRows * T::kUnits && T::kThreads % T::kUnits == 0 && T::kPieces == 8);
     extern __shared__ u32x4 lds[];
     // Blocks of the same columns side by side on one XCD: W comes from memory once, then from that L2.
     const int xcd = blockIdx.x & 7, index = blockIdx.x >> 3;
@@ -225,7 +234,8 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
     const int x_first = static_cast<int>(threadIdx.x) / T::kUnits, x_rows = T::kThreads / T::kUnits;
 
     struct {  // what a thread has loaded of the step that is staged next
-        u32x4 w[kWLoads], scale_bytes, x[kXLoads][F32 ? 2 : 1];
+        u32x4 w[kWLoads], x[kXLoads][F32 ? 2 : 1];
+        u32x2 scale_bytes;
     } ahead;
     auto load = [&](int step) {
         // Past K: the last group's, x is zeroed when it is staged, and that group counts anyway.
@@ -240,18 +250,8 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
         if (static_cast<int>(threadIdx.x) < T::kCols) {
             const uint8_t* const from = scales + static_cast<int64_t>(min(static_cast<int>(threadIdx.x), p.N - 1 - n0)) * groups;
             const int first = step * T::kPieces;
-            if constexpr (T::kPieces == 8) {
-                typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
-                if (first + 8 <= groups) {
-                    const u32x2 v = *reinterpret_cast<const u32x2_any*>(from + first);
-                    ahead.scale_bytes[0] = v[0];
-                    ahead.scale_bytes[1] = v[1];
-                }
-            } else {
-                static_assert(T::kPieces == 16);
-                typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
-                if (first + 16 <= groups) ahead.scale_bytes = *reinterpret_cast<const u32x4_byte*>(from + first);
-            }
+            typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+            if (first + T::kPieces <= groups) ahead.scale_bytes = *reinterpret_cast<const u32x2_any*>(from + first);
             if (first + T::kPieces > groups) {
 #pragma unroll
                 for (int i = 0; i < T::kPieces / 4; ++i) {
@@ -264,7 +264,8 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
         const int kx = min(step * T::kK + 8 * unit, p.K - 8) * kBytes;
 #pragma unroll
         for (int i = 0; i < kXLoads; ++i) {
-            const char* const from = xs + (static_cast<uint32_t>(min(x_first + i * x_rows, p.rows - 1 - m0)) * static_cast<uint32_t>(p.x_stride * kBytes) + kx);
+            const uint32_t row = static_cast<uint32_t>(min(x_first + i * x_rows, p.rows - 1 - m0));
+            const char* const from = xs + (row * static_cast<uint32_t>(p.x_stride * kBytes) + kx);
 #pragma unroll
             for (int j = 0; j < (F32 ? 2 : 1); ++j) ahead.x[i][j] = reinterpret_cast<const u32x4_any*>(from)[j];
         }
@@ -401,22 +402,21 @@ __global__ __launch_bounds__(64 * WN * KW) void linear_fp4_tile_kernel(Fp4Linear
     }
 }
 
-template <bool F32, int WN, int KW, int NT, int MT>
+template <bool F32, int NT, int MT>
 void launch_tile(const Fp4LinearArgs& p, hipStream_t s) {
-    using T = TileShape<F32, WN, KW, NT, MT>;
+    using T = TileShape<F32, NT, MT>;
     static_assert(T::kLds <= 160 * 1024);
     const int64_t n_tiles = ceil_div(p.N, T::kCols), m_tiles = ceil_div(p.rows, T::kRows);
-    hipLaunchKernelGGL((linear_fp4_tile_kernel<F32, WN, KW, NT, MT>), dim3(static_cast<unsigned>(8 * ceil_div(n_tiles, 8) * m_tiles)),
+    hipLaunchKernelGGL((linear_fp4_tile_kernel<F32, NT, MT>), dim3(static_cast<unsigned>(8 * ceil_div(n_tiles, 8) * m_tiles)),
                        dim3(T::kThreads), T::kLds, s, p, static_cast<int>(n_tiles), static_cast<int>(m_tiles));
 }
 template <bool F32, int NT>
 void launch_stream(const Fp4LinearArgs& p, hipStream_t s) {
-    constexpr int KW = 8, U = 2;
     const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 16 * NT)), static_cast<unsigned>(ceil_div(p.rows, 16)));
     if (p.rows <= kFew) {
-        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, false, KW, NT, U>), grid, dim3(KW * 64), 0, s, p);
+        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, false, NT>), grid, dim3(kWaves * 64), 0, s, p);
     } else {
-        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, true, KW, NT, U>), grid, dim3(KW * 64), 0, s, p);
+        hipLaunchKernelGGL((linear_fp4_stream_kernel<F32, true, NT>), grid, dim3(kWaves * 64), 0, s, p);
     }
 }
 
@@ -445,13 +445,14 @@ void launch(const Fp4LinearArgs& p, hipStream_t s) {
     const bool offsets_fit = p.x_stride < (int64_t{1} << 24);  // a tile's rows of x are addressed in 32 bits
     const bool few = p.rows <= kFew;
     if constexpr (F32) {
-        if (offsets_fit && 30 * rounds(128, 32) < 12 * full(64)) return launch_tile<true, 2, 4, 4, 2>(p, s);
+        if (offsets_fit && 30 * rounds(128, 32) < 12 * full(64)) return launch_tile<true, 4, 2>(p, s);
         const double by16 = (few ? 5.2 : 6.7) * rounds(16, 16), by32 = (few ? 6.8 : 8.1) * rounds(32, 16), by64 = (few ? 9.5 : 11.6) * rounds(64, 16);
         if (by64 < std::min(by16, by32)) return launch_stream<true, 4>(p, s);
         by16 <= by32 ? launch_stream<true, 1>(p, s) : launch_stream<true, 2>(p, s);
     } else {
         const double stream = 3.7 * full(32), narrow = 15.5 * rounds(64, 64), wide = 22 * rounds(128, 64);
-        if (offsets_fit && std::min(narrow, wide) < stream) return narrow < wide ? launch_tile<false, 2, 4, 2, 4>(p, s) : launch_tile<false, 2, 4, 4, 4>(p, s);
+        if (offsets_fit && std::min(narrow, wide) < stream)
+            return narrow < wide ? launch_tile<false, 2, 4>(p, s) : launch_tile<false, 4, 4>(p, s);
         (few ? 2.9 : 4.0) * rounds(16, 16) <= (few ? 3.8 : 4.9) * rounds(32, 16) ? launch_stream<false, 1>(p, s) : launch_stream<false, 2>(p, s);
     }
 }
@@ -473,7 +474,8 @@ extern "C" mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_fea
     MLK_CHECK(x && codes && scales && out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
               "codes and out must be 16-byte aligned");
-    Fp4LinearArgs p{x, x_stride, codes, scales, bias, out, static_cast<int32_t>(rows), static_cast<int32_t>(in_features), static_cast<int32_t>(out_features)};
+    Fp4LinearArgs p{x, x_stride, codes, scales, bias, out, static_cast<int32_t>(rows), static_cast<int32_t>(in_features),
+                    static_cast<int32_t>(out_features)};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (dtype == MLK_DTYPE_F32) {
         launch<true>(p, s);
