@@ -442,7 +442,8 @@ mlk_status mlk_mamba3_siso_step(const float* projected, int64_t streams, int64_t
  * anything. Both are contiguous int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes, 16-byte aligned, page_size a
  * multiple of 16 up to 1024, head_dim 32, 64, 128 or 256. A (page, head) holds key codes [page_size][head_dim / 2], value
  * codes [head_dim / 2][page_size], key scales [page_size][head_dim / 32], value scales [head_dim / 32][page_size].
- * Strides are {sequence, token, head} in elements, head_dim dense. */
+ * Strides are {sequence, token, head} in elements, head_dim dense. A call that needs 2^32 threads or more is refused: 2^26
+ * head rows of a norm, 2^29 of an append or a read, 2^27 query head rows of an attention. */
 
 /* RMSNorm over head_dim of every head of q [batch, length, heads, head_dim] and k [.., kv_heads, ..], each with its fp32
  * weight [head_dim], then the rotation (rotate_half, as mlk_mla_rope_qk) of the last rope_dim lanes by the tables' row
@@ -484,7 +485,7 @@ mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dt
 
 /* y [rows, out_features] = x W^T + bias with four-bit weights: codes [out_features, in_features / 2] (16-byte aligned),
  * scales [out_features, in_features / 32], bias fp32 or NULL. x rows `x_stride` elements apart; y contiguous, of x's
- * dtype. in_features: a multiple of 32 below 2^24; out_features below 2^26. */
+ * dtype. in_features: a multiple of 32 below 2^24; out_features below 2^26; rows below 2^20 - 16, y up to 2^34 elements. */
 mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int64_t x_stride, int32_t dtype,
                           const uint8_t* codes, const uint8_t* scales, const float* bias, int64_t out_features, void* out,
                           mlk_stream_t stream);

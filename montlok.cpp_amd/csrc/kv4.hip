@@ -1117,6 +1117,8 @@ mlk_status cache_of(Cache& c, uint8_t* bytes, int64_t pages, int64_t page_size, 
     return MLK_OK;
 }
 
+constexpr int64_t kThreads = int64_t{1} << 32;  // a launch's threads stay below
+
 // Rows of all (sequence, key head) pairs below 2^31: every count of the plan then fits.
 bool rows_fit(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads) {
     if (batch <= 0 || length <= 0 || kv_heads <= 0) return true;  // nothing to do, or refused as geometry
@@ -1129,6 +1131,8 @@ struct Plan {
     int64_t splits, rows, part_rows;
     bool many;  // kv4_attention_rows_kernel
     size_t bytes;
+
+    int64_t row_tiles(bool f32) const { return ceil_div(rows, many ? 16 * W * (f32 ? kRowTiles<true> : kRowTiles<false>) : 16); }
 };
 // Few blocks are split over the keys, as far as the chip takes them at once (256 blocks of eight waves, 512 with heads up to
 // 64; a second round of them cost more than uneven shares: 131072 keys, 8 key heads 67 us with 512 blocks, 39 with 256), a
@@ -1166,7 +1170,7 @@ Plan plan_of(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int
 
 template <int D, bool F32>
 void launch_attention(AttentionArgs p, const Plan& t, hipStream_t s) {
-    p.row_tiles = static_cast<int32_t>(ceil_div(t.rows, t.many ? 16 * W * kRowTiles<F32> : 16));
+    p.row_tiles = static_cast<int32_t>(t.row_tiles(F32));
     const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * p.row_tiles * t.splits;
     if (t.many) {
         if constexpr (D == kSharedDim) hipLaunchKernelGGL(kv4_attention_rows_kernel<F32>, dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
@@ -1200,7 +1204,7 @@ extern "C" mlk_status mlk_kv4_append(const void* k, const int64_t* k_strides, co
     if (status != MLK_OK || batch == 0 || length == 0) return status;
     MLK_CHECK(k && k_strides && v && v_strides, "null tensor pointer");
     const int64_t waves = ceil_div(batch * length, 16) * kv_heads * 2;
-    MLK_CHECK(waves < (int64_t{1} << 33), "too many tokens for one launch");
+    MLK_CHECK(ceil_div(waves, 4) * 256 < kThreads, "too many tokens for one launch");
     const Rows3 kr{k, k_strides[0], k_strides[1], k_strides[2]}, vr{v, v_strides[0], v_strides[1], v_strides[2]};
     by_dim(head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
@@ -1222,7 +1226,7 @@ extern "C" mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t 
     MLK_CHECK(k && v, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(k) & 15) == 0 && (reinterpret_cast<uintptr_t>(v) & 15) == 0, "k and v must be 16-byte aligned");
     const int64_t waves = ceil_div(batch * length, 16) * kv_heads * 2;
-    MLK_CHECK(waves < (int64_t{1} << 33), "too many tokens for one launch");
+    MLK_CHECK(ceil_div(waves, 4) * 256 < kThreads, "too many tokens for one launch");
     by_dim(head_dim, [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_read_kernel<D, true> : kv4_read_kernel<D, false>;
@@ -1255,7 +1259,7 @@ extern "C" mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides,
     MLK_CHECK(q && q_strides && out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(out) & 15) == 0, "out must be 16-byte aligned");
     const Plan t = plan_of(batch, length, heads, kv_heads, head_dim, page_size * table_width);
-    MLK_CHECK(batch * kv_heads * ceil_div(t.rows, 16) * t.splits < (int64_t{1} << 31), "too many tokens for one launch");
+    MLK_CHECK(batch * kv_heads * t.row_tiles(dtype == MLK_DTYPE_F32) * t.splits * (64 * W) < kThreads, "too many tokens for one launch");
     MLK_CHECK(workspace_bytes >= t.bytes && (t.bytes == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)),
               "workspace must be 16-byte aligned and hold mlk_kv4_attention_workspace_bytes");
     p.q = q;

@@ -468,7 +468,9 @@ extern "C" mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_fea
     MLK_CHECK(dtype == MLK_DTYPE_F32 || dtype == MLK_DTYPE_BF16, "dtype must be f32 or bf16");
     MLK_CHECK(rows >= 0 && out_features > 0, "invalid linear geometry");
     MLK_CHECK(in_features > 0 && in_features % kGroup == 0, "in_features must be a positive multiple of 32");
-    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 24) && out_features < (int64_t{1} << 26), "too many rows or features");
+    MLK_CHECK(rows < (int64_t{1} << 20) - 16 && in_features < (int64_t{1} << 24) && out_features < (int64_t{1} << 26) &&
+                  rows * out_features <= (int64_t{1} << 34),
+              "too many rows or features");  // the grids: 65,535 blocks along y, 2^32 threads along x
     MLK_CHECK(x_stride >= 0, "x_stride must not be negative");
     if (rows == 0) return MLK_OK;
     MLK_CHECK(x && codes && scales && out, "null tensor pointer");

@@ -201,7 +201,7 @@ void launch_vec(const NormArgs& p, hipStream_t s) {
 template <bool F32>
 bool launch_vec(const NormArgs& p, hipStream_t s) {
     constexpr int E = F32 ? 4 : 8;
-    if (p.rope / 2 % E != 0 || p.dim % E != 0 || p.tokens * (p.heads + p.kv_heads) >= (int64_t{1} << 31)) return false;
+    if (p.rope / 2 % E != 0 || p.dim % E != 0) return false;
     switch (p.dim / E) {
         case 4: launch_vec<F32, 4>(p, s); return true;
         case 8: launch_vec<F32, 8>(p, s); return true;
@@ -229,7 +229,7 @@ extern "C" mlk_status mlk_qk_norm_rope(const void* q, const int64_t* q_strides, 
     MLK_CHECK(heads < (int64_t{1} << 20) && kv_heads < (int64_t{1} << 20), "too many heads");
     MLK_CHECK(batch < (int64_t{1} << 31) && length < (int64_t{1} << 31) && batch * length < (int64_t{1} << 36), "too many tokens");
     const int64_t blocks = ceil_div(batch * length * (heads + kv_heads), 4);
-    MLK_CHECK(blocks < (int64_t{1} << 31), "too many tokens for one launch");
+    MLK_CHECK(blocks < (int64_t{1} << 24), "too many tokens for one launch");  // of 256 threads: below 2^32
     if (batch == 0 || length == 0) return MLK_OK;
     MLK_CHECK(q && q_strides && k && k_strides && q_weight && k_weight && positions && q_out && k_out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(q_out) & 15) == 0 && (reinterpret_cast<uintptr_t>(k_out) & 15) == 0, "outputs must be 16-byte aligned");

@@ -167,3 +167,24 @@ def test_weights_that_do_not_fit_are_refused(w):
 
     with pytest.raises(RuntimeError, match="weight must be"):
         _C.fp4_weights(w)
+
+
+def test_calls_past_a_launch_are_refused(lib):
+    """More threads than a grid holds, with pointers that nothing reads before the refusal."""
+    memory = (C.c_uint8 * 64)()
+    at = C.c_void_p((C.addressof(memory) + 15) & ~15)
+    strides = (C.c_int64 * 3)(64, 64, 64)
+    for status in (
+            lib.mlk_kv4_append(at, strides, at, strides, 1, 1, 2 ** 26, 8, 64, at, 4, 64, at, 2, at, None),
+            lib.mlk_kv4_read(at, 4, 64, at, 2, at, 1, 2 ** 26, 8, 64, 1, at, at, None),
+            lib.mlk_kv4_attention(at, strides, 1, 1, 2 ** 24, 16, 16, 64, at, 4, 64, at, 2, at, 1.0, at, None, 0, None),
+            lib.mlk_qk_norm_rope(at, strides, at, strides, 1, at, at, 1e-5, at, at, 8, 4, at, 1, 2 ** 22, 32, 8, 64, at, at, None),
+            lib.mlk_linear_fp4(at, 2 ** 19, 64, 64, 1, at, at, None, 2 ** 16, at, None)):
+        assert status == 1 and "too many" in lib.mlk_last_error().decode()
+
+
+def test_negative_row_strides_are_refused(lib):
+    memory = (C.c_uint8 * 64)()
+    at = C.c_void_p((C.addressof(memory) + 15) & ~15)
+    assert lib.mlk_linear_fp4(at, 2, 64, -64, 1, at, at, None, 8, at, None) == 1
+    assert "x_stride" in lib.mlk_last_error().decode()
