@@ -653,8 +653,8 @@ def fp4_weights(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     size = torch.where(fine, groups, 0.0).abs()
     # most = m 2^e with m in [0.5, 1) and 6 = 0.75 * 2^3: the power is e - 3 up to 0.75 and e - 2 above.
     m, e = torch.frexp(size.amax(-1, keepdim=True))
-    byte = torch.where(m == 0, 3, (e + 124 + (m > 0.75)).clamp(3, 252))
-    size = torch.ldexp(size, 127 - byte)
+    byte = torch.where(m == 0, 3, (e + 124 + (m > 0.75)).clamp(3, 252)).int()
+    size = size * (254 - byte << 23).view(torch.float32)  # 2^(127 - byte)
     # Halves between two codes go to the even one.
     code = ((size > 0.25).int() + (size >= 0.75) + (size > 1.25) + (size >= 1.75) + (size > 2.5) + (size >= 3.5) + (size > 5.0))
     code = torch.where(fine, code + 8 * torch.signbit(groups), 0).to(torch.uint8).flatten(1)

@@ -155,3 +155,19 @@ def test_graph_replays(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, _C.linear_fp4(x, codes, scales)), f"replay {replay}"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weights_are_quantised_alike_on_the_gpu(dev, dtype):
+    """The codes and scales of weights on the GPU are those of the same weights on the CPU, and ``linear_fp4`` of the unit
+    rows gives their values back."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(47)
+    w = (torch.randn(130, 192, generator=g) * 2.0 ** torch.randint(-30, 30, (130, 1), generator=g)).to(dtype)
+    w[3, :32], w[4, 32:64] = 0.0, 2.0 ** -100
+    codes, scales = _C.fp4_weights(w)
+    on_gpu = _C.fp4_weights(w.to(dev))
+    assert torch.equal(on_gpu[0].cpu(), codes) and torch.equal(on_gpu[1].cpu(), scales)
+    got = _C.linear_fp4(torch.eye(192, dtype=dtype, device=dev), *on_gpu)
+    assert torch.equal(got.cpu().double(), ref.nearest(w).t())
