@@ -135,12 +135,12 @@ struct Place {
     int offset;
     bool run;
 };
-__device__ __forceinline__ Place place_of(const Cache& c, int64_t token, int head) {
+__device__ __forceinline__ Place place_of(const Cache& c, uint32_t token, uint32_t b, int head) {
     Place p{nullptr, 0, false};
     const int i = (threadIdx.x >> 2) & 3;
-    if (token < static_cast<int64_t>(c.batch) * c.length) {
+    if (token < static_cast<uint32_t>(c.batch) * static_cast<uint32_t>(c.length)) {
         const int at = c.positions[token];
-        if (at >= 0) p.record = record_of(c, static_cast<int>(token / c.length), at, head, p.offset);
+        if (at >= 0) p.record = record_of(c, static_cast<int>(b), at, head, p.offset);
     }
     bool same = p.record != nullptr && (p.offset & 3) == i;
 #pragma unroll
@@ -156,20 +156,21 @@ __device__ __forceinline__ Place place_of(const Cache& c, int64_t token, int hea
 }
 
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, Rows3 k, Rows3 v, int64_t waves) {
+__global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, Rows3 k, Rows3 v, uint32_t waves) {
     constexpr int S = D / 32;
     using Scales = typename Bytes<S>::type;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if (id >= waves) return;
     const bool values = id & 1;
-    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) % c.kv_heads);
-    const int64_t token = (id >> 1) / c.kv_heads * 16 + (lane >> 2), all = static_cast<int64_t>(c.batch) * c.length, held = min(token, all - 1);
+    const uint32_t tile = (id >> 1) / static_cast<uint32_t>(c.kv_heads), length = static_cast<uint32_t>(c.length);
+    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) - tile * c.kv_heads);
+    const uint32_t token = tile * 16 + (lane >> 2), held = min(token, c.batch * length - 1), b = held / length;
     const Rows3& r = values ? v : k;
-    const int64_t b = held / c.length, from = b * r.bs + (held - b * c.length) * r.ts + head * r.hs + 8 * q;
+    const int64_t from = b * r.bs + static_cast<int64_t>(held - b * length) * r.ts + head * r.hs + 8 * q;
     float x[S][8];
 #pragma unroll
     for (int s = 0; s < S; ++s) load8<F32>(r.p, from + 32 * s, x[s]);
-    const Place place = place_of(c, token, head);
+    const Place place = place_of(c, token, b, head);
     uint32_t codes[S];
     uint64_t bytes = 0;
 #pragma unroll
@@ -222,15 +223,16 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, Rows3 k, Rows3
 }
 
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, void* k, void* v, int64_t waves) {
+__global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, void* k, void* v, uint32_t waves) {
     constexpr int S = D / 32;
     using Scales = typename Bytes<S>::type;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if (id >= waves) return;
     const bool values = id & 1;
-    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) % c.kv_heads);
-    const int64_t token = (id >> 1) / c.kv_heads * 16 + (lane >> 2), all = static_cast<int64_t>(c.batch) * c.length;
-    const Place place = place_of(c, token, head);
+    const uint32_t tile = (id >> 1) / static_cast<uint32_t>(c.kv_heads), length = static_cast<uint32_t>(c.length);
+    const int lane = threadIdx.x & 63, q = lane & 3, i = lane >> 2 & 3, head = static_cast<int>((id >> 1) - tile * c.kv_heads);
+    const uint32_t token = tile * 16 + (lane >> 2), all = c.batch * length;
+    const Place place = place_of(c, token, token / length, head);
     const int64_t half = static_cast<int64_t>(c.page_size) * (D / 2);
     uint32_t codes[S];
     uint64_t bytes = 0;
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, void* k, void* v
     }
     if (token >= all) return;
     if (place.record == nullptr) bytes = c.positions[token] < 0 ? 0 : ~uint64_t{0};  // zero codes, or NaN
-    const int64_t to = (token * c.kv_heads + head) * D + 8 * q;
+    const int64_t to = (static_cast<int64_t>(token) * c.kv_heads + head) * D + 8 * q;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const bf16x8 x = fp4_octet(codes[s], scale_of(static_cast<uint32_t>(bytes >> (8 * s)) & 0xFF));
@@ -1210,7 +1212,7 @@ extern "C" mlk_status mlk_kv4_append(const void* k, const int64_t* k_strides, co
         constexpr int D = decltype(dim)::value;
         const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_append_kernel<D, true> : kv4_append_kernel<D, false>;
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0,
-                           reinterpret_cast<hipStream_t>(stream), c, kr, vr, waves);
+                           reinterpret_cast<hipStream_t>(stream), c, kr, vr, static_cast<uint32_t>(waves));
     });
     return launch_status("kv4 append");
 }
@@ -1231,7 +1233,7 @@ extern "C" mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t 
         constexpr int D = decltype(dim)::value;
         const auto kernel = dtype == MLK_DTYPE_F32 ? kv4_read_kernel<D, true> : kv4_read_kernel<D, false>;
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(waves, 4))), dim3(256), 0,
-                           reinterpret_cast<hipStream_t>(stream), c, k, v, waves);
+                           reinterpret_cast<hipStream_t>(stream), c, k, v, static_cast<uint32_t>(waves));
     });
     return launch_status("kv4 read");
 }

@@ -27,7 +27,7 @@ struct NormArgs {
     const float* cosine;
     const float* sine;
     const int32_t* positions;
-    int64_t table_rows, tokens, length;
+    int64_t table_rows, tokens, length;  // tokens below 2^26
     int32_t heads, kv_heads, dim, rope;
     double eps;
 };
@@ -69,18 +69,18 @@ template <bool F32, int LPG, int R>
 __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsigned chunks, unsigned q_chunks) {
     constexpr int E = F32 ? 4 : 8, D = LPG * E, G = 64 / LPG;
     const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int64_t token = wave / chunks;
+    const unsigned token = wave / chunks;  // below 2^26, as a launch's waves
     if (token >= p.tokens) return;
-    const unsigned chunk = wave - static_cast<unsigned>(token) * chunks;
+    const unsigned chunk = wave - token * chunks, length = static_cast<unsigned>(p.length), b = token / length;
     const bool query = chunk < q_chunks;
     const Head& t = query ? p.q : p.k;
     const int rows = query ? p.heads : p.kv_heads;
     const int lane = threadIdx.x & 63, d = lane % LPG * E, first = static_cast<int>(query ? chunk : chunk - q_chunks) * (G * R) + lane / LPG;
-    const int64_t at = p.positions[token], b = token / p.length;
+    const int64_t at = p.positions[token];
     const int nope = D - p.rope, half = p.rope / 2;
     const bool turned = d >= nope, upper = d >= nope + half, inside = at >= 0 && at < p.table_rows;
     const int other = !turned ? d : upper ? d - half : d + half;
-    const int64_t from = b * t.bs + (token - b * p.length) * t.ts;
+    const int64_t from = b * t.bs + static_cast<int64_t>(token - b * length) * t.ts;
     u32x4 x[R], y[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsig
 #pragma unroll
             for (int i = 0; i < E; ++i) out[i] = at < 0 ? 0.0f : NAN;
         }
-        const int64_t to = (token * rows + row) * D + d;
+        const int64_t to = (static_cast<int64_t>(token) * rows + row) * D + d;
         if constexpr (F32) {
             *reinterpret_cast<f32x4*>(static_cast<float*>(t.out) + to) = f32x4{out[0], out[1], out[2], out[3]};
         } else {
@@ -146,14 +146,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsig
 template <bool F32>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormArgs p) {
     const int per_token = p.heads + p.kv_heads, lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
-    const int64_t token = row / per_token;
+    const unsigned row = blockIdx.x * 4 + threadIdx.x / 64, token = row / static_cast<unsigned>(per_token);
     if (token >= p.tokens) return;
     const int which = static_cast<int>(row - token * per_token), head = which < p.heads ? which : which - p.heads;
     const Head& t = which < p.heads ? p.q : p.k;
-    const int64_t b = token / p.length;
-    const int64_t from = b * t.bs + (token - b * p.length) * t.ts + head * t.hs;
-    const int64_t to = (token * (which < p.heads ? p.heads : p.kv_heads) + head) * p.dim;
+    const unsigned length = static_cast<unsigned>(p.length), b = token / length;
+    const int64_t from = b * t.bs + static_cast<int64_t>(token - b * length) * t.ts + head * t.hs;
+    const int64_t to = (static_cast<int64_t>(token) * (which < p.heads ? p.heads : p.kv_heads) + head) * p.dim;
     double sum = 0.0;
     for (int d = lane; d < p.dim; d += 64) {
         const double v = Element<F32>::get(t.x, from + d);
