@@ -295,6 +295,13 @@ struct AttentionArgs {
     int64_t part_rows;
 };
 
+// Of 16 lanes each: `v` of the lane 4, 8 or 12 below (kUp) or above (kDown), or 4 or 8 around, in the lanes of the
+// quarters that `kQuarters` names; `old` elsewhere, 0 past the ends.
+constexpr int kDown4 = 0x104, kDown8 = 0x108, kDown12 = 0x10C, kUp4 = 0x114, kUp8 = 0x118, kUp12 = 0x11C, kAround4 = 0x124, kAround8 = 0x128;
+template <int kMove, int kQuarters>
+__device__ __forceinline__ float from_lanes(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), kMove, 0xF, kQuarters, true));
+}
 __device__ __forceinline__ float max_over_groups(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, kWave));
     return fmaxf(v, __shfl_xor(v, 32, kWave));
@@ -318,9 +325,9 @@ struct TileLds {
 
 // A block takes 16 rows of a (sequence, key head) and every p.splits-th group of W tiles of 64 keys, a tile a wave.
 //
-// Bound by memory with 8 waves of bf16 (64 sequences of 10000 keys, 8 key heads of 128: 132 us, 5.3 TB/s), by the issue of
-// some 500 vector instructions a tile in fp32 (182 us, 3.8 TB/s: three planes of each weight) and below 64 elements (4 a
-// key pair to convert, turn and scale); one tile a wave alone takes about 5 us, most of it waiting for memory.
+// Bound by memory in bf16 (64 sequences of 10000 keys, 32 heads on 8 of 128: 127 us, 5.5 TB/s), by the latencies of some
+// 400 vector and 96 matrix instructions a tile in fp32 (172 us, 4.0 TB/s: three planes of each query and weight), with the
+// two waves a SIMD that the registers allow; one tile a wave alone takes about 5 us, most of it waiting for memory.
 //
 // Scores are key tile x q^T, so that lane (g, l) holds row l's scores of 16 tokens, in the registers from which the
 // product with the values takes its weights: nothing moves between lanes but the maximum (a column's sum is formed at
@@ -328,7 +335,10 @@ struct TileLds {
 // every tile) are its 16 tokens 16 g .. 16 g + 15 of the value product.
 // WHOLE: pages of whole tiles. A tile then has one page, and its addresses are scalar. Not for D = 256, where the
 // registers that this takes are spilled (64 x 4000 keys of 8 heads, fp32: 161 against 138 us).
-template <int D, bool F32, bool WHOLE>
+// FEW: up to four rows, a token of as many query heads a key head. 12 of 16 columns of a product are then idle, and their
+// lanes take three quarters of the rows' softmax (64 x 10000 keys, fp32 181 -> 172 us; 16 x 16000 of 8 heads of 64, fp32
+// 45 -> 41; of 32, bf16 22 -> 20).
+template <int D, bool F32, bool WHOLE, bool FEW>
 __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void kv4_attention_kernel(AttentionArgs p) {
     constexpr int S = D / 32;       // k steps of a score product, groups of a token, 1 KB loads of a tile's keys (or values)
     constexpr int P = F32 ? 3 : 1;  // bf16 operands that make up a query or a weight
@@ -553,39 +563,86 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
 #pragma unroll
             for (int i = 0; i < 16; ++i) score[i / 4][i % 4] = first + 16 * g + i > position ? -INFINITY : score[i / 4][i % 4];
         }
-        float most = -INFINITY;
+        // Scores to weights 2^(scale (score - top)), `top` the largest of a row so far.
+        auto soften = [&](auto& v, auto over_lanes) {
+            float most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[i / 4][i % 4]);
-        const float now = fmaxf(top, max_over_groups(most));
-        if (__ballot(now != top) != 0) {  // seldom after the first tiles
-            const float shrink = __builtin_amdgcn_exp2f(fmaf(top, scale, -finite_or_zero(now) * scale));
-            top = now;
-            sum *= shrink;
+            for (float x : v) most = fmaxf(most, x);
+            const float now = fmaxf(top, max_over_groups(over_lanes(most)));
+            if (__ballot(now != top) != 0) {  // seldom after the first tiles
+                const float shrink = __builtin_amdgcn_exp2f(fmaf(top, scale, -finite_or_zero(now) * scale));
+                top = now;
+                sum *= shrink;
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                acc[s][0] *= shrink;
-                acc[s][1] *= shrink;
+                for (int s = 0; s < S; ++s) {
+                    acc[s][0] *= shrink;
+                    acc[s][1] *= shrink;
+                }
             }
-        }
-        bf16x8 weight[P][2];
-        const float base = finite_or_zero(top) * scale;
+            const float base = finite_or_zero(top) * scale;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(fmaf(score[2 * h + i / 4][i % 4], scale, -base));
-                sum += w[i];
+            for (float& x : v) {
+                x = __builtin_amdgcn_exp2f(fmaf(x, scale, -base));
+                sum += x;
             }
+        };
+        // Eight weights as operands. fp32: of finite values, or NaN. bf16: rounded to nearest, 2^-9 of a weight, which a mean
+        // over many keys loses; the sum is of the unrounded.
+        auto operand_of = [&](const float (&w)[8], bf16x8 (&to)[P]) {
             if constexpr (F32) {
-                bf16x8 plane[3];
-                planes_of<false>(w, plane);  // of finite values, or NaN
-#pragma unroll
-                for (int i = 0; i < 3; ++i) weight[i][h] = plane[i];
+                planes_of<false>(w, to);
             } else {
-                // Rounded to nearest: 2^-9 of a weight, which a mean over many keys loses; the sum is of the unrounded.
 #pragma unroll
-                for (int i = 0; i < 8; ++i) weight[0][h][i] = static_cast<__bf16>(w[i]);
+                for (int i = 0; i < 8; ++i) to[0][i] = static_cast<__bf16>(w[i]);
+            }
+        };
+        bf16x8 weight[P][2];
+        if constexpr (FEW) {
+            // Lane 4 a + r of 16 takes row r's scores of key tile a from lane r, and gives its weights back.
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = score[0][i];
+                v[i] = from_lanes<kUp4, 2>(v[i], score[1][i]);
+                v[i] = from_lanes<kUp8, 4>(v[i], score[2][i]);
+                v[i] = from_lanes<kUp12, 8>(v[i], score[3][i]);
+            }
+            soften(v, [](float most) {
+                most = fmaxf(most, from_lanes<kAround4, 15>(most, most));
+                return fmaxf(most, from_lanes<kAround8, 15>(most, most));
+            });
+            const float both[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+            bf16x8 mine_of[P];
+            operand_of(both, mine_of);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const u32x4 w = __builtin_bit_cast(u32x4, mine_of[i]);
+                u32x4 first, second;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float x = __uint_as_float(w[j]);
+                    first[j] = w[j];
+                    first[2 + j] = __float_as_uint(from_lanes<kDown4, 15>(0.0f, x));
+                    second[j] = __float_as_uint(from_lanes<kDown8, 15>(0.0f, x));
+                    second[2 + j] = __float_as_uint(from_lanes<kDown12, 15>(0.0f, x));
+                }
+                weight[i][0] = __builtin_bit_cast(bf16x8, first);
+                weight[i][1] = __builtin_bit_cast(bf16x8, second);
+            }
+        } else {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = score[i / 4][i % 4];
+            soften(v, [](float most) { return most; });
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i];
+                bf16x8 to[P];
+                operand_of(w, to);
+#pragma unroll
+                for (int i = 0; i < P; ++i) weight[i][h] = to[i];
             }
         }
 
@@ -641,6 +698,10 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
     // The waves' parts joined: each writes its own, wave s adds up elements 32 s .. 32 s + 31 of the rows.
     __syncthreads();
     auto& stats = lds.end.stats;
+    if constexpr (FEW) {
+        sum += __shfl_xor(sum, 4, kWave);
+        sum += __shfl_xor(sum, 8, kWave);
+    }
     sum = sum_over_groups(sum);
     if (g == 0) {
         stats[wave][0][l] = top;
@@ -1176,10 +1237,17 @@ void launch_attention(AttentionArgs p, const Plan& t, hipStream_t s) {
     const int64_t blocks = int64_t{p.c.batch} * p.c.kv_heads * p.row_tiles * t.splits;
     if (t.many) {
         if constexpr (D == kSharedDim) hipLaunchKernelGGL(kv4_attention_rows_kernel<F32>, dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
-    } else if (D < 256 && p.c.runs % 4 == 0) {
-        if constexpr (D < 256) hipLaunchKernelGGL((kv4_attention_kernel<D, F32, true>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
     } else {
-        hipLaunchKernelGGL((kv4_attention_kernel<D, F32, false>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
+        auto launch = [&](auto whole, auto few) {
+            constexpr bool kWhole = decltype(whole)::value, kFew = decltype(few)::value;
+            hipLaunchKernelGGL((kv4_attention_kernel<D, F32, kWhole, kFew>), dim3(static_cast<unsigned>(blocks)), dim3(W * 64), 0, s, p);
+        };
+        auto by_rows = [&](auto whole) { t.rows <= 4 ? launch(whole, std::true_type{}) : launch(whole, std::false_type{}); };
+        if (D < 256 && p.c.runs % 4 == 0) {
+            by_rows(std::bool_constant<D < 256>{});
+        } else {
+            by_rows(std::false_type{});
+        }
     }
     if (t.splits == 1) return;
     const int64_t rows = t.part_rows / t.splits;
