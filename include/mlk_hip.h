@@ -473,9 +473,10 @@ mlk_status mlk_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, 
 /* softmax(q k^T * scale) v of q [batch, length, heads, head_dim] over the cached keys 0 .. position of each token (heads
  * a multiple of kv_heads: query head h reads key head h * kv_heads / heads). out: contiguous, 16-byte aligned. A token at
  * a negative position sees no key and gives zeros; one past the page table, or that sees a key on a page outside
- * [0, pages), gives NaN. What the cache holds behind a token's position does not reach it. fp32 q runs with fp32
- * accuracy, bf16 q with the softmax weights rounded to bf16 for the value product. The workspace is 16-byte aligned and
- * private to the call until it has run. */
+ * [0, pages), gives NaN. What the cache holds behind a token's position, of any bytes, does not reach it; a group of
+ * values under byte 253 or 254 that a token sees may count as NaN. fp32 q runs with fp32 accuracy, bf16 q with the
+ * softmax weights rounded to bf16 for the value product. The workspace is 16-byte aligned and private to the call until
+ * it has run. */
 size_t mlk_kv4_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                          int64_t page_size, int64_t table_width);
 mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dtype, int64_t batch, int64_t length,

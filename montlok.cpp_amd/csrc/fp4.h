@@ -23,6 +23,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kGroup = 32;  // values under one scale
+constexpr uint32_t kMostScale = 252;  // the largest byte whose values are all finite in bf16 (6 * 2^126 is 1.5 * 2^128)
 
 // The float whose exponent bits are the scale byte: what the conversions take as scale.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }

@@ -651,11 +651,11 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
         for (int s = 0; s < S; ++s) {
             u32x4 vs = reinterpret_cast<const u32x4*>(mine.value_scale)[4 * s + g];
             if (masked) {
-                // A value that no row may see must not reach a sum as 0 * NaN: its NaN scale goes, and the rows that do see
-                // it are made NaN below.
+                // A value that no row may see must not reach a sum as 0 * NaN, or 0 * infinity (values under bytes 253 and
+                // 254 can pass bf16's largest): such a scale goes, and the rows that do see it are made NaN below.
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if ((vs[i / 4] >> (8 * (i % 4)) & 0xFF) == 0xFF) {
+                    if ((vs[i / 4] >> (8 * (i % 4)) & 0xFF) > kMostScale) {
                         vs[i / 4] &= ~(0xFFu << (8 * (i % 4)));
                         if (first + 16 * g + i <= position) poison |= 1u << s;
                     }
@@ -776,7 +776,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
     };
     __shared__ Raw raw[2];
     __shared__ bf16x8 key_lds[2][kKeyUnits][64], value_lds[2][kValueUnits][2][64];
-    __shared__ int nan_tile[2];  // the last tile of the buffer that held a NaN value group, plus one
+    __shared__ int nan_tile[2];  // the last tile of the buffer that held a value group under a byte above kMostScale, plus one
     __shared__ int wave_last[W];
     const Cache& c = p.c;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
@@ -862,13 +862,13 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
         for (int w = 0; w < 2; ++w) {
             const uint32_t code = codes[w];
             uint32_t scales = scales_of[w];
-            // A NaN group must not meet the weight 0 of a row that does not see it: it counts as small here, and the
-            // rows that see it are made NaN by themselves.
-            if (((scales & 0x7F7F7F7Fu) + 0x01010101u) & scales & 0x80808080u) {
+            // A NaN group, or one that may hold infinities, must not meet the weight 0 of a row that does not see it: it
+            // counts as small here, and the rows that see it are made NaN by themselves.
+            if (((scales & 0x7F7F7F7Fu) + 0x01010101u * (0x7F - (kMostScale & 0x7F))) & scales & 0x80808080u) {
                 nan = true;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if ((scales >> (8 * e) & 0xFF) == 0xFF) scales &= ~(0xFFu << (8 * e));
+                    if ((scales >> (8 * e) & 0xFF) > kMostScale) scales &= ~(0xFFu << (8 * e));
             }
             pair[4 * w] = fp4_pair<0>(code, scale_at<0>(scales));
             pair[4 * w + 1] = fp4_pair<1>(code, scale_at<1>(scales));
@@ -1045,7 +1045,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_rows_kernel(Attention
                     for (int s = 0; s < S; ++s) {
                         int poison = 0;
                         for (int i = 0; i < 16; ++i)
-                            if (first + 16 * g + i <= position[m] && scales[(S + s) * c.page_size + static_cast<int>(token) + i] == 0xFF) poison = 1;
+                            if (first + 16 * g + i <= position[m] && scales[(S + s) * c.page_size + static_cast<int>(token) + i] > kMostScale) poison = 1;
                         poison |= __shfl_xor(poison, 16, kWave);
                         poison |= __shfl_xor(poison, 32, kWave);
                         if (poison) acc[m][s][0] = acc[m][s][1] = f32x4{NAN, NAN, NAN, NAN};

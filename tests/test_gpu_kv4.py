@@ -515,3 +515,103 @@ def test_shared_keys_at_other_scales(dev, dtype, scale):
     keys, values = ref.contents(cache, 64, 128)
     out, size, spread = ref.attention(q, keys, values, table, positions, scale)
     _within(got, out, ref.attention_bound(size, spread, out, int(positions.max()) + 1, 128, dtype))
+
+
+# ------------------------------------------------------------------ scale bytes whose values leave bf16
+
+
+def _junk(g, cache, page, D, used):
+    """The cache with any bytes at the places [pages, page] that no token needs: every scale byte, half of them 253 and 254,
+    whose larger codes stand for 2^128 and more."""
+    dirty = cache.clone()
+    any_byte = lambda t: torch.randint(0, 256, t.shape, generator=g, dtype=torch.uint8)
+    kc, vc, ks, vs = ref.parts(dirty, page, D)
+    for codes, scales, place in ((kc, ks, used[:, None, :, None]), (vc, vs, used[:, None, None, :])):
+        codes.copy_(torch.where(place, codes, any_byte(codes)))
+        huge = torch.randint(253, 255, scales.shape, generator=g, dtype=torch.uint8)
+        scales.copy_(torch.where(place, scales, torch.where(torch.rand(scales.shape, generator=g) < 0.5, huge, any_byte(scales))))
+    return dirty
+
+
+def _places(table, positions, pages, page):
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for b in range(len(table)):
+        for t in range(int(positions[b].max()) + 1):
+            used[table[b, t // page].long(), t % page] = True
+    return used
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D,page", [(32, 16), (32, 64), (64, 48), (64, 128), (128, 32), (128, 64), (256, 128)])
+@pytest.mark.parametrize("L", [1, 30])
+def test_any_bytes_behind_a_position_do_not_reach_it(dev, dtype, D, page, L):
+    g = torch.Generator().manual_seed(3 * D + L)
+    total = torch.tensor([max(L, 1), 71, 64, 333, 130])
+    positions = (total[:, None] - L + torch.arange(L)).to(torch.int32)
+    positions[3, 0] = 20
+    width = -(-int(total.max()) // page)
+    cache = ref.random_cache(g, 5 * width + 1, 2, page, D)
+    table = ref.random_table(g, 5, width, len(cache))
+    q = torch.randn(5, L, 6, D, generator=g).to(dtype)
+    first = _check(dev, g, 5, L, 6, 2, D, page, positions, dtype, cache=cache, table=table, q=q)
+    dirty = _junk(g, cache, page, D, _places(table, positions, len(cache), page))
+    assert torch.equal(first, _c().kv4_attention(q.to(dev), dirty.to(dev), table.to(dev), positions.to(dev), D ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page,room", [(48, 48 * 350), (64, 1 << 14)])
+def test_shared_keys_any_bytes_behind_a_position(dev, dtype, page, room):
+    """The same for the waves that share the keys."""
+    g = torch.Generator().manual_seed(page)
+    q, cache, table, wide, positions = _shared_case(g, 2, 150, 6, 2, page, room, dtype)
+    dirty = _junk(g, cache, page, 128, _places(table, positions, len(cache), page))
+    call = lambda c: _c().kv4_attention(q.to(dev), c.to(dev), wide.to(dev), positions.to(dev), 0.09)
+    first = call(cache)
+    assert torch.isfinite(first).all() and torch.equal(first, call(dirty))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,D,page,room", [(1, 1, 64, 16, 0), (1, 3, 128, 32, 0), (1, 70, 128, 48, 48 * 1500), (1, 70, 32, 16, 0)])
+def test_a_missing_page_reaches_only_the_rows_that_need_it(dev, dtype, B, L, D, page, room):
+    """Whatever the cache's first page holds: in a tile of keys of which one page is missing, the rows before it keep their
+    bits, beside rows that need it."""
+    g = torch.Generator().manual_seed(L + D)
+    width = 4
+    cache = ref.random_cache(g, 9, 2, page, D)
+    table = torch.tensor([[5, 3, 7, 2]], dtype=torch.int32)
+    positions = torch.arange(page // 2, page // 2 + L, dtype=torch.int32)[None]  # the first page, the second of long chunks
+    q = torch.randn(B, L, 8, D, generator=g).to(dtype)
+    wide = _wide(table, max(width, room // page))
+    call = lambda c, t: _c().kv4_attention(q.to(dev), c.to(dev), t.to(dev), positions.to(dev), D ** -0.5).cpu()
+    first = call(cache, wide)
+    dirty = cache.clone()
+    kc, vc, ks, vs = ref.parts(dirty, page, D)
+    kc[0], vc[0], ks[0], vs[0] = 0x77, 0x77, 254, 254
+    gone = wide.clone()
+    gone[0, 1:4] = torch.tensor([-1, 9, 2 ** 30], dtype=torch.int32)
+    got = call(dirty, gone)
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[0] = (positions[0] >= page)[:, None, None]
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], first[~nan])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("room", [0, 1 << 17])
+def test_huge_values_reach_only_the_rows_that_see_them(dev, dtype, room):
+    """A value under byte 254 in a tile that some rows do not see whole: the rows before it and the other groups of 32 keep
+    their bits, in both forms."""
+    g = torch.Generator().manual_seed(53)
+    page, D, L = 64, 128, 70
+    cache = ref.random_cache(g, 4, 1, page, D)
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    positions = torch.arange(60, 60 + L, dtype=torch.int32)[None]
+    q = torch.randn(1, L, 4, D, generator=g).to(dtype)
+    wide = _wide(table, max(3, room // page))
+    call = lambda c: _c().kv4_attention(q.to(dev), c.to(dev), wide.to(dev), positions.to(dev), 0.09).cpu()
+    first = call(cache)
+    kc, vc, ks, vs = ref.parts(cache, page, D)
+    vs[0, 0, 1, 70 - page], vc[0, 0, 16:32, 70 - page] = 254, 0x77
+    got = call(cache)
+    sees = torch.zeros(got.shape, dtype=torch.bool)
+    sees[0, :, :, 32:64] = (positions[0] >= 70)[:, None, None]
+    assert torch.equal(got[~sees], first[~sees]) and not torch.isfinite(got[sees]).any()
