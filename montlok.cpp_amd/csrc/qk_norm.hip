@@ -60,10 +60,21 @@ __device__ __forceinline__ double element(const u32x4& v, int i) {
     return __uint_as_float(i % 2 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
 }
 
+// The float that v is stored through. For bf16 the upper word of v, and a float's last bit where the lower word is not 0: the
+// middle between two bf16 values only where v is one, so that v is rounded once (from 2^-126 on; a subnormal float may lose
+// that bit).
+template <bool F32>
+__device__ __forceinline__ float to_store(double v) {
+    if constexpr (F32) return static_cast<float>(v);
+    uint32_t cut = __double2loint(v);
+    asm("v_min_u32 %0, 1, %0" : "+v"(cut));  // the compiler makes a comparison and a selection of it
+    return static_cast<float>(__hiloint2double(__double2hiint(v), static_cast<int>(cut << 29)));
+}
+
 // A head row on LPG lanes of E elements (16 bytes) each, a wave on R * 64 / LPG query rows, or key rows, of one token.
 // What the rows share is formed once, weight times cosine and partner's weight times sine in double, so that an element
 // costs three double operations beside its square (with all of it per row, 8000 tokens x 40 heads of 128 in bf16 took
-// 56 us). A rotated lane loads its partners' 16 bytes as well (from the L1: the partner lane has them) instead of
+// 56 us, and 39 so). A rotated lane loads its partners' 16 bytes as well (from the L1: the partner lane has them) instead of
 // exchanging doubles. Every load is issued before the first sum.
 template <bool F32, int LPG, int R>
 __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsigned chunks, unsigned q_chunks) {
@@ -100,6 +111,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsig
         load_floats<E>(p.cosine + at * p.rope + (d - nope), cosine);
         load_floats<E>(p.sine + at * p.rope + (d - nope), sine);
     }
+    const uint32_t fill = at < 0 ? 0 : F32 ? 0x7FC00000u : 0x7FC07FC0u;  // zeros, or NaN, where the position has no row
     double sum[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsig
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         own[i] = static_cast<double>(weight[i]) * cosine[i];
-        others[i] = static_cast<double>(upper ? partner[i] : -partner[i]) * sine[i];
+        others[i] = turned ? static_cast<double>(upper ? partner[i] : -partner[i]) * sine[i] : 0.0;
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -122,23 +134,17 @@ __global__ __launch_bounds__(256) void qk_norm_rope_vec_kernel(NormArgs p, unsig
         float out[E];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            // A lane that is not rotated has no partner: its element is not to meet the sine's 0 as an infinity.
-            const double v = turned ? fma(element<F32>(y[r], i), others[i], element<F32>(x[r], i) * own[i]) : element<F32>(x[r], i) * own[i];
-            out[i] = static_cast<float>(v * by);
+            // A lane that is not rotated is its own partner, times 0: an infinity of it is NaN here, and in its row's norm.
+            out[i] = to_store<F32>(fma(element<F32>(y[r], i), others[i], element<F32>(x[r], i) * own[i]) * by);
         }
-        if (!inside) {
+        u32x4 w;
 #pragma unroll
-            for (int i = 0; i < E; ++i) out[i] = at < 0 ? 0.0f : NAN;
+        for (int i = 0; i < 4; ++i) {
+            w[i] = F32 ? __float_as_uint(out[i]) : __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(out[E / 4 * i]), static_cast<__bf16>(out[E / 4 * i + E / 8])});
+            w[i] = inside ? w[i] : fill;
         }
         const int64_t to = (static_cast<int64_t>(token) * rows + row) * D + d;
-        if constexpr (F32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(t.out) + to) = f32x4{out[0], out[1], out[2], out[3]};
-        } else {
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = float_to_bf16(out[2 * i]) | float_to_bf16(out[2 * i + 1]) << 16;
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(t.out) + to) = w;
-        }
+        *reinterpret_cast<u32x4*>(static_cast<char*>(t.out) + to * (F32 ? 4 : 2)) = w;
     }
 }
 
@@ -176,7 +182,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormArgs p) {
             }
             if (!inside) y = NAN;
         }
-        Element<F32>::put(t.out, to + d, static_cast<float>(y));
+        Element<F32>::put(t.out, to + d, to_store<F32>(y));
     }
 }
 

@@ -157,3 +157,40 @@ def test_refusals(dev):
                        (lambda: _C.qk_norm_rope(x, x, w, w.cpu(), 1e-5, t, t, at), "k_weight must be on the same GPU")):
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def _nearest_bf16(y):
+    """The bf16 values next to float64 ones of ordinary size, straight from them: torch's cast rounds to float32 on its way."""
+    step = 2.0 ** (torch.floor(torch.log2(y.abs())) - 7)
+    return (torch.round(y / step) * step).to(torch.float32).to(BF16)  # ties, which torch.round gives the even one, as bf16's are
+
+
+@pytest.mark.parametrize("D,rope", [(32, 0), (32, 32), (64, 32), (128, 128), (256, 256), (512, 256), (96, 32), (100, 100)])
+def test_bf16_results_next_to_a_tie_are_rounded_once(dev, D, rope):
+    """Weights, or cosines, that bring each result within 2^-23 of the middle between two bf16 values, where a rounding to
+    float32 before that to bf16 lands on the middle and then on the wrong side."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(D + rope)
+    wrong = 0
+    for _ in range(4):
+        x = torch.randn(1, 1, 1, D, generator=g).to(BF16)
+        x[x == 0] = 1
+        middle = (1 + (2 * torch.randint(0, 64, (D,), generator=g) + 1).double() / 256) * (1 - 2.0 * torch.randint(0, 2, (D,), generator=g))
+        by = (x[0, 0, 0].double() / torch.sqrt(x.double().square().mean() + 1e-6))
+        weight = (middle / by).float()
+        cos, sin = torch.ones(1, rope), torch.zeros(1, rope)
+        if rope:  # rotated lanes: cos = (middle + what the sine takes) / own
+            y = (by * weight)[D - rope:]
+            a, b = y.chunk(2)
+            sin = (torch.rand(1, rope, generator=g) - 0.5)
+            other = torch.cat([-b, a]) * sin[0].double()
+            cos = ((middle[D - rope:] - other) / y).float()[None]
+        at = torch.zeros(1, 1, dtype=torch.int32)
+        expect = _reference(x, weight, 1e-6, cos, sin, at)
+        q, k = _C.qk_norm_rope(x.to(dev), x.to(dev), weight.to(dev), weight.to(dev), 1e-6, cos.to(dev), sin.to(dev), at.to(dev))
+        nearest = _nearest_bf16(expect)
+        clear = (expect - torch.round(expect * 256) / 256).abs() > 2.0 ** -44  # of the middles, by more than float64's own error
+        wrong += int((expect.float().to(BF16) != nearest)[clear].sum())
+        assert torch.equal(q.cpu()[clear], nearest[clear]) and torch.equal(k.cpu()[clear], nearest[clear])
+    assert wrong >= D // 4
