@@ -171,3 +171,117 @@ def test_weights_are_quantised_alike_on_the_gpu(dev, dtype):
     assert torch.equal(on_gpu[0].cpu(), codes) and torch.equal(on_gpu[1].cpu(), scales)
     got = _C.linear_fp4(torch.eye(192, dtype=dtype, device=dev), *on_gpu)
     assert torch.equal(got.cpu().double(), ref.nearest(w).t())
+
+
+# ------------------------------------------------------------------ every form of the kernel
+
+
+def _form(rows, n, dtype, stride=0):
+    """Which form a call takes: the rule of the launch, by rounds of blocks on 256 compute units."""
+    up = lambda a, b: -(-a // b)
+    rounds = lambda c, r: up(up(n, c) * up(rows, r), 256)
+    full = lambda c: max(1.0, up(n, c) * up(rows, 16) / 256)
+    few, tiles = rows <= 4, stride < 1 << 24
+    if dtype == F32:
+        if tiles and 30 * rounds(128, 32) < 12 * full(64):
+            return "tile 128"
+        by = {c: t * rounds(c, 16) for c, t in zip((16, 32, 64), (5.2, 6.8, 9.5) if few else (6.7, 8.1, 11.6))}
+        columns = 64 if by[64] < min(by[16], by[32]) else 16 if by[16] <= by[32] else 32
+    else:
+        narrow, wide = 15.5 * rounds(64, 64), 22 * rounds(128, 64)
+        if tiles and min(narrow, wide) < 3.7 * full(32):
+            return "tile 64" if narrow < wide else "tile 128"
+        one, two = (2.9, 3.8) if few else (4.0, 4.9)
+        columns = 16 if one * rounds(16, 16) <= two * rounds(32, 16) else 32
+    return f"{'few' if few else 'turned'} {columns}"
+
+
+FORMS = [(F32, "few 16", 3, 3000), (F32, "few 32", 3, 6001), (F32, "few 64", 2, 8199), (F32, "turned 16", 17, 1001), (F32, "turned 32", 70, 1301),
+         (F32, "turned 64", 300, 2050), (F32, "tile 128", 600, 1501), (F32, "tile 128", 130, 12290), (F32, "tile 128", 70, 9001),
+         (BF16, "few 16", 4, 3003), (BF16, "few 32", 2, 5002), (BF16, "turned 16", 40, 1001), (BF16, "turned 32", 70, 9001),
+         (BF16, "tile 64", 257, 2050), (BF16, "tile 64", 600, 1501), (BF16, "tile 64", 2000, 300), (BF16, "tile 128", 256, 4099),
+         (BF16, "tile 128", 130, 12290), (BF16, "tile 128", 300, 6004)]
+
+
+@pytest.mark.parametrize("dtype,form,rows,n", FORMS)
+@pytest.mark.parametrize("k", [32, 224, 512, 544])
+def test_every_form_against_float64(dev, dtype, form, rows, n, k):
+    """Ragged rows, columns and K (whole steps of 256 are one of the four), with and without a bias."""
+    from montlok import _C
+
+    assert _form(rows, n, dtype) == form
+    g = torch.Generator().manual_seed(rows + n + k)
+    codes, scales = _weights(g, n, k)
+    x = torch.randn(rows, k, generator=g).to(dtype)
+    bias = torch.randn(n, generator=g) if k % 64 else None
+    got = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev), None if bias is None else bias.to(dev))
+    assert got.shape == (rows, n) and got.dtype == dtype
+    _check(got, x, codes, scales, bias, dtype)
+
+
+@pytest.mark.parametrize("dtype,form,rows,n", [f for f in FORMS if "tile" in f[1]])
+def test_tiles_of_views_and_of_infinities(dev, dtype, form, rows, n):
+    """Rows of any alignment give a copy's bits; infinities and NaN stay in their rows and columns, also in the last group
+    of a K that ends inside a step."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(rows * 3 + n)
+    codes, scales = _weights(g, n, 160)
+    codes |= 0x11  # no weight is zero: an infinity gives an infinity
+    dc, ds = codes.to(dev), scales.to(dev)
+    wide = torch.randn(rows, 171, generator=g).to(dtype)
+    x = wide[:, 3:163].contiguous()
+    clean = _C.linear_fp4(x.to(dev), dc, ds)
+    for lead in (1, 2, 3, 8):
+        moved = torch.roll(wide, lead - 3, 1).to(dev)[:, lead:lead + 160]
+        assert torch.equal(_C.linear_fp4(moved, dc, ds), clean)
+    same = x[:1].to(dev).expand(rows, 160)  # rows at a stride of 0
+    assert torch.equal(_C.linear_fp4(same, dc, ds), _C.linear_fp4(same.contiguous(), dc, ds))
+    x[0, 3], x[rows // 2, 100], x[rows - 1, 159] = torch.inf, -torch.inf, torch.nan
+    scales[9, 2], scales[n - 1, 4] = 255, 255
+    got, clean = _C.linear_fp4(x.to(dev), dc, scales.to(dev)).cpu(), clean.cpu()
+    expect = x.double() @ ref.value_of(codes, scales).t()
+    assert torch.equal(torch.isnan(got), torch.isnan(expect)) and torch.equal(torch.isinf(got), torch.isinf(expect))
+    assert torch.equal(torch.sign(got[0, :9].double()), torch.sign(expect[0, :9]))
+    rest, keep = torch.ones(rows, dtype=torch.bool), torch.ones(n, dtype=torch.bool)
+    rest[[0, rows // 2, rows - 1]], keep[[9, n - 1]] = False, False
+    assert torch.equal(got[rest][:, keep], clean[rest][:, keep])
+
+
+@pytest.mark.parametrize("dtype,rows,n", [(BF16, 257, 2050), (F32, 70, 9001)])
+@pytest.mark.parametrize("stride", [(1 << 24) - 1, 1 << 24])
+def test_rows_far_apart(dev, dtype, rows, n, stride):
+    """The widest stride that tiles address in 32 bits, and the first that goes to the other form."""
+    from montlok import _C
+
+    assert _form(rows, n, dtype, stride).startswith("tile") == (stride < 1 << 24) and _form(rows, n, dtype).startswith("tile")
+    g = torch.Generator().manual_seed(n)
+    codes, scales = _weights(g, n, 160)
+    x = torch.randn(rows, 160, generator=g).to(dtype)
+    far = torch.empty(rows * stride, dtype=dtype, device=dev).as_strided((rows, 160), (stride, 1)).copy_(x)
+    _check(_C.linear_fp4(far, codes.to(dev), scales.to(dev)), x, codes, scales, None, dtype)
+
+
+@pytest.mark.parametrize("dtype,rows,n", [(BF16, 257, 2050), (BF16, 256, 4099), (F32, 600, 1501)])
+def test_tiles_in_a_graph(dev, dtype, rows, n):
+    from montlok import _C
+
+    assert _form(rows, n, dtype).startswith("tile")
+    g = torch.Generator().manual_seed(rows)
+    codes, scales = (t.to(dev) for t in _weights(g, n, 288))
+    x = torch.zeros(rows, 288, dtype=dtype, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _C.linear_fp4(x, codes, scales)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _C.linear_fp4(x, codes, scales)
+    for replay in range(4):
+        x.copy_(torch.randn(x.shape, generator=g).to(dtype))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, _C.linear_fp4(x, codes, scales)), f"replay {replay}"
