@@ -194,3 +194,40 @@ def test_bf16_results_next_to_a_tie_are_rounded_once(dev, D, rope):
         wrong += int((expect.float().to(BF16) != nearest)[clear].sum())
         assert torch.equal(q.cpu()[clear], nearest[clear]) and torch.equal(k.cpu()[clear], nearest[clear])
     assert wrong >= D // 4
+
+
+def _rows_a_wave(tokens, H, Hkv, D, dtype):
+    """How many head rows a lane group takes: the rule of the launch."""
+    groups = 64 // (D // (4 if dtype == F32 else 8))
+    slots = lambda r: sum(-(-heads // (groups * r)) for heads in (H, Hkv)) * r
+    for r in (4, 2):
+        if tokens * slots(r) >= 4096 * r and 4 * slots(r) <= 5 * slots(1):
+            return r
+    return 1
+
+
+@pytest.mark.parametrize("dtype,each,B,L,H,Hkv,D,rope", [
+    (BF16, 4, 3, 700, 30, 8, 128, 64), (BF16, 4, 2, 1030, 60, 50, 32, 16), (BF16, 4, 1, 2051, 7, 8, 256, 256), (BF16, 4, 1, 1400, 7, 4, 512, 0),
+    (BF16, 2, 2, 1030, 15, 10, 64, 32), (BF16, 2, 1, 2077, 8, 5, 128, 128), (BF16, 1, 3, 1037, 8, 2, 64, 32),
+    (F32, 4, 2, 500, 30, 7, 128, 128), (F32, 4, 3, 700, 16, 15, 64, 64), (F32, 4, 1, 1400, 7, 4, 256, 128), (F32, 4, 1, 1030, 60, 50, 32, 0),
+    (F32, 2, 2, 1030, 7, 6, 64, 32), (F32, 2, 1, 2077, 4, 3, 128, 32), (F32, 2, 5, 411, 16, 9, 32, 32)])
+def test_several_rows_a_wave(dev, dtype, each, B, L, H, Hkv, D, rope):
+    """Heads that leave a group's last turns empty, padding, positions past the tables, a head with a NaN and one with an
+    infinity, q and k as views."""
+    from montlok import _C
+
+    assert _rows_a_wave(B * L, H, Hkv, D, dtype) == each
+    g = torch.Generator().manual_seed(D + H + L)
+    qkv = torch.randn(B, L, H + 2 * Hkv, D, generator=g)
+    qkv[0, 3, H - 1, D - 1], qkv[B - 1, L - 1, H, 0] = torch.nan, torch.inf
+    qkv = qkv.to(dtype)
+    weights = 1 + 0.3 * torch.randn(2, D, generator=g)
+    cos, sin = _tables(g, L, rope)
+    positions = torch.arange(L, dtype=torch.int32).expand(B, L).clone()
+    positions[torch.rand(B, L, generator=g) < 0.1] = -1
+    positions[torch.rand(B, L, generator=g) < 0.05] = L
+    positions[0, 3], positions[B - 1, L - 1] = 1, 2
+    d = qkv.to(dev)
+    q, k = _C.qk_norm_rope(d[:, :, :H], d[:, :, H:H + Hkv], weights[0].to(dev), weights[1].to(dev), 1e-5, cos.to(dev), sin.to(dev), positions.to(dev))
+    _check(q, _reference(qkv[:, :, :H], weights[0], 1e-5, cos, sin, positions), dtype)
+    _check(k, _reference(qkv[:, :, H:H + Hkv], weights[1], 1e-5, cos, sin, positions), dtype)
