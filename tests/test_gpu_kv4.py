@@ -615,3 +615,51 @@ def test_huge_values_reach_only_the_rows_that_see_them(dev, dtype, room):
     sees = torch.zeros(got.shape, dtype=torch.bool)
     sees[0, :, :, 32:64] = (positions[0] >= 70)[:, None, None]
     assert torch.equal(got[~sees], first[~sees]) and not torch.isfinite(got[sees]).any()
+
+
+# ------------------------------------------------------------------ the forms and splits that a call's sizes choose
+
+
+def _splits(lib, B, L, H, Hkv, D, page, width):
+    """Parts of a row, from the workspace's size."""
+    return lib.mlk_kv4_attention_workspace_bytes(B, L, H, Hkv, D, page, width) // (4 * (D + 2) * B * L * H)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("page,L,H,Hkv", [(64, 7, 6, 2), (128, 1, 17, 1), (192, 2, 6, 2), (64, 1, 3, 1), (128, 1, 2, 1), (64, 40, 1, 1)])
+def test_rows_on_pages_of_whole_tiles(dev, dtype, D, page, L, H, Hkv):
+    g = torch.Generator().manual_seed(D + page + L)
+    total = torch.tensor([L, 77, 64, 301, 129 + L]).clamp(min=L)
+    positions = (total[:, None] - L + torch.arange(L)).to(torch.int32)
+    positions[4, L // 2] = -1
+    _check(dev, g, 5, L, H, Hkv, D, page, positions, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D,page,L,H,Hkv,length,splits", [(32, 64, 1, 4, 1, 9700, 19), (64, 48, 1, 8, 2, 9300, 19), (128, 64, 1, 4, 1, 10240, 20),
+                                                          (256, 32, 1, 3, 1, 9001, 18), (32, 16, 5, 4, 1, 8711, 18), (64, 128, 3, 7, 1, 16001, 32),
+                                                          (256, 256, 2, 6, 1, 16384, 32), (128, 16, 6, 6, 2, 20011, 20)])
+def test_many_parts_that_all_hold_keys(dev, dtype, D, page, L, H, Hkv, length, splits):
+    """More than 16 parts of every row, joined by groups of lanes; among the rows short ones, whose parts are mostly empty."""
+    width = -(-length // page)
+    assert _splits(_c().library(), 2, L, H, Hkv, D, page, width) == splits
+    g = torch.Generator().manual_seed(length)
+    positions = torch.stack([torch.arange(L) + length - L, torch.arange(L) * 613 % length]).to(torch.int32)
+    _check(dev, g, 2, L, H, Hkv, D, page, positions, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_shared_keys_many_parts_that_all_hold_keys(dev, dtype):
+    g = torch.Generator().manual_seed(59)
+    page, D, L, H, Hkv, length, width = 64, 128, 16, 64, 8, 6000, 256
+    assert _splits(_c().library(), 1, L, H, Hkv, D, page, width) == 32  # by strides of 32 tiles, 94 of them in use
+    positions = (torch.arange(L) * 400).to(torch.int32)[None]
+    positions[0, L - 1] = length - 1
+    used = -(-length // page)
+    cache, table = ref.random_cache(g, used, Hkv, page, D), ref.random_table(g, 1, used, used)
+    q = torch.randn(1, L, H, D, generator=g).to(dtype)
+    got = _c().kv4_attention(q.to(dev), cache.to(dev), _wide(table, width).to(dev), positions.to(dev), D ** -0.5)
+    keys, values = ref.contents(cache, page, D)
+    out, size, spread = ref.attention(q, keys, values, table, positions, D ** -0.5)
+    _within(got, out, ref.attention_bound(size, spread, out, length, D, dtype))
