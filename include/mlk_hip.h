@@ -435,7 +435,9 @@ mlk_status mlk_mamba3_siso_step(const float* projected, int64_t streams, int64_t
  *
  * Four-bit values are OCP MX: codes of four bits (sign, e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32 consecutive ones under a
  * scale byte that stands for 2^(byte - 127); 255 makes the group NaN. Byte j of a row of codes holds elements 2 j (low
- * four bits) and 2 j + 1.
+ * four bits) and 2 j + 1. Values of 2^128 and more (bytes 253 and 254, which no call here writes) count as infinities.
+ * An fp32 activation is multiplied as the sum of three bf16 numbers: exactly from 2^-110 on, without what lies below 2^-133
+ * of a smaller one.
  *
  * `positions` [batch, length] gives every token its place in its sequence; a negative one is padding. `page_table`
  * [batch, table_width] names a sequence's pages, 2^28 tokens at most; entries of pages that no token needs may be
@@ -485,8 +487,9 @@ mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dt
                              double scale, void* out, void* workspace, size_t workspace_bytes, mlk_stream_t stream);
 
 /* y [rows, out_features] = x W^T + bias with four-bit weights: codes [out_features, in_features / 2] (16-byte aligned),
- * scales [out_features, in_features / 32], bias fp32 or NULL. x rows `x_stride` elements apart; y contiguous, of x's
- * dtype. in_features: a multiple of 32 below 2^24; out_features below 2^26; rows below 2^20 - 16, y up to 2^34 elements. */
+ * scales [out_features, in_features / 32], bias fp32 or NULL. An output that takes an infinite weight is infinite or NaN,
+ * whatever x holds there. x rows `x_stride` elements apart; y contiguous, of x's dtype. in_features: a multiple of 32 below
+ * 2^24; out_features below 2^26; rows below 2^20 - 16, y up to 2^34 elements. */
 mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int64_t x_stride, int32_t dtype,
                           const uint8_t* codes, const uint8_t* scales, const float* bias, int64_t out_features, void* out,
                           mlk_stream_t stream);

@@ -3,13 +3,15 @@
 //
 //   value = (-1)^(code >> 3) * {0, 0.5, 1, 1.5, 2, 3, 4, 6}[code & 7] * 2^(byte - 127);  byte 255: NaN
 //
-// A value has two significant bits, so every one of them is exact in bf16 and
-// its product with a bf16 number is exact in fp32: sums over it on the bf16
-// matrix cores round only in their fp32 accumulation. The conversions are
-// gfx950's v_cvt_scalef32_pk_*: over all 256 bytes and all codes they give the
-// values above (NaN for 255, 2^-127 for byte 0), and the way back rounds to
-// nearest with ties to the even code and saturates at 6 (49,160 values on and
-// next to every border, at 8 scales).
+// A value has two significant bits, so up to byte 252 every one of them is exact
+// in bf16 and its product with a bf16 number is exact in fp32: sums over it on
+// the bf16 matrix cores round only in their fp32 accumulation. Under bytes 253
+// and 254 the larger codes stand for 2^128 and more, infinities in bf16; the
+// package's own quantisation ends at 252. The conversions are gfx950's
+// v_cvt_scalef32_pk_*: over all 256 bytes and all codes they give the values
+// above (infinities from 2^128 on, NaN for 255, 2^-127 for byte 0), and the way
+// back rounds to nearest with ties to the even code and saturates at 6 (49,160
+// values on and next to every border, at 8 scales).
 #pragma once
 
 #include "mlk_common.h"
@@ -55,8 +57,8 @@ __device__ __forceinline__ uint32_t scale_byte(float most) {
     return static_cast<uint32_t>(min(max(byte, 3), 252));
 }
 
-// An fp32 value as the sum of three bf16 values, exactly: its leading 8 significant bits, the next 8, the rest
-// (each cut off, so that none of them overflows). An infinity or a NaN stays alone with CAREFUL, and makes the rest NaN
+// An fp32 value as the sum of three bf16 values: its leading 8 significant bits, the next 8, the rest (each cut off, so that
+// none of them overflows). Exact from 2^-110 on; below, what is smaller than bf16's least number, 2^-133, is lost. An infinity or a NaN stays alone with CAREFUL, and makes the rest NaN
 // without: half the instructions, for callers that look at their result.
 struct Parts3 {
     float a, b, c;

@@ -1,7 +1,7 @@
 // y = x W^T + b with four-bit weights (groups of 32 under a power of two), on
-// the bf16 matrix cores with fp32 accumulation. Every weight is exact in bf16,
-// a bf16 x is too, and an fp32 x is the exact sum of three bf16 values, so the
-// only rounding is that of the sums.
+// the bf16 matrix cores with fp32 accumulation. Every weight below 2^128 is
+// exact in bf16, a bf16 x is too, and an fp32 x from 2^-110 on is the exact sum
+// of three bf16 values, so the only rounding is that of the sums.
 #include <algorithm>
 #include <type_traits>
 

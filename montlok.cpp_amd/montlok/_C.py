@@ -588,9 +588,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: int, scal
 # ------------------------------------------------------------------ streaming over a 4-bit cache
 #
 # No counterparts in the reference. Four-bit values are OCP MX: codes (sign, e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32
-# consecutive ones under a scale byte for 2^(byte - 127), 255 for NaN. ``positions`` [batch, length] (int32) is each
-# token's place in its sequence, negative for padding; ``page_table`` [batch, n] (int32) names a sequence's pages.
-# Activations are float32 or bfloat16; the tensors of a call are on one GPU, whose current stream it uses.
+# consecutive ones under a scale byte for 2^(byte - 127), 255 for NaN (values of 2^128 and more, under 253 and 254, count
+# as infinities; nothing here writes those bytes). ``positions`` [batch, length] (int32) is each token's place in its
+# sequence, negative for padding; ``page_table`` [batch, n] (int32) names a sequence's pages. Activations are float32 or
+# bfloat16; the tensors of a call are on one GPU, whose current stream it uses.
 
 
 def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device=None) -> torch.Tensor:
@@ -666,7 +667,8 @@ def linear_fp4(input: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                bias: torch.Tensor | None = None) -> torch.Tensor:
     """input [..., K] @ W^T + bias with W in four bits, as ``fp4_weights`` gives it: codes uint8 [N, K / 2] (element 2 j in
     the low bits of byte j), scales uint8 [N, K / 32], bias float32 [N]. The result has the input's dtype; sums are in
-    float32 and the products exact, for float32 input too."""
+    float32 and the products exact, for float32 input too (what lies below 2^-133 of a value under 2^-110 is lost). An
+    output that takes an infinite weight is infinite or NaN."""
     return (_native or _ops()).linear_fp4(input, codes, scales, bias)
 
 

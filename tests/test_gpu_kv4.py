@@ -663,3 +663,21 @@ def test_shared_keys_many_parts_that_all_hold_keys(dev, dtype):
     keys, values = ref.contents(cache, page, D)
     out, size, spread = ref.attention(q, keys, values, table, positions, D ** -0.5)
     _within(got, out, ref.attention_bound(size, spread, out, length, D, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_every_scale_byte_and_code_is_read_as_its_value(dev, dtype):
+    """All 256 bytes under all 16 codes: exactly the value, an infinity from 2^128 on (bytes 253 and 254), NaN for 255."""
+    page, D = 256, 32
+    cache = torch.zeros(1, 1, page * (D + D // 16), dtype=torch.uint8)
+    kc, vc, ks, vs = ref.parts(cache, page, D)
+    kc[0, 0] = torch.arange(16, dtype=torch.uint8) * 16 + torch.arange(16, dtype=torch.uint8).flip(0)
+    vc[0, 0] = kc[0, 0].t()
+    ks[0, 0, :, 0] = vs[0, 0, 0] = torch.arange(256, dtype=torch.int32).to(torch.uint8)
+    positions = torch.arange(page, dtype=torch.int32, device=dev)[None]
+    keys, values = ref.contents(cache, page, D)
+    assert torch.equal(keys.nan_to_num(nan=0.5), values.nan_to_num(nan=0.5))
+    expect = torch.where(keys.abs() >= 2.0 ** 128, torch.sign(keys) * torch.inf, keys)[0, 0][None, :, None]
+    assert int(torch.isinf(expect).sum()) == 8 + 16  # of 32 elements each: codes 6 and 7 under 253, 4 to 7 under 254
+    for got in _c().kv4_read(cache.to(dev), torch.zeros(1, 1, dtype=torch.int32, device=dev), positions, D, dtype):
+        assert _same(got, expect)

@@ -285,3 +285,44 @@ def test_tiles_in_a_graph(dev, dtype, rows, n):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, _C.linear_fp4(x, codes, scales)), f"replay {replay}"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(3, 40), (40, 40), (600, 1501)])
+def test_weights_past_the_largest_number(dev, dtype, rows, n):
+    """Bytes 253 and 254: weights below 2^128 are exact, an output with a larger one is infinite or NaN, the others keep
+    their bits."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(rows)
+    codes, scales = _weights(g, n, 96)
+    x = (torch.randn(rows, 96, generator=g) * 2.0 ** -20).to(dtype)
+    clean = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    scales[3, 1], scales[4, 2], scales[5, 2], scales[6, 0] = 253, 254, 253, 254
+    codes[3, 16:32], codes[4, 32:48] = 0x75, 0x94  # 6 and 3 times 2^126; 2 and -0.5 times 2^127
+    codes[5, 32:48], codes[6, :16] = 0xD5, 0x3B  # 3 times 2^126; 1.5 times 2^127: exact
+    got = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)).cpu()
+    assert not torch.isfinite(got[:, 3:5]).any()
+    _check(got[:, 5:7], x, codes[5:7], scales[5:7], None, dtype)
+    rest = torch.ones(n, dtype=torch.bool)
+    rest[3:7] = False
+    assert torch.equal(got[:, rest], clean[:, rest])
+
+
+@pytest.mark.parametrize("rows,n", [(2, 33), (40, 33), (600, 1501)])
+@pytest.mark.parametrize("power", [-110, -111, -120, -132, -140, -148])
+def test_the_smallest_inputs(dev, rows, n, power):
+    """float32 values of one power of two, down to the subnormal ones: their parts are exact from 2^-110 on, and lose less
+    than 2^-133 of a smaller value."""
+    from montlok import _C
+
+    g = torch.Generator().manual_seed(rows - power)
+    codes, scales = _weights(g, n, 96, 220, 224)
+    x = (1 + torch.rand(rows, 96, generator=g)).double() * (1 - 2.0 * torch.randint(0, 2, (rows, 96), generator=g)) * 2.0 ** power
+    x = x.float()
+    got = _C.linear_fp4(x.to(dev), codes.to(dev), scales.to(dev)).double().cpu()
+    w = ref.value_of(codes, scales)
+    bound = (3 * 96 + 8) * 2.0 ** -24 * (x.double().abs() @ w.abs().t())
+    if power < -110:
+        bound = bound + 2.0 ** -133 * w.abs().sum(1)
+    assert ((got - x.double() @ w.t()).abs() <= bound).all()
