@@ -441,11 +441,13 @@ mlk_status mlk_mamba3_siso_step(const float* projected, int64_t streams, int64_t
  *
  * `positions` [batch, length] gives every token its place in its sequence; a negative one is padding. `page_table`
  * [batch, table_width] names a sequence's pages, 2^28 tokens at most; entries of pages that no token needs may be
- * anything. Both are contiguous int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes, 16-byte aligned, page_size a
- * multiple of 16 up to 1024, head_dim 32, 64, 128 or 256. A (page, head) holds key codes [page_size][head_dim / 2], value
- * codes [head_dim / 2][page_size], key scales [page_size][head_dim / 32], value scales [head_dim / 32][page_size].
- * Strides are {sequence, token, head} in elements, head_dim dense. A call that needs 2^32 threads or more is refused: 2^26
- * head rows of a norm, 2^29 of an append or a read, 2^27 query head rows of an attention. */
+ * anything. Both are contiguous int32. The cache is [pages, kv_heads, page_size * (head_dim + head_dim / 16)] bytes,
+ * 16-byte aligned, page_size a multiple of 16 up to 1024, head_dim 32, 64, 128 or 256. A (page, head) holds key codes
+ * [page_size][head_dim / 2], value codes [head_dim / 2][page_size], key scales [page_size][head_dim / 32], value scales
+ * [head_dim / 32][page_size]. Strides are {sequence, token, head} in elements, head_dim dense. A call that needs 2^32
+ * threads or more is refused: 2^26 head rows of a norm, 2^29 of an append or a read, 2^23 blocks of an attention, one to
+ * 16 rows (token and query head) of a sequence's key head, however few they are: batch * kv_heads *
+ * ceil(length * heads / kv_heads / 16). */
 
 /* RMSNorm over head_dim of every head of q [batch, length, heads, head_dim] and k [.., kv_heads, ..], each with its fp32
  * weight [head_dim], then the rotation (rotate_half, as mlk_mla_rope_qk) of the last rope_dim lanes by the tables' row

@@ -188,3 +188,14 @@ def test_negative_row_strides_are_refused(lib):
     at = C.c_void_p((C.addressof(memory) + 15) & ~15)
     assert lib.mlk_linear_fp4(at, 2, 64, -64, 1, at, at, None, 8, at, None) == 1
     assert "x_stride" in lib.mlk_last_error().decode()
+
+
+def test_attention_is_refused_by_blocks(lib):
+    """2^23 blocks of up to 16 rows of a (sequence, key head), however few of the rows there are."""
+    memory = (C.c_uint8 * 64)()
+    at = C.c_void_p((C.addressof(memory) + 15) & ~15)
+    strides = (C.c_int64 * 3)(64, 64, 64)
+    for batch, length, heads, kv_heads in ((2 ** 20, 1, 32, 8), (2 ** 23, 1, 1, 1), (2 ** 19, 17, 8, 8), (2 ** 19 + 1, 1, 255, 15)):
+        assert batch * kv_heads * -(-(length * heads // kv_heads) // 16) >= 2 ** 23
+        assert lib.mlk_kv4_attention(at, strides, 1, batch, length, heads, kv_heads, 64, at, 4, 64, at, 2, at, 1.0, at, None, 0, None) == 1
+        assert "too many" in lib.mlk_last_error().decode()
