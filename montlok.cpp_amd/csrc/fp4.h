@@ -23,6 +23,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // at any element's alignment
 
 constexpr int kGroup = 32;  // values under one scale
 constexpr uint32_t kMostScale = 252;  // the largest byte whose values are all finite in bf16 (6 * 2^126 is 1.5 * 2^128)
@@ -102,13 +103,11 @@ __device__ __forceinline__ uint32_t float_to_bf16(float x) {
 // Element access by the tensors' type.
 template <bool F32>
 struct Element {
-    using type = float;
     static __device__ __forceinline__ float get(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
 };
 template <>
 struct Element<false> {
-    using type = uint16_t;
     static __device__ __forceinline__ float get(const void* p, int64_t i) { return bf16_to_float(static_cast<const uint16_t*>(p)[i]); }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(float_to_bf16(v)); }
 };

@@ -67,13 +67,12 @@ struct Rows3 {
 // Eight elements of a row at any alignment.
 template <bool F32>
 __device__ __forceinline__ void load8(const void* p, int64_t first, float (&x)[8]) {
-    typedef uint32_t Four __attribute__((ext_vector_type(4), aligned(2)));
     if constexpr (F32) {
-        const Four* const from = reinterpret_cast<const Four*>(static_cast<const float*>(p) + first);
+        const u32x4_any* const from = reinterpret_cast<const u32x4_any*>(static_cast<const float*>(p) + first);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(from[i / 4][i % 4]);
     } else {
-        const Four v = *reinterpret_cast<const Four*>(static_cast<const uint16_t*>(p) + first);
+        const u32x4 v = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(p) + first);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i % 2 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
     }

@@ -20,9 +20,6 @@ struct Fp4LinearArgs {
     int32_t rows, K, N;
 };
 
-// Sixteen bytes at any element's alignment.
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-
 // Four results side by side; `first` a multiple of 4 from an aligned base.
 template <bool F32>
 __device__ __forceinline__ void put4(void* out, int64_t first, const float (&y)[4]) {

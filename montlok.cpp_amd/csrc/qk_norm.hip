@@ -51,8 +51,7 @@ __device__ __forceinline__ void load_floats(const float* from, float (&v)[E]) {
 }
 template <bool F32>
 __device__ __forceinline__ u32x4 load_elements(const void* p, int64_t first) {
-    typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
-    return *reinterpret_cast<const Any*>(static_cast<const char*>(p) + first * (F32 ? 4 : 2));
+    return *reinterpret_cast<const u32x4_any*>(static_cast<const char*>(p) + first * (F32 ? 4 : 2));
 }
 template <bool F32>
 __device__ __forceinline__ double element(const u32x4& v, int i) {
