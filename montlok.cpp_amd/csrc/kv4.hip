@@ -585,8 +585,10 @@ __global__ __launch_bounds__(W * 64, D == 32 || (D == 64 && !F32) ? 4 : 2) void 
                 sum += x;
             }
         };
-        // Eight weights as operands. fp32: of finite values, or NaN. bf16: rounded to nearest, 2^-9 of a weight, which a mean
-        // over many keys loses; the sum is of the unrounded.
+        // Eight weights as operands. fp32: of finite values, or NaN. bf16: rounded to nearest, by up to 2^-8 of a weight; the
+        // sum is of the unrounded. An output's error grows by it from the 0.0016 or 0.0017 of its own rounding to 0.0017 (one
+        // stream of 131072 keys) to 0.0020 (32 x 8000); what is left of each weight as a second operand would take it away
+        // again, in 5 to 8% more time (32 x 8000 keys 40.2 -> 43.5 us, 64 x 10000 93 -> 98).
         auto operand_of = [&](const float (&w)[8], bf16x8 (&to)[P]) {
             if constexpr (F32) {
                 planes_of<false>(w, to);
@@ -757,8 +759,8 @@ constexpr int kRowTiles = F32 ? 1 : 2;
 // operands in LDS. A wave of the kernel above spends most of its instructions on converting keys and values, for 16 rows
 // (512 tokens of two sequences over 8192 keys took 270 us so); here it converts an eighth of them, for 128 MT. A tile
 // passes through registers (three tiles ahead), LDS as it lies in memory (two ahead) and LDS as operands (one ahead).
-// 1 x 512 tokens over 8192 keys, 32 heads on 8: 111 us, 620 TFLOP/s; a SIMD's two waves issue vector instructions for 54%
-// of the time, products for 33%, and LDS hands out operands for 28%. Converting at the end of a tile in one of the two
+// 1 x 512 tokens over 8192 keys, 32 heads on 8: 111 us, 620 TFLOP/s; while a CU is at work its vector units issue for 55%
+// of the time, its matrix cores are busy for 33% and its LDS for 29%. Converting at the end of a tile in one of the two
 // waves, so that the other's products meet it, took 6% longer.
 //
 // Operands: key tile a, k step s is unit a S + s; values of group s and half h of a lane's 16 tokens, their even and odd

@@ -192,9 +192,9 @@ __global__ __launch_bounds__(kWaves * 64) void linear_fp4_stream_kernel(Fp4Linea
 // row m of x lies at u * rows + (m ^ (u & 7)), piece c (32 codes) of row n of W at n * pieces + (c ^ (n & 7)): what
 // 8 lanes write, or read, together lies in different banks. The KW partial sums meet in LDS.
 //
-// 256 rows of bf16, 8192 x 8192: 40 us, 860 TFLOP/s, two thirds of what a large library product reaches. Of a wave's
-// cycles the matrix cores are busy for 37%, vector instructions 31%, LDS 38%, and one block a CU leaves little to overlap
-// them with; a step staged after its products, or two steps in registers, took 2 to 6 us longer.
+// 256 rows of bf16, 8192 x 8192: 38 us, 900 TFLOP/s, 69% of what a large library product reaches. While a CU is at work its
+// matrix cores are busy for 39% of the time, its vector units issue for 28%, its LDS is busy for 39%, and one block a CU
+// leaves little to overlap them with; a step staged after its products, or two steps in registers, took 2 to 6 us longer.
 template <bool F32, int NT, int MT>
 struct TileShape {
     static constexpr int WN = 2, KW = 4;
