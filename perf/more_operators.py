@@ -299,8 +299,8 @@ def _write(rows, latent, k_rope, case):
     fine = torch.isfinite(x).all(-1, keepdim=True)
     most = torch.where(fine, x, 0.0).abs().amax(-1, keepdim=True)
     power = (((most.view(torch.int32) + 0x1FFFFF) >> 23) - 135).clamp(-117, 119)  # the least with most <= 448 * 2^power
-    codes = torch.where(fine, torch.ldexp(x, -power), 0.0).to(torch.float8_e4m3fn)
-    scale = torch.where(fine, torch.ldexp(torch.ones_like(most), power), torch.nan)
+    codes = torch.where(fine, x * (127 - power << 23).view(torch.float32), 0.0).to(torch.float8_e4m3fn)
+    scale = torch.where(fine, (127 + power << 23).view(torch.float32), torch.nan)
     rows[:, :rank], rows[:, rank:rank + k_rope.shape[1]] = codes.view(torch.uint8), k_rope
     rows[:, rank + k_rope.shape[1]:rank + k_rope.shape[1] + 4] = scale.view(torch.uint8)
 
@@ -383,8 +383,8 @@ def _plain_rope(s, case):
 
 
 def _two(power):
-    """2^power, exactly (the device's pow is not)."""
-    return torch.ldexp(torch.ones_like(power), power.int())
+    """2^power in float64, from its exponent bits (the device's pow and ldexp are not exact)."""
+    return (power.long() + 1023 << 52).view(torch.float64)
 
 
 def _e4m3_64(codes):
