@@ -36,10 +36,11 @@ extern "C" {
 
 typedef struct ihipStream_t* mlk_stream_t; /* identical to hipStream_t */
 
-/* Element type of a weight operand. */
+/* Element type of an operand. */
 typedef enum mlk_dtype {
     MLK_DTYPE_F32 = 0,
-    MLK_DTYPE_BF16 = 1
+    MLK_DTYPE_BF16 = 1,
+    MLK_DTYPE_E4M3 = 2 /* of a latent cache alone */
 } mlk_dtype;
 
 /* Attention mask (which keys j a query i sees; queries sit at the trailing
@@ -495,6 +496,72 @@ mlk_status mlk_kv4_attention(const void* q, const int64_t* q_strides, int32_t dt
 mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int64_t x_stride, int32_t dtype,
                           const uint8_t* codes, const uint8_t* scales, const float* bias, int64_t out_features, void* out,
                           mlk_stream_t stream);
+
+/* ------------------------------------------- streaming latent attention -- */
+
+/* The operators of a streamed MLA layer in its absorbed form; the reference has none of them (its MLA forms every key of the
+ * window again, montlok.cpp:1159-1211). A token is cached as its latent (rank R) and a rotated key part (P = rope_dim) that
+ * all heads share; W_k and W_v, the latent's products for a head's keys and values, go to the query and to the output:
+ *   q . (W_k c) = (W_k^T q) . c,     sum_t w_t (W_v c_t) = W_v sum_t w_t c_t.
+ * Activations are fp32 or bf16 (`dtype`, an mlk_dtype), sums are held in fp32 or more, results are rounded once.
+ *
+ * The cache is [pages, page_size, row] bytes, 16-byte aligned, page_size 1 to 65536, R 64, 128, 256 or 512, P 16, 32 or 64.
+ * With MLK_DTYPE_E4M3 a row is R e4m3 codes, P bf16 and 16 bytes that begin with the fp32 scale of the codes; with
+ * MLK_DTYPE_BF16 it is R + P bf16 and 16 unused bytes. `positions` [batch, length] gives every token its place in its
+ * sequence, a negative one is padding; `page_table` [batch, table_width] names a sequence's pages, 2^28 tokens at most.
+ * Entries of pages that no token needs may be anything. Both are contiguous int32. Calls of 2^32 threads or more are
+ * refused: 2^26 tokens of an append or a read, 2^22 blocks of 16 rows (token and head, of one sequence) of an attention. */
+
+/* Rotation of the last rope_dim lanes of every head of q [batch, length, heads, head_dim] and k [.., kv_heads, ..] by
+ * position * frequencies[i] (fp64 [rope_dim / 2], radians): (a, b) -> magnitude (a cos - b sin, b cos + a sin), a and b the
+ * lanes 2 i and 2 i + 1 where `interleaved`, else i and i + rope_dim / 2. The other lanes are copied. Angles in double at
+ * every position; double arithmetic, one rounding. Tokens at negative positions give zeros. Strides are {sequence, token,
+ * head}; q_out, k_out contiguous. head_dim up to 1024. */
+mlk_status mlk_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int32_t dtype,
+                    const double* frequencies, int64_t rope_dim, int32_t interleaved, double magnitude,
+                    const int32_t* positions, int64_t batch, int64_t length, int64_t heads, int64_t kv_heads,
+                    int64_t head_dim, void* q_out, void* k_out, mlk_stream_t stream);
+
+/* Latents [batch, length, R] and key parts [batch, length, P] (strides {sequence, token}) into the cache. e4m3: a row's scale
+ * is the smallest power of two whose 448-fold reaches its largest magnitude (2^-117 to 2^119; larger values are held at 448 *
+ * 2^119), codes are rounded to nearest, ties to even. bf16: rounded to nearest. A latent with an infinity or a NaN (bf16: that rounds to an infinity) becomes NaN.
+ * Tokens at negative positions, past the page table or on a page outside [0, pages) are dropped. The places of one call's
+ * tokens must be distinct. */
+mlk_status mlk_latent_append(const void* latent, const int64_t* latent_strides, const void* k_rope,
+                             const int64_t* k_rope_strides, int32_t dtype, int64_t batch, int64_t length, int64_t rank,
+                             int64_t rope_dim, uint8_t* cache, int32_t cache_dtype, int64_t pages, int64_t page_size,
+                             const int32_t* page_table, int64_t table_width, const int32_t* positions, mlk_stream_t stream);
+
+/* What the cache holds at `positions`, into contiguous latent [batch, length, R] and k_rope [batch, length, P]. Negative
+ * positions give zeros, places that the page table does not name NaN. */
+mlk_status mlk_latent_read(const uint8_t* cache, int32_t cache_dtype, int64_t pages, int64_t page_size,
+                           const int32_t* page_table, int64_t table_width, const int32_t* positions, int64_t batch,
+                           int64_t length, int64_t rank, int64_t rope_dim, int32_t dtype, void* latent, void* k_rope,
+                           mlk_stream_t stream);
+
+/* softmax((q_latent . c + q_rope . r) * scale) c over cached tokens, q_latent [batch, length, heads, R], q_rope [.., P],
+ * strides {sequence, token, head}; out [batch, length, heads, R] contiguous, 16-byte aligned. Without `ancestors` a token
+ * sees the cached tokens 0 .. its position. With ancestors [batch, length] (int64, length <= 64) the call's tokens are a
+ * tree that lies in the cache in the call's order: token i at the place p sees the places below p - i, and p - i + j for
+ * every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one past the page
+ * table, or that sees a token on a page outside [0, pages), NaN. What the cache holds where a token does not see it, of any
+ * bytes, does not reach it. fp32 queries run with fp32 accuracy, bf16 ones with the softmax weights rounded to bf16 for
+ * the product with the latents. The workspace is 16-byte aligned and private to the call until it has run. */
+size_t mlk_latent_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t rank, int64_t rope_dim,
+                                            int32_t dtype, int32_t cache_dtype, int64_t page_size, int64_t table_width);
+mlk_status mlk_latent_attention(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,
+                                const int64_t* q_rope_strides, int32_t dtype, int64_t batch, int64_t length, int64_t heads,
+                                int64_t rank, int64_t rope_dim, const uint8_t* cache, int32_t cache_dtype, int64_t pages,
+                                int64_t page_size, const int32_t* page_table, int64_t table_width, const int32_t* positions,
+                                const int64_t* ancestors, double scale, void* out, void* workspace, size_t workspace_bytes,
+                                mlk_stream_t stream);
+
+/* y[t, h] = W[h] x[t, h]: x [tokens, heads, in_features] (strides {token, head}, in_features dense), W [heads, out_features,
+ * in_features] (strides {head, out, in}, one of the last two 1), y [tokens, heads, out_features] contiguous, 16-byte aligned,
+ * of x's dtype. weight_dtype: bf16, or fp32 with fp32 x. fp32 x keeps fp32 accuracy in both. */
+mlk_status mlk_head_linear(const void* x, int64_t tokens, int64_t heads, int64_t in_features, const int64_t* x_strides,
+                           int32_t dtype, const void* weight, const int64_t* weight_strides, int32_t weight_dtype,
+                           int64_t out_features, void* out, mlk_stream_t stream);
 
 /* --------------------------------------------------------- diagnostics -- */
 

@@ -78,7 +78,8 @@ using OptTensor = std::optional<Tensor>;
     X(mlk_linear_residual) X(mlk_rms_norm_linear) X(mlk_linear_swiglu) X(mlk_mhc_prepare) X(mlk_mhc_combine) X(mlk_mhc_combine_prepare) \
     X(mlk_mamba3_workspace_bytes) X(mlk_mamba3_siso_forward) X(mlk_mamba3_siso_step)                               \
     X(mlk_rms_norm_mamba3_forward) X(mlk_mla_rope_qk) X(mlk_attention) X(mlk_qk_norm_rope) X(mlk_kv4_append)       \
-    X(mlk_kv4_read) X(mlk_kv4_attention_workspace_bytes) X(mlk_kv4_attention) X(mlk_linear_fp4)
+    X(mlk_kv4_read) X(mlk_kv4_attention_workspace_bytes) X(mlk_kv4_attention) X(mlk_linear_fp4)  \
+    X(mlk_rope) X(mlk_latent_append) X(mlk_latent_read) X(mlk_latent_attention_workspace_bytes) X(mlk_latent_attention) X(mlk_head_linear)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -721,6 +722,126 @@ Tensor linear_fp4(const OptTensor& input, const OptTensor& codes_, const OptTens
     return out;
 }
 
+// ------------------------------------------------------------------ streaming latent attention
+
+std::tuple<Tensor, Tensor> rope(const OptTensor& q_, const OptTensor& k_, const OptTensor& frequencies, const OptTensor& positions,
+                                bool interleaved, Real magnitude) {
+    const Tensor &q = activation(q_, "q", 4), &k = activation(k_, "k", 4);
+    const c10::DeviceGuard guard(q.device());
+    typed(k_, "k", q.scalar_type(), "of q's dtype", q);
+    const int64_t batch = q.size(0), length = q.size(1), heads = q.size(2), dim = q.size(3), kv_heads = k.size(2);
+    REQUIRE(k.size(0) == batch && k.size(1) == length && k.size(3) == dim, "k must be [batch, length, kv_heads, head_dim] as q");
+    const Tensor f = typed(frequencies, "frequencies", at::kDouble, "float64", q).contiguous();
+    REQUIRE(f.dim() == 1 && f.size(0) > 0 && 2 * f.size(0) <= dim, "frequencies must be [rope_dim / 2], rope_dim at most head_dim");
+    const Tensor at = positions_of(positions, q, batch, length);
+    const Tensor q_out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    const Tensor k_out = at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous));
+    done(lib.mlk_rope(q.const_data_ptr(), strides_of(q), k.const_data_ptr(), strides_of(k), dtype_of(q),
+                      static_cast<const double*>(f.const_data_ptr()), 2 * f.size(0), interleaved, magnitude, at.const_data_ptr<int32_t>(), batch,
+                      length, heads, kv_heads, dim, q_out.data_ptr(), k_out.data_ptr(), stream()));
+    return {q_out, k_out};
+}
+
+// A latent cache [pages, page_size, row]: what it holds follows from the bytes of a row.
+struct LatentView {
+    Tensor pages, table;
+    int64_t count, page_size, width;
+    int32_t dtype;
+};
+LatentView latent_cache_of(const OptTensor& cache_, const OptTensor& table, const Tensor& like, int64_t batch, int64_t rank, int64_t rope_dim) {
+    const Tensor& cache = typed(cache_, "cache", at::kByte, "uint8", like);
+    REQUIRE(cache.dim() == 3 && cache.is_contiguous(), "cache must be contiguous [pages, page_size, row]");
+    const int64_t row = cache.size(2);
+    const bool e4m3 = row == rank + 2 * rope_dim + 16, bf16 = row == 2 * (rank + rope_dim) + 16;
+    REQUIRE(e4m3 || bf16, "a row of the cache, " + std::to_string(row) + " bytes, does not hold rank " + std::to_string(rank) + " and rope_dim " + std::to_string(rope_dim));
+    LatentView v{cache, index_of(table, "page_table", like), cache.size(0), cache.size(1), 0, e4m3 ? MLK_DTYPE_E4M3 : MLK_DTYPE_BF16};
+    REQUIRE(v.table.size(0) == batch, "page_table must have a row for each sequence");
+    v.width = v.table.size(1);
+    return v;
+}
+
+void latent_append(const OptTensor& latent_, const OptTensor& k_rope_, const OptTensor& cache, const OptTensor& page_table, const OptTensor& positions) {
+    const Tensor &latent = activation(latent_, "latent", 3), &k_rope = activation(k_rope_, "k_rope", 3);
+    const c10::DeviceGuard guard(latent.device());
+    typed(k_rope_, "k_rope", latent.scalar_type(), "of the latent's dtype", latent);
+    const int64_t batch = latent.size(0), length = latent.size(1), rank = latent.size(2), rope_dim = k_rope.size(2);
+    REQUIRE(k_rope.size(0) == batch && k_rope.size(1) == length, "k_rope must be [batch, length, rope_dim] as the latent");
+    const LatentView c = latent_cache_of(cache, page_table, latent, batch, rank, rope_dim);
+    const Tensor at = positions_of(positions, latent, batch, length);
+    const int64_t ls[2] = {latent.stride(0), latent.stride(1)}, rs[2] = {k_rope.stride(0), k_rope.stride(1)};
+    done(lib.mlk_latent_append(latent.const_data_ptr(), ls, k_rope.const_data_ptr(), rs, dtype_of(latent), batch, length, rank, rope_dim,
+                               static_cast<uint8_t*>(c.pages.data_ptr()), c.dtype, c.count, c.page_size, c.table.const_data_ptr<int32_t>(), c.width,
+                               at.const_data_ptr<int32_t>(), stream()));
+}
+
+std::tuple<Tensor, Tensor> latent_read(const OptTensor& cache, const OptTensor& page_table, const OptTensor& positions, Count rank, Count rope_dim,
+                                       bool bf16) {
+    REQUIRE(cache.has_value() && cache->defined(), "cache must be defined");
+    REQUIRE(cache->is_cuda(), "cache must be on the GPU");
+    const c10::DeviceGuard guard(cache->device());
+    const Tensor at = index_of(positions, "positions", *cache);
+    const int64_t batch = at.size(0), length = at.size(1);
+    const LatentView c = latent_cache_of(cache, page_table, *cache, batch, rank, rope_dim);
+    REQUIRE(rank > 0 && rope_dim > 0, "rank and rope_dim must be positive");
+    const auto options = at::TensorOptions().dtype(bf16 ? at::kBFloat16 : at::kFloat).device(cache->device());
+    const Tensor latent = at::empty({batch, length, rank}, options), k_rope = at::empty({batch, length, rope_dim}, options);
+    done(lib.mlk_latent_read(static_cast<const uint8_t*>(c.pages.const_data_ptr()), c.dtype, c.count, c.page_size, c.table.const_data_ptr<int32_t>(),
+                             c.width, at.const_data_ptr<int32_t>(), batch, length, rank, rope_dim, dtype_of(latent), latent.data_ptr(),
+                             k_rope.data_ptr(), stream()));
+    return {latent, k_rope};
+}
+
+Tensor latent_attention(const OptTensor& q_latent_, const OptTensor& q_rope_, const OptTensor& cache, const OptTensor& page_table,
+                        const OptTensor& positions, Real scale, const OptTensor& ancestors_) {
+    const Tensor &q = activation(q_latent_, "q_latent", 4), &qr = activation(q_rope_, "q_rope", 4);
+    const c10::DeviceGuard guard(q.device());
+    typed(q_rope_, "q_rope", q.scalar_type(), "of q_latent's dtype", q);
+    const int64_t batch = q.size(0), length = q.size(1), heads = q.size(2), rank = q.size(3), rope_dim = qr.size(3);
+    REQUIRE(qr.size(0) == batch && qr.size(1) == length && qr.size(2) == heads, "q_rope must be [batch, length, heads, rope_dim] as q_latent");
+    const LatentView c = latent_cache_of(cache, page_table, q, batch, rank, rope_dim);
+    const Tensor at = positions_of(positions, q, batch, length);
+    Tensor ancestors;
+    if (ancestors_.has_value() && ancestors_->defined()) {
+        ancestors = typed(ancestors_, "ancestors", at::kLong, "int64", q).contiguous();
+        REQUIRE(ancestors.dim() == 2 && ancestors.size(0) == batch && ancestors.size(1) == length, "ancestors must be [batch, length]");
+    }
+    const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    const size_t bytes = lib.mlk_latent_attention_workspace_bytes(batch, length, heads, rank, rope_dim, dtype_of(q), c.dtype, c.page_size, c.width);
+    const Tensor ws = bytes == 0 ? Tensor() : at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+    done(lib.mlk_latent_attention(q.const_data_ptr(), strides_of(q), qr.const_data_ptr(), strides_of(qr), dtype_of(q), batch, length, heads, rank,
+                                  rope_dim, static_cast<const uint8_t*>(c.pages.const_data_ptr()), c.dtype, c.count, c.page_size,
+                                  c.table.const_data_ptr<int32_t>(), c.width, at.const_data_ptr<int32_t>(),
+                                  ancestors.defined() ? ancestors.const_data_ptr<int64_t>() : nullptr, scale, out.data_ptr(),
+                                  bytes == 0 ? nullptr : ws.data_ptr(), bytes, stream()));
+    return out;
+}
+
+Tensor head_linear(const OptTensor& x_, const OptTensor& weight_) {
+    REQUIRE(x_.has_value() && x_->defined(), "x must be defined");
+    REQUIRE(x_->is_cuda(), "x must be on the GPU");
+    REQUIRE(x_->scalar_type() == at::kFloat || x_->scalar_type() == at::kBFloat16, "x must be float32 or bfloat16");
+    const Tensor& x = *x_;
+    REQUIRE(x.dim() >= 2, "x must be [..., heads, in_features]");
+    const c10::DeviceGuard guard(x.device());
+    REQUIRE(weight_.has_value() && weight_->defined(), "weight must be defined");
+    REQUIRE(weight_->is_cuda() && weight_->device() == x.device(), "weight must be on the same GPU as the others");
+    REQUIRE(weight_->scalar_type() == at::kBFloat16 || (weight_->scalar_type() == at::kFloat && x.scalar_type() == at::kFloat),
+            "weight must be bfloat16, or float32 with float32 x");
+    REQUIRE(weight_->dim() == 3, "weight must be [heads, out_features, in_features]");
+    const int64_t heads = x.size(-2), k = x.size(-1), n = weight_->size(1);
+    REQUIRE(weight_->size(0) == heads && weight_->size(2) == k, "weight must be [heads, out_features, in_features] with x's heads and features");
+    REQUIRE(heads > 0 && k > 0 && n > 0, "heads and features must be positive");
+    Tensor w = *weight_;
+    if (w.stride(1) != 1 && w.stride(2) != 1) w = w.contiguous();
+    Tensor r = x.dim() == 3 ? x : x.reshape({-1, heads, k});
+    if (r.stride(2) != 1 && k != 1) r = r.contiguous();
+    std::vector<int64_t> sizes = with_last(x, n);
+    const Tensor out = at::empty(sizes, x.options().memory_format(at::MemoryFormat::Contiguous));
+    const int64_t xs[2] = {r.stride(0), r.stride(1)}, ws[3] = {w.stride(0), w.stride(1), w.stride(2)};
+    done(lib.mlk_head_linear(r.const_data_ptr(), r.size(0), heads, k, xs, dtype_of(x), w.const_data_ptr(), ws, dtype_of(w), n, out.data_ptr(), stream()));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -750,5 +871,10 @@ PYBIND11_MODULE(_torch_ops, m) {
     OPERATOR(kv4_read);
     OPERATOR(kv4_attention);
     OPERATOR(linear_fp4);
+    OPERATOR(rope);
+    OPERATOR(latent_append);
+    OPERATOR(latent_read);
+    OPERATOR(latent_attention);
+    OPERATOR(head_linear);
 #undef OPERATOR
 }

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import json
+import math
 import os
 import weakref
 from pathlib import Path
@@ -72,6 +73,12 @@ def _load():
         "mlk_kv4_attention": [_vp, _vp, C.c_int32] + [_i64] * 5 + [_vp, _i64, _i64, _vp, _i64, _vp, _dbl, _vp, _vp,
                                                                    C.c_size_t, _vp],
         "mlk_linear_fp4": [_vp, _i64, _i64, _i64, C.c_int32, _vp, _vp, _vp, _i64, _vp, _vp],
+        "mlk_rope": [_vp, _vp, _vp, _vp, C.c_int32, _vp, _i64, C.c_int32, _dbl, _vp] + [_i64] * 5 + [_vp, _vp, _vp],
+        "mlk_latent_append": [_vp, _vp, _vp, _vp, C.c_int32] + [_i64] * 4 + [_vp, C.c_int32, _i64, _i64, _vp, _i64, _vp, _vp],
+        "mlk_latent_read": [_vp, C.c_int32, _i64, _i64, _vp, _i64, _vp] + [_i64] * 4 + [C.c_int32, _vp, _vp, _vp],
+        "mlk_latent_attention": [_vp, _vp, _vp, _vp, C.c_int32] + [_i64] * 5 +
+                                [_vp, C.c_int32, _i64, _i64, _vp, _i64, _vp, _vp, _dbl, _vp, _vp, C.c_size_t, _vp],
+        "mlk_head_linear": [_vp, _i64, _i64, _i64, _vp, C.c_int32, _vp, _vp, C.c_int32, _i64, _vp, _vp],
         "mlk_math_check": [_vp, _i64, _vp, _vp],
         "mlk_mamba3_siso_recurrent": [_vp, _vp] * 7 + [_vp] + [_i64] * 5 + [_vp, _vp, C.c_size_t, _vp],
         "mlk_mamba3_siso_recurrent_noalloc": [_vp, _vp] * 7 + [_vp] + [_i64] * 5 + [_vp, _vp],
@@ -92,6 +99,8 @@ def _load():
     lib.mlk_mamba3_workspace_bytes.restype = C.c_size_t
     lib.mlk_kv4_attention_workspace_bytes.argtypes = [_i64] * 7
     lib.mlk_kv4_attention_workspace_bytes.restype = C.c_size_t
+    lib.mlk_latent_attention_workspace_bytes.argtypes = [_i64] * 5 + [C.c_int32] * 2 + [_i64] * 2
+    lib.mlk_latent_attention_workspace_bytes.restype = C.c_size_t
     lib.mlk_mla_packed_elems.argtypes = [_i64] * 5
     lib.mlk_mla_packed_elems.restype = C.c_int64
     _lib = lib
@@ -672,6 +681,104 @@ def linear_fp4(input: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     return (_native or _ops()).linear_fp4(input, codes, scales, bias)
 
 
+# ------------------------------------------------------------------ streaming latent attention
+#
+# No counterparts in the reference, whose MLA forms every key of the window again. A token is cached as its latent and a
+# rotated key part that all heads share; the heads' key and value weights go to the query and to the output
+# (``head_linear``). ``positions`` and ``page_table`` are as for the 4-bit cache above.
+
+
+def rope_frequencies(rope_dim: int, theta: float = 10000.0, factor: float = 1.0, original_length: int = 0,
+                     fast: float = 32.0, slow: float = 1.0, device=None) -> tuple[torch.Tensor, float]:
+    """The ``frequencies`` (float64 [rope_dim / 2], radians a position) and ``magnitude`` of ``rope``.
+
+    theta^(-2 i / rope_dim); divided by ``factor`` for contexts that are ``factor`` times as long. With ``original_length``
+    (the context before) pairs that turn more than ``fast`` times over it are kept and those that turn less than ``slow``
+    times are divided, with a straight ramp over the pairs between, and the magnitude is 0.1 ln(factor) + 1 (the method
+    published as YaRN)."""
+    _check(rope_dim > 0 and rope_dim % 2 == 0, "rope_dim must be even and positive")
+    _check(theta > 1 and factor >= 1 and original_length >= 0, "theta must exceed 1, factor be at least 1, original_length not negative")
+    index = torch.arange(rope_dim // 2, dtype=torch.float64)
+    frequencies = theta ** (-2.0 * index / rope_dim)
+    magnitude = 1.0
+    if factor != 1.0 and original_length == 0:
+        frequencies = frequencies / factor
+    elif factor != 1.0:
+        _check(fast > slow > 0, "fast must exceed slow, slow be positive")
+
+        def pair(turns: float) -> float:
+            return rope_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rope_dim // 2 - 1)
+        ramp = ((index - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        frequencies = frequencies * (1 - ramp) + frequencies / factor * ramp
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return frequencies.to("cuda" if device is None else device), magnitude
+
+
+def rope(q: torch.Tensor, k: torch.Tensor, frequencies: torch.Tensor, positions: torch.Tensor, interleaved: bool = False,
+         magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The last R lanes of every head of q [B, L, H, D] and k [B, L, Hkv, D] rotated by position * ``frequencies`` (float64
+    [R / 2]) and multiplied by ``magnitude``, the others copied: lanes 2 i and 2 i + 1 paired where ``interleaved``, else
+    i and i + R / 2. float64 angles and arithmetic, one rounding, new tensors. A negative position gives zeros."""
+    return (_native or _ops()).rope(q, k, frequencies, positions, interleaved, magnitude)
+
+
+def latent_cache(pages: int, page_size: int, rank: int, rope_dim: int, dtype: torch.dtype = torch.float8_e4m3fn,
+                 device=None) -> torch.Tensor:
+    """An empty cache of ``pages`` pages of ``page_size`` tokens (1 to 65536): uint8 [pages, page_size, row], a token's
+    latent of ``rank`` (64, 128, 256 or 512) in eight bits under one power of two (``torch.float8_e4m3fn``) or in bfloat16,
+    and its key part of ``rope_dim`` (16, 32 or 64) in bfloat16. A row's bytes are described in ``include/mlk_hip.h``."""
+    _check(dtype in (torch.float8_e4m3fn, torch.bfloat16), "dtype must be float8_e4m3fn or bfloat16")
+    _check(rank in (64, 128, 256, 512), "rank must be 64, 128, 256 or 512")
+    _check(rope_dim in (16, 32, 64), "rope_dim must be 16, 32 or 64")
+    _check(0 < page_size <= 65536, "page_size must be between 1 and 65536")
+    _check(pages > 0, "pages must be positive")
+    row = rank + 2 * rope_dim + 16 if dtype == torch.float8_e4m3fn else 2 * (rank + rope_dim) + 16
+    return torch.zeros(pages, page_size, row, dtype=torch.uint8, device="cuda" if device is None else device)
+
+
+def latent_append(latent: torch.Tensor, k_rope: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
+                  positions: torch.Tensor) -> None:
+    """latent [B, L, R] and k_rope [B, L, P] into the cache, in place. In eight bits a token's latent is rounded to nearest
+    (ties to even) under the smallest power of two whose 448-fold reaches its largest magnitude; a latent with an infinity
+    or a NaN becomes NaN. Tokens at negative positions or on pages that the table does not name are dropped.
+
+    The places of one call's tokens must be distinct: which token stays at a shared one is not defined."""
+    (_native or _ops()).latent_append(latent, k_rope, cache, page_table, positions)
+
+
+def latent_read(cache: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor, rank: int, rope_dim: int,
+                dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The latents [B, L, R] and key parts [B, L, P] that the cache holds at ``positions`` [B, L]. Negative positions give
+    zeros, places on pages that the table does not name NaN."""
+    _check(dtype in (torch.float32, torch.bfloat16), "dtype must be float32 or bfloat16")
+    return (_native or _ops()).latent_read(cache, page_table, positions, rank, rope_dim, dtype == torch.bfloat16)
+
+
+def latent_attention(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
+                     positions: torch.Tensor, scale: float, ancestors: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax((q_latent . c + q_rope . r) * scale) c over the cached tokens (latent c, key part r) 0 .. ``positions[b, l]``:
+    q_latent [B, L, H, R], q_rope [B, L, H, P] -> [B, L, H, R].
+
+    One new token a sequence, a chunk of a prompt and padded batches are the same call. With ``ancestors`` [B, L] (int64,
+    L <= 64) the tokens of the call are a tree, cached at successive places: token i, at the place p, sees the places below
+    p - i, and p - i + j for every bit j < L that is set (its own bit i among them, if it is to see itself). A token at a
+    negative position, or that sees nothing, gives zeros; one past the page table, or that sees a token on a page that the
+    table does not name, NaN; what the cache holds where a token does not see it does not reach it. float32 queries run
+    with float32 accuracy."""
+    return (_native or _ops()).latent_attention(q_latent, q_rope, cache, page_table, positions, scale, ancestors)
+
+
+def head_linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """Every head's own matrix times its part of x: x [..., H, K], weight [H, N, K] -> [..., H, N], y[h] = weight[h] x[h].
+
+    The weight is dense along its last or its middle dimension (others are copied), so that the rows [H, K, N] of a
+    projection serve as ``w.transpose(1, 2)`` where they are multiplied into the query. bfloat16 weights with x of either
+    type, float32 ones with float32 x; float32 x keeps float32 accuracy."""
+    return (_native or _ops()).head_linear(x, weight)
+
+
 def mla_forward(x, in_proj_weight, q_weight, kv_norm_weight, kv_norm_bias, kv_norm_eps, kv_up_weight, out_weight,
                 cosine, sine, n_heads, head_dim, nope_dim, kv_lora_rank, n_last, causal, scale):
     """montlok.cpp:1159-1211: projection, latent LayerNorm, kv_up, RoPE, attention and output projection.
@@ -996,7 +1103,8 @@ def exported_symbols() -> list[str]:
             "mlk_layer_norm_bf16", "mlk_mla_rope_qk", "mlk_attention", "mlk_mla_attend", "mlk_mla_attend_normed",
             "mlk_mla_forward", "mlk_mla_packed_elems", "mlk_mla_pack_weights", "mlk_mla_forward_packed",
             "mlk_qk_norm_rope", "mlk_kv4_append", "mlk_kv4_read", "mlk_kv4_attention_workspace_bytes",
-            "mlk_kv4_attention", "mlk_linear_fp4"]
+            "mlk_kv4_attention", "mlk_linear_fp4", "mlk_rope", "mlk_latent_append", "mlk_latent_read",
+            "mlk_latent_attention_workspace_bytes", "mlk_latent_attention", "mlk_head_linear"]
 
 
 def empty_kernel(blocks: int, threads: int, dynamic_lds_bytes: int = 0) -> None:

@@ -1,0 +1,263 @@
+"""latent_attention on the GPU against float64: formats, sizes, masks, trees, missing pages, bytes that no token sees."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import latent_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _c():
+    from montlok import _C
+
+    return _C
+
+
+def _queries(g, B, L, H, rank, rope, dtype):
+    return torch.randn(B, L, H, rank, generator=g).to(dtype), torch.randn(B, L, H, rope, generator=g).to(dtype)
+
+
+def _within(got, out, bound):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(out))
+    fine = ~torch.isnan(out)
+    off = ((got - out).abs() / bound)[fine]
+    assert not fine.any() or float(off.max()) <= 1.0, f"{float(off.max()):.3g} of the bound"
+
+
+def _check(dev, q, qr, cache, table, positions, store, scale=None, ancestors=None):
+    rank, rope = q.shape[3], qr.shape[3]
+    scale = (rank + rope) ** -0.5 if scale is None else scale
+    got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), scale,
+                                None if ancestors is None else ancestors.to(dev))
+    out, size, spread = ref.attention(q, qr, cache, table, positions, scale, store, ancestors)
+    assert got.shape == q.shape and got.dtype == q.dtype and got.is_contiguous()
+    _within(got, out, ref.attention_bound(size, spread, out, max(1, int(positions.max()) + 1), rank + rope, q.dtype))
+    return got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("rank", [64, 128, 256, 512])
+@pytest.mark.parametrize("rope", [16, 32, 64])
+@pytest.mark.parametrize("H", [3, 24, 70])
+def test_every_form(dev, dtype, store, rank, rope, H):
+    """One token of two sequences over a short past, and five with a row of padding: every built form once."""
+    g = torch.Generator().manual_seed(rank + rope + H)
+    for L, lengths, page, width in ((1, (1, 200), 64, 4), (5, (67, 130), 24, 40)):
+        table = ref.random_table(g, 2, width, 2 * width + 1)
+        cache = ref.random_cache(g, 2 * width + 1, page, rank, rope, store)
+        positions = torch.tensor([[n - L + i for i in range(L)] for n in lengths], dtype=torch.int32)
+        if L > 1:
+            positions[1, 3] = -1
+        q, qr = _queries(g, 2, L, H, rank, rope, dtype)
+        _check(dev, q, qr, cache, table, positions, store)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("B,L,H,rank,rope,page,lengths", [
+    (1, 1, 1, 64, 16, 1, [1]), (1, 1, 16, 512, 64, 64, [63]), (1, 1, 16, 512, 64, 64, [64]), (1, 1, 17, 512, 64, 64, [65]),
+    (3, 1, 8, 64, 16, 32, [480, 1, 129]), (2, 7, 12, 128, 32, 48, [7, 300]), (1, 1, 128, 512, 64, 256, [1000]),
+    (1, 64, 5, 256, 64, 16, [64]), (2, 33, 16, 64, 32, 100, [33, 150]), (5, 1, 33, 256, 32, 7, [1, 2, 63, 128, 129]),
+    (1, 100, 4, 64, 64, 1000, [613]), (1, 1, 4, 64, 16, 16, [5000])])
+def test_sizes(dev, dtype, store, B, L, H, rank, rope, page, lengths):
+    g = torch.Generator().manual_seed(sum(lengths) + H)
+    width = -(-max(lengths) // page)
+    table = ref.random_table(g, B, width, B * width + 2)
+    cache = ref.random_cache(g, B * width + 2, page, rank, rope, store)
+    positions = torch.tensor([[n - L + i for i in range(L)] for n in lengths], dtype=torch.int32)
+    q, qr = _queries(g, B, L, H, rank, rope, dtype)
+    _check(dev, q, qr, cache, table, positions, store)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("L,H,rank", [(1, 8, 64), (7, 16, 128), (48, 5, 256), (64, 3, 64), (63, 2, 512)])
+def test_trees(dev, dtype, store, L, H, rank):
+    """Random ancestors, words with bits of no token, a tree over no cached text, a padded token and one that sees nothing."""
+    g = torch.Generator().manual_seed(L)
+    B, page, width = 4, 20, 12
+    table = ref.random_table(g, B, width, B * width)
+    cache = ref.random_cache(g, B * width, page, rank, 16, store)
+    base = [0, 1, 100, width * page - L]
+    positions = torch.tensor([[n + i for i in range(L)] for n in base], dtype=torch.int32)
+    ancestors = torch.randint(-2 ** 63, 2 ** 63 - 1, (B, L), generator=g)
+    ancestors[0, 0] = 0
+    ancestors[1] = -1
+    if L > 2:
+        positions[2, 1] = -1
+    q, qr = _queries(g, B, L, H, rank, 16, dtype)
+    got = _check(dev, q, qr, cache, table, positions, store, ancestors=ancestors)
+    assert (got[0, 0] == 0).all()
+    # A chain is the plain call.
+    chain = torch.tensor([[min(2 ** (i + 1) - 1, 2 ** 63 - 1) if i < 63 else -1 for i in range(L)]] * B)
+    scale = (rank + 16) ** -0.5
+    args = (q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), scale)
+    assert torch.equal(_c().latent_attention(*args, chain.to(dev)), _c().latent_attention(*args))
+
+
+@pytest.mark.parametrize("store", [E4M3, BF16])
+def test_a_tree_at_places_before_the_sequence(dev, store):
+    """Token i at a place below i: the tree would begin before the sequence, and what lies there is not seen."""
+    g = torch.Generator().manual_seed(9)
+    table, cache = ref.random_table(g, 1, 2, 2), ref.random_cache(g, 2, 16, 64, 16, store)
+    positions = torch.tensor([[0, 0, 1, 5]], dtype=torch.int32)
+    ancestors = torch.tensor([[1, 3, 7, 15]])
+    q, qr = _queries(g, 1, 4, 2, 64, 16, F32)
+    _check(dev, q, qr, cache, table, positions, store, ancestors=ancestors)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("rank,H", [(64, 4), (512, 16), (512, 64), (128, 40)])
+def test_what_no_token_sees_does_not_reach_it(dev, dtype, store, rank, H):
+    """Any bytes behind each token's position, in the same tile and page, and pages that only later tokens name."""
+    g = torch.Generator().manual_seed(rank + H)
+    page, width, L = 48, 5, 3
+    table = ref.random_table(g, 2, width, 2 * width)
+    cache = ref.random_cache(g, 2 * width, page, rank, 32, store)
+    positions = torch.tensor([[30, 70, 71], [5, -1, 100]], dtype=torch.int32)
+    q, qr = _queries(g, 2, L, H, rank, 32, dtype)
+    clean = _check(dev, q, qr, cache, table, positions, store)
+    for b, last in ((0, 71), (1, 100)):
+        flat = cache[table[b].long()].flatten(0, 1)
+        flat[last + 1:] = 255  # NaN in every format
+        flat[last + 1::3] = torch.randint(0, 256, flat[last + 1::3].shape, generator=g, dtype=torch.uint8)
+        cache[table[b].long()] = flat.view(width, page, -1)
+    table[0, 2:], table[1, 3:] = -1, 2 ** 31 - 1
+    assert torch.equal(_check(dev, q, qr, cache, table, positions, store), clean)
+    # A row of no numbers between tokens of one call: those before it keep their results, those after it get NaN.
+    row = cache[table[0, 1].item(), 50 - page]
+    row[:] = 255
+    got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), (rank + 32) ** -0.5)
+    assert torch.equal(got[0, 0], clean[0, 0]) and torch.isnan(got[0, 1:]).all() and torch.equal(got[1], clean[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_infinite_latent_of_another_token(dev, dtype):
+    """Bytes of infinities in a bf16 cache, seen by the later token only."""
+    g = torch.Generator().manual_seed(3)
+    cache, table = ref.random_cache(g, 1, 64, 64, 16, BF16), torch.zeros(1, 1, dtype=torch.int32)
+    positions = torch.tensor([[9, 20]], dtype=torch.int32)
+    q, qr = _queries(g, 1, 2, 4, 64, 16, dtype)
+    clean = _check(dev, q, qr, cache, table, positions, BF16)
+    cache[0, 15].view(BF16)[3] = torch.inf
+    got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), 80 ** -0.5)
+    assert torch.equal(got[0, 0], clean[0, 0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_missing_pages_and_places_past_the_table(dev, dtype):
+    g = torch.Generator().manual_seed(6)
+    cache = ref.random_cache(g, 4, 16, 64, 16, E4M3)
+    table = torch.tensor([[1, -1, 4, 0], [2, 3, 2 ** 31 - 1, -2 ** 31], [0, 1, 2, 3]], dtype=torch.int32)
+    positions = torch.tensor([[15, 16, 40, 63, 64], [31, 32, -1, 2 ** 31 - 1, 0], [63, 10 ** 6, -2 ** 31, 62, 64]], dtype=torch.int32)
+    q, qr = _queries(g, 3, 5, 6, 64, 16, dtype)
+    got = _check(dev, q, qr, cache, table, positions, E4M3)
+    assert torch.isnan(got).all(-1).all(-1).tolist() == [[False, True, True, True, True], [False, True, False, True, False],
+                                                        [False, True, False, False, True]]
+
+
+@pytest.mark.parametrize("store", [E4M3, BF16])
+def test_rows_of_nan_and_of_extreme_scales(dev, store):
+    """A token that append made NaN; latents near the largest and the smallest numbers."""
+    c = _c()
+    x = torch.randn(1, 40, 64, generator=torch.Generator().manual_seed(8))
+    x[0, 10] *= 1e30
+    x[0, 20] *= 1e-30
+    words = torch.randn(1, 40, 16, generator=torch.Generator().manual_seed(9))
+    table = torch.tensor([[1, 0, 2]], dtype=torch.int32)
+    cache = c.latent_cache(3, 16, 64, 16, store, dev)
+    at = torch.arange(40, dtype=torch.int32)[None]
+    c.latent_append(x.to(dev), words.to(dev), cache, table.to(dev), at.to(dev))
+    q, qr = _queries(torch.Generator().manual_seed(7), 1, 40, 4, 64, 16, F32)
+    q[:, :, 1] = 0
+    _check(dev, q * 1e-3, qr, cache.cpu(), table, at, store, scale=1e-4)
+    x[0, 30, 5] = torch.nan
+    c.latent_append(x.to(dev), words.to(dev), cache, table.to(dev), at.to(dev))
+    got = c.latent_attention(q.to(dev), qr.to(dev), cache, table.to(dev), at.to(dev), 1e-4)
+    assert not torch.isnan(got[0, :30]).any() and torch.isnan(got[0, 30:]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,rank", [(5, 64), (16, 512), (40, 512)])
+def test_long_and_uneven_sequences_in_parts(dev, dtype, H, rank):
+    """Keys in parts over the chip, a sequence so short that most parts are empty, a table with room to spare."""
+    g = torch.Generator().manual_seed(H)
+    page, width = 64, 320
+    lengths = [9000, 3, 4096, 1]
+    pages = sum(-(-n // page) for n in lengths)
+    cache = ref.random_cache(g, pages, page, rank, 32, E4M3)
+    table, at = torch.full((4, width), -1, dtype=torch.int32), 0
+    for b, n in enumerate(lengths):
+        need = -(-n // page)
+        table[b, :need] = torch.arange(at, at + need)
+        at += need
+    positions = torch.tensor([[n - 1] for n in lengths], dtype=torch.int32)
+    q, qr = _queries(g, 4, 1, H, rank, 32, dtype)
+    q *= 3  # a few tokens carry the weight
+    _check(dev, q, qr, cache, table, positions, E4M3)
+    # Scores that rise towards the end: the maximum moves in every tile.
+    cache = cache.clone()
+    flat = cache.view(-1, cache.shape[-1])
+    flat[:141 * 64, rank:rank + 2] = (torch.arange(141 * 64)[:, None] / 100).to(BF16).view(torch.uint8)
+    qr[..., 0] = rank ** 0.5 * 3
+    _check(dev, q, qr, cache, table, positions, E4M3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_views_at_any_alignment_and_order(dev, dtype):
+    """Queries as parts of wider heads at odd elements, heads before tokens, and a table and positions that are views."""
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(2, 6, 5, 64 + 16 + 3, generator=g).to(dtype)  # [B, H, L, ..]
+    cache, table = ref.random_cache(g, 8, 16, 64, 16, E4M3), ref.random_table(g, 2, 4, 8)
+    positions = torch.tensor([[50, 51, 52, 53, 54], [3, 4, 5, 6, 7]], dtype=torch.int32)
+    q, qr = wide[..., 1:65].transpose(1, 2), wide[..., 66:82].transpose(1, 2)
+    expect = _check(dev, q.contiguous(), qr.contiguous(), cache, table, positions, E4M3)
+    d = wide.to(dev)
+    got = _c().latent_attention(d[..., 1:65].transpose(1, 2), d[..., 66:82].transpose(1, 2), cache.to(dev),
+                                table.t().contiguous().to(dev).t(), positions.t().contiguous().to(dev).t(), 80 ** -0.5)
+    assert torch.equal(got, expect)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tree", [False, True])
+def test_in_a_graph_and_on_streams(dev, dtype, tree):
+    """A captured call, replayed at further positions with other queries, and eager calls between the replays; two streams at
+    once. Each result equals the eager call's, bit for bit."""
+    c, g = _c(), torch.Generator().manual_seed(11)
+    B, L, H, rank, page, width = 3, 4, 16, 512, 64, 40
+    cache, table = ref.random_cache(g, B * width, page, rank, 64, E4M3).to(dev), ref.random_table(g, B, width, B * width).to(dev)
+    q, qr = (t.to(dev) for t in _queries(g, B, L, H, rank, 64, dtype))
+    at = torch.tensor([[100 + 50 * b + i for i in range(L)] for b in range(B)], dtype=torch.int32, device=dev)
+    words = torch.randint(0, 16, (B, L), generator=g).to(dev) if tree else None
+    call = lambda: c.latent_attention(q, qr, cache, table, at, 0.04, words)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for replay in range(4):
+        q.copy_(torch.randn(q.shape, generator=g).to(dtype))
+        at += 311
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call()), f"replay {replay}"
+    expect = call()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        one = [call() for _ in range(5)]
+    two = [call() for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, expect) for t in one + two)
