@@ -11,7 +11,9 @@ rotate_half halves, attention with the reference's mask conventions, o_proj.
 RoPE tables are built with torch on the CPU exactly as the upstream
 token-index RoPE does (rope.py:9-16, 138-166) and cached per device. With bf16
 weights the attention contractions also run on bf16 matrix cores.
-KV caches, padding masks and morphological RoPE are not built.
+``step`` takes new tokens of streams whose latents are cached (``new_state``):
+kv_up's products go to the query and to the output, so that the heads read the
+cached latents themselves. Padding masks and morphological RoPE are not built.
 """
 
 from __future__ import annotations
@@ -120,7 +122,8 @@ class MLAHIP(nn.Module):
 
     def _check(self, x, word_pos=None, morph_depth=None, attn_mask=None, cache=None) -> None:
         if cache is not None or attn_mask is not None or word_pos is not None or morph_depth is not None:
-            raise RuntimeError("MLAHIP: KV caches, attention masks and morphological positions are not built")
+            raise RuntimeError("MLAHIP: attention masks, morphological positions and the caches of other modules are not "
+                               "built (new_state and step serve streams)")
         if self.training:
             raise RuntimeError("MLAHIP: inference only (call .eval())")
         require_gpu_inference(type(self).__name__, x, _FAMILY)
@@ -190,6 +193,48 @@ class MLAHIP(nn.Module):
         precision = torch.bfloat16 if self.o_proj.weight.dtype == torch.bfloat16 else torch.float32
         out = c.attention(q, k, v, mask, self.scale, precision).view(bsz, n_last, self.d_model)
         return c.linear(out, self.o_proj.weight)
+
+    def new_state(self, streams: int, max_length: int, dtype: torch.dtype = torch.bfloat16, page_size: int = 64,
+                  device=None) -> dict:
+        """An empty cache for ``streams`` sequences of up to ``max_length`` tokens, latents in bfloat16 or, as
+        ``torch.float8_e4m3fn``, in eight bits (kv_lora_rank 64, 128, 256 or 512, rope_dim 16, 32 or 64)."""
+        if streams <= 0 or max_length <= 0 or page_size <= 0:
+            raise ValueError("streams, max_length and page_size must be positive")
+        device = device if device is not None else self.o_proj.weight.device
+        pages = -(-max_length // page_size)
+        table = torch.arange(streams * pages, dtype=torch.int32, device=device).view(streams, pages)
+        return {"cache": ext().latent_cache(streams * pages, page_size, self.kv_lora_rank, self.rope_dim, dtype, device),
+                "page_table": table, "length": torch.zeros(streams, 1, dtype=torch.int32, device=device),
+                "frequencies": self.rope.freqs.double().to(device)}
+
+    def step(self, u: torch.Tensor, state: dict) -> torch.Tensor:
+        """The next token ``u [S, d_model]`` of every stream, or the next ``[S, L, d_model]``; ``state`` advances in place
+        and outputs have u's shape. Each token sees what its stream held and the call's tokens up to itself. The result is
+        ``forward``'s over the stream but for the cached latents' and key parts' rounding; tokens past max_length give
+        NaN."""
+        if u.ndim not in (2, 3) or u.shape[-1] != self.d_model:
+            raise ValueError("MLAHIP.step expects [streams, d_model] or [streams, length, d_model]")
+        if self.training:
+            raise RuntimeError("MLAHIP: inference only (call .eval())")
+        require_gpu_inference(type(self).__name__, u, _FAMILY)
+        c = ext()
+        x = u.unsqueeze(1) if u.ndim == 2 else u
+        with_q = self.q_lora_rank == 0
+        projected = c.linear(x, self._in_proj_weight(with_q))
+        q_width = self.n_heads * self.head_dim if with_q else 0
+        q = (projected[..., :q_width] if with_q else self._project_q_rows(x)).unflatten(-1, (self.n_heads, self.head_dim))
+        latent = c.layer_norm(projected[..., q_width:q_width + self.kv_lora_rank], self.kv_norm.weight, self.kv_norm.bias,
+                              self.kv_norm.eps)
+        at = state["length"] + torch.arange(x.shape[1], dtype=torch.int32, device=x.device)
+        q_rope, k_rope = c.rope(q[..., self.nope_dim:], projected[..., None, q_width + self.kv_lora_rank:],
+                                state["frequencies"], at)
+        c.latent_append(latent, k_rope[:, :, 0], state["cache"], state["page_table"], at)
+        rows = self.kv_up.weight.detach().view(self.n_heads, self.nope_dim + self.head_dim, self.kv_lora_rank)
+        q_latent = c.head_linear(q[..., :self.nope_dim], rows[:, :self.nope_dim].transpose(1, 2))
+        seen = c.latent_attention(q_latent, q_rope, state["cache"], state["page_table"], at, self.scale)
+        values = c.head_linear(seen, rows[:, self.nope_dim:])
+        state["length"] += x.shape[1]
+        return c.linear(values.flatten(2), self.o_proj.weight).view(u.shape)
 
 
 MLACPU = MLAHIP
