@@ -33,12 +33,13 @@ __device__ __forceinline__ Byte* row_of(Byte* bytes, const LatentCache& c, int64
     return bytes + (static_cast<int64_t>(id) * c.page_size + (token - page * static_cast<uint32_t>(c.page_size))) * row;
 }
 
-// Eight e4m3 codes as bf16 values, exactly (NaN for 0x7F and 0xFF).
-__device__ __forceinline__ bf16x8 e4m3_octet(uint32_t lo, uint32_t hi) {
-    const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
-                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+// Eight e4m3 codes times a power of two as bf16 values, exactly (NaN for 0x7F and 0xFF, and under a scale of NaN: all codes
+// under every exponent byte).
+__device__ __forceinline__ bf16x8 e4m3_octet(uint32_t lo, uint32_t hi, float scale) {
+    const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
     return __builtin_bit_cast(bf16x8, v);
 }
 

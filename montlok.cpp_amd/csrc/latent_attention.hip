@@ -5,6 +5,7 @@
 // One pass over a sequence's rows with a running maximum and sum; all heads of a token, and all tokens of a call, read the
 // same rows.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -16,6 +17,15 @@ namespace {
 // Read in place of rows that no page holds, or that no token of a block sees.
 __device__ const uint8_t kZeroRow[2 * (512 + 64) + 16] __attribute__((aligned(16))) = {};
 
+// Read in place of rows on pages that the table does not name: NaN in every format.
+struct Filled {
+    uint8_t bytes[2 * (512 + 64) + 16];
+    constexpr explicit Filled(uint8_t v) : bytes{} {
+        for (auto& b : bytes) b = v;
+    }
+};
+__device__ const Filled kMissingRow __attribute__((aligned(16))) (0xFF);
+
 struct LatentAttentionArgs {
     const void *q, *qr;
     int64_t qs[3], rs[3];
@@ -24,8 +34,12 @@ struct LatentAttentionArgs {
     const int64_t* ancestors;  // or null
     void* out;
     float* partial;  // [sequence][row][split][R], then the maxima and sums [sequence][row][split][2]
+    float* stats;     // maxima and sums of the parts
+    int32_t* starts;  // tiles before each unit
     int32_t length, heads, rows, row_blocks, splits;
-    float scale;  // times log2(e)
+    int32_t units, shares;  // 0 shares: a unit a block
+    float scale;      // times log2(e), not negative
+    uint32_t negate;  // the sign bits of two bf16 where it was
 };
 
 constexpr int kTile = 64;   // tokens of a tile
@@ -56,6 +70,7 @@ __device__ __forceinline__ void load_row_pieces(const uint8_t* from, uint32_t to
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void wait_for_rows() {
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0, the other counters at their most
     asm volatile("" ::: "memory");
 }
@@ -146,6 +161,8 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
                         v[4 + i] = __uint_as_float(hi[i]);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = p.negate == 0 ? v[i] : -v[i];
                 bf16x8 plane[3];
                 planes_of<true>(v, plane);
 #pragma unroll
@@ -219,7 +236,7 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
 #pragma unroll
             for (int t = 0; t < KS / 2; ++t) {
                 const u32x4 v = *reinterpret_cast<const u32x4*>(key + 64 * t + 16 * g);
-                const bf16x8 a = e4m3_octet(v[0], v[1]), c = e4m3_octet(v[2], v[3]);
+                const bf16x8 a = e4m3_octet(v[0], v[1], 1.0f), c = e4m3_octet(v[2], v[3], 1.0f);
 #pragma unroll
                 for (int m = 0; m < RT; ++m)
 #pragma unroll
@@ -358,7 +375,7 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
                 if constexpr (E4M3) {
                     const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                         (__attribute__((address_space(3))) i32x2*)(rows + (32 * t + 8 * g + l / 2) * ROW + column + 8 * (l & 1)));
-                    v = e4m3_octet(x[0], x[1]);
+                    v = e4m3_octet(x[0], x[1], 1.0f);
                 } else {
                     i16x4 x[2];
 #pragma unroll
@@ -421,27 +438,611 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
     }
 }
 
-// The parts of a row, R / 4 lanes a row.
-template <int R, bool F32>
-__global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, const float* stats, int64_t rows, int splits, void* out) {
-    constexpr int LANES = R / 4;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
-    const int column = threadIdx.x % LANES * 4;
-    if (row >= rows) return;
-    float top = -INFINITY;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, stats[(row * splits + i) * 2]);
-    const float under = finite_or_zero(top);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float sum = 0.0f;
-    for (int i = 0; i < splits; ++i) {
-        const int64_t part = row * splits + i;
-        const float by = __builtin_amdgcn_exp2f(stats[part * 2] - under), total = stats[part * 2 + 1];
-        if (total == 0.0f) continue;  // nothing seen: its sums may not have been written
-        sum = fmaf(total, by, sum);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(partial + part * R + column);
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// The maximum, or the sum, of a row: its scores lie with the lanes l and l + 32.
+__device__ __forceinline__ float max_over_halves(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(x[0]), __int_as_float(x[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(x[0]) + __int_as_float(x[1]);
+}
+
+// At most N of the loads that this wave asked for are still on their way.
+template <int N>
+__device__ __forceinline__ void wait_for_rows_but() {
+    static_assert(N >= 0 && N < 64, "the counter's range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | 0x0F70 | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+
+// A row's sums are rescaled when its maximum has grown by more than this (log2): weights are then at most 2^16, which
+// changes no rounding, and after a row's first tokens next to no tile rescales.
+constexpr float kSlack = 16.0f;
+
+// What a token of a call sees: the places below `base`, and base + j where bit j is set; nothing from `end` on.
+struct Sight {
+    int base, end;
+    uint64_t bits;
+    bool beyond;  // past the table
+};
+__device__ __forceinline__ Sight sight_of(const LatentAttentionArgs& p, int64_t sequence, int token) {
+    const int64_t at = sequence * p.length + token;
+    const int32_t position = p.positions[at];
+    Sight s{0, 0, 0, position >= static_cast<int64_t>(p.c.width) * p.c.page_size};
+    if (position < 0 || s.beyond) return s;
+    s.end = s.base = position + 1;
+    if (p.ancestors == nullptr) return s;
+    s.base = position - token;
+    s.bits = static_cast<uint64_t>(p.ancestors[at]);
+    if (p.length < 64) s.bits &= (uint64_t{1} << p.length) - 1;
+    s.end = max(s.bits == 0 ? s.base : s.base + 64 - __builtin_clzll(s.bits), 0);
+    return s;
+}
+
+constexpr int kMaxUnits = 1024;  // that blocks share out among them
+constexpr int kLeastShare = 2;   // tiles of a block, so that a block is worth its beginning
+constexpr int kIds = 512;  // page numbers that are looked up at a time
+
+// Waves of two kinds, RW groups of 32 rows: a scorer takes the rows' scores of 32 tokens of a tile (KW of them a group) and
+// turns them into weights, a summer adds those tokens' latents to half of the rows' columns, and sees to the loads. Scorers
+// hold the queries, summers the sums: what either holds leaves room for a wave of the other kind on its SIMD, and the one's
+// exponents and conversions run beside the other's products (both in one wave, which then has a SIMD to itself: 6500 cycles a
+// tile of 64 tokens and 64 rows, of which the matrix cores are busy for 2200).
+//
+// A tile is scored while the one before it is summed, with one barrier between.
+template <int R, int P, bool E4M3, int RW>
+struct Shape {
+    static constexpr int ROW = row_bytes<E4M3>(R, P), KW = 64 * ROW * 3 <= 140 * 1024 ? 2 : 1, KEYS = 32 * KW, BYTES = KEYS * ROW;
+    static constexpr int STAGES = BYTES * 4 <= 76 * 1024 ? 4 : 3;
+    static constexpr int SCORERS = RW * KW, SUMMERS = RW * 2, WAVES = SCORERS + SUMMERS;
+    static constexpr int LOADS = BYTES / 1024 + (BYTES % 1024 != 0);  // of 64 lanes, 16 bytes each
+};
+
+template <int R, int P, bool E4M3, int RW>
+__global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent_attention_rows_kernel(LatentAttentionArgs p) {
+    using S = Shape<R, P, E4M3, RW>;
+    constexpr int ROW = S::ROW, KW = S::KW, KEYS = S::KEYS, STAGES = S::STAGES, SUMMERS = S::SUMMERS, PIECES = ROW / 16;
+    constexpr int KS = R / 16, RS = P / 16, CT = R / 64;  // 16-deep steps over the latent and the key part, 32-wide tiles of columns
+    // Tiles are asked for AHEAD iterations before they are scored; their rows' addresses are set one before that, and the page
+    // numbers for these looked up one before that again, so that each is there for all summers after a barrier.
+    constexpr int AHEAD = STAGES - 2;
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[STAGES][S::BYTES];
+    __shared__ bf16x8 shared_weights[2][RW][KW][2][64];
+    __shared__ const uint8_t* row_at[2][KEYS];
+    __shared__ __attribute__((aligned(16))) float scales[S::SCORERS][32];
+    __shared__ float tops[RW][KW][32], factors[RW][32];
+    __shared__ int32_t ids[2][kIds];
+    __shared__ int ends[RW];
+    __shared__ int starts[kMaxUnits + 1];
+    __shared__ int grown[2], odd[2];  // 1 + the tile where a maximum has outgrown its row's, or a score is no number
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const bool scorer = wave < S::SCORERS;
+    const int rw = scorer ? wave / KW : (wave - S::SCORERS) / 2, part = scorer ? wave % KW : (wave - S::SCORERS) % 2;
+
+    // The block's share: of the tiles of all units (RW * 32 rows of a sequence), laid end to end, as many as any other block's;
+    // or one unit.
+    int unit = blockIdx.x, from_tile = 0, until = INT_MAX, share_first = 0;
+    if (p.shares != 0) {
+        for (int u = threadIdx.x; u < p.units; u += S::WAVES * 64) {
+            const int64_t sequence = u / p.row_blocks;
+            const int row0 = static_cast<int>(u - sequence * p.row_blocks) * (RW * 32), row1 = min(row0 + RW * 32, p.rows) - 1;
+            int end = 1;  // a unit that sees nothing has outputs all the same
+            for (int t = row0 / p.heads; t <= row1 / p.heads; ++t) end = max(end, sight_of(p, sequence, t).end);
+            starts[u + 1] = (end + KEYS - 1) / KEYS;
+        }
+        __syncthreads();
+        if (wave == 0) {  // sums of everything before: a run of units a lane, then the lanes
+            const int lane = threadIdx.x;
+            const int run = (p.units + 63) / 64, u0 = min(lane * run, p.units), u1 = min(u0 + run, p.units);
+            int sum = 0;
+            for (int u = u0; u < u1; ++u) sum += starts[u + 1];
+            int before = sum;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = fmaf(v[j], by, acc[j]);
+            for (int m = 1; m < 64; m *= 2) {
+                const int other = __shfl_up(before, m, kWave);
+                before += lane >= m ? other : 0;
+            }
+            before -= sum;
+            for (int u = u0; u < u1; ++u) starts[u + 1] = before += starts[u + 1];
+            if (lane == 0) starts[0] = 0;
+        }
+        __syncthreads();
+        const int total = starts[p.units], each = max((total + p.shares - 1) / p.shares, kLeastShare);
+        share_first = blockIdx.x * each;
+        until = min(share_first + each, total);
+        if (blockIdx.x == 0) {  // for the join
+            for (int u = threadIdx.x; u <= p.units; u += S::WAVES * 64) p.starts[u] = starts[u];
+        }
+        if (share_first >= until) return;
+        int low = 0, high = p.units - 1;  // the last unit that begins at or before the share
+        while (low < high) {
+            const int middle = (low + high + 1) / 2;
+            if (starts[middle] <= share_first) low = middle;
+            else high = middle - 1;
+        }
+        unit = __builtin_amdgcn_readfirstlane(low);
+        from_tile = __builtin_amdgcn_readfirstlane(share_first - starts[unit]);
+        until = __builtin_amdgcn_readfirstlane(until);
     }
+
+    for (int part_of_share = 0;; ++part_of_share) {
+    // Formed anew for every part: what follows from the lane alone is otherwise kept through all of them, in registers that the
+    // loop over tiles needs.
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int h = lane >> 5, l = lane & 31;
+    const int64_t b = unit / p.row_blocks;
+    const int row0 = static_cast<int>(unit - b * p.row_blocks) * (RW * 32), row = row0 + 32 * rw + l;
+    const bool real = row < p.rows;
+    const int token_of_row = row / p.heads, head = row - token_of_row * p.heads;
+    Sight sight{0, 0, 0, false};
+    if (real) sight = sight_of(p, b, token_of_row);
+    const bool beyond = sight.beyond;
+    const int base = sight.base;
+    const uint64_t bits = sight.bits;
+    int all = sight.end, every = real ? base : INT_MAX;  // where the tokens that some row sees end, and those that every row of the wave sees
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        all = max(all, __shfl_xor(all, m, kWave));
+        every = min(every, __shfl_xor(every, m, kWave));
+    }
+    const int plain = __builtin_amdgcn_readfirstlane(every);
+    if (!scorer) ends[rw] = all;
+    if (threadIdx.x < 2) grown[threadIdx.x] = odd[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RW; ++i) all = max(all, ends[i]);
+    all = __builtin_amdgcn_readfirstlane(all);
+
+    const int tile_count = (all + KEYS - 1) / KEYS;
+    const int unit_start = p.shares == 0 ? 0 : starts[unit], unit_end = p.shares == 0 ? INT_MAX : starts[unit + 1];
+    const int first = min(from_tile, tile_count), last = p.shares == 0 ? tile_count : min(until - unit_start, tile_count);
+    const bool whole = p.shares == 0 || (from_tile == 0 && until >= unit_end);
+    // A share has at most two parts of units, its first and its last.
+    const int64_t at_row = b * p.rows + row, place = (static_cast<int64_t>(blockIdx.x) * 2 + (part_of_share != 0)) * (RW * 32) + 32 * rw + l;
+
+    if (scorer) {
+        float top = -INFINITY, sum = 0.0f;
+        if (first < last) {
+            bf16x8 q[KS + RS];
+            {
+                // A lane without a row takes the first row's: what it makes of it goes nowhere.
+                const int64_t ql = b * p.qs[0] + (real ? token_of_row * p.qs[1] + head * p.qs[2] : 0);
+                const int64_t qr = b * p.rs[0] + (real ? token_of_row * p.rs[1] + head * p.rs[2] : 0);
+#pragma unroll
+                for (int t = 0; t < KS + RS; ++t) {
+                    // The dimensions that the lane's piece of a row holds: codes come 16 to a piece, bf16 values 8.
+                    const int d = t >= KS ? 16 * (t - KS) + 8 * h : E4M3 ? 32 * (t / 2) + 16 * h + 8 * (t % 2) : 16 * t + 8 * h;
+                    u32x4 v = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(t < KS ? p.q : p.qr) + (t < KS ? ql : qr) + d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] ^= p.negate;  // a negative scale is the queries'
+                    q[t] = __builtin_bit_cast(bf16x8, v);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD + 2; ++i) __syncthreads();  // page numbers, the rows' addresses of AHEAD tiles, the first tile
+            int stage = 0;
+            for (int tile = first; tile < last; ++tile) {
+                const uint8_t* const rows = tiles[stage];
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+                // Scores of the wave's tokens with the lane's row: register i holds token 8 (i / 4) + 4 h + i % 4. Pieces of the
+                // key row are read four ahead of their use, and turned into an operand beside the product before theirs; nothing
+                // moves over the bars (the scheduler on its own reads each piece right before it is used).
+                f32x16 s = {};
+                const uint8_t* const key = rows + (32 * part + l) * ROW;
+                constexpr int PARTS = E4M3 ? KS / 2 : KS, ALL = PARTS + RS, RING = ALL < 4 ? ALL : 4;
+                auto piece = [&](int t) {
+                    return *reinterpret_cast<const u32x4*>(key + (t < PARTS ? 32 * t : (E4M3 ? R : 2 * R) + 32 * (t - PARTS)) + 16 * h);
+                };
+                float scale = 1.0f;
+                if constexpr (E4M3) scale = *reinterpret_cast<const float*>(key + R + 2 * P);
+                u32x4 ring[RING];
+#pragma unroll
+                for (int t = 0; t < RING; ++t) ring[t] = piece(t);
+                if constexpr (E4M3) scales[wave][l] = scale;
+                __builtin_amdgcn_sched_barrier(0);
+                auto operand = [&](int k) {  // of product k; its piece makes room for the one four on
+                    const int t = !E4M3 ? k : k < KS ? k / 2 : k - KS + PARTS;
+                    const u32x4 x = ring[t % RING];
+                    const bool codes = E4M3 && k < KS;
+                    if (t + RING < ALL && (!codes || k % 2 == 1)) ring[t % RING] = piece(t + RING);
+                    return codes ? e4m3_octet(x[k % 2 * 2], x[k % 2 * 2 + 1], scale) : __builtin_bit_cast(bf16x8, x);
+                };
+                bf16x8 next = operand(0);
+#pragma unroll
+                for (int k = 0; k < KS + RS; ++k) {
+                    const bf16x8 now = next;
+                    if (k + 1 < KS + RS) next = operand(k + 1);
+                    s = mfma(now, q[k], s);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int first_token = tile * KEYS + 32 * part;
+                const bool masked = first_token + 32 > plain;
+                if (masked) {
+                    float none = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        none = fmaf(s[i], 0.0f, none);  // NaN once a score is an infinity or none
+                        const int past = first_token + 8 * (i / 4) + 4 * h + i % 4 - base;
+                        const bool seen = (past < 0) | ((past < 64) & static_cast<bool>(bits >> (past & 63) & 1));
+                        s[i] = seen ? s[i] : -INFINITY;
+                    }
+                    if (__any(none != none)) odd[tile & 1] = tile + 1;
+                }
+                float most = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+                most = max_over_halves(most);
+                most = most == -INFINITY ? most : most * p.scale;  // a scale of 0 is one too
+
+                float total;
+                auto weigh = [&] {
+                    const float under = finite_or_zero(top);
+                    total = 0.0f;
+                    u32x4 packed[2];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        f32x4 key_scale;
+                        if constexpr (E4M3) key_scale = *reinterpret_cast<const f32x4*>(&scales[wave][2 * i + 4 * h]);
+                        float e[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], p.scale, -under));
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) e[j] = s[i + j] == -INFINITY ? 0.0f : e[j];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) total += e[j];
+                        if constexpr (E4M3) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) e[j] = e[j] * key_scale[j];
+                            if (masked) {  // a scale of NaN is no matter to a row that does not see its token
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) e[j] = s[i + j] == -INFINITY ? 0.0f : e[j];
+                            }
+                        }
+                        // Rounded to bf16 for the product with the latents: 2^-8 of a weight at most, without a bias; the sum keeps them whole.
+                        packed[i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(e[0]), static_cast<__bf16>(e[1])});
+                        packed[i / 8][i / 2 % 4 + 1] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(e[2]), static_cast<__bf16>(e[3])});
+                    }
+                    shared_weights[tile & 1][rw][part][0][lane] = __builtin_bit_cast(bf16x8, packed[0]);
+                    shared_weights[tile & 1][rw][part][1][lane] = __builtin_bit_cast(bf16x8, packed[1]);
+                };
+                // Weights under the maximum so far, which all waves of the rows know. Where it is outgrown they learn the others'
+                // and weigh again, and the summers rescale.
+                weigh();
+                tops[rw][part][l] = most;
+                if (__any(most > top + kSlack)) grown[tile & 1] = tile + 1;
+                __syncthreads();
+                if (__builtin_expect(grown[tile & 1] == tile + 1, 0)) {
+                    float now = top;
+#pragma unroll
+                    for (int i = 0; i < KW; ++i) now = fmaxf(now, tops[rw][i][l]);
+                    const float by = __builtin_amdgcn_exp2f(top - finite_or_zero(now));
+                    if (part == 0) factors[rw][l] = by;
+                    top = now;
+                    sum *= by;
+                    weigh();
+                    __syncthreads();
+                }
+                sum += total;
+            }
+        }
+        sum = sum_over_halves(sum);
+        tops[rw][part][l] = sum;
+        __syncthreads();
+        if (!whole && part == 0 && h == 0) {
+#pragma unroll
+            for (int i = 1; i < KW; ++i) sum += tops[rw][i][l];
+            p.stats[place * 2] = top;
+            p.stats[place * 2 + 1] = beyond ? NAN : sum;
+        }
+    } else {
+
+    // A summer. Row addresses: of the pages whose numbers ids[] holds, by one wave, a token a lane.
+    const int own = wave - S::SCORERS;
+    const uint32_t page_size = static_cast<uint32_t>(p.c.page_size);
+    int held_page[2] = {0, 0}, held_end = first, holds = 0;  // ids[i] begins with page held_page[i]; ids[holds] serves tiles before held_end
+    auto hold = [&](int tile) {
+        const int page0 = static_cast<int>(static_cast<uint32_t>(tile) * KEYS / page_size);
+        held_end = static_cast<int>((static_cast<int64_t>(page0) + kIds) * page_size / KEYS);
+        holds ^= 1;
+        held_page[holds] = page0;
+        for (int i = own * 64 + lane; i < kIds; i += SUMMERS * 64) {
+            const int page = page0 + i;
+            ids[holds][i] = page < p.c.width ? p.c.table[b * p.c.width + page] : -1;
+        }
+    };
+    auto set_rows = [&](int tile, int which) {
+        if (lane < KEYS) {
+            const uint32_t token = static_cast<uint32_t>(tile) * KEYS + lane, page = token / page_size;
+            const uint8_t* at = kZeroRow;
+            if (static_cast<int>(token) < all) {
+                const int32_t page_id = ids[which][page - held_page[which]];
+                const bool held = page_id >= 0 && page_id < p.c.pages;
+                at = held ? p.c.bytes + (static_cast<int64_t>(page_id) * page_size + (token - page * page_size)) * ROW : kMissingRow.bytes;
+            }
+            row_at[tile & 1][lane] = at;
+        }
+    };
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)tiles[0]));
+    auto load_tile = [&](int tile, int stage) {
+        // All addresses are read before the first load: the compiler moves nothing past one.
+        constexpr int N = (S::LOADS + SUMMERS - 1) / SUMMERS;
+        const uint8_t* from[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = min((i * SUMMERS + own) * 64 + lane, KEYS * PIECES - 1), r = piece / PIECES;
+            from[i] = row_at[tile & 1][r] + (piece - r * PIECES) * 16;
+        }
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * S::BYTES + own * 1024);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((i + 1) * SUMMERS * 64 <= KEYS * PIECES || (i * SUMMERS + own) * 64 + lane < KEYS * PIECES) load_row_pieces(from[i], to + i * SUMMERS * 1024);
+    };
+    f32x16 acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = f32x16{};
+
+    // The latents of the tokens whose weights a lane holds, eight of a column: the rows' bytes turned as they are read.
+    auto add_tile = [&](int tile, const uint8_t* rows) {
+        constexpr int VS = 2 * KW, GROUP = E4M3 && CT % 2 == 0 ? 2 : 1, N = GROUP * VS;  // column tiles read ahead of their products
+        struct Codes {
+            i32x2 v;
+        };
+        struct Words {
+            i16x4 lo, hi;
+        };
+        using Fragment = std::conditional_t<E4M3, Codes, Words>;
+        const uint8_t* const at0 = rows + (E4M3 ? 1 : 2) * (part * CT * 32 + 16 * (lane >> 4 & 1)) +
+                                   (E4M3 ? ((lane >> 1 & 3) + 8 * (lane >> 3 & 1) + 4 * h) * ROW + 8 * (lane & 1) : ((lane >> 2 & 3) + 4 * h) * ROW + 8 * (lane & 3));
+        auto read = [&](Fragment (&f)[N], int c) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint8_t* const at = at0 + (i / GROUP) * 16 * ROW + (c + i % GROUP) * (E4M3 ? 32 : 64);
+                if constexpr (E4M3) {
+                    f[i].v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)at);
+                } else {
+                    f[i].lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
+                    f[i].hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at + 8 * ROW));
+                }
+            }
+        };
+        // A latent that is no number makes its scores none, and the weight of every row that sees it; where a row does not, its
+        // weight 0 has to meet a number. Seldom: rows that were written hold numbers, and a scale of NaN.
+        auto scrub = [&](Fragment (&f)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t byte = 255u << (8 * (k & 3)), nan = 127u << (8 * (k & 3)), word = static_cast<uint32_t>(f[i].v[k / 4]);
+                        if ((word & nan) == nan) f[i].v[k / 4] = static_cast<int>(word & ~byte);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if ((f[i].lo[k] & 0x7F80) == 0x7F80) f[i].lo[k] = 0;
+                        if ((f[i].hi[k] & 0x7F80) == 0x7F80) f[i].hi[k] = 0;
+                    }
+                }
+            }
+        };
+        Fragment ahead[2][N];
+        read(ahead[0], 0);
+        bf16x8 w[VS];
+#pragma unroll
+        for (int i = 0; i < VS; ++i) w[i] = shared_weights[tile & 1][rw][i / 2][i % 2][lane];
+        const bool tainted = odd[tile & 1] == tile + 1;
+#pragma unroll
+        for (int c = 0; c < CT; c += GROUP) {
+            Fragment(&f)[N] = ahead[c / GROUP & 1];
+            if (c + GROUP < CT) read(ahead[c / GROUP + 1 & 1], c + GROUP);
+            if (__builtin_expect(tainted, 0)) scrub(f);
+            auto latents = [&](int i) {
+                if constexpr (E4M3) return e4m3_octet(f[i].v[0], f[i].v[1], 1.0f);
+                else return __builtin_bit_cast(bf16x8, __builtin_shufflevector(f[i].lo, f[i].hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            bf16x8 next = latents(0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bf16x8 now = next;
+                if (i + 1 < N) next = latents(i + 1);
+                acc[c + i % GROUP] = mfma(now, w[i / GROUP], acc[c + i % GROUP]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    if (first < last) {
+        hold(first);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (own == 0) set_rows(first + i, holds);
+            __syncthreads();
+            if (first + i < last) load_tile(first + i, i);
+        }
+        if (own == 0) set_rows(first + AHEAD, holds);
+        if (first + AHEAD <= last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
+        else wait_for_rows();
+        __syncthreads();
+        int stage = 0;  // of the tile that is scored
+        for (int tile = first; tile < last; ++tile) {
+            // The stage that is loaded now was summed in the iteration before this one.
+            if (tile + AHEAD < last) load_tile(tile + AHEAD, stage >= STAGES - AHEAD ? stage + AHEAD - STAGES : stage + AHEAD);
+            const int which = holds;
+            if (tile + AHEAD + 2 < last && tile + AHEAD + 2 >= held_end) hold(tile + AHEAD + 2);
+            if (own == tile % SUMMERS && tile + AHEAD + 1 < last) set_rows(tile + AHEAD + 1, which);
+            if (tile > first) add_tile(tile - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1]);
+            if (tile + AHEAD < last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
+            else wait_for_rows();
+            __syncthreads();
+            if (__builtin_expect(grown[tile & 1] == tile + 1, 0)) {
+                __syncthreads();
+                if (tile > first) {
+                    const float by = factors[rw][l];
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] *= by;
+                }
+            }
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        }
+        add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1]);
+    }
+    __syncthreads();  // the rows' sums
+    const int column = part * (R / 2) + 4 * h;
+    if (whole && real) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) sum += tops[rw][i][l];
+        // A row that sees nothing has no sum: zeros. One past the table: NaN.
+        const float inverse = beyond ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* const to = static_cast<uint16_t*>(p.out) + at_row * R + column;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[c][4 * j + e] * inverse;
+                *reinterpret_cast<u32x2*>(to + 32 * c + 8 * j) = u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1])}),
+                                                                       __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[2]), static_cast<__bf16>(x[3])})};
+            }
+    } else if (!whole && first < last) {
+        float* const to = p.partial + place * R + column;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4*>(to + 32 * c + 8 * j) = f32x4{acc[c][4 * j], acc[c][4 * j + 1], acc[c][4 * j + 2], acc[c][4 * j + 3]};
+    }
+    }
+    if (p.shares == 0 || until <= unit_end) return;
+    ++unit;
+    from_tile = 0;
+    __syncthreads();
+    }
+}
+
+// The parts of a unit's rows: a row and COLUMNS of its columns a block, 4 a lane, as many parts at a time as the lanes allow.
+template <int R, int COLUMNS>
+__global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionArgs p, int rows_per_unit) {
+    constexpr int LANES = COLUMNS / 4, GROUPS = 256 / LANES, BATCH = 8;
+    __shared__ float by[256];
+    __shared__ float reduced[4];
+    __shared__ f32x4 sums[GROUPS][LANES];
+    const int unit = blockIdx.x / (rows_per_unit * (R / COLUMNS)), in = blockIdx.x % (rows_per_unit * (R / COLUMNS));
+    const int r = in / (R / COLUMNS), column = in % (R / COLUMNS) * COLUMNS + threadIdx.x % LANES * 4, group = threadIdx.x / LANES;
+    const int64_t b = unit / p.row_blocks;
+    const int row = static_cast<int>(unit - b * p.row_blocks) * rows_per_unit + r;
+    if (row >= p.rows) return;
+    // The shares that hold the unit's tiles: share g is of tiles each * g ..; where it is a share's first unit its part is the first.
+    const int begin = p.starts[unit], end = p.starts[unit + 1], total = p.starts[p.units];
+    const int each = max((total + p.shares - 1) / p.shares, kLeastShare), g0 = begin / each, parts = (end - 1) / each - g0 + 1;
+    if (parts == 1) return;
+    auto place = [&](int i) { return (static_cast<int64_t>(g0 + i) * 2 + (i == 0 && begin > g0 * each)) * rows_per_unit + r; };
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const bool mine = static_cast<int>(threadIdx.x) < parts;  // at most 256 of them
+    const float top = mine ? p.stats[place(threadIdx.x) * 2] : -INFINITY;
+    const float sum0 = mine ? p.stats[place(threadIdx.x) * 2 + 1] : 0.0f;
+    float most = top;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m, kWave));
+    if (lane == 0) reduced[wave] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(reduced[0], reduced[1]), fmaxf(reduced[2], reduced[3]));
+    const float factor = __builtin_amdgcn_exp2f(top - finite_or_zero(most));
+    by[threadIdx.x] = sum0 == 0.0f ? 0.0f : factor;  // of a part that saw nothing: its sums may not have been written
+    float sum = sum0 == 0.0f ? 0.0f : sum0 * factor;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m, kWave);
+    __syncthreads();
+    if (lane == 0) reduced[wave] = sum;
+    __syncthreads();
+    sum = (reduced[0] + reduced[1]) + (reduced[2] + reduced[3]);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = group; i < parts; i += GROUPS * BATCH) {
+        f32x4 v[BATCH];
+        float f[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int j = i + k * GROUPS;
+            f[k] = j < parts ? by[j] : 0.0f;
+            if (f[k] != 0.0f) v[k] = *reinterpret_cast<const f32x4*>(p.partial + place(j) * R + column);
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (f[k] != 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = fmaf(v[k][j], f[k], acc[j]);
+            }
+        }
+    }
+    if constexpr (GROUPS > 1) {
+        sums[group][threadIdx.x % LANES] = acc;
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i) acc += sums[i][threadIdx.x];
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    acc *= inverse;
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + (b * p.rows + row) * R + column) =
+        u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[0]), static_cast<__bf16>(acc[1])}),
+              __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[2]), static_cast<__bf16>(acc[3])})};
+}
+
+// The parts of a row, 64 columns a block: 16 lanes side by side, 16 parts at a time.
+template <int R, bool F32>
+__global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, const float* stats, int splits, void* out) {
+    __shared__ float by[256];
+    __shared__ float reduced[4];
+    __shared__ f32x4 sums[16][16];
+    const int64_t row = blockIdx.x / (R / 64);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, group = threadIdx.x / 16, column = blockIdx.x % (R / 64) * 64 + threadIdx.x % 16 * 4;
+    const float* const from = partial + (row * splits + group) * R + column;
+    // Every load is issued before the first is waited for; a part that saw nothing may hold anything.
+    f32x4 v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (group + 16 * i < splits) v[i] = *reinterpret_cast<const f32x4*>(from + 16 * i * R);
+    const bool mine = static_cast<int>(threadIdx.x) < splits;  // at most 256 of them
+    const float top = mine ? stats[(row * splits + threadIdx.x) * 2] : -INFINITY;
+    const float total = mine ? stats[(row * splits + threadIdx.x) * 2 + 1] : 0.0f;
+    float most = top;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m, kWave));
+    if (lane == 0) reduced[wave] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(reduced[0], reduced[1]), fmaxf(reduced[2], reduced[3]));
+    const float factor = __builtin_amdgcn_exp2f(top - finite_or_zero(most));
+    by[threadIdx.x] = total == 0.0f ? 0.0f : factor;
+    float sum = total == 0.0f ? 0.0f : total * factor;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m, kWave);
+    __syncthreads();
+    if (lane == 0) reduced[wave] = sum;
+    __syncthreads();
+    sum = (reduced[0] + reduced[1]) + (reduced[2] + reduced[3]);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float f = group + 16 * i < splits ? by[group + 16 * i] : 0.0f;
+        if (f != 0.0f) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = fmaf(v[i][j], f, acc[j]);
+        }
+    }
+    sums[group][threadIdx.x % 16] = acc;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) acc += sums[i][threadIdx.x];
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc *= inverse;
     if constexpr (F32) {
@@ -454,48 +1055,64 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, 
 }
 
 struct Plan {
-    int tiles;  // of 16 rows a block
-    int64_t row_blocks, splits, workspace;
+    int64_t row_blocks, splits, units, shares, workspace;
 };
-// Row tiles a block by the rows a sequence has: the cache is read, and turned into bf16, once for all of them.
+constexpr int kChip = 256;  // compute units
+// Rows a block by the rows a sequence has: the cache is read, and turned into bf16, once for all of them.
+int64_t rows_per_block(int64_t rows, bool f32) { return f32 ? 16 : rows <= 32 ? 32 : 64; }
 Plan plan_of(int64_t batch, int64_t rows, int64_t rank, bool f32, int64_t capacity) {
     Plan plan{};
-    plan.tiles = f32 || rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    plan.row_blocks = ceil_div(rows, 16 * plan.tiles);
-    const int64_t blocks = batch * plan.row_blocks, tiles = ceil_div(capacity, kTile);
-    plan.splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(tiles / 2, 256), ceil_div(512, std::max<int64_t>(blocks, 1))));
-    plan.workspace = plan.splits == 1 ? 0 : batch * rows * plan.splits * (rank + 2) * 4;
+    const int64_t per = rows_per_block(rows, f32);
+    plan.row_blocks = ceil_div(rows, per);
+    plan.units = batch * plan.row_blocks;
+    const int64_t tiles = ceil_div(capacity, kTile);
+    if (f32) {
+        plan.splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(tiles / 2, 256), ceil_div(512, std::max<int64_t>(plan.units, 1))));
+        plan.workspace = plan.splits == 1 ? 0 : batch * rows * plan.splits * (rank + 2) * 4;
+        return plan;
+    }
+    // Shares where there are few units; with more a unit a block balances well enough, and has nothing to join.
+    if (plan.units <= kMaxUnits && tiles > kLeastShare && plan.units * 2 * tiles < (int64_t{1} << 31)) {
+        plan.shares = kChip;
+        plan.workspace = plan.shares * 2 * per * (rank + 2) * 4 + (kMaxUnits + 1) * 4;
+    }
     return plan;
 }
 
 template <int R, int P, bool F32, bool E4M3>
-void launch_attention(const LatentAttentionArgs& p, int tiles, int64_t blocks, hipStream_t s) {
+void launch_attention(const LatentAttentionArgs& p, int64_t blocks, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(blocks));
     if constexpr (F32) {
         hipLaunchKernelGGL((latent_attention_kernel<R, P, true, E4M3, 1, 4>), grid, dim3(256), 0, s, p);
     } else {
-        if (tiles == 1) hipLaunchKernelGGL((latent_attention_kernel<R, P, false, E4M3, 1, 4>), grid, dim3(256), 0, s, p);
-        else if (tiles == 2) hipLaunchKernelGGL((latent_attention_kernel<R, P, false, E4M3, 2, 4>), grid, dim3(256), 0, s, p);
-        else if constexpr (R >= 256) hipLaunchKernelGGL((latent_attention_kernel<R, P, false, E4M3, 4, 8>), grid, dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((latent_attention_kernel<R, P, false, E4M3, 4, 4>), grid, dim3(256), 0, s, p);
+        const int64_t rows = rows_per_block(p.rows, false);
+        if (rows == 32) hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, 1>), grid, dim3(Shape<R, P, E4M3, 1>::WAVES * 64), 0, s, p);
+        else hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, 2>), grid, dim3(Shape<R, P, E4M3, 2>::WAVES * 64), 0, s, p);
     }
 }
 template <int R, int P>
-void launch_attention(const LatentAttentionArgs& p, bool f32, bool e4m3, int tiles, int64_t blocks, hipStream_t s) {
-    if (f32) e4m3 ? launch_attention<R, P, true, true>(p, tiles, blocks, s) : launch_attention<R, P, true, false>(p, tiles, blocks, s);
-    else e4m3 ? launch_attention<R, P, false, true>(p, tiles, blocks, s) : launch_attention<R, P, false, false>(p, tiles, blocks, s);
+void launch_attention(const LatentAttentionArgs& p, bool f32, bool e4m3, int64_t blocks, hipStream_t s) {
+    if (f32) e4m3 ? launch_attention<R, P, true, true>(p, blocks, s) : launch_attention<R, P, true, false>(p, blocks, s);
+    else e4m3 ? launch_attention<R, P, false, true>(p, blocks, s) : launch_attention<R, P, false, false>(p, blocks, s);
 }
 template <int R>
-void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool e4m3, int tiles, int64_t blocks, hipStream_t s) {
-    if (rope == 16) launch_attention<R, 16>(p, f32, e4m3, tiles, blocks, s);
-    else if (rope == 32) launch_attention<R, 32>(p, f32, e4m3, tiles, blocks, s);
-    else launch_attention<R, 64>(p, f32, e4m3, tiles, blocks, s);
+void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool e4m3, int64_t blocks, hipStream_t s) {
+    if (rope == 16) launch_attention<R, 16>(p, f32, e4m3, blocks, s);
+    else if (rope == 32) launch_attention<R, 32>(p, f32, e4m3, blocks, s);
+    else launch_attention<R, 64>(p, f32, e4m3, blocks, s);
+    if (!f32) {
+        if (p.shares == 0) return;
+        const int per = static_cast<int>(rows_per_block(p.rows, false));
+        // Few rows of many parts: 64 columns a block.
+        if (p.units * 16 <= p.shares) hipLaunchKernelGGL((latent_join_rows_kernel<R, 64>), dim3(static_cast<unsigned>(p.units * per * (R / 64))), dim3(256), 0, s, p, per);
+        else hipLaunchKernelGGL((latent_join_rows_kernel<R, R>), dim3(static_cast<unsigned>(p.units * per)), dim3(256), 0, s, p, per);
+        return;
+    }
     if (p.splits == 1) return;
     const int64_t rows = blocks / p.splits / p.row_blocks * p.rows;
     const float* const stats = p.partial + rows * p.splits * R;
-    const dim3 grid(static_cast<unsigned>(ceil_div(rows, 1024 / R)));
-    if (f32) hipLaunchKernelGGL((latent_join_kernel<R, true>), grid, dim3(256), 0, s, p.partial, stats, rows, p.splits, p.out);
-    else hipLaunchKernelGGL((latent_join_kernel<R, false>), grid, dim3(256), 0, s, p.partial, stats, rows, p.splits, p.out);
+    const dim3 grid(static_cast<unsigned>(rows * (R / 64)));
+    hipLaunchKernelGGL((latent_join_kernel<R, true>), grid, dim3(256), 0, s, p.partial, stats, p.splits, p.out);
 }
 
 mlk_status check_attention(int64_t batch, int64_t length, int64_t heads) {
@@ -552,14 +1169,22 @@ extern "C" mlk_status mlk_latent_attention(const void* q_latent, const int64_t* 
     p.rows = static_cast<int32_t>(length * heads);
     p.row_blocks = static_cast<int32_t>(plan.row_blocks);
     p.splits = static_cast<int32_t>(plan.splits);
-    p.scale = static_cast<float>(scale * 1.4426950408889634074);
-    const int64_t blocks = batch * plan.row_blocks * plan.splits;
+    p.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634074);
+    p.negate = std::signbit(scale) ? 0x80008000u : 0;
+    p.units = static_cast<int32_t>(plan.units);
+    p.shares = static_cast<int32_t>(plan.shares);
+    if (plan.shares != 0) {
+        const int64_t parts = plan.shares * 2 * rows_per_block(p.rows, f32);
+        p.stats = p.partial + parts * rank;
+        p.starts = reinterpret_cast<int32_t*>(p.stats + parts * 2);
+    }
+    const int64_t blocks = f32 ? plan.units * plan.splits : plan.shares != 0 ? plan.shares : plan.units;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (rank) {
-        case 64: launch_attention<64>(p, rope_dim, f32, e4m3, plan.tiles, blocks, s); break;
-        case 128: launch_attention<128>(p, rope_dim, f32, e4m3, plan.tiles, blocks, s); break;
-        case 256: launch_attention<256>(p, rope_dim, f32, e4m3, plan.tiles, blocks, s); break;
-        default: launch_attention<512>(p, rope_dim, f32, e4m3, plan.tiles, blocks, s); break;
+        case 64: launch_attention<64>(p, rope_dim, f32, e4m3, blocks, s); break;
+        case 128: launch_attention<128>(p, rope_dim, f32, e4m3, blocks, s); break;
+        case 256: launch_attention<256>(p, rope_dim, f32, e4m3, blocks, s); break;
+        default: launch_attention<512>(p, rope_dim, f32, e4m3, blocks, s); break;
     }
     return launch_status("latent attention");
 }
