@@ -38,6 +38,7 @@ struct LatentAttentionArgs {
     int32_t* starts;  // tiles before each unit
     int32_t length, heads, rows, row_blocks, splits;
     int32_t units, shares;  // 0 shares: a unit a block
+    int32_t wide;           // the cache is larger than an offset of 32 bits reaches
     float scale;      // times log2(e), not negative
     uint32_t negate;  // the sign bits of two bf16 where it was
 };
@@ -67,6 +68,11 @@ typedef __attribute__((address_space(3))) const uint8_t LdsByte;
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 as a clobber: nothing else here uses it
 __device__ __forceinline__ void load_row_pieces(const uint8_t* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+}
+// The same from `from` + offset. Beside waves that keep the matrix cores busy the form above is issued once in 246 cycles, this
+// one once in 71 as without them: a vector of 64-bit addresses waits for the matrix instructions' operands.
+__device__ __forceinline__ void load_row_pieces(const uint8_t* from, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(to) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void wait_for_rows() {
@@ -502,17 +508,19 @@ struct Shape {
     static constexpr int LOADS = BYTES / 1024 + (BYTES % 1024 != 0);  // of 64 lanes, 16 bytes each
 };
 
-template <int R, int P, bool E4M3, int RW>
+template <int R, int P, bool E4M3, int RW, bool WIDE>
 __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent_attention_rows_kernel(LatentAttentionArgs p) {
     using S = Shape<R, P, E4M3, RW>;
     constexpr int ROW = S::ROW, KW = S::KW, KEYS = S::KEYS, STAGES = S::STAGES, SUMMERS = S::SUMMERS, PIECES = ROW / 16;
     constexpr int KS = R / 16, RS = P / 16, CT = R / 64;  // 16-deep steps over the latent and the key part, 32-wide tiles of columns
-    // Tiles are asked for AHEAD iterations before they are scored; their rows' addresses are set one before that, and the page
-    // numbers for these looked up one before that again, so that each is there for all summers after a barrier.
-    constexpr int AHEAD = STAGES - 2;
+    // Tiles are asked for AHEAD iterations before they are scored. Where their pieces lie is read at the end of the iteration
+    // before that, from addresses set in the one before, from page numbers looked up one before that: each is there for all
+    // summers after a barrier.
+    constexpr int AHEAD = STAGES - 2, SLOTS = AHEAD == 1 ? 4 : 8;
     __shared__ __attribute__((aligned(16))) uint8_t tiles[STAGES][S::BYTES];
     __shared__ bf16x8 shared_weights[2][RW][KW][2][64];
-    __shared__ const uint8_t* row_at[2][KEYS];
+    __shared__ uint64_t row_at[SLOTS][KEYS];      // offsets of a tile's rows in the cache, or addresses where these are wide
+    __shared__ uint32_t missing[SLOTS][KEYS];     // all ones where a token's page is missing: its row becomes NaN
     __shared__ __attribute__((aligned(16))) float scales[S::SCORERS][32];
     __shared__ float tops[RW][KW][32], factors[RW][32];
     __shared__ int32_t ids[2][kIds];
@@ -525,7 +533,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
 
     // The block's share: of the tiles of all units (RW * 32 rows of a sequence), laid end to end, as many as any other block's;
     // or one unit.
-    int unit = blockIdx.x, from_tile = 0, until = INT_MAX, share_first = 0;
+    int unit = blockIdx.x, from_tile = 0, until = INT_MAX, share = 0;
     if (p.shares != 0) {
         for (int u = threadIdx.x; u < p.units; u += S::WAVES * 64) {
             const int64_t sequence = u / p.row_blocks;
@@ -552,7 +560,9 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
         }
         __syncthreads();
         const int total = starts[p.units], each = max((total + p.shares - 1) / p.shares, kLeastShare);
-        share_first = blockIdx.x * each;
+        // Neighbouring shares on one XCD, whose cache then holds one sequence's rows for many units.
+        share = blockIdx.x % 8 * (p.shares / 8) + blockIdx.x / 8;
+        const int share_first = share * each;
         until = min(share_first + each, total);
         if (blockIdx.x == 0) {  // for the join
             for (int u = threadIdx.x; u <= p.units; u += S::WAVES * 64) p.starts[u] = starts[u];
@@ -603,7 +613,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     const int first = min(from_tile, tile_count), last = p.shares == 0 ? tile_count : min(until - unit_start, tile_count);
     const bool whole = p.shares == 0 || (from_tile == 0 && until >= unit_end);
     // A share has at most two parts of units, its first and its last.
-    const int64_t at_row = b * p.rows + row, place = (static_cast<int64_t>(blockIdx.x) * 2 + (part_of_share != 0)) * (RW * 32) + 32 * rw + l;
+    const int64_t at_row = b * p.rows + row, place = (static_cast<int64_t>(share) * 2 + (part_of_share != 0)) * (RW * 32) + 32 * rw + l;
 
     if (scorer) {
         float top = -INFINITY, sum = 0.0f;
@@ -624,7 +634,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 }
             }
 #pragma unroll
-            for (int i = 0; i < AHEAD + 2; ++i) __syncthreads();  // page numbers, the rows' addresses of AHEAD tiles, the first tile
+            for (int i = 0; i < 3; ++i) __syncthreads();  // page numbers, row addresses, the first tile
             int stage = 0;
             for (int tile = first; tile < last; ++tile) {
                 const uint8_t* const rows = tiles[stage];
@@ -640,10 +650,12 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 };
                 float scale = 1.0f;
                 if constexpr (E4M3) scale = *reinterpret_cast<const float*>(key + R + 2 * P);
+                const uint32_t lost = missing[tile % SLOTS][32 * part + l];
                 u32x4 ring[RING];
 #pragma unroll
                 for (int t = 0; t < RING; ++t) ring[t] = piece(t);
                 if constexpr (E4M3) scales[wave][l] = scale;
+                ring[0][0] |= lost;
                 __builtin_amdgcn_sched_barrier(0);
                 auto operand = [&](int k) {  // of product k; its piece makes room for the one four on
                     const int t = !E4M3 ? k : k < KS ? k / 2 : k - KS + PARTS;
@@ -653,11 +665,15 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                     return codes ? e4m3_octet(x[k % 2 * 2], x[k % 2 * 2 + 1], scale) : __builtin_bit_cast(bf16x8, x);
                 };
                 bf16x8 next = operand(0);
+                f32x4 key_scale[4];
 #pragma unroll
                 for (int k = 0; k < KS + RS; ++k) {
                     const bf16x8 now = next;
                     if (k + 1 < KS + RS) next = operand(k + 1);
                     s = mfma(now, q[k], s);
+                    if constexpr (E4M3) {
+                        if (k >= KS + RS - 4) key_scale[k - (KS + RS - 4)] = *reinterpret_cast<const f32x4*>(&scales[wave][8 * (k - (KS + RS - 4)) + 4 * h]);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const int first_token = tile * KEYS + 32 * part;
@@ -670,6 +686,8 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                         const int past = first_token + 8 * (i / 4) + 4 * h + i % 4 - base;
                         const bool seen = (past < 0) | ((past < 64) & static_cast<bool>(bits >> (past & 63) & 1));
                         s[i] = seen ? s[i] : -INFINITY;
+                        // A scale of NaN is no matter to a row that does not see its token.
+                        if constexpr (E4M3) key_scale[i / 4][i % 4] = seen ? key_scale[i / 4][i % 4] : 0.0f;
                     }
                     if (__any(none != none)) odd[tile & 1] = tile + 1;
                 }
@@ -683,31 +701,23 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 auto weigh = [&] {
                     const float under = finite_or_zero(top);
                     total = 0.0f;
+                    float e[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale, -under));
+                    if (masked && p.scale == 0.0f) {  // the infinity of an unseen token times 0
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) e[i] = s[i] == -INFINITY ? 0.0f : e[i];
+                    }
                     u32x4 packed[2];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        f32x4 key_scale;
-                        if constexpr (E4M3) key_scale = *reinterpret_cast<const f32x4*>(&scales[wave][2 * i + 4 * h]);
-                        float e[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], p.scale, -under));
-                        if (masked) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) e[j] = s[i + j] == -INFINITY ? 0.0f : e[j];
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) total += e[j];
+                    for (int i = 0; i < 16; i += 2) {
+                        total += e[i] + e[i + 1];
                         if constexpr (E4M3) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) e[j] = e[j] * key_scale[j];
-                            if (masked) {  // a scale of NaN is no matter to a row that does not see its token
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) e[j] = s[i + j] == -INFINITY ? 0.0f : e[j];
-                            }
+                            e[i] *= key_scale[i / 4][i % 4];
+                            e[i + 1] *= key_scale[i / 4][i % 4 + 1];
                         }
                         // Rounded to bf16 for the product with the latents: 2^-8 of a weight at most, without a bias; the sum keeps them whole.
-                        packed[i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(e[0]), static_cast<__bf16>(e[1])});
-                        packed[i / 8][i / 2 % 4 + 1] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(e[2]), static_cast<__bf16>(e[3])});
+                        packed[i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(e[i]), static_cast<__bf16>(e[i + 1])});
                     }
                     shared_weights[tile & 1][rw][part][0][lane] = __builtin_bit_cast(bf16x8, packed[0]);
                     shared_weights[tile & 1][rw][part][1][lane] = __builtin_bit_cast(bf16x8, packed[1]);
@@ -759,37 +769,67 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     };
     auto set_rows = [&](int tile, int which) {
         if (lane < KEYS) {
-            const uint32_t token = static_cast<uint32_t>(tile) * KEYS + lane, page = token / page_size;
-            const uint8_t* at = kZeroRow;
-            if (static_cast<int>(token) < all) {
-                const int32_t page_id = ids[which][page - held_page[which]];
-                const bool held = page_id >= 0 && page_id < p.c.pages;
-                at = held ? p.c.bytes + (static_cast<int64_t>(page_id) * page_size + (token - page * page_size)) * ROW : kMissingRow.bytes;
-            }
-            row_at[tile & 1][lane] = at;
+            // Behind the last token that some row sees that token's row again, which stands for nothing there.
+            const uint32_t token = min(static_cast<uint32_t>(tile) * KEYS + lane, static_cast<uint32_t>(all) - 1), page = token / page_size;
+            const int32_t page_id = ids[which][page - held_page[which]];
+            const bool held = page_id >= 0 && page_id < p.c.pages;
+            const uint64_t at = held ? (static_cast<uint64_t>(page_id) * page_size + (token - page * page_size)) * ROW : 0;
+            row_at[tile % SLOTS][lane] = WIDE ? reinterpret_cast<uint64_t>(p.c.bytes) + at : at;
+            missing[tile % SLOTS][lane] = held ? 0 : 0xFFFFFFFFu;
         }
     };
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)tiles[0]));
-    auto load_tile = [&](int tile, int stage) {
-        // All addresses are read before the first load: the compiler moves nothing past one.
-        constexpr int N = (S::LOADS + SUMMERS - 1) / SUMMERS;
-        const uint8_t* from[N];
+    // A wave's loads of a tile, in two steps: all their places, which are read from LDS, then the loads one by one.
+    constexpr int ASKS = (S::LOADS + SUMMERS - 1) / SUMMERS;
+    struct Asks {
+        uint32_t offset[ASKS], to;
+    };
+    auto whole_wave = [&](int i) { return (i + 1) * SUMMERS * 64 <= KEYS * PIECES; };
+    auto active = [&](int i) { return (i * SUMMERS + own) * 64 + lane < KEYS * PIECES; };
+    uint32_t places[WIDE ? 1 : ASKS];  // a piece's row in the upper half and bytes in the lower, one register for both
+    if constexpr (!WIDE) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < ASKS; ++i) {
             const int piece = min((i * SUMMERS + own) * 64 + lane, KEYS * PIECES - 1), r = piece / PIECES;
-            from[i] = row_at[tile & 1][r] + (piece - r * PIECES) * 16;
+            places[i] = static_cast<uint32_t>(r * 8) << 16 | (piece - r * PIECES) * 16;
+            asm volatile("" : "+v"(places[i]));
         }
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * S::BYTES + own * 1024);
+    }
+    auto find = [&](Asks& asks, int tile, int stage) {
+        asks.to = __builtin_amdgcn_readfirstlane(lds0 + stage * S::BYTES + own * 1024);
+        const uint8_t* const table = reinterpret_cast<const uint8_t*>(row_at[tile % SLOTS]);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if ((i + 1) * SUMMERS * 64 <= KEYS * PIECES || (i * SUMMERS + own) * 64 + lane < KEYS * PIECES) load_row_pieces(from[i], to + i * SUMMERS * 1024);
+        for (int i = 0; i < ASKS; ++i) asks.offset[i] = *reinterpret_cast<const uint32_t*>(table + (places[i] >> 16)) + (places[i] & 0xFFFF);
+    };
+    auto ask = [&](const Asks& asks, int i) {
+        if (whole_wave(i) || active(i)) load_row_pieces(p.c.bytes, asks.offset[i], __builtin_amdgcn_readfirstlane(asks.to + i * SUMMERS * 1024));
+    };
+    auto ask_wide = [&](int tile, int stage) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + stage * S::BYTES + own * 1024);
+        for (int i = 0; i < ASKS; ++i) {
+            const int piece = (i * SUMMERS + own) * 64 + lane, r = piece / PIECES;
+            const uint32_t at = __builtin_amdgcn_readfirstlane(to + i * SUMMERS * 1024);
+            if (piece < KEYS * PIECES) load_row_pieces(reinterpret_cast<const uint8_t*>(row_at[tile % SLOTS][r] + (piece - r * PIECES) * 16), at);
+        }
+    };
+    auto load_tile = [&](int tile, int stage) {
+        if constexpr (WIDE) {
+            ask_wide(tile, stage);
+        } else {
+            Asks asks;
+            find(asks, tile, stage);
+#pragma unroll
+            for (int i = 0; i < ASKS; ++i) ask(asks, i);
+        }
     };
     f32x16 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = f32x16{};
 
     // The latents of the tokens whose weights a lane holds, eight of a column: the rows' bytes turned as they are read.
-    auto add_tile = [&](int tile, const uint8_t* rows) {
+    // Beside its products go the loads of a later tile: at once they would fill the memory's queue and hold the wave up (1450
+    // cycles of a tile's 4400).
+    auto add_tile = [&](int tile, const uint8_t* rows, const Asks& asks, auto with_asks) {
         constexpr int VS = 2 * KW, GROUP = E4M3 && CT % 2 == 0 ? 2 : 1, N = GROUP * VS;  // column tiles read ahead of their products
         struct Codes {
             i32x2 v;
@@ -853,6 +893,10 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 const bf16x8 now = next;
                 if (i + 1 < N) next = latents(i + 1);
                 acc[c + i % GROUP] = mfma(now, w[i / GROUP], acc[c + i % GROUP]);
+                constexpr int PER = (ASKS + CT * VS - 1) / (CT * VS);  // loads a product
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (decltype(with_asks)::value && (c * VS + i) * PER + k < ASKS) ask(asks, (c * VS + i) * PER + k);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -861,24 +905,35 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     if (first < last) {
         hold(first);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (own == 0) set_rows(first + i, holds);
-            __syncthreads();
-            if (first + i < last) load_tile(first + i, i);
+        if (own == 0) {
+            for (int i = 0; i < AHEAD + 2; ++i) set_rows(first + i, holds);
         }
-        if (own == 0) set_rows(first + AHEAD, holds);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (first + i < last) load_tile(first + i, i);
         if (first + AHEAD <= last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
         else wait_for_rows();
+        Asks asks{};
+        if constexpr (!WIDE) find(asks, first + AHEAD, AHEAD);
         __syncthreads();
         int stage = 0;  // of the tile that is scored
         for (int tile = first; tile < last; ++tile) {
-            // The stage that is loaded now was summed in the iteration before this one.
-            if (tile + AHEAD < last) load_tile(tile + AHEAD, stage >= STAGES - AHEAD ? stage + AHEAD - STAGES : stage + AHEAD);
-            const int which = holds;
-            if (tile + AHEAD + 2 < last && tile + AHEAD + 2 >= held_end) hold(tile + AHEAD + 2);
-            if (own == tile % SUMMERS && tile + AHEAD + 1 < last) set_rows(tile + AHEAD + 1, which);
-            if (tile > first) add_tile(tile - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1]);
+            // The stage that is loaded now was summed in the iteration before this one. Behind the last tile that tile is loaded
+            // again, and not read.
+            const int free_stage = stage >= STAGES - AHEAD ? stage + AHEAD - STAGES : stage + AHEAD;
+            if constexpr (WIDE) {
+                if (tile + AHEAD < last) ask_wide(tile + AHEAD, free_stage);
+            }
+            if (tile > first) {
+                add_tile(tile - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], asks, std::bool_constant<!WIDE>{});
+            } else if constexpr (!WIDE) {
+#pragma unroll
+                for (int i = 0; i < ASKS; ++i) ask(asks, i);
+            }
+            if (own == tile % SUMMERS && tile + AHEAD + 2 < last) set_rows(tile + AHEAD + 2, holds);
+            if (tile + AHEAD + 3 < last && tile + AHEAD + 3 >= held_end) hold(tile + AHEAD + 3);
+            if constexpr (!WIDE) find(asks, min(tile + AHEAD + 1, last - 1), free_stage == STAGES - 1 ? 0 : free_stage + 1);
             if (tile + AHEAD < last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
             else wait_for_rows();
             __syncthreads();
@@ -892,7 +947,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
             }
             stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
-        add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1]);
+        add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], Asks{}, std::false_type{});
     }
     __syncthreads();  // the rows' sums
     const int column = part * (R / 2) + 4 * h;
@@ -1086,8 +1141,14 @@ void launch_attention(const LatentAttentionArgs& p, int64_t blocks, hipStream_t 
         hipLaunchKernelGGL((latent_attention_kernel<R, P, true, E4M3, 1, 4>), grid, dim3(256), 0, s, p);
     } else {
         const int64_t rows = rows_per_block(p.rows, false);
-        if (rows == 32) hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, 1>), grid, dim3(Shape<R, P, E4M3, 1>::WAVES * 64), 0, s, p);
-        else hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, 2>), grid, dim3(Shape<R, P, E4M3, 2>::WAVES * 64), 0, s, p);
+        auto go = [&](auto groups) {
+            constexpr int RW = decltype(groups)::value;
+            const dim3 threads(Shape<R, P, E4M3, RW>::WAVES * 64);
+            if (p.wide) hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, RW, true>), grid, threads, 0, s, p);
+            else hipLaunchKernelGGL((latent_attention_rows_kernel<R, P, E4M3, RW, false>), grid, threads, 0, s, p);
+        };
+        if (rows == 32) go(std::integral_constant<int, 1>{});
+        else go(std::integral_constant<int, 2>{});
     }
 }
 template <int R, int P>
@@ -1171,6 +1232,7 @@ extern "C" mlk_status mlk_latent_attention(const void* q_latent, const int64_t* 
     p.splits = static_cast<int32_t>(plan.splits);
     p.scale = static_cast<float>(std::fabs(scale) * 1.4426950408889634074);
     p.negate = std::signbit(scale) ? 0x80008000u : 0;
+    p.wide = pages * page_size * (e4m3 ? rank + 2 * rope_dim + 16 : 2 * (rank + rope_dim) + 16) > (int64_t{1} << 32);
     p.units = static_cast<int32_t>(plan.units);
     p.shares = static_cast<int32_t>(plan.shares);
     if (plan.shares != 0) {
