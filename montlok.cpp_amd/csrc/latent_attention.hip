@@ -640,11 +640,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 const uint8_t* const rows = tiles[stage];
                 stage = stage == STAGES - 1 ? 0 : stage + 1;
                 // Scores of the wave's tokens with the lane's row: register i holds token 8 (i / 4) + 4 h + i % 4. Pieces of the
-                // key row are read four ahead of their use, and turned into an operand beside the product before theirs; nothing
+                // key row are read six ahead of their use, and turned into an operand beside the product before theirs; nothing
                 // moves over the bars (the scheduler on its own reads each piece right before it is used).
                 f32x16 s = {};
                 const uint8_t* const key = rows + (32 * part + l) * ROW;
-                constexpr int PARTS = E4M3 ? KS / 2 : KS, ALL = PARTS + RS, RING = ALL < 4 ? ALL : 4;
+                constexpr int PARTS = E4M3 ? KS / 2 : KS, ALL = PARTS + RS, RING = ALL < 6 ? ALL : 6;
                 auto piece = [&](int t) {
                     return *reinterpret_cast<const u32x4*>(key + (t < PARTS ? 32 * t : (E4M3 ? R : 2 * R) + 32 * (t - PARTS)) + 16 * h);
                 };
@@ -657,7 +657,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 if constexpr (E4M3) scales[wave][l] = scale;
                 ring[0][0] |= lost;
                 __builtin_amdgcn_sched_barrier(0);
-                auto operand = [&](int k) {  // of product k; its piece makes room for the one four on
+                auto operand = [&](int k) {  // of product k; its piece makes room for a later one
                     const int t = !E4M3 ? k : k < KS ? k / 2 : k - KS + PARTS;
                     const u32x4 x = ring[t % RING];
                     const bool codes = E4M3 && k < KS;
@@ -893,10 +893,14 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 const bf16x8 now = next;
                 if (i + 1 < N) next = latents(i + 1);
                 acc[c + i % GROUP] = mfma(now, w[i / GROUP], acc[c + i % GROUP]);
-                constexpr int PER = (ASKS + CT * VS - 1) / (CT * VS);  // loads a product
+                if constexpr (decltype(with_asks)::value) {
+                    // One load with every second product, with fewer products as many as it takes.
+                    constexpr int STEPS = CT * VS, PER = (ASKS + STEPS - 1) / STEPS, EVERY = STEPS >= 2 * ASKS ? 2 : 1;
+                    const int step = c * VS + i;
 #pragma unroll
-                for (int k = 0; k < PER; ++k)
-                    if (decltype(with_asks)::value && (c * VS + i) * PER + k < ASKS) ask(asks, (c * VS + i) * PER + k);
+                    for (int k = 0; k < PER; ++k)
+                        if (step % EVERY == 0 && step / EVERY * PER + k < ASKS) ask(asks, step / EVERY * PER + k);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
