@@ -233,12 +233,12 @@ __device__ __forceinline__ u32x4 numbers(u32x2 v) { return u32x4{v[0] << 16, v[0
 // SPLIT: all waves make the same 32 x 32, from a quarter of the inputs each, and the first adds the four in order; else each
 // makes a quarter of 64 x 64.
 template <bool W32, bool IN_DENSE, bool SPLIT>
-__global__ __launch_bounds__(256, 4) void head_linear_f32_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
+__global__ __launch_bounds__(256, SPLIT ? 6 : 4) void head_linear_f32_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
     constexpr int TILE = SPLIT ? 32 : 64, TK = SPLIT ? 64 : 32, STEPS = SPLIT ? 1 : 2;
     // Rows of x and of an IN_DENSE w hold TK inputs, else those of w TILE outputs; with 4 more, rows that are read together
     // (16 of 16 bytes, or every fourth) lie on other banks.
     constexpr int X_ROW = TK + 4, W_ROW = IN_DENSE ? TK + 4 : TILE + 4, W_SIZE = IN_DENSE ? TILE * W_ROW : TK * W_ROW;
-    __shared__ __attribute__((aligned(16))) float shared[2][TILE * X_ROW + W_SIZE];
+    __shared__ __attribute__((aligned(16))) float shared[SPLIT ? 1 : 2][TILE * X_ROW + W_SIZE];
     static_assert(sizeof shared >= 3 * 64 * 20 * sizeof(float), "the waves' parts take the same LDS");
     const unsigned id = unit_of(blocks);
     if (id >= blocks) return;
@@ -266,7 +266,8 @@ __global__ __launch_bounds__(256, 4) void head_linear_f32_kernel(HeadArgs p, uns
     load(begin, 0);
     int half = 0;
     for (int64_t t0 = begin; t0 < end; t0 += TILE) {
-        for (int k0 = 0; k0 < p.k; k0 += TK, half ^= 1) {
+        for (int k0 = 0; k0 < p.k; k0 += TK, half ^= !SPLIT) {
+            if (SPLIT && k0 > 0) __syncthreads();
             float* const xs = shared[half];
             float* const ws = xs + TILE * X_ROW;
 #pragma unroll
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(256, 4) void head_linear_f32_kernel(HeadArgs p, uns
             }
             __syncthreads();  // one a tile: a wave writes a half again only behind the next barrier, which follows its readers' products
             if (k0 + TK < p.k) load(t0, k0 + TK);
-            else if (t0 + TILE < end) load(t0 + TILE, 0);
+            else if (!SPLIT && t0 + TILE < end) load(t0 + TILE, 0);
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 const int k = at_k + 16 * s;
@@ -333,6 +334,7 @@ __global__ __launch_bounds__(256, 4) void head_linear_f32_kernel(HeadArgs p, uns
                 }
             }
         }
+        if constexpr (SPLIT) break;
     }
 }
 
