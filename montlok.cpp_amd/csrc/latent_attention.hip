@@ -494,7 +494,7 @@ constexpr int kLeastShare = 2;   // tiles of a block, so that a block is worth i
 constexpr int kIds = 512;  // page numbers that are looked up at a time
 
 // Waves of two kinds, RW groups of 32 rows: a scorer takes the rows' scores of 32 tokens of a tile (KW of them a group) and
-// turns them into weights, a summer adds those tokens' latents to half of the rows' columns, and sees to the loads. Scorers
+// turns them into weights, a summer adds all tokens' latents to a part of the columns, and sees to the loads. Scorers
 // hold the queries, summers the sums: what either holds leaves room for a wave of the other kind on its SIMD, and the one's
 // exponents and conversions run beside the other's products (both in one wave, which then has a SIMD to itself: 6500 cycles a
 // tile of 64 tokens and 64 rows, of which the matrix cores are busy for 2200).
@@ -505,6 +505,9 @@ struct Shape {
     static constexpr int ROW = row_bytes<E4M3>(R, P), KW = 64 * ROW * 3 <= 140 * 1024 ? 2 : 1, KEYS = 32 * KW, BYTES = KEYS * ROW;
     static constexpr int STAGES = BYTES * 4 <= 76 * 1024 ? 4 : 3;
     static constexpr int SCORERS = RW * KW, SUMMERS = RW * 2, WAVES = SCORERS + SUMMERS;
+    // A summer takes all rows of a quarter of the columns where it can: it then turns and converts half as many latents as for
+    // one group's rows of half of the columns, with as many sums.
+    static constexpr int GROUPS = RW == 2 && R % 128 == 0 ? 2 : 1, COLUMNS = R / (2 * GROUPS);
     static constexpr int LOADS = BYTES / 1024 + (BYTES % 1024 != 0);  // of 64 lanes, 16 bytes each
 };
 
@@ -512,7 +515,7 @@ template <int R, int P, bool E4M3, int RW, bool WIDE>
 __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent_attention_rows_kernel(LatentAttentionArgs p) {
     using S = Shape<R, P, E4M3, RW>;
     constexpr int ROW = S::ROW, KW = S::KW, KEYS = S::KEYS, STAGES = S::STAGES, SUMMERS = S::SUMMERS, PIECES = ROW / 16;
-    constexpr int KS = R / 16, RS = P / 16, CT = R / 64;  // 16-deep steps over the latent and the key part, 32-wide tiles of columns
+    constexpr int KS = R / 16, RS = P / 16, RG = S::GROUPS, CT = S::COLUMNS / 32;  // 16-deep steps over the latent and the key part, 32-wide tiles of columns
     // Tiles are asked for AHEAD iterations before they are scored. Where their pieces lie is read at the end of the iteration
     // before that, from addresses set in the one before, from page numbers looked up one before that: each is there for all
     // summers after a barrier.
@@ -529,7 +532,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     __shared__ int grown[2], odd[2];  // 1 + the tile where a maximum has outgrown its row's, or a score is no number
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const bool scorer = wave < S::SCORERS;
-    const int rw = scorer ? wave / KW : (wave - S::SCORERS) / 2, part = scorer ? wave % KW : (wave - S::SCORERS) % 2;
+    const int rw = scorer ? wave / KW : (wave - S::SCORERS) / 2, part = scorer ? wave % KW : RG == 1 ? (wave - S::SCORERS) % 2 : wave - S::SCORERS;
 
     // The block's share: of the tiles of all units (RW * 32 rows of a sequence), laid end to end, as many as any other block's;
     // or one unit.
@@ -613,7 +616,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     const int first = min(from_tile, tile_count), last = p.shares == 0 ? tile_count : min(until - unit_start, tile_count);
     const bool whole = p.shares == 0 || (from_tile == 0 && until >= unit_end);
     // A share has at most two parts of units, its first and its last.
-    const int64_t at_row = b * p.rows + row, place = (static_cast<int64_t>(share) * 2 + (part_of_share != 0)) * (RW * 32) + 32 * rw + l;
+    const int64_t place = (static_cast<int64_t>(share) * 2 + (part_of_share != 0)) * (RW * 32) + 32 * rw + l;
 
     if (scorer) {
         float top = -INFINITY, sum = 0.0f;
@@ -822,9 +825,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
             for (int i = 0; i < ASKS; ++i) ask(asks, i);
         }
     };
-    f32x16 acc[CT];
+    f32x16 acc[RG][CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c] = f32x16{};
+    for (int r = 0; r < RG; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[r][c] = f32x16{};
 
     // The latents of the tokens whose weights a lane holds, eight of a column: the rows' bytes turned as they are read.
     // Beside its products go the loads of a later tile: at once they would fill the memory's queue and hold the wave up (1450
@@ -874,9 +879,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
         };
         Fragment ahead[2][N];
         read(ahead[0], 0);
-        bf16x8 w[VS];
+        bf16x8 w[RG][VS];
 #pragma unroll
-        for (int i = 0; i < VS; ++i) w[i] = shared_weights[tile & 1][rw][i / 2][i % 2][lane];
+        for (int r = 0; r < RG; ++r)
+#pragma unroll
+            for (int i = 0; i < VS; ++i) w[r][i] = shared_weights[tile & 1][RG == 1 ? rw : r][i / 2][i % 2][lane];
         const bool tainted = odd[tile & 1] == tile + 1;
 #pragma unroll
         for (int c = 0; c < CT; c += GROUP) {
@@ -892,14 +899,17 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
             for (int i = 0; i < N; ++i) {
                 const bf16x8 now = next;
                 if (i + 1 < N) next = latents(i + 1);
-                acc[c + i % GROUP] = mfma(now, w[i / GROUP], acc[c + i % GROUP]);
-                if constexpr (decltype(with_asks)::value) {
-                    // One load with every second product, with fewer products as many as it takes.
-                    constexpr int STEPS = CT * VS, PER = (ASKS + STEPS - 1) / STEPS, EVERY = STEPS >= 2 * ASKS ? 2 : 1;
-                    const int step = c * VS + i;
 #pragma unroll
-                    for (int k = 0; k < PER; ++k)
-                        if (step % EVERY == 0 && step / EVERY * PER + k < ASKS) ask(asks, step / EVERY * PER + k);
+                for (int r = 0; r < RG; ++r) {
+                    acc[r][c + i % GROUP] = mfma(now, w[r][i / GROUP], acc[r][c + i % GROUP]);
+                    if constexpr (decltype(with_asks)::value) {
+                        // One load with every second product, with fewer products as many as it takes.
+                        constexpr int STEPS = CT * VS * RG, PER = (ASKS + STEPS - 1) / STEPS, EVERY = STEPS >= 2 * ASKS ? 2 : 1;
+                        const int step = (c * VS + i) * RG + r;
+#pragma unroll
+                        for (int k = 0; k < PER; ++k)
+                            if (step % EVERY == 0 && step / EVERY * PER + k < ASKS) ask(asks, step / EVERY * PER + k);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -944,9 +954,12 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
             if (__builtin_expect(grown[tile & 1] == tile + 1, 0)) {
                 __syncthreads();
                 if (tile > first) {
-                    const float by = factors[rw][l];
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) acc[c] *= by;
+                    for (int r = 0; r < RG; ++r) {
+                        const float by = factors[RG == 1 ? rw : r][l];
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) acc[r][c] *= by;
+                    }
                 }
             }
             stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -954,31 +967,39 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
         add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], Asks{}, std::false_type{});
     }
     __syncthreads();  // the rows' sums
-    const int column = part * (R / 2) + 4 * h;
-    if (whole && real) {
-        float sum = 0.0f;
+    const int column = part * S::COLUMNS + 4 * h;
 #pragma unroll
-        for (int i = 0; i < KW; ++i) sum += tops[rw][i][l];
-        // A row that sees nothing has no sum: zeros. One past the table: NaN.
-        const float inverse = beyond ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t* const to = static_cast<uint16_t*>(p.out) + at_row * R + column;
+    for (int r = 0; r < RG; ++r) {
+        const int group = RG == 1 ? rw : r, in_unit = 32 * group + l, out_row = row0 + in_unit;
+        if (whole && out_row < p.rows) {
+            float sum = 0.0f;
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+            for (int i = 0; i < KW; ++i) sum += tops[group][i][l];
+            // A row that sees nothing has no sum: zeros. One past the table: NaN.
+            const bool past = RG == 1 ? beyond : p.positions[b * p.length + out_row / p.heads] >= static_cast<int64_t>(p.c.width) * p.c.page_size;
+            const float inverse = past ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint16_t* const to = static_cast<uint16_t*>(p.out) + (b * p.rows + out_row) * R + column;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x[4];
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = acc[c][4 * j + e] * inverse;
-                *reinterpret_cast<u32x2*>(to + 32 * c + 8 * j) = u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1])}),
-                                                                       __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[2]), static_cast<__bf16>(x[3])})};
-            }
-    } else if (!whole && first < last) {
-        float* const to = p.partial + place * R + column;
+                for (int j = 0; j < 4; ++j) {
+                    float x[4];
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+                    for (int e = 0; e < 4; ++e) x[e] = acc[r][c][4 * j + e] * inverse;
+                    *reinterpret_cast<u32x2*>(to + 32 * c + 8 * j) =
+                        u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1])}),
+                              __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[2]), static_cast<__bf16>(x[3])})};
+                }
+        } else if (!whole && first < last) {
+            float* const to = p.partial + (static_cast<int64_t>(share) * 2 + (part_of_share != 0)) * (RW * 32) * R + in_unit * R + column;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<f32x4*>(to + 32 * c + 8 * j) = f32x4{acc[c][4 * j], acc[c][4 * j + 1], acc[c][4 * j + 2], acc[c][4 * j + 3]};
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x16& v = acc[r][c];
+                    *reinterpret_cast<f32x4*>(to + 32 * c + 8 * j) = f32x4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+                }
+        }
     }
     }
     if (p.shares == 0 || until <= unit_end) return;
