@@ -445,6 +445,7 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // The maximum, or the sum, of a row: its scores lie with the lanes l and l + 32.
@@ -1077,6 +1078,64 @@ __global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionAr
               __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[2]), static_cast<__bf16>(acc[3])})};
 }
 
+// The same where rows have few parts: a wave a row (of 64 lanes or as many as its columns take, 4 or 8 a lane), eight parts and
+// their statistics asked for at a time, under a running maximum.
+template <int R>
+__global__ __launch_bounds__(256) void latent_join_few_kernel(LatentAttentionArgs p, int rows_per_unit) {
+    constexpr int LANES = R / 4 < 64 ? R / 4 : 64, ROWS = 256 / LANES, EACH = R / 4 / LANES, BATCH = 8;
+    const int blocks = rows_per_unit / ROWS, unit = blockIdx.x / blocks, r = (blockIdx.x - unit * blocks) * ROWS + threadIdx.x / LANES;
+    const int column = threadIdx.x % LANES * 4;
+    const int begin = p.starts[unit], end = p.starts[unit + 1], total = p.starts[p.units];
+    const int each = max((total + p.shares - 1) / p.shares, kLeastShare), g0 = begin / each, parts = (end - 1) / each - g0 + 1;
+    const int64_t b = unit / p.row_blocks;
+    const int row = static_cast<int>(unit - b * p.row_blocks) * rows_per_unit + r;
+    if (parts == 1 || row >= p.rows) return;
+    float most = -INFINITY, sum = 0.0f;
+    f32x4 acc[EACH] = {};
+    for (int i = 0; i < parts; i += BATCH) {
+        f32x2 stats[BATCH];
+        f32x4 v[BATCH][EACH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            stats[k] = f32x2{-INFINITY, 0.0f};
+            if (i + k >= parts) continue;
+            const int part = i + k;
+            const int64_t place = (static_cast<int64_t>(g0 + part) * 2 + (part == 0 && begin > g0 * each)) * rows_per_unit + r;
+            stats[k] = *reinterpret_cast<const f32x2*>(p.stats + place * 2);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) v[k][j] = *reinterpret_cast<const f32x4*>(p.partial + place * R + column + 256 * j);
+        }
+        float now = most;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) now = fmaxf(now, stats[k][0]);
+        const float before = __builtin_amdgcn_exp2f(most - finite_or_zero(now));
+        most = now;
+        sum *= before;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) acc[j] *= before;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            // Of a part that saw nothing the sums may not have been written; one past the table has a sum of NaN.
+            const float f = stats[k][1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(stats[k][0] - finite_or_zero(now));
+            sum = fmaf(stats[k][1], f, sum);
+            if (f != 0.0f) {
+#pragma unroll
+                for (int j = 0; j < EACH; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(v[k][j][e], f, acc[j][e]);
+            }
+        }
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const f32x4 x = acc[j] * inverse;
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + (b * p.rows + row) * R + column + 256 * j) =
+            u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1])}),
+                  __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x[2]), static_cast<__bf16>(x[3])})};
+    }
+}
+
 // The parts of a row, 64 columns a block: 16 lanes side by side, 16 parts at a time.
 template <int R, bool F32>
 __global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, const float* stats, int splits, void* out) {
@@ -1191,7 +1250,7 @@ void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool
         const int per = static_cast<int>(rows_per_block(p.rows, false));
         // Few rows of many parts: 64 columns a block.
         if (p.units * 16 <= p.shares) hipLaunchKernelGGL((latent_join_rows_kernel<R, 64>), dim3(static_cast<unsigned>(p.units * per * (R / 64))), dim3(256), 0, s, p, per);
-        else hipLaunchKernelGGL((latent_join_rows_kernel<R, R>), dim3(static_cast<unsigned>(p.units * per)), dim3(256), 0, s, p, per);
+        else hipLaunchKernelGGL((latent_join_few_kernel<R>), dim3(static_cast<unsigned>(p.units * per / (R / 4 < 64 ? 1024 / R : 4))), dim3(256), 0, s, p, per);
         return;
     }
     if (p.splits == 1) return;
