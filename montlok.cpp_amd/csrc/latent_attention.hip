@@ -539,19 +539,18 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     // or one unit.
     int unit = blockIdx.x, from_tile = 0, until = INT_MAX, share = 0;
     if (p.shares != 0) {
-        for (int u = threadIdx.x; u < p.units; u += S::WAVES * 64) {
-            const int64_t sequence = u / p.row_blocks;
-            const int row0 = static_cast<int>(u - sequence * p.row_blocks) * (RW * 32), row1 = min(row0 + RW * 32, p.rows) - 1;
-            int end = 1;  // a unit that sees nothing has outputs all the same
-            for (int t = row0 / p.heads; t <= row1 / p.heads; ++t) end = max(end, sight_of(p, sequence, t).end);
-            starts[u + 1] = (end + KEYS - 1) / KEYS;
+        for (int u = threadIdx.x; u < p.units; u += S::WAVES * 64) starts[u + 1] = 1;  // a unit that sees nothing has outputs all the same
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.units / p.row_blocks * p.length; i += S::WAVES * 64) {
+            const int sequence = i / p.length, token = i - sequence * p.length, row0 = token * p.heads, end = sight_of(p, sequence, token).end;
+            for (int u = row0 / (RW * 32); u <= (row0 + p.heads - 1) / (RW * 32); ++u) atomicMax(&starts[sequence * p.row_blocks + u + 1], end);
         }
         __syncthreads();
         if (wave == 0) {  // sums of everything before: a run of units a lane, then the lanes
             const int lane = threadIdx.x;
             const int run = (p.units + 63) / 64, u0 = min(lane * run, p.units), u1 = min(u0 + run, p.units);
             int sum = 0;
-            for (int u = u0; u < u1; ++u) sum += starts[u + 1];
+            for (int u = u0; u < u1; ++u) sum += starts[u + 1] = (starts[u + 1] + KEYS - 1) / KEYS;
             int before = sum;
 #pragma unroll
             for (int m = 1; m < 64; m *= 2) {
@@ -593,6 +592,28 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     const int row0 = static_cast<int>(unit - b * p.row_blocks) * (RW * 32), row = row0 + 32 * rw + l;
     const bool real = row < p.rows;
     const int token_of_row = row / p.heads, head = row - token_of_row * p.heads;
+    // Page numbers for the summers, looked up kIds at a time.
+    const int own = wave - S::SCORERS;
+    const uint32_t page_size = static_cast<uint32_t>(p.c.page_size);
+    int held_page = 0, held_end = 0, holds = 0;  // ids[holds] begins with page held_page and serves tiles before held_end
+    auto hold = [&](int tile) {
+        constexpr int EACH = kIds / (SUMMERS * 64);
+        static_assert(kIds % (SUMMERS * 64) == 0, "as many for every lane");
+        const int page0 = static_cast<int>(static_cast<uint32_t>(tile) * KEYS / page_size);
+        held_end = static_cast<int>((static_cast<int64_t>(page0) + kIds) * page_size / KEYS);
+        holds ^= 1;
+        held_page = page0;
+        int32_t id[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int page = page0 + (i * SUMMERS + own) * 64 + lane;
+            id[i] = -1;
+            if (page < p.c.width) id[i] = p.c.table[b * p.c.width + page];
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) ids[holds][(i * SUMMERS + own) * 64 + lane] = id[i];
+    };
+    if (!scorer) hold(from_tile);
     Sight sight{0, 0, 0, false};
     if (real) sight = sight_of(p, b, token_of_row);
     const bool beyond = sight.beyond;
@@ -638,7 +659,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 3; ++i) __syncthreads();  // page numbers, row addresses, the first tile
+            for (int i = 0; i < 2; ++i) __syncthreads();  // row addresses, the first tile
             int stage = 0;
             for (int tile = first; tile < last; ++tile) {
                 const uint8_t* const rows = tiles[stage];
@@ -758,24 +779,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     } else {
 
     // A summer. Row addresses: of the pages whose numbers ids[] holds, by one wave, a token a lane.
-    const int own = wave - S::SCORERS;
-    const uint32_t page_size = static_cast<uint32_t>(p.c.page_size);
-    int held_page[2] = {0, 0}, held_end = first, holds = 0;  // ids[i] begins with page held_page[i]; ids[holds] serves tiles before held_end
-    auto hold = [&](int tile) {
-        const int page0 = static_cast<int>(static_cast<uint32_t>(tile) * KEYS / page_size);
-        held_end = static_cast<int>((static_cast<int64_t>(page0) + kIds) * page_size / KEYS);
-        holds ^= 1;
-        held_page[holds] = page0;
-        for (int i = own * 64 + lane; i < kIds; i += SUMMERS * 64) {
-            const int page = page0 + i;
-            ids[holds][i] = page < p.c.width ? p.c.table[b * p.c.width + page] : -1;
-        }
-    };
-    auto set_rows = [&](int tile, int which) {
+    auto set_rows = [&](int tile) {
         if (lane < KEYS) {
             // Behind the last token that some row sees that token's row again, which stands for nothing there.
             const uint32_t token = min(static_cast<uint32_t>(tile) * KEYS + lane, static_cast<uint32_t>(all) - 1), page = token / page_size;
-            const int32_t page_id = ids[which][page - held_page[which]];
+            const int32_t page_id = ids[holds][page - held_page];
             const bool held = page_id >= 0 && page_id < p.c.pages;
             const uint64_t at = held ? (static_cast<uint64_t>(page_id) * page_size + (token - page * page_size)) * ROW : 0;
             row_at[tile % SLOTS][lane] = WIDE ? reinterpret_cast<uint64_t>(p.c.bytes) + at : at;
@@ -918,11 +926,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
     };
 
     if (first < last) {
-        hold(first);
-        __syncthreads();
-        if (own == 0) {
-            for (int i = 0; i < AHEAD + 2; ++i) set_rows(first + i, holds);
-        }
+        for (int i = own; i < AHEAD + 2; i += SUMMERS) set_rows(first + i);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
@@ -946,7 +950,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent
 #pragma unroll
                 for (int i = 0; i < ASKS; ++i) ask(asks, i);
             }
-            if (own == tile % SUMMERS && tile + AHEAD + 2 < last) set_rows(tile + AHEAD + 2, holds);
+            if (own == tile % SUMMERS && tile + AHEAD + 2 < last) set_rows(tile + AHEAD + 2);
             if (tile + AHEAD + 3 < last && tile + AHEAD + 3 >= held_end) hold(tile + AHEAD + 3);
             if constexpr (!WIDE) find(asks, min(tile + AHEAD + 1, last - 1), free_stage == STAGES - 1 ? 0 : free_stage + 1);
             if (tile + AHEAD < last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
