@@ -17,15 +17,6 @@ namespace {
 // Read in place of rows that no page holds, or that no token of a block sees.
 __device__ const uint8_t kZeroRow[2 * (512 + 64) + 16] __attribute__((aligned(16))) = {};
 
-// Read in place of rows on pages that the table does not name: NaN in every format.
-struct Filled {
-    uint8_t bytes[2 * (512 + 64) + 16];
-    constexpr explicit Filled(uint8_t v) : bytes{} {
-        for (auto& b : bytes) b = v;
-    }
-};
-__device__ const Filled kMissingRow __attribute__((aligned(16))) (0xFF);
-
 struct LatentAttentionArgs {
     const void *q, *qr;
     int64_t qs[3], rs[3];
@@ -33,8 +24,8 @@ struct LatentAttentionArgs {
     const int32_t* positions;
     const int64_t* ancestors;  // or null
     void* out;
-    float* partial;  // [sequence][row][split][R], then the maxima and sums [sequence][row][split][2]
-    float* stats;     // maxima and sums of the parts
+    float* partial;   // sums of the parts: of fp32 rows [sequence][row][split][R], else [share][2][row of a unit][R]
+    float* stats;     // maxima and sums of the parts' weights, two in place of R
     int32_t* starts;  // tiles before each unit
     int32_t length, heads, rows, row_blocks, splits;
     int32_t units, shares;  // 0 shares: a unit a block
@@ -43,7 +34,7 @@ struct LatentAttentionArgs {
     uint32_t negate;  // the sign bits of two bf16 where it was
 };
 
-constexpr int kTile = 64;   // tokens of a tile
+constexpr int kTile = 64;   // tokens of a tile, for plans and fp32 queries
 constexpr int kPPitch = 72;  // bf16 elements from one row of weights to the next in LDS: 36 dwords, eight rows on eight bank groups
 
 __device__ __forceinline__ float max_over_groups(float v) {
@@ -81,57 +72,51 @@ __device__ __forceinline__ void wait_for_rows() {
     asm volatile("" ::: "memory");
 }
 
-// MT tiles of 16 rows (a row is a token and a query head) of one sequence over every `splits`-th part of its tokens.
-// Wave (rg, kg) scores the row tiles of group rg with 16 tokens of a tile, then takes R / WAVES columns of all rows' sums.
-// Every product has the rows as its columns (scores are tokens x rows, sums are columns x rows), so that a lane's numbers all
-// belong to row lane & 15 of a tile: its maximum, sum and rescaling are one number, its weights of four tokens and its sums
-// of four columns lie side by side.
-template <int R, int P, bool F32, bool E4M3, int MT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attention_kernel(LatentAttentionArgs p) {
-    constexpr int ROW = row_bytes<E4M3>(R, P), PIECES = ROW / 16, kPlanes = F32 ? 3 : 1;
-    constexpr int RG = WAVES / 4, RT = MT / RG, COLS = R / WAVES, CT = COLS / 16;
+// What a token of a call sees: the places below `base`, and base + j where bit j is set; nothing from `end` on.
+struct Sight {
+    int base, end;
+    uint64_t bits;
+    bool beyond;  // past the table
+};
+__device__ __forceinline__ Sight sight_of(const LatentAttentionArgs& p, int64_t sequence, int token) {
+    const int64_t at = sequence * p.length + token;
+    const int32_t position = p.positions[at];
+    Sight s{0, 0, 0, position >= static_cast<int64_t>(p.c.width) * p.c.page_size};
+    if (position < 0 || s.beyond) return s;
+    s.end = s.base = position + 1;
+    if (p.ancestors == nullptr) return s;
+    s.base = position - token;
+    s.bits = static_cast<uint64_t>(p.ancestors[at]);
+    if (p.length < 64) s.bits &= (uint64_t{1} << p.length) - 1;
+    s.end = max(s.bits == 0 ? s.base : s.base + 64 - __builtin_clzll(s.bits), 0);
+    return s;
+}
+
+// fp32 queries: 16 rows (a row is a token and a query head) of one sequence over every `splits`-th part of its tokens. Queries
+// and weights are three bf16 planes each, which hold every bit of them, so that products with the cache's values are exact.
+// Wave i scores tokens 16 i .. of a tile of 64, then takes R / 4 columns of all rows' sums. Every product has the rows as its
+// columns (scores are tokens x rows, sums are columns x rows), so that a lane's numbers all belong to row lane & 15: its
+// maximum, sum and rescaling are one number, its weights of four tokens and its sums of four columns lie side by side.
+template <int R, int P, bool E4M3>
+__global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttentionArgs p) {
+    constexpr int ROW = row_bytes<E4M3>(R, P), PIECES = ROW / 16, COLS = R / 4, CT = COLS / 16, kPlanes = 3;
     constexpr int KS = R / 32, RS = (P + 31) / 32;  // 32-deep steps over the latent and the key part
-    static_assert(MT % RG == 0 && COLS % 16 == 0, "rows and columns fall to whole tiles");
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][kTile * ROW];
-    __shared__ __attribute__((aligned(16))) uint16_t weights[kPlanes][MT * 16 * kPPitch];
-    __shared__ float maxima[4][MT * 16];
+    __shared__ __attribute__((aligned(16))) uint16_t weights[kPlanes][16 * kPPitch];
+    __shared__ float maxima[4][16];
     __shared__ const uint8_t* row_at[kTile];
     __shared__ float missing[2][kTile];  // NaN where a token's page is missing, else 0
     __shared__ int tainted[2];           // some score of the tile is not finite
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4, l = lane & 15;
-    const int kg = wave % 4, rg = wave / 4;
     unsigned id = blockIdx.x;
     const int split = id % p.splits;
     id /= p.splits;
-    const int row0 = static_cast<int>(id % p.row_blocks) * (MT * 16);
+    const int row = static_cast<int>(id % p.row_blocks) * 16 + l, token_of_row = row / p.heads, head = row - token_of_row * p.heads;
     const int64_t b = id / p.row_blocks;
-
-    // What each of the lane's rows sees: tokens below `base`, and base + j where bit j is set. A plain row sees base = its
-    // position + 1 tokens.
-    int base[MT], end = 0, at[MT];
-    uint64_t bits[MT];
-    bool beyond[MT];
-    const int64_t capacity = static_cast<int64_t>(p.c.width) * p.c.page_size;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = row0 + 16 * m + l;
-        const int token = row / p.heads;
-        at[m] = row < p.rows ? p.positions[b * p.length + token] : -1;
-        beyond[m] = at[m] >= capacity;
-        base[m] = 0;
-        bits[m] = 0;
-        if (at[m] >= 0 && !beyond[m]) {
-            if (p.ancestors == nullptr) {
-                base[m] = at[m] + 1;
-                end = max(end, base[m]);
-            } else {
-                base[m] = at[m] - token;
-                bits[m] = static_cast<uint64_t>(p.ancestors[b * p.length + token]);
-                if (p.length < 64) bits[m] &= (uint64_t{1} << p.length) - 1;
-                end = max(end, bits[m] == 0 ? base[m] : base[m] + 64 - __builtin_clzll(bits[m]));
-            }
-        }
-    }
+    const bool real = row < p.rows;
+    Sight sight{0, 0, 0, false};
+    if (real) sight = sight_of(p, b, token_of_row);
+    int end = sight.end;
 #pragma unroll
     for (int m = 1; m < 16; m *= 2) end = max(end, __shfl_xor(end, m, kWave));
     end = __builtin_amdgcn_readfirstlane(end);
@@ -139,46 +124,25 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
     const int tile_count = (end + kTile - 1) / kTile, per_split = (tile_count + p.splits - 1) / p.splits;
     const int first = min(split * per_split, tile_count), last = min(first + per_split, tile_count);
 
-    // The lane's queries: of row tile m, step s, the dimensions that its piece of a key row holds.
-    bf16x8 q[RT][KS + RS][kPlanes];
-    auto dimension = [&](int s) {  // of the latent; codes come 16 to a piece, bf16 values 8
-        return E4M3 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-    };
+    // The lane's queries: of each step the dimensions that its piece of a key row holds (codes come 16 to a piece, bf16 values 8).
+    bf16x8 q[KS + RS][kPlanes];
+    const int64_t ql = b * p.qs[0] + token_of_row * p.qs[1] + head * p.qs[2], qr = b * p.rs[0] + token_of_row * p.rs[1] + head * p.rs[2];
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
-        const int row = row0 + 16 * (rg * RT + m) + l, token = row / p.heads, head = row - token * p.heads;
-        const bool real = row < p.rows;
-        const int64_t ql = b * p.qs[0] + token * p.qs[1] + head * p.qs[2], qr = b * p.rs[0] + token * p.rs[1] + head * p.rs[2];
+    for (int t = 0; t < KS + RS; ++t) {
+        const int d = t >= KS ? 32 * (t - KS) + 8 * g : E4M3 ? 64 * (t / 2) + 16 * g + 8 * (t % 2) : 32 * t + 8 * g;
+        const float* const from = static_cast<const float*>(t < KS ? p.q : p.qr) + (t < KS ? ql : qr) + d;
+        float v[8] = {};
+        if (real && (t < KS || d < P)) {
+            const u32x4 lo = *reinterpret_cast<const u32x4_any*>(from), hi = *reinterpret_cast<const u32x4_any*>(from + 4);
 #pragma unroll
-        for (int s = 0; s < KS + RS; ++s) {
-            const bool in_latent = s < KS;
-            const int d = in_latent ? dimension(s) : 32 * (s - KS) + 8 * g;
-            const void* const from = in_latent ? p.q : p.qr;
-            const int64_t start = (in_latent ? ql : qr) + d;
-            const bool take = real && (in_latent || d < P);
-            if constexpr (F32) {
-                float v[8] = {};
-                if (take) {
-                    const u32x4 lo = *reinterpret_cast<const u32x4_any*>(static_cast<const float*>(from) + start);
-                    const u32x4 hi = *reinterpret_cast<const u32x4_any*>(static_cast<const float*>(from) + start + 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[i] = __uint_as_float(lo[i]);
-                        v[4 + i] = __uint_as_float(hi[i]);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = p.negate == 0 ? v[i] : -v[i];
-                bf16x8 plane[3];
-                planes_of<true>(v, plane);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) q[m][s][i] = plane[i];
-            } else {
-                u32x4 v = {0, 0, 0, 0};
-                if (take) v = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(from) + start);
-                q[m][s][0] = __builtin_bit_cast(bf16x8, v);
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __uint_as_float(lo[i]);
+                v[4 + i] = __uint_as_float(hi[i]);
             }
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p.negate == 0 ? v[i] : -v[i];
+        planes_of<true>(v, q[t]);
     }
 
     // Row addresses of a tile: by the first wave, a token a lane.
@@ -197,26 +161,17 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
     auto load_tile = [&](int tile) {
         const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)tiles[tile & 1]));
 #pragma unroll
-        for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i) {
-            const int part = i * WAVES + wave;  // 64 pieces
+        for (int i = 0; i < (PIECES + 3) / 4; ++i) {
+            const int part = i * 4 + wave;  // 64 pieces
             if (part < PIECES) {
-                const int piece = part * 64 + lane, row = piece / PIECES;
-                load_row_pieces(row_at[row] + (piece - row * PIECES) * 16, __builtin_amdgcn_readfirstlane(to + part * 1024));
+                const int piece = part * 64 + lane, from = piece / PIECES;
+                load_row_pieces(row_at[from] + (piece - from * PIECES) * 16, __builtin_amdgcn_readfirstlane(to + part * 1024));
             }
         }
     };
 
-    f32x4 acc[MT][CT];
-    float top[MT], sum[RT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        top[m] = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) acc[m][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-#pragma unroll
-    for (int m = 0; m < RT; ++m) sum[m] = 0.0f;
-
+    f32x4 acc[CT] = {};
+    float top = -INFINITY, sum = 0.0f;
     if (first < last) {
         if (wave == 0) set_rows(first, page_of(first));
         if (threadIdx.x == 0) tainted[0] = tainted[1] = 0;
@@ -233,118 +188,79 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
         if (tile + 1 < last) load_tile(tile + 1);
         const uint8_t* const rows = tiles[tile & 1];
 
-        // Scores of tokens 16 kg + 4 g + i with row l of each row tile.
-        f32x4 s[RT], r[RT];
+        // Scores of tokens 16 wave + 4 g + i with the lane's row.
+        f32x4 s = {}, r = {};
+        const uint8_t* const key = rows + (16 * wave + l) * ROW;
 #pragma unroll
-        for (int m = 0; m < RT; ++m) s[m] = r[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const uint8_t* const key = rows + (16 * kg + l) * ROW;
-        if constexpr (E4M3) {
-#pragma unroll
-            for (int t = 0; t < KS / 2; ++t) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(key + 64 * t + 16 * g);
+        for (int t = 0; t < KS; t += E4M3 ? 2 : 1) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(key + (E4M3 ? 32 : 64) * t + 16 * g);
+            if constexpr (E4M3) {
                 const bf16x8 a = e4m3_octet(v[0], v[1], 1.0f), c = e4m3_octet(v[2], v[3], 1.0f);
 #pragma unroll
-                for (int m = 0; m < RT; ++m)
+                for (int i = kPlanes - 1; i >= 0; --i) {
+                    s = mfma(a, q[t][i], s);
+                    s = mfma(c, q[t + 1][i], s);
+                }
+            } else {
 #pragma unroll
-                    for (int i = kPlanes - 1; i >= 0; --i) {
-                        s[m] = mfma(a, q[m][2 * t][i], s[m]);
-                        s[m] = mfma(c, q[m][2 * t + 1][i], s[m]);
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < KS; ++t) {
-                const bf16x8 a = *reinterpret_cast<const bf16x8*>(key + 64 * t + 16 * g);
-#pragma unroll
-                for (int m = 0; m < RT; ++m)
-#pragma unroll
-                    for (int i = kPlanes - 1; i >= 0; --i) s[m] = mfma(a, q[m][t][i], s[m]);
+                for (int i = kPlanes - 1; i >= 0; --i) s = mfma(__builtin_bit_cast(bf16x8, v), q[t][i], s);
             }
         }
 #pragma unroll
         for (int t = 0; t < RS; ++t) {
             const int d = 32 * t + 8 * g;
-            // Where the key part is 16 wide the upper lanes' queries are zeros; they read the row's tail or zeros in its place.
+            // Where the key part is 16 wide the upper lanes' queries are zeros, and so are their keys.
             bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
             if (P >= 32 || d < P) a = *reinterpret_cast<const bf16x8*>(key + (E4M3 ? R : 2 * R) + 2 * d);
 #pragma unroll
-            for (int m = 0; m < RT; ++m)
-#pragma unroll
-                for (int i = kPlanes - 1; i >= 0; --i) r[m] = mfma(a, q[m][KS + t][i], r[m]);
+            for (int i = kPlanes - 1; i >= 0; --i) r = mfma(a, q[KS + t][i], r);
         }
-        float key_scale[4], lost[4];
+        float key_scale[4];
+        bool odd = false;
+        float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int token = 16 * kg + 4 * g + i;
-            key_scale[i] = E4M3 ? *reinterpret_cast<const float*>(rows + token * ROW + R + 2 * P) : 1.0f;
-            lost[i] = missing[tile & 1][token];
+            const int in_tile = 16 * wave + 4 * g + i, past = tile * kTile + in_tile - sight.base;
+            key_scale[i] = E4M3 ? *reinterpret_cast<const float*>(rows + in_tile * ROW + R + 2 * P) : 1.0f;
+            const float v = (E4M3 ? fmaf(s[i], key_scale[i], r[i]) : s[i] + r[i]) * p.scale + missing[tile & 1][in_tile];
+            odd |= !(fabsf(v) < INFINITY);
+            const bool seen = past < 0 || (past < 64 && (sight.bits >> (past & 63) & 1));
+            s[i] = seen ? v : -INFINITY;
+            most = fmaxf(most, s[i]);
         }
-        bool odd = false;
-#pragma unroll
-        for (int m = 0; m < RT; ++m) {
-            const int row = rg * RT + m;
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int token = tile * kTile + 16 * kg + 4 * g + i, past = token - base[row];
-                float v = (E4M3 ? fmaf(s[m][i], key_scale[i], r[m][i]) : s[m][i] + r[m][i]) * p.scale + lost[i];
-                odd |= !(fabsf(v) < INFINITY);
-                const bool seen = past < 0 || (past < 64 && (bits[row] >> (past & 63) & 1));
-                v = seen ? v : -INFINITY;
-                s[m][i] = v;
-                most = fmaxf(most, v);
-            }
-            most = max_over_groups(most);
-            if (g == 0) maxima[kg][16 * row + l] = most;
-        }
+        most = max_over_groups(most);
+        if (g == 0) maxima[wave][l] = most;
         if (odd) tainted[tile & 1] = 1;
         __syncthreads();  // the rows' maxima
         const bool clean = tainted[tile & 1] == 0;
         if (threadIdx.x == 0) tainted[~tile & 1] = 0;
-        float by[MT];
+        most = top;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float most = top[m];
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, maxima[i][l]);
+        const float under = finite_or_zero(most), by = __builtin_amdgcn_exp2f(top - under);
+        top = most;
+        float w[4], total = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) most = fmaxf(most, maxima[i][16 * m + l]);
-            by[m] = __builtin_amdgcn_exp2f(top[m] - finite_or_zero(most));
-            top[m] = most;
+        for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[i] - under);
+            total += e;
+            w[i] = E4M3 ? (s[i] == -INFINITY ? 0.0f : e * key_scale[i]) : e;
         }
+        sum = fmaf(sum, by, total);
+        Parts3 x[4];
 #pragma unroll
-        for (int m = 0; m < RT; ++m) {
-            const int row = rg * RT + m;
-            const float under = finite_or_zero(top[row]);
-            float w[4], total = 0.0f;
+        for (int i = 0; i < 4; ++i) x[i] = parts_of<true>(w[i]);
+        const int to = l * kPPitch + 16 * wave + 4 * g;
+        *reinterpret_cast<u32x2*>(&weights[0][to]) = u32x2{pack_upper(x[0].a, x[1].a), pack_upper(x[2].a, x[3].a)};
+        *reinterpret_cast<u32x2*>(&weights[1][to]) = u32x2{pack_upper(x[0].b, x[1].b), pack_upper(x[2].b, x[3].b)};
+        *reinterpret_cast<u32x2*>(&weights[2][to]) = u32x2{pack_upper(x[0].c, x[1].c), pack_upper(x[2].c, x[3].c)};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(s[m][i] - under);
-                total += e;
-                w[i] = E4M3 ? (s[m][i] == -INFINITY ? 0.0f : e * key_scale[i]) : e;
-            }
-            sum[m] = fmaf(sum[m], by[row], total);
-            uint16_t* const to = &weights[0][(16 * row + l) * kPPitch + 16 * kg + 4 * g];
-            if constexpr (F32) {
-                Parts3 x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = parts_of<true>(w[i]);
-                *reinterpret_cast<u32x2*>(to) = u32x2{pack_upper(x[0].a, x[1].a), pack_upper(x[2].a, x[3].a)};
-                *reinterpret_cast<u32x2*>(to + MT * 16 * kPPitch) = u32x2{pack_upper(x[0].b, x[1].b), pack_upper(x[2].b, x[3].b)};
-                *reinterpret_cast<u32x2*>(to + 2 * MT * 16 * kPPitch) = u32x2{pack_upper(x[0].c, x[1].c), pack_upper(x[2].c, x[3].c)};
-            } else {
-                // Rounded to bf16 for the product with the latents: 2^-8 of a weight at most, without a bias; the sum keeps them whole.
-                *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(w[0]), static_cast<__bf16>(w[1])}),
-                                                      __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(w[2]), static_cast<__bf16>(w[3])})};
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int c = 0; c < CT; ++c) acc[m][c] *= by[m];
+        for (int c = 0; c < CT; ++c) acc[c] *= by;
         if (!clean) {
             // A latent that is no number makes its scores none, and the weight of every row that sees it; where a row does not,
             // its weight 0 has to meet a number. Seldom: rows of a cache hold numbers, or codes 0 under a scale of NaN.
             uint8_t* const mine = tiles[tile & 1];
-            for (int i = threadIdx.x; i < kTile * R / 4; i += WAVES * 64) {
+            for (int i = threadIdx.x; i < kTile * R / 4; i += 256) {
                 const int token = i / (R / 4), d = i % (R / 4) * 4;
                 if constexpr (E4M3) {
                     uint32_t* const at4 = reinterpret_cast<uint32_t*>(mine + token * ROW + d);
@@ -368,32 +284,28 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
         __syncthreads();  // the weights
 #pragma unroll
         for (int t = 0; t < kTile / 32; ++t) {
-            bf16x8 w[MT][kPlanes];
+            bf16x8 w8[kPlanes];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int i = 0; i < kPlanes; ++i) w[m][i] = *reinterpret_cast<const bf16x8*>(&weights[i][(16 * m + l) * kPPitch + 32 * t + 8 * g]);
+            for (int i = 0; i < kPlanes; ++i) w8[i] = *reinterpret_cast<const bf16x8*>(&weights[i][l * kPPitch + 32 * t + 8 * g]);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 // Eight tokens of a column a lane: the rows' bytes turned as they are read.
                 const int column = wave * COLS + 16 * c;
                 bf16x8 v;
                 if constexpr (E4M3) {
-                    const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    const i32x2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                         (__attribute__((address_space(3))) i32x2*)(rows + (32 * t + 8 * g + l / 2) * ROW + column + 8 * (l & 1)));
-                    v = e4m3_octet(x[0], x[1], 1.0f);
+                    v = e4m3_octet(y[0], y[1], 1.0f);
                 } else {
-                    i16x4 x[2];
+                    i16x4 y[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        x[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        y[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) i16x4*)(rows + (32 * t + 8 * g + 4 * h + l / 4) * ROW + 2 * column + 8 * (l & 3)));
-                    v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
                 }
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int i = kPlanes - 1; i >= 0; --i) acc[m][c] = mfma(v, w[m][i], acc[m][c]);
+                for (int i = kPlanes - 1; i >= 0; --i) acc[c] = mfma(v, w8[i], acc[c]);
             }
         }
         wait_for_rows();  // of the next tile
@@ -402,44 +314,26 @@ __global__ __launch_bounds__(WAVES * 64, F32 ? 1 : WAVES / 4) void latent_attent
 
     // A row's sum lies with the lanes and waves that scored its tokens.
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < RT; ++m) {
-        const float total = sum_over_groups(sum[m]);
-        if (g == 0) maxima[kg][16 * (rg * RT + m) + l] = total;
-    }
+    sum = sum_over_groups(sum);
+    if (g == 0) maxima[wave][l] = sum;
     __syncthreads();
+    if (!real) return;
+    sum = maxima[0][l] + maxima[1][l] + maxima[2][l] + maxima[3][l];
+    const int64_t at_row = b * p.rows + row;
+    if (p.splits == 1) {
+        // A row that sees nothing has no sum: zeros. One past the table: NaN.
+        const float inverse = sight.beyond ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = row0 + 16 * m + l;
-        if (row >= p.rows) continue;
-        const float total = maxima[0][16 * m + l] + maxima[1][16 * m + l] + maxima[2][16 * m + l] + maxima[3][16 * m + l];
-        const int64_t at_row = b * p.rows + row;
-        if (p.splits == 1) {
-            // A row that sees nothing has no sum: zeros. One past the table: NaN.
-            const float inverse = beyond[m] ? NAN : total == 0.0f ? 0.0f : 1.0f / total;
+        for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at_row * R + wave * COLS + 16 * c + 4 * g) = acc[c] * inverse;
+    } else {
+        const int64_t part = at_row * p.splits + split;
+        if (first < last) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const int64_t to = at_row * R + wave * COLS + 16 * c + 4 * g;
-                const f32x4 v = acc[m][c] * inverse;
-                if constexpr (F32) {
-                    *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + to) = v;
-                } else {
-                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + to) =
-                        u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(v[0]), static_cast<__bf16>(v[1])}),
-                              __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(v[2]), static_cast<__bf16>(v[3])})};
-                }
-            }
-        } else {
-            const int64_t part = at_row * p.splits + split;
-            if (first < last) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(p.partial + part * R + wave * COLS + 16 * c + 4 * g) = acc[m][c];
-            }
-            if (wave == 0 && g == 0) {
-                float* const stats = p.partial + static_cast<int64_t>(gridDim.x / (p.splits * p.row_blocks)) * p.rows * p.splits * R + part * 2;
-                stats[0] = first < last ? top[m] : -INFINITY;
-                stats[1] = beyond[m] ? NAN : first < last ? total : 0.0f;
-            }
+            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(p.partial + part * R + wave * COLS + 16 * c + 4 * g) = acc[c];
+        }
+        if (wave == 0 && g == 0) {
+            p.stats[part * 2] = first < last ? top : -INFINITY;
+            p.stats[part * 2 + 1] = sight.beyond ? NAN : first < last ? sum : 0.0f;
         }
     }
 }
@@ -470,26 +364,6 @@ __device__ __forceinline__ void wait_for_rows_but() {
 // changes no rounding, and after a row's first tokens next to no tile rescales.
 constexpr float kSlack = 16.0f;
 
-// What a token of a call sees: the places below `base`, and base + j where bit j is set; nothing from `end` on.
-struct Sight {
-    int base, end;
-    uint64_t bits;
-    bool beyond;  // past the table
-};
-__device__ __forceinline__ Sight sight_of(const LatentAttentionArgs& p, int64_t sequence, int token) {
-    const int64_t at = sequence * p.length + token;
-    const int32_t position = p.positions[at];
-    Sight s{0, 0, 0, position >= static_cast<int64_t>(p.c.width) * p.c.page_size};
-    if (position < 0 || s.beyond) return s;
-    s.end = s.base = position + 1;
-    if (p.ancestors == nullptr) return s;
-    s.base = position - token;
-    s.bits = static_cast<uint64_t>(p.ancestors[at]);
-    if (p.length < 64) s.bits &= (uint64_t{1} << p.length) - 1;
-    s.end = max(s.bits == 0 ? s.base : s.base + 64 - __builtin_clzll(s.bits), 0);
-    return s;
-}
-
 constexpr int kMaxUnits = 1024;  // that blocks share out among them
 constexpr int kLeastShare = 2;   // tiles of a block, so that a block is worth its beginning
 constexpr int kIds = 512;  // page numbers that are looked up at a time
@@ -513,7 +387,7 @@ struct Shape {
 };
 
 template <int R, int P, bool E4M3, int RW, bool WIDE>
-__global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), 2) void latent_attention_rows_kernel(LatentAttentionArgs p) {
+__global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void latent_attention_rows_kernel(LatentAttentionArgs p) {
     using S = Shape<R, P, E4M3, RW>;
     constexpr int ROW = S::ROW, KW = S::KW, KEYS = S::KEYS, STAGES = S::STAGES, SUMMERS = S::SUMMERS, PIECES = ROW / 16;
     constexpr int KS = R / 16, RS = P / 16, RG = S::GROUPS, CT = S::COLUMNS / 32;  // 16-deep steps over the latent and the key part, 32-wide tiles of columns
@@ -1140,9 +1014,9 @@ __global__ __launch_bounds__(256) void latent_join_few_kernel(LatentAttentionArg
     }
 }
 
-// The parts of a row, 64 columns a block: 16 lanes side by side, 16 parts at a time.
-template <int R, bool F32>
-__global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, const float* stats, int splits, void* out) {
+// The parts of a row of fp32, 64 columns a block: 16 lanes side by side, 16 parts at a time.
+template <int R>
+__global__ __launch_bounds__(256) void latent_join_f32_kernel(const float* partial, const float* stats, int splits, float* out) {
     __shared__ float by[256];
     __shared__ float reduced[4];
     __shared__ f32x4 sums[16][16];
@@ -1188,13 +1062,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const float* partial, 
     for (int i = 1; i < 16; ++i) acc += sums[i][threadIdx.x];
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc *= inverse;
-    if constexpr (F32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(out) + row * R + column) = acc;
-    } else {
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + row * R + column) =
-            u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[0]), static_cast<__bf16>(acc[1])}),
-                  __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[2]), static_cast<__bf16>(acc[3])})};
-    }
+    *reinterpret_cast<f32x4*>(out + row * R + column) = acc;
 }
 
 struct Plan {
@@ -1226,7 +1094,7 @@ template <int R, int P, bool F32, bool E4M3>
 void launch_attention(const LatentAttentionArgs& p, int64_t blocks, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(blocks));
     if constexpr (F32) {
-        hipLaunchKernelGGL((latent_attention_kernel<R, P, true, E4M3, 1, 4>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((latent_attention_f32_kernel<R, P, E4M3>), grid, dim3(256), 0, s, p);
     } else {
         const int64_t rows = rows_per_block(p.rows, false);
         auto go = [&](auto groups) {
@@ -1258,10 +1126,9 @@ void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool
         return;
     }
     if (p.splits == 1) return;
-    const int64_t rows = blocks / p.splits / p.row_blocks * p.rows;
-    const float* const stats = p.partial + rows * p.splits * R;
-    const dim3 grid(static_cast<unsigned>(rows * (R / 64)));
-    hipLaunchKernelGGL((latent_join_kernel<R, true>), grid, dim3(256), 0, s, p.partial, stats, p.splits, p.out);
+    const int64_t rows = static_cast<int64_t>(p.units) / p.row_blocks * p.rows;
+    hipLaunchKernelGGL((latent_join_f32_kernel<R>), dim3(static_cast<unsigned>(rows * (R / 64))), dim3(256), 0, s, p.partial, p.stats, p.splits,
+                       static_cast<float*>(p.out));
 }
 
 mlk_status check_attention(int64_t batch, int64_t length, int64_t heads) {
@@ -1323,6 +1190,7 @@ extern "C" mlk_status mlk_latent_attention(const void* q_latent, const int64_t* 
     p.wide = pages * page_size * (e4m3 ? rank + 2 * rope_dim + 16 : 2 * (rank + rope_dim) + 16) > (int64_t{1} << 32);
     p.units = static_cast<int32_t>(plan.units);
     p.shares = static_cast<int32_t>(plan.shares);
+    if (f32) p.stats = p.partial + batch * p.rows * plan.splits * rank;
     if (plan.shares != 0) {
         const int64_t parts = plan.shares * 2 * rows_per_block(p.rows, f32);
         p.stats = p.partial + parts * rank;

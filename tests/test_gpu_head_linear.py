@@ -75,3 +75,39 @@ def test_values_that_are_no_numbers_stay_in_their_row_and_column(dev, dtype, wty
     expect = torch.zeros(40, 2, 48, dtype=torch.bool, device=dev)
     expect[7, 0], expect[20, 1], expect[:, 1, 5] = True, True, True
     assert torch.equal(bad, expect) and (got[~bad] == 64).all()
+
+
+@pytest.mark.parametrize("dtype,wtype", TYPES)
+@pytest.mark.parametrize("inner_dense", [True, False])
+@pytest.mark.parametrize("T,H,K,N", [(5001, 8, 32, 256), (3000, 16, 61, 300), (3001, 16, 128, 520), (2999, 16, 200, 256), (3000, 16, 500, 130),
+                                     (300, 16, 600, 100)])
+def test_many_tokens(dev, dtype, wtype, inner_dense, T, H, K, N):
+    """Blocks that go over several tiles of tokens, the last of them short."""
+    g = torch.Generator().manual_seed(T + K)
+    x = torch.randn(T, H, K, generator=g).to(dtype)
+    w = (torch.randn(H, N, K, generator=g) * K ** -0.5).to(wtype)
+    d = w.to(dev) if inner_dense else w.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    _check(_c().head_linear(x.to(dev), d), x, w)
+
+
+def test_in_a_graph_and_on_streams(dev):
+    """Captured calls of both directions, replayed on other inputs with eager calls between; each equals the eager call's."""
+    c, g = _c(), torch.Generator().manual_seed(2)
+    w = torch.randn(16, 256, 128, generator=g).to(BF16).to(dev)
+    x = torch.randn(24, 16, 128, generator=g).to(BF16).to(dev)
+    call = lambda: c.head_linear(c.head_linear(x, w), w.transpose(1, 2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for replay in range(3):
+        x.copy_(torch.randn(x.shape, generator=g).to(BF16))
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call()), f"replay {replay}"

@@ -261,3 +261,94 @@ def test_in_a_graph_and_on_streams(dev, dtype, tree):
     two = [call() for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(t, expect) for t in one + two)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("H,rank", [(5, 64), (70, 128), (16, 512)])
+@pytest.mark.parametrize("scale", [0.0, -0.05])
+def test_scales_that_are_not_positive(dev, dtype, store, H, rank, scale):
+    """A scale of 0 weighs every token alike, a negative one the other way round; in parts and trees too."""
+    g = torch.Generator().manual_seed(H)
+    cache, table = ref.random_cache(g, 16, 48, rank, 16, store), ref.random_table(g, 2, 8, 16)
+    positions = torch.tensor([[200, 201, 202], [5, 6, 7]], dtype=torch.int32)
+    q, qr = _queries(g, 2, 3, H, rank, 16, dtype)
+    _check(dev, q, qr, cache, table, positions, store, scale=scale)
+    _check(dev, q, qr, cache, table, positions, store, scale=scale, ancestors=torch.tensor([[1, 2, 5], [0, 3, 6]]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("H", [2, 40])
+def test_more_sequences_than_are_shared_out(dev, dtype, store, H):
+    g = torch.Generator().manual_seed(H)
+    B, page, width = 1100, 16, 16
+    cache = ref.random_cache(g, 60, page, 64, 16, store)
+    table = torch.randint(0, 60, (B, width), generator=g, dtype=torch.int32)
+    positions = torch.randint(-1, page * width, (B, 1), generator=g, dtype=torch.int32)
+    q, qr = _queries(g, B, 1, H, 64, 16, dtype)
+    _check(dev, q, qr, cache, table, positions, store)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,rank,B,most", [(16, 512, 20, 3000), (70, 64, 300, 200), (40, 256, 7, 5000), (4, 128, 600, 150)])
+def test_shares_of_many_uneven_sequences(dev, dtype, H, rank, B, most):
+    """Parts that begin and end inside a sequence, hold several whole ones, or are empty; one sequence sees nothing."""
+    g = torch.Generator().manual_seed(B)
+    page, width = 32, 160
+    cache = ref.random_cache(g, 200, page, rank, 16, E4M3)
+    table = torch.randint(0, 200, (B, width), generator=g, dtype=torch.int32)
+    positions = (torch.rand(B, 1, generator=g) ** 2 * most).to(torch.int32)
+    positions[B // 2] = -1
+    q, qr = _queries(g, B, 1, H, rank, 16, dtype)
+    _check(dev, q, qr, cache, table, positions, E4M3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("H,rank,page", [(8, 64, 1), (70, 64, 1), (40, 512, 3)])
+def test_small_pages_of_a_long_sequence(dev, dtype, store, H, rank, page):
+    """More pages than are looked up at a time, in one block's share and over the chip; one of them missing."""
+    g = torch.Generator().manual_seed(page)
+    n = 2500
+    width = -(-n // page)
+    cache, table = ref.random_cache(g, width + 3, page, rank, 16, store), ref.random_table(g, 1, width, width + 3)
+    positions = torch.tensor([[n - 2, n - 1]], dtype=torch.int32)
+    q, qr = _queries(g, 1, 2, H, rank, 16, dtype)
+    _check(dev, q, qr, cache, table, positions, store)
+    # Many short-lived units make a block's share as long as a sequence.
+    many = 300
+    at = torch.full((many, 1), n - 1, dtype=torch.int32)
+    at[3:] = torch.randint(0, 900, (many - 3, 1), generator=g, dtype=torch.int32)
+    q, qr = _queries(g, many, 1, H, rank, 16, dtype)
+    _check(dev, q, qr, cache, table.expand(many, width).contiguous(), at, store)
+    table[0, 777] = -1
+    _check(dev, q[:4], qr[:4], cache, table.expand(4, width).contiguous(), at[:4], store)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store,rank,rope,H", [(E4M3, 512, 64, 16), (E4M3, 512, 64, 64), (BF16, 256, 32, 40), (E4M3, 64, 16, 24)])
+@pytest.mark.parametrize("size", [2 ** 32 - 2 ** 20, 2 ** 32 + 2 ** 28])
+def test_a_large_cache(dev, dtype, store, rank, rope, H, size):
+    """Pages all over a cache of just under 4 GiB, and of more, give bit for bit what they give in a small one."""
+    g = torch.Generator().manual_seed(rank)
+    page, width, row = 64, 10, ref.row_bytes(rank, rope, store)
+    small, table = ref.random_cache(g, 2 * width, page, rank, rope, store).to(dev), ref.random_table(g, 2, width, 2 * width)
+    pages = size // (page * row)
+    large = torch.empty(pages, page, row, dtype=torch.uint8, device=dev)
+    far = (torch.arange(2 * width) * ((pages - 1) // (2 * width - 1))).flip(0)
+    far[0] = pages - 1
+    large[far.to(dev)] = small
+    q, qr = (t.to(dev) for t in _queries(g, 2, 2, H, rank, rope, dtype))
+    positions = torch.tensor([[630, 631], [200, 201]], dtype=torch.int32, device=dev)
+    expect = _c().latent_attention(q, qr, small, table.to(dev), positions, 0.05)
+    got = _c().latent_attention(q, qr, large, far[table.long()].to(torch.int32).to(dev), positions, 0.05)
+    assert torch.isfinite(expect).all() and torch.equal(got, expect)
+    # What append writes there, read gives back.
+    x, words = torch.randn(2, 1, rank, generator=g).to(dtype).to(dev), torch.randn(2, 1, rope, generator=g).to(dtype).to(dev)
+    at = positions[:, 1:].contiguous()
+    for cache, ids in ((small, table.to(dev)), (large, far[table.long()].to(torch.int32).to(dev))):
+        _c().latent_append(x, words, cache, ids, at)
+    one = _c().latent_read(small, table.to(dev), at, rank, rope, dtype)
+    two = _c().latent_read(large, far[table.long()].to(torch.int32).to(dev), at, rank, rope, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
