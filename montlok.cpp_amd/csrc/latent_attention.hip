@@ -681,11 +681,14 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
             asm volatile("" : "+v"(places[i]));
         }
     }
+    auto find_one = [&](Asks& asks, int tile, int i) {
+        const uint8_t* const table = reinterpret_cast<const uint8_t*>(row_at[tile % SLOTS]);
+        asks.offset[i] = *reinterpret_cast<const uint32_t*>(table + (places[i] >> 16)) + (places[i] & 0xFFFF);
+    };
     auto find = [&](Asks& asks, int tile, int stage) {
         asks.to = __builtin_amdgcn_readfirstlane(lds0 + stage * S::BYTES + own * 1024);
-        const uint8_t* const table = reinterpret_cast<const uint8_t*>(row_at[tile % SLOTS]);
 #pragma unroll
-        for (int i = 0; i < ASKS; ++i) asks.offset[i] = *reinterpret_cast<const uint32_t*>(table + (places[i] >> 16)) + (places[i] & 0xFFFF);
+        for (int i = 0; i < ASKS; ++i) find_one(asks, tile, i);
     };
     auto ask = [&](const Asks& asks, int i) {
         if (whole_wave(i) || active(i)) load_row_pieces(p.c.bytes, asks.offset[i], __builtin_amdgcn_readfirstlane(asks.to + i * SUMMERS * 1024));
@@ -715,9 +718,9 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
         for (int c = 0; c < CT; ++c) acc[r][c] = f32x16{};
 
     // The latents of the tokens whose weights a lane holds, eight of a column: the rows' bytes turned as they are read.
-    // Beside its products go the loads of a later tile: at once they would fill the memory's queue and hold the wave up (1450
-    // cycles of a tile's 4400).
-    auto add_tile = [&](int tile, const uint8_t* rows, const Asks& asks, auto with_asks) {
+    // Beside its products go the loads of a later tile (at once they would fill the memory's queue and hold the wave up, 1450
+    // cycles of a tile's 4400), then the places of the one after that, `find_tile`.
+    auto add_tile = [&](int tile, const uint8_t* rows, Asks& asks, int find_tile, auto with_asks) {
         constexpr int VS = 2 * KW, GROUP = E4M3 && CT % 2 == 0 ? 2 : 1, N = GROUP * VS;  // column tiles read ahead of their products
         struct Codes {
             i32x2 v;
@@ -792,6 +795,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
 #pragma unroll
                         for (int k = 0; k < PER; ++k)
                             if (step % EVERY == 0 && step / EVERY * PER + k < ASKS) ask(asks, step / EVERY * PER + k);
+                        // Their registers are free for the next places, one a product, the last product's for what is left.
+                        constexpr int FREE = ((ASKS + PER - 1) / PER - 1) * EVERY + 1;
+#pragma unroll
+                        for (int k = 0; k < ASKS; ++k)
+                            if (k == step - FREE || (step == STEPS - 1 && k > step - FREE)) find_one(asks, find_tile, k);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -819,14 +827,15 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
                 if (tile + AHEAD < last) ask_wide(tile + AHEAD, free_stage);
             }
             if (tile > first) {
-                add_tile(tile - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], asks, std::bool_constant<!WIDE>{});
+                add_tile(tile - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], asks, min(tile + AHEAD + 1, last - 1), std::bool_constant<!WIDE>{});
             } else if constexpr (!WIDE) {
 #pragma unroll
                 for (int i = 0; i < ASKS; ++i) ask(asks, i);
+                find(asks, min(tile + AHEAD + 1, last - 1), 0);
             }
+            if constexpr (!WIDE) asks.to = __builtin_amdgcn_readfirstlane(lds0 + (free_stage == STAGES - 1 ? 0 : free_stage + 1) * S::BYTES + own * 1024);
             if (own == tile % SUMMERS && tile + AHEAD + 2 < last) set_rows(tile + AHEAD + 2);
             if (tile + AHEAD + 3 < last && tile + AHEAD + 3 >= held_end) hold(tile + AHEAD + 3);
-            if constexpr (!WIDE) find(asks, min(tile + AHEAD + 1, last - 1), free_stage == STAGES - 1 ? 0 : free_stage + 1);
             if (tile + AHEAD < last) wait_for_rows_but<(AHEAD - 1) * (S::LOADS / SUMMERS)>();
             else wait_for_rows();
             __syncthreads();
@@ -843,7 +852,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
             }
             stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
-        add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], Asks{}, std::false_type{});
+        add_tile(last - 1, tiles[stage == 0 ? STAGES - 1 : stage - 1], asks, 0, std::false_type{});
     }
     __syncthreads();  // the rows' sums
     const int column = part * S::COLUMNS + 4 * h;
