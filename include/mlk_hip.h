@@ -506,9 +506,10 @@ mlk_status mlk_linear_fp4(const void* x, int64_t rows, int64_t in_features, int6
  * Activations are fp32 or bf16 (`dtype`, an mlk_dtype), sums are held in fp32 or more, results are rounded once.
  *
  * The cache is [pages, page_size, row] bytes, 16-byte aligned, page_size 1 to 65536, R 64, 128, 256 or 512, P 16, 32 or 64.
- * With MLK_DTYPE_E4M3 a row is R e4m3 codes, P bf16 and 16 bytes that begin with the fp32 scale of the codes; with
- * MLK_DTYPE_BF16 it is R + P bf16 and 16 unused bytes. `positions` [batch, length] gives every token its place in its
- * sequence, a negative one is padding; `page_table` [batch, table_width] names a sequence's pages, 2^28 tokens at most.
+ * With MLK_DTYPE_E4M3 a row is R e4m3 codes, P bf16 and 16 bytes that begin with the fp32 scale of the codes (a power of two
+ * from 2^-117 to 2^119, 0 with codes of 0, or NaN; other scales give other results in each operator); with MLK_DTYPE_BF16
+ * it is R + P bf16 and 16 unused bytes. `positions` [batch, length] gives every token its place in its sequence, a negative
+ * one is padding; `page_table` [batch, table_width] names a sequence's pages, 2^28 tokens at most.
  * Entries of pages that no token needs may be anything. Both are contiguous int32. Calls of 2^32 threads or more are
  * refused: 2^26 tokens of an append or a read, 2^22 blocks of 16 rows (token and head, of one sequence) of an attention. */
 
@@ -524,7 +525,8 @@ mlk_status mlk_rope(const void* q, const int64_t* q_strides, const void* k, cons
 
 /* Latents [batch, length, R] and key parts [batch, length, P] (strides {sequence, token}) into the cache. e4m3: a row's scale
  * is the smallest power of two whose 448-fold reaches its largest magnitude (2^-117 to 2^119; larger values are held at 448 *
- * 2^119), codes are rounded to nearest, ties to even. bf16: rounded to nearest. A latent with an infinity or a NaN (bf16: that rounds to an infinity) becomes NaN.
+ * 2^119), codes are rounded to nearest, ties to even. bf16: rounded to nearest. A latent with an infinity or a NaN (bf16: that
+ * rounds to an infinity) becomes NaN.
  * Tokens at negative positions, past the page table or on a page outside [0, pages) are dropped. The places of one call's
  * tokens must be distinct. */
 mlk_status mlk_latent_append(const void* latent, const int64_t* latent_strides, const void* k_rope,
@@ -546,7 +548,7 @@ mlk_status mlk_latent_read(const uint8_t* cache, int32_t cache_dtype, int64_t pa
  * every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one past the page
  * table, or that sees a token on a page outside [0, pages), NaN. What the cache holds where a token does not see it, of any
  * bytes, does not reach it. fp32 queries run with fp32 accuracy, bf16 ones with the softmax weights rounded to bf16 for
- * the product with the latents. The workspace is 16-byte aligned and private to the call until it has run. */
+ * the product with the latents; theirs hold latents of up to 2^110 in size (larger ones may give an infinity). The workspace is 16-byte aligned and private to the call until it has run. */
 size_t mlk_latent_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t rank, int64_t rope_dim,
                                             int32_t dtype, int32_t cache_dtype, int64_t page_size, int64_t table_width);
 mlk_status mlk_latent_attention(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,

@@ -2,8 +2,8 @@
 // queries into the latents' space and its attended latents back to the heads' values. W is dense along its inputs or along
 // its outputs, so that both products read the same projection's rows.
 //
-// A wave takes 32 outputs of a head and goes over tokens, 32 (or 64) at a time: products have the outputs as rows and the
-// tokens as columns, so that a lane ends with runs of outputs of one token. All waves of a block read the same tokens.
+// Products have the outputs as rows and the tokens as columns, so that a lane ends with runs of outputs of one token. Sums are
+// fp32, and rounded once.
 #include <algorithm>
 #include <type_traits>
 
@@ -110,6 +110,10 @@ __device__ __forceinline__ void store_outputs(const HeadArgs& p, const f32x16& a
 
 // bf16 in and out, many tokens. A wave's weights, of NT x 32 outputs and all inputs, are kept in registers and read once; the
 // tokens of all waves go through LDS, the next 32 being loaded while these are multiplied.
+//
+// Bound by memory: 512 outputs of 128 inputs make 51 operations a byte. 4096 tokens of 64 heads take 140 us (W dense along its
+// inputs) or 122 with 512 outputs of 128 inputs, 91 with 128 of 512: 2.4, 2.8 and 3.7 TB/s (210 and 275 with each wave reading
+// the tokens by itself, 32 bytes of a row a load).
 template <int KS, int NT, bool IN_DENSE>
 __global__ __launch_bounds__(256, 2) void head_linear_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
     constexpr int ROW = KS * 16 + 8, PIECES = 64 * KS, EACH = (PIECES + 255) / 256;
@@ -159,6 +163,9 @@ __global__ __launch_bounds__(256, 2) void head_linear_kernel(HeadArgs p, unsigne
 
 // bf16 in and out, few tokens: 32 tokens x 32 outputs a block, whose WAVES waves take KS steps of the inputs each; the first
 // adds their sums in order.
+//
+// Bound by latency, one load of everything and a store: 24 tokens of 64 heads, 512 outputs of 128 inputs, 4.1 us a call (10 MB
+// at 5 TB/s are 2.1); with 512 inputs 4.5 to 5.4 (7.7 to 9.6 where one wave takes all of them).
 template <int KS, int WAVES, bool IN_DENSE>
 __global__ __launch_bounds__(WAVES * 64) void head_linear_few_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
     constexpr int TURN = (KS < kBatch ? KS : kBatch) * 16 * kTurn, TURNED = IN_DENSE ? 0 : WAVES * TURN, PARTS = (WAVES - 1) * 64 * 40;
@@ -231,7 +238,11 @@ __device__ __forceinline__ u32x4 numbers(u32x2 v) { return u32x4{v[0] << 16, v[0
 // takes the j-th of each.
 //
 // SPLIT: all waves make the same 32 x 32, from a quarter of the inputs each, and the first adds the four in order; else each
-// makes a quarter of 64 x 64.
+// makes a quarter of 64 x 64. One half of LDS is enough to split, where the sixth block on a compute unit is worth more.
+//
+// Bound by the fp32 products: 600 tokens of 24 heads, 96 outputs of 512 inputs, take 21 us (9.2 at the 154 TFLOP/s of a large
+// fp32 product; 31 with operands read from memory lane by lane, 16 rows a load), 4096 tokens of 64 heads, 512 of 128, 365 us,
+// 94 TFLOP/s. Both types of weights take the same.
 template <bool W32, bool IN_DENSE, bool SPLIT>
 __global__ __launch_bounds__(256, SPLIT ? 6 : 4) void head_linear_f32_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
     constexpr int TILE = SPLIT ? 32 : 64, TK = SPLIT ? 64 : 32, STEPS = SPLIT ? 1 : 2;
@@ -338,7 +349,7 @@ __global__ __launch_bounds__(256, SPLIT ? 6 : 4) void head_linear_f32_kernel(Hea
     }
 }
 
-// bf16 with more inputs than a wave's registers hold: 32 tokens x 32 outputs a block, sums in fp32.
+// bf16 with more inputs than a wave's registers hold (above 512): 32 tokens x 32 outputs a block on the vector units.
 __global__ __launch_bounds__(256) void head_linear_any_kernel(HeadArgs p, unsigned token_tiles, unsigned n_tiles) {
     __shared__ float xs[32][33], ws[32][33];
     const unsigned id = blockIdx.x, tile = id % token_tiles, rest = id / token_tiles, nt = rest % n_tiles, head = rest / n_tiles;
@@ -381,9 +392,11 @@ template <int KS>
 void launch_bf16(HeadArgs p, hipStream_t s) {
     constexpr int NT = KS > 8 ? 1 : 2;
     const bool in_dense = p.ws_in == 1;
-    // A block of many tokens reads its weights once for all of them: four such a compute unit, where they fill half of it.
+    // A block of many tokens reads its weights once for all of them; up to four such a compute unit, at least one: of 456
+    // blocks (600 tokens of 24 heads, 512 -> 96) 10.8 us against 13.4 in tiles of few tokens, of 256 (64 of 64 heads, 128 ->
+    // 512) 5.6 against 6.6, of 160 (300 of 16 heads, 512 -> 128) 8.0 against 7.8.
     const unsigned wide = static_cast<unsigned>(ceil_div(p.n, 128 * NT)), chunks = cut(p, 32, p.heads * wide, 4 * kChip);
-    if (const unsigned blocks = p.heads * wide * chunks; blocks >= 2 * kChip) {
+    if (const unsigned blocks = p.heads * wide * chunks; blocks >= kChip) {
         if (in_dense) hipLaunchKernelGGL((head_linear_kernel<KS, NT, true>), grid_of(blocks), dim3(256), 0, s, p, wide, chunks, blocks);
         else hipLaunchKernelGGL((head_linear_kernel<KS, NT, false>), grid_of(blocks), dim3(256), 0, s, p, wide, chunks, blocks);
     } else {
@@ -405,7 +418,8 @@ void launch_f32(HeadArgs p, hipStream_t s) {
         if (p.ws_in == 1) hipLaunchKernelGGL((head_linear_f32_kernel<W32, true, SPLIT>), grid_of(blocks), dim3(256), 0, s, p, n_blocks, chunks, blocks);
         else hipLaunchKernelGGL((head_linear_f32_kernel<W32, false, SPLIT>), grid_of(blocks), dim3(256), 0, s, p, n_blocks, chunks, blocks);
     };
-    // Tiles of 32 x 32 that give every SIMD two waves or more are not split.
+    // Tiles of 32 x 32 that give every SIMD two waves are not split: 2048 tiles (64 tokens of 64 heads, 128 -> 512) take 9.4 us,
+    // split 11.1; 1368 (600 tokens of 24 heads, 512 -> 96) 24.7, split 21.6; 640 (300 of 16, 512 -> 128) 16.2, split 12.0.
     if (p.heads * ceil_div(p.n, 32) * ceil_div(p.tokens, 32) >= 8 * kChip) launch(std::false_type{});
     else launch(std::true_type{});
 }
