@@ -542,7 +542,7 @@ mlk_status mlk_latent_read(const uint8_t* cache, int32_t cache_dtype, int64_t pa
                            mlk_stream_t stream);
 
 /* softmax((q_latent . c + q_rope . r) * scale) c over cached tokens, q_latent [batch, length, heads, R], q_rope [.., P],
- * strides {sequence, token, head}; out [batch, length, heads, R] contiguous, 16-byte aligned. Without `ancestors` a token
+ * strides {sequence, token, head}; scale finite, of any sign; out [batch, length, heads, R] contiguous, 16-byte aligned. Without `ancestors` a token
  * sees the cached tokens 0 .. its position. With ancestors [batch, length] (int64, length <= 64) the call's tokens are a
  * tree that lies in the cache in the call's order: token i at the place p sees the places below p - i, and p - i + j for
  * every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one past the page
@@ -560,7 +560,8 @@ mlk_status mlk_latent_attention(const void* q_latent, const int64_t* q_latent_st
 
 /* y[t, h] = W[h] x[t, h]: x [tokens, heads, in_features] (strides {token, head}, in_features dense), W [heads, out_features,
  * in_features] (strides {head, out, in}, one of the last two 1), y [tokens, heads, out_features] contiguous, 16-byte aligned,
- * of x's dtype. weight_dtype: bf16, or fp32 with fp32 x. fp32 x keeps fp32 accuracy in both. */
+ * of x's dtype. weight_dtype: bf16, or fp32 with fp32 x. fp32 x keeps fp32 accuracy in both. At most 2^23 tiles of 32 tokens
+ * and 32 outputs of a head a call. */
 mlk_status mlk_head_linear(const void* x, int64_t tokens, int64_t heads, int64_t in_features, const int64_t* x_strides,
                            int32_t dtype, const void* weight, const int64_t* weight_strides, int32_t weight_dtype,
                            int64_t out_features, void* out, mlk_stream_t stream);

@@ -1184,6 +1184,7 @@ extern "C" mlk_status mlk_latent_attention(const void* q_latent, const int64_t* 
     if (checked == MLK_OK) checked = check_attention(batch, length, heads);
     if (checked != MLK_OK) return checked;
     MLK_CHECK(ancestors == nullptr || length <= 64, "a tree holds at most 64 tokens");
+    MLK_CHECK(std::isfinite(static_cast<float>(scale * 1.4426950408889634074)), "scale must be finite");
     if (batch == 0 || length == 0) return MLK_OK;
     MLK_CHECK(q_latent && q_latent_strides && q_rope && q_rope_strides && cache && page_table && positions && out, "null tensor pointer");
     MLK_CHECK((reinterpret_cast<uintptr_t>(cache) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "cache and out must be 16-byte aligned");

@@ -352,3 +352,53 @@ def test_a_large_cache(dev, dtype, store, rank, rope, H, size):
     one = _c().latent_read(small, table.to(dev), at, rank, rope, dtype)
     two = _c().latent_read(large, far[table.long()].to(torch.int32).to(dev), at, rank, rope, dtype)
     assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,rank", [(5, 64), (40, 512), (70, 128)])
+def test_one_token_carries_all_the_weight(dev, dtype, H, rank):
+    """Scores of thousands, so that a row's result is one latent (its weight and the result rounded, to bf16 at the coarsest);
+    and a query of zeros, whose result is their mean."""
+    g = torch.Generator().manual_seed(H)
+    cache, table = ref.random_cache(g, 20, 32, rank, 32, E4M3), ref.random_table(g, 2, 10, 20)
+    positions = torch.tensor([[318, 319], [0, 77]], dtype=torch.int32)
+    q, qr = _queries(g, 2, 2, H, rank, 32, dtype)
+    _check(dev, q * 0, qr * 0, cache, table, positions, E4M3)
+    got = _c().latent_attention((q * 512).to(dev), (qr * 512).to(dev), cache.to(dev), table.to(dev), positions.to(dev), 1.0).double().cpu()
+    latent, words = ref.contents(cache, rank, 32, E4M3)
+    for b in range(2):
+        for i in range(2):
+            n = int(positions[b, i]) + 1
+            c, r = latent[table[b].long()].flatten(0, 1)[:n], words[table[b].long()].flatten(0, 1)[:n]
+            score = 512 * (q[b, i].double() @ c.t() + qr[b, i].double() @ r.t())
+            best = score.topk(min(2, n), -1)
+            sure = torch.ones(H, dtype=torch.bool) if n == 1 else best.values[:, 0] - best.values[:, 1] > 60
+            expect = c[best.indices[:, 0]]
+            assert sure.any() and ((got[b, i] - expect).abs()[sure] <= 2.02 * ref.half_step(BF16) * expect.abs()[sure] + 1e-12).all()
+
+
+@pytest.mark.parametrize("B,L", [(0, 1), (2, 0), (0, 0)])
+def test_empty_calls(dev, B, L):
+    c = _c()
+    cache = c.latent_cache(2, 16, 64, 16, E4M3, dev)
+    at, table = torch.zeros(B, L, dtype=torch.int32, device=dev), torch.zeros(B, 2, dtype=torch.int32, device=dev)
+    for dtype in (F32, BF16):
+        q, qr = torch.zeros(B, L, 3, 64, dtype=dtype, device=dev), torch.zeros(B, L, 3, 16, dtype=dtype, device=dev)
+        assert c.latent_attention(q, qr, cache, table, at, 1.0).shape == (B, L, 3, 64)
+        assert c.latent_attention(q, qr, cache, table, at, 1.0, torch.zeros(B, L, dtype=torch.int64, device=dev)).shape == (B, L, 3, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tensors_of_one_storage_and_expanded_ones(dev, dtype):
+    """Every sequence with the same table, positions and queries, expanded without a copy."""
+    g = torch.Generator().manual_seed(12)
+    cache, table = ref.random_cache(g, 8, 16, 64, 16, BF16), ref.random_table(g, 1, 8, 8)
+    positions = torch.tensor([[99, 100, 101]], dtype=torch.int32)
+    q, qr = _queries(g, 1, 1, 6, 64, 16, dtype)
+    spread = lambda t, *s: t.to(dev).expand(*s)
+    got = _c().latent_attention(spread(q, 4, 3, 6, 64), spread(qr, 4, 3, 6, 16), cache.to(dev), spread(table, 4, 8), spread(positions, 4, 3), 0.1)
+    one = _check(dev, q.expand(1, 3, 6, 64), qr.expand(1, 3, 6, 16), cache, table, positions, BF16, scale=0.1)
+    out, size, span = ref.attention(q.expand(1, 3, 6, 64), qr.expand(1, 3, 6, 16), cache, table, positions, 0.1, BF16)
+    bound = ref.attention_bound(size, span, out, 102, 80, dtype)
+    for b in range(4):
+        _within(got[b:b + 1], out, bound)

@@ -156,3 +156,12 @@ def test_past_the_end_and_refusals(dev):
             m.new_state(*bad)
     with pytest.raises(RuntimeError, match="rank must be"):
         _module(dev, rank=48).new_state(1, 16)
+
+
+def test_no_tokens_leave_the_state(dev):
+    m = _module(dev)
+    x = torch.randn(2, 3, m.d_model, generator=torch.Generator().manual_seed(5)).to(dev)
+    state, twin = m.new_state(2, 16), m.new_state(2, 16)
+    with torch.no_grad():
+        assert m.step(x[:, :0], state).shape == (2, 0, m.d_model)
+        assert torch.equal(m.step(x, state), m.step(x, twin)) and torch.equal(state["cache"], twin["cache"])

@@ -163,3 +163,9 @@ def test_frequencies():
     assert (ratio[turns > 33] > 0.97).all() and torch.allclose(ratio[turns < 0.9], torch.tensor(1 / 40.0, dtype=torch.float64), rtol=1e-12)
     assert (ratio[1:] <= ratio[:-1] + 1e-15).all() and ((ratio < 0.97) & (ratio > 0.03)).sum() > 5
     assert torch.equal(_C.rope_frequencies(64, factor=1.0, original_length=4096, device="cpu")[0], plain)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e300, -3e38])
+def test_scales_that_fp32_does_not_hold_are_refused(lib, scale):
+    status = lib.mlk_latent_attention(None, None, None, None, 1, 1, 1, 4, 64, 16, None, 2, 4, 64, None, 2, None, None, scale, None, None, 0, None)
+    assert status == 1 and "scale must be finite" in lib.mlk_last_error().decode()
