@@ -908,11 +908,11 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
     }
 }
 
-// The parts of a unit's rows: a row and COLUMNS of its columns a block, 4 a lane, as many parts at a time as the lanes allow.
+// The parts of a unit's rows: a row and 64 of its columns a block, 4 a lane, 16 parts at a time.
 // 256 parts of 32 rows of 512 columns (17 MB): 6.8 us.
-template <int R, int COLUMNS>
+template <int R>
 __global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionArgs p, int rows_per_unit) {
-    constexpr int LANES = COLUMNS / 4, GROUPS = 256 / LANES, BATCH = 8;
+    constexpr int COLUMNS = 64, LANES = COLUMNS / 4, GROUPS = 256 / LANES, BATCH = 8;
     __shared__ float by[256];
     __shared__ float reduced[4];
     __shared__ f32x4 sums[GROUPS][LANES];
@@ -963,13 +963,11 @@ __global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionAr
             }
         }
     }
-    if constexpr (GROUPS > 1) {
-        sums[group][threadIdx.x % LANES] = acc;
-        __syncthreads();
-        if (group != 0) return;
+    sums[group][threadIdx.x % LANES] = acc;
+    __syncthreads();
+    if (group != 0) return;
 #pragma unroll
-        for (int i = 1; i < GROUPS; ++i) acc += sums[i][threadIdx.x];
-    }
+    for (int i = 1; i < GROUPS; ++i) acc += sums[i][threadIdx.x];
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc *= inverse;
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + (b * p.rows + row) * R + column) =
@@ -1145,7 +1143,7 @@ void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool
         const int per = static_cast<int>(rows_per_block(p.rows, false));
         // A row of many parts falls to several blocks of 64 columns: 256 parts of each of 32 rows 35.0 us with the attention, by
         // one wave a row 78.9. Where rows have some ten parts a wave each is faster: 24 units 6.0 us, by 64 columns 9.8.
-        if (p.units * 16 <= p.shares) hipLaunchKernelGGL((latent_join_rows_kernel<R, 64>), dim3(static_cast<unsigned>(p.units * per * (R / 64))), dim3(256), 0, s, p, per);
+        if (p.units * 16 <= p.shares) hipLaunchKernelGGL((latent_join_rows_kernel<R>), dim3(static_cast<unsigned>(p.units * per * (R / 64))), dim3(256), 0, s, p, per);
         else hipLaunchKernelGGL((latent_join_few_kernel<R>), dim3(static_cast<unsigned>(p.units * per / (R / 4 < 64 ? 1024 / R : 4))), dim3(256), 0, s, p, per);
         return;
     }
