@@ -381,7 +381,7 @@ constexpr int kIds = 512;  // page numbers that are looked up at a time
 // A tile is scored while the one before it is summed, with one barrier between.
 //
 // Measured with R = 512, P = 64 in eight bits: 24 sequences of up to 8000 tokens, 16 heads, 32.6 us; one of 131072 tokens, 32
-// heads, 28.5 us (84 MB); 64 of up to 16384, 64 heads, 128 us (435 MB, 3.4 TB/s, 720 TFLOP/s); two chunks of 256 tokens of 24
+// heads, 28.5 us (84 MB); 64 of up to 16384, 64 heads, 125 us (435 MB, 3.5 TB/s, 735 TFLOP/s); two chunks of 256 tokens of 24
 // heads over up to 8000 183 us (900 TFLOP/s). A launch's first 8 us (positions, page numbers, row addresses, a tile, each after
 // the other) and its last 2 are no work on tiles; a tile of 64 rows and 64 tokens then takes 2.0 us where its products alone
 // take 1.1: LDS reads and conversions of the operands share the SIMD with them (a product of 32 cycles takes 47 beside its
@@ -829,6 +829,8 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
         Asks asks{};
         if constexpr (!WIDE) find(asks, first + AHEAD, AHEAD);
         __syncthreads();
+        // Before the scorers, whose weights are not needed until the barrier: 64 x 16384 tokens 141 -> 135 us.
+        __builtin_amdgcn_s_setprio(2);
         int stage = 0;  // of the tile that is scored
         for (int tile = first; tile < last; ++tile) {
             // The stage that is loaded now was summed in the iteration before this one. Behind the last tile that tile is loaded
