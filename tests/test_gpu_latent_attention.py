@@ -402,3 +402,17 @@ def test_tensors_of_one_storage_and_expanded_ones(dev, dtype):
     bound = ref.attention_bound(size, span, out, 102, 80, dtype)
     for b in range(4):
         _within(got[b:b + 1], out, bound)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("name", [-1, -2, -3, 4, 5, 2 ** 30])
+def test_every_number_outside_the_pages_is_a_missing_page(dev, dtype, store, name):
+    """In a whole tile, in a tile that ends with the sequence, and where no token sees it."""
+    g = torch.Generator().manual_seed(12)
+    cache = ref.random_cache(g, 4, 64, 64, 16, store)
+    table = torch.tensor([[name, 1, 2], [0, name, 3], [2, 3, name]], dtype=torch.int32)
+    positions = torch.tensor([[63, 130, 5], [63, 64, 191], [127, 128, 150]], dtype=torch.int32)
+    q, qr = _queries(g, 3, 3, 4, 64, 16, dtype)
+    got = _check(dev, q, qr, cache, table, positions, store)
+    assert torch.isnan(got).all(-1).all(-1).tolist() == [[True, True, True], [False, True, True], [False, True, True]]
