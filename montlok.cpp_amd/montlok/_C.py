@@ -694,7 +694,8 @@ def rope_frequencies(rope_dim: int, theta: float = 10000.0, factor: float = 1.0,
 
     theta^(-2 i / rope_dim); divided by ``factor`` for contexts that are ``factor`` times as long. With ``original_length``
     (the context before) pairs that turn more than ``fast`` times over it are kept and those that turn less than ``slow``
-    times are divided, with a straight ramp over the pairs between, and the magnitude is 0.1 ln(factor) + 1 (the method
+    times are divided, with a straight ramp over the pairs between (from the pair before ``fast`` turns, 0 at the least, to
+    the one behind ``slow`` turns, which may lie behind the last), and the magnitude is 0.1 ln(factor) + 1 (the method
     published as YaRN)."""
     _check(rope_dim > 0 and rope_dim % 2 == 0, "rope_dim must be even and positive")
     _check(theta > 1 and factor >= 1 and original_length >= 0, "theta must exceed 1, factor be at least 1, original_length not negative")
@@ -709,7 +710,7 @@ def rope_frequencies(rope_dim: int, theta: float = 10000.0, factor: float = 1.0,
         def pair(turns: float) -> float:
             return rope_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rope_dim // 2 - 1)
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rope_dim - 1)
         ramp = ((index - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
         frequencies = frequencies * (1 - ramp) + frequencies / factor * ramp
         magnitude = 0.1 * math.log(factor) + 1.0

@@ -169,3 +169,24 @@ def test_frequencies():
 def test_scales_that_fp32_does_not_hold_are_refused(lib, scale):
     status = lib.mlk_latent_attention(None, None, None, None, 1, 1, 1, 4, 64, 16, None, 2, 4, 64, None, 2, None, None, scale, None, None, 0, None)
     assert status == 1 and "scale must be finite" in lib.mlk_last_error().decode()
+
+
+@pytest.mark.parametrize("rope_dim,original", [(16, 32768), (64, 131072), (16, 500000), (16, 4096), (64, 4096), (128, 10 ** 6)])
+@pytest.mark.parametrize("factor", [4.0, 40.0])
+def test_frequencies_where_the_slowest_pair_still_turns(rope_dim, original, factor):
+    """Every pair against the ramp written out from how often it turns: the fastest turns original / (2 pi) times, each next
+    one theta^(2 / rope_dim) times less often. It ends where a pair would turn once, wherever the last pair lies."""
+    from montlok import _C
+
+    plain = _C.rope_frequencies(rope_dim, device="cpu")[0].tolist()
+    got = _C.rope_frequencies(rope_dim, factor=factor, original_length=original, device="cpu")[0].tolist()
+    fewer = math.log(10000.0) * 2 / rope_dim
+    low = max(0, math.floor(math.log(original / (2 * math.pi) / 32) / fewer))
+    high = math.ceil(math.log(original / (2 * math.pi)) / fewer)
+    assert high < rope_dim
+    for i, (f, y) in enumerate(zip(plain, got)):
+        slowed = min(1.0, max(0.0, (i - low) / (high - low)))
+        assert abs(y / f - (1 - slowed + slowed / factor)) <= 1e-13
+        turns = original * f / (2 * math.pi)
+        assert turns > 1 or abs(y / f * factor - 1) <= 1e-12
+        assert turns <= 1 or y / f > 1 / factor + 1e-3
