@@ -693,10 +693,10 @@ def rope_frequencies(rope_dim: int, theta: float = 10000.0, factor: float = 1.0,
     """The ``frequencies`` (float64 [rope_dim / 2], radians a position) and ``magnitude`` of ``rope``.
 
     theta^(-2 i / rope_dim); divided by ``factor`` for contexts that are ``factor`` times as long. With ``original_length``
-    (the context before) pairs that turn more than ``fast`` times over it are kept and those that turn less than ``slow``
-    times are divided, with a straight ramp over the pairs between (from the pair before ``fast`` turns, 0 at the least, to
-    the one behind ``slow`` turns, which may lie behind the last), and the magnitude is 0.1 ln(factor) + 1 (the method
-    published as YaRN)."""
+    (the context before, more than 2 pi ``slow`` positions) pairs that turn more than ``fast`` times over it are kept and
+    those that turn less than ``slow`` times are divided, with a straight ramp over the pairs between (from the pair before
+    ``fast`` turns, 0 at the least, to the one behind ``slow`` turns, which may lie behind the last), and the magnitude is
+    0.1 ln(factor) + 1 (the method published as YaRN)."""
     _check(rope_dim > 0 and rope_dim % 2 == 0, "rope_dim must be even and positive")
     _check(theta > 1 and factor >= 1 and original_length >= 0, "theta must exceed 1, factor be at least 1, original_length not negative")
     index = torch.arange(rope_dim // 2, dtype=torch.float64)
@@ -706,6 +706,7 @@ def rope_frequencies(rope_dim: int, theta: float = 10000.0, factor: float = 1.0,
         frequencies = frequencies / factor
     elif factor != 1.0:
         _check(fast > slow > 0, "fast must exceed slow, slow be positive")
+        _check(original_length > 2 * math.pi * slow, "original_length must hold slow turns of the fastest pair")
 
         def pair(turns: float) -> float:
             return rope_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))

@@ -190,3 +190,13 @@ def test_frequencies_where_the_slowest_pair_still_turns(rope_dim, original, fact
         turns = original * f / (2 * math.pi)
         assert turns > 1 or abs(y / f * factor - 1) <= 1e-12
         assert turns <= 1 or y / f > 1 / factor + 1e-3
+
+
+def test_frequencies_of_a_context_that_no_pair_turns_in_are_refused():
+    from montlok import _C
+
+    for bad in (dict(original_length=1), dict(original_length=6), dict(original_length=100, slow=16.0)):
+        with pytest.raises(RuntimeError, match="original_length"):
+            _C.rope_frequencies(16, factor=4.0, device="cpu", **bad)
+    _C.rope_frequencies(16, factor=4.0, original_length=7, device="cpu")
+    assert torch.equal(_C.rope_frequencies(16, original_length=1, device="cpu")[0], _C.rope_frequencies(16, device="cpu")[0])
