@@ -205,6 +205,7 @@ class MLAHIP(nn.Module):
         table = torch.arange(streams * pages, dtype=torch.int32, device=device).view(streams, pages)
         return {"cache": ext().latent_cache(streams * pages, page_size, self.kv_lora_rank, self.rope_dim, dtype, device),
                 "page_table": table, "length": torch.zeros(streams, 1, dtype=torch.int32, device=device),
+                "max_length": max_length,
                 "frequencies": self.rope.freqs.double().to(device)}
 
     def step(self, u: torch.Tensor, state: dict) -> torch.Tensor:
@@ -226,6 +227,9 @@ class MLAHIP(nn.Module):
         latent = c.layer_norm(projected[..., q_width:q_width + self.kv_lora_rank], self.kv_norm.weight, self.kv_norm.bias,
                               self.kv_norm.eps)
         at = state["length"] + torch.arange(x.shape[1], dtype=torch.int32, device=x.device)
+        held = state["page_table"].shape[1] * state["cache"].shape[1]
+        if held > state["max_length"]:  # the last page is longer than the stream: behind its end is behind the table
+            at.masked_fill_(at >= state["max_length"], held)
         q_rope, k_rope = c.rope(q[..., self.nope_dim:], projected[..., None, q_width + self.kv_lora_rank:],
                                 state["frequencies"], at)
         c.latent_append(latent, k_rope[:, :, 0], state["cache"], state["page_table"], at)

@@ -165,3 +165,21 @@ def test_no_tokens_leave_the_state(dev):
     with torch.no_grad():
         assert m.step(x[:, :0], state).shape == (2, 0, m.d_model)
         assert torch.equal(m.step(x, state), m.step(x, twin)) and torch.equal(state["cache"], twin["cache"])
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("length,page_size", [(20, 16), (9, 64), (33, 7)])
+def test_the_end_inside_a_page(dev, store, length, page_size):
+    """max_length holds to the token where pages reach beyond it: token by token, in a chunk that passes it, and behind it.
+    Against float64 from what the cache holds, as test_tokens_and_chunks_in_turn."""
+    m = _module(dev)
+    x = torch.randn(2, length + 5, m.d_model, generator=torch.Generator().manual_seed(6))
+    state = m.new_state(2, length, store, page_size)
+    cuts = [0, 4, 5, length - 2, length + 2, length + 5]
+    with torch.no_grad():
+        y = torch.cat([m.step(x[:, i:j].to(dev), state) for i, j in zip(cuts, cuts[1:])], 1)
+        assert torch.isnan(y[:, length:]).all() and torch.isnan(m.step(x[:, 0].to(dev), state)).all()
+    for b in range(2):
+        latents, words = ref.contents(_rows(state, b, length), m.kv_lora_rank, m.rope_dim, store)
+        expect = _reference(m, x[b, :length], latents, words)
+        assert (y[b, :length].double().cpu() - expect).abs().max() <= 1e-5 * expect.abs().max()
