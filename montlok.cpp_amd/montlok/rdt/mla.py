@@ -234,7 +234,10 @@ class MLAHIP(nn.Module):
                                 state["frequencies"], at)
         c.latent_append(latent, k_rope[:, :, 0], state["cache"], state["page_table"], at)
         rows = self.kv_up.weight.detach().view(self.n_heads, self.nope_dim + self.head_dim, self.kv_lora_rank)
-        q_latent = c.head_linear(q[..., :self.nope_dim], rows[:, :self.nope_dim].transpose(1, 2))
+        if self.nope_dim > 0:
+            q_latent = c.head_linear(q[..., :self.nope_dim], rows[:, :self.nope_dim].transpose(1, 2))
+        else:  # heads that are rotated whole: nothing of their scores is the latents'
+            q_latent = q.new_zeros(*q.shape[:3], self.kv_lora_rank)
         seen = c.latent_attention(q_latent, q_rope, state["cache"], state["page_table"], at, self.scale)
         values = c.head_linear(seen, rows[:, self.nope_dim:])
         state["length"] += x.shape[1]

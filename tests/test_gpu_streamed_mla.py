@@ -183,3 +183,21 @@ def test_the_end_inside_a_page(dev, store, length, page_size):
         latents, words = ref.contents(_rows(state, b, length), m.kv_lora_rank, m.rope_dim, store)
         expect = _reference(m, x[b, :length], latents, words)
         assert (y[b, :length].double().cpu() - expect).abs().max() <= 1e-5 * expect.abs().max()
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+def test_heads_that_are_rotated_whole(dev, store):
+    """nope_head_dim 0, which forward has too: scores are of the key parts alone. Against float64 from what the cache holds, as
+    test_tokens_and_chunks_in_turn, and against forward, as test_a_stream_is_the_whole_windows_forward."""
+    m = _module(dev, nope=0)
+    x = torch.randn(2, 20, m.d_model, generator=torch.Generator().manual_seed(7))
+    state = m.new_state(2, 20, store, 16)
+    with torch.no_grad():
+        y = torch.cat([m.step(x[:, :19].to(dev), state), m.step(x[:, 19].to(dev), state)[:, None]], 1)
+        whole = m(x.to(dev))
+    for b in range(2):
+        latents, words = ref.contents(_rows(state, b, 20), m.kv_lora_rank, m.rope_dim, store)
+        expect = _reference(m, x[b], latents, words)
+        assert (y[b].double().cpu() - expect).abs().max() <= 1e-5 * expect.abs().max()
+    if store == BF16:
+        assert (y - whole).abs().max() <= 2e-2 * whole.abs().max()
