@@ -206,7 +206,7 @@ class MLAHIP(nn.Module):
         return {"cache": ext().latent_cache(streams * pages, page_size, self.kv_lora_rank, self.rope_dim, dtype, device),
                 "page_table": table, "length": torch.zeros(streams, 1, dtype=torch.int32, device=device),
                 "max_length": max_length,
-                "frequencies": self.rope.freqs.double().to(device)}
+                "frequencies": _build_freqs(self.rope_dim, self.rope.theta).double().to(device)}
 
     def step(self, u: torch.Tensor, state: dict) -> torch.Tensor:
         """The next token ``u [S, d_model]`` of every stream, or the next ``[S, L, d_model]``; ``state`` advances in place

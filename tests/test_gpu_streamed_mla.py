@@ -201,3 +201,15 @@ def test_heads_that_are_rotated_whole(dev, store):
         assert (y[b].double().cpu() - expect).abs().max() <= 1e-5 * expect.abs().max()
     if store == BF16:
         assert (y - whole).abs().max() <= 2e-2 * whole.abs().max()
+
+
+def test_frequencies_of_a_module_that_was_cast(dev):
+    """Casting a module's weights casts its buffers as well; the rotation keeps its frequencies, as forward does."""
+    m, cast = _module(dev, weights=BF16), _module(dev, weights=BF16).to(BF16)
+    cast.kv_norm.float()
+    cast.kv_norm.load_state_dict(m.kv_norm.state_dict())
+    x = torch.randn(2, 30, m.d_model, generator=torch.Generator().manual_seed(8)).to(dev)
+    state, other = m.new_state(2, 30), cast.new_state(2, 30)
+    assert torch.equal(state["frequencies"], other["frequencies"])
+    with torch.no_grad():
+        assert torch.equal(m(x), cast(x)) and torch.equal(m.step(x, state), cast.step(x, other))
