@@ -832,12 +832,12 @@ Tensor head_linear(const OptTensor& x_, const OptTensor& weight_) {
     REQUIRE(weight_->size(0) == heads && weight_->size(2) == k, "weight must be [heads, out_features, in_features] with x's heads and features");
     REQUIRE(heads > 0 && k > 0 && n > 0, "heads and features must be positive");
     Tensor w = *weight_;
-    if (w.stride(1) != 1 && w.stride(2) != 1) w = w.contiguous();
+    if (w.stride(1) != 1 && w.stride(2) != 1 && k != 1) w = w.contiguous();
     Tensor r = x.dim() == 3 ? x : x.reshape({-1, heads, k});
     if (r.stride(2) != 1 && k != 1) r = r.contiguous();
     std::vector<int64_t> sizes = with_last(x, n);
     const Tensor out = at::empty(sizes, x.options().memory_format(at::MemoryFormat::Contiguous));
-    const int64_t xs[2] = {r.stride(0), r.stride(1)}, ws[3] = {w.stride(0), w.stride(1), w.stride(2)};
+    const int64_t xs[2] = {r.stride(0), r.stride(1)}, ws[3] = {w.stride(0), w.stride(1), k == 1 ? 1 : w.stride(2)};  // one input is dense at any stride
     done(lib.mlk_head_linear(r.const_data_ptr(), r.size(0), heads, k, xs, dtype_of(x), w.const_data_ptr(), ws, dtype_of(w), n, out.data_ptr(), stream()));
     return out;
 }

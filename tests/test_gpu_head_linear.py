@@ -111,3 +111,13 @@ def test_in_a_graph_and_on_streams(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, call()), f"replay {replay}"
+
+
+@pytest.mark.parametrize("dtype,wtype", TYPES)
+@pytest.mark.parametrize("N,K", [(1, 1), (1, 5), (5, 1)])
+def test_weights_of_one_input_or_output_in_any_order(dev, dtype, wtype, N, K):
+    """Parts of a tensor whose heads lie side by side, which count as contiguous where both sizes are 1."""
+    g = torch.Generator().manual_seed(13)
+    w = torch.randn(8, 7, 3, generator=g).to(wtype)
+    x = torch.randn(40, 3, K, generator=g).to(dtype)
+    _check(_c().head_linear(x.to(dev), w.to(dev).permute(2, 0, 1)[:, :N, :K]), x, w.permute(2, 0, 1)[:, :N, :K])
