@@ -149,21 +149,17 @@ __global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttenti
         planes_of<true>(v, q[t]);
     }
 
-    // Row addresses of a tile: by the first wave, a token a lane. A page's number, kMissing for any that is none, kBehind for
-    // tokens that no row sees.
-    constexpr int kMissing = -1, kBehind = -2;
+    // Row addresses of a tile: by the first wave, a token a lane. The page's number is looked at a tile after it was asked for.
     auto page_of = [&](int tile) {
-        const uint32_t token = static_cast<uint32_t>(tile) * kTile + lane;
-        if (static_cast<int>(token) >= end) return kBehind;
-        const uint32_t page = token / static_cast<uint32_t>(p.c.page_size);
-        if (page >= static_cast<uint32_t>(p.c.width)) return kMissing;
-        const int page_id = p.c.table[b * p.c.width + page];
-        return page_id >= 0 && page_id < p.c.pages ? page_id : kMissing;
+        const uint32_t token = static_cast<uint32_t>(tile) * kTile + lane, page = token / static_cast<uint32_t>(p.c.page_size);
+        return static_cast<int>(token) < end && page < static_cast<uint32_t>(p.c.width) ? p.c.table[b * p.c.width + page] : -1;
     };
     auto set_rows = [&](int tile, int page_id) {
         const uint32_t token = static_cast<uint32_t>(tile) * kTile + lane, in_page = token % static_cast<uint32_t>(p.c.page_size);
-        row_at[lane] = page_id >= 0 ? p.c.bytes + (static_cast<int64_t>(page_id) * p.c.page_size + in_page) * ROW : kZeroRow;
-        missing[tile & 1][lane] = page_id == kMissing ? NAN : 0.0f;
+        const bool held = page_id >= 0 && page_id < p.c.pages;
+        row_at[lane] = held ? p.c.bytes + (static_cast<int64_t>(page_id) * p.c.page_size + in_page) * ROW : kZeroRow;
+        // Tokens that no row sees are no missing ones.
+        missing[tile & 1][lane] = held || static_cast<int>(token) >= end ? 0.0f : NAN;
     };
     auto load_tile = [&](int tile) {
         const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)tiles[tile & 1]));
