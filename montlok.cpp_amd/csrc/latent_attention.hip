@@ -6,6 +6,7 @@
 // same rows: 16 heads make 56 operations a byte of eight-bit rows (bound by memory), 64 heads 224 (memory and products alike),
 // a chunk's tokens any number (products).
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -73,25 +74,33 @@ __device__ __forceinline__ void wait_for_rows() {
     asm volatile("" ::: "memory");
 }
 
-// What a token of a call sees: the places below `base`, and base + j where bit j is set; nothing from `end` on.
+// What a token of a call sees: the places below `base`, and base + j where bit j is set; nothing from `end` on. The base is
+// kNowhere where that is nothing, 0 past the table, where it is nothing either but the result NaN.
 struct Sight {
     int base, end;
     uint64_t bits;
-    bool beyond;  // past the table
 };
+constexpr int kNowhere = -(1 << 30);
 __device__ __forceinline__ Sight sight_of(const LatentAttentionArgs& p, int64_t sequence, int token) {
     const int64_t at = sequence * p.length + token;
     const int32_t position = p.positions[at];
-    Sight s{0, 0, 0, position >= static_cast<int64_t>(p.c.width) * p.c.page_size};
-    if (position < 0 || s.beyond) return s;
+    Sight s{position < 0 ? kNowhere : 0, 0, 0};
+    if (position < 0 || position >= static_cast<int64_t>(p.c.width) * p.c.page_size) return s;
     s.end = s.base = position + 1;
     if (p.ancestors == nullptr) return s;
     s.base = position - token;
     s.bits = static_cast<uint64_t>(p.ancestors[at]);
     if (p.length < 64) s.bits &= (uint64_t{1} << p.length) - 1;
     s.end = max(s.bits == 0 ? s.base : s.base + 64 - __builtin_clzll(s.bits), 0);
+    if (s.end == 0) s.base = kNowhere;
     return s;
 }
+
+// What a row's sums are multiplied by. Where it sees tokens its sum is 1 at least, its largest weight; it is 0 where it sees
+// nothing, which gives zeros, and where all its scores are -infinity or it is past the table, which gives NaN. A part's maximum
+// tells the join which: -infinity for the first, kNoWeight for the others where no weight of theirs is in the part.
+__device__ __forceinline__ float inverse_of(float sum, bool nothing) { return sum != 0.0f ? 1.0f / sum : nothing ? 0.0f : NAN; }
+constexpr float kNoWeight = -FLT_MAX;
 
 // fp32 queries: 16 rows (a row is a token and a query head) of one sequence over every `splits`-th part of its tokens. Queries
 // and weights are three bf16 planes each, which hold every bit of them, so that products with the cache's values are exact.
@@ -118,7 +127,7 @@ __global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttenti
     const int row = static_cast<int>(id % p.row_blocks) * 16 + l, token_of_row = row / p.heads, head = row - token_of_row * p.heads;
     const int64_t b = id / p.row_blocks;
     const bool real = row < p.rows;
-    Sight sight{0, 0, 0, false};
+    Sight sight{0, 0, 0};
     if (real) sight = sight_of(p, b, token_of_row);
     int end = sight.end;
 #pragma unroll
@@ -323,9 +332,10 @@ __global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttenti
     if (!real) return;
     sum = maxima[0][l] + maxima[1][l] + maxima[2][l] + maxima[3][l];
     const int64_t at_row = b * p.rows + row;
+    // Asked for again where it matters: held through the loop over tiles it costs more (64 x 4096 tokens 259 us for 257).
+    const bool nothing = top == -INFINITY && sight_of(p, b, row / p.heads).base == kNowhere;
     if (p.splits == 1) {
-        // A row that sees nothing has no sum: zeros. One past the table: NaN.
-        const float inverse = sight.beyond ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inverse = inverse_of(sum, nothing);
 #pragma unroll
         for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at_row * R + wave * COLS + 16 * c + 4 * g) = acc[c] * inverse;
     } else {
@@ -335,8 +345,8 @@ __global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttenti
             for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(p.partial + part * R + wave * COLS + 16 * c + 4 * g) = acc[c];
         }
         if (wave == 0 && g == 0) {
-            p.stats[part * 2] = first < last ? top : -INFINITY;
-            p.stats[part * 2 + 1] = sight.beyond ? NAN : first < last ? sum : 0.0f;
+            p.stats[part * 2] = top == -INFINITY && !nothing ? kNoWeight : top;
+            p.stats[part * 2 + 1] = sum;
         }
     }
 }
@@ -498,9 +508,8 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
         for (int i = 0; i < EACH; ++i) ids[holds][(i * SUMMERS + own) * 64 + lane] = id[i];
     };
     if (!scorer) hold(from_tile);
-    Sight sight{0, 0, 0, false};
+    Sight sight{0, 0, 0};
     if (real) sight = sight_of(p, b, token_of_row);
-    const bool beyond = sight.beyond;
     const int base = sight.base;
     const uint64_t bits = sight.bits;
     int all = sight.end, every = real ? base : INT_MAX;  // where the tokens that some row sees end, and those that every row of the wave sees
@@ -652,13 +661,14 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
             }
         }
         sum = sum_over_halves(sum);
-        tops[rw][part][l] = sum;
+        const bool weightless = top == -INFINITY && base != kNowhere;
+        tops[rw][part][l] = whole && weightless ? NAN : sum;
         __syncthreads();
         if (!whole && part == 0 && h == 0) {
 #pragma unroll
             for (int i = 1; i < KW; ++i) sum += tops[rw][i][l];
-            p.stats[place * 2] = top;
-            p.stats[place * 2 + 1] = beyond ? NAN : sum;
+            p.stats[place * 2] = weightless ? kNoWeight : top;
+            p.stats[place * 2 + 1] = sum;
         }
     } else {
 
@@ -875,9 +885,7 @@ __global__ __launch_bounds__((Shape<R, P, E4M3, RW>::WAVES * 64), RW) void laten
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < KW; ++i) sum += tops[group][i][l];
-            // A row that sees nothing has no sum: zeros. One past the table: NaN.
-            const bool past = RG == 1 ? beyond : p.positions[b * p.length + out_row / p.heads] >= static_cast<int64_t>(p.c.width) * p.c.page_size;
-            const float inverse = past ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inverse = inverse_of(sum, true);
             uint16_t* const to = static_cast<uint16_t*>(p.out) + (b * p.rows + out_row) * R + column;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
@@ -946,6 +954,7 @@ __global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionAr
     if (lane == 0) reduced[wave] = sum;
     __syncthreads();
     sum = (reduced[0] + reduced[1]) + (reduced[2] + reduced[3]);
+    const float inverse = inverse_of(sum, most == -INFINITY);
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i = group; i < parts; i += GROUPS * BATCH) {
         f32x4 v[BATCH];
@@ -969,7 +978,6 @@ __global__ __launch_bounds__(256) void latent_join_rows_kernel(LatentAttentionAr
     if (group != 0) return;
 #pragma unroll
     for (int i = 1; i < GROUPS; ++i) acc += sums[i][threadIdx.x];
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc *= inverse;
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + (b * p.rows + row) * R + column) =
         u32x2{__builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(acc[0]), static_cast<__bf16>(acc[1])}),
@@ -1014,7 +1022,7 @@ __global__ __launch_bounds__(256) void latent_join_few_kernel(LatentAttentionArg
         for (int j = 0; j < EACH; ++j) acc[j] *= before;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-            // Of a part that saw nothing the sums may not have been written; one past the table has a sum of NaN.
+            // Of a part that saw nothing the sums may not have been written.
             const float f = stats[k][1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(stats[k][0] - finite_or_zero(now));
             sum = fmaf(stats[k][1], f, sum);
             if (f != 0.0f) {
@@ -1025,7 +1033,7 @@ __global__ __launch_bounds__(256) void latent_join_few_kernel(LatentAttentionArg
             }
         }
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inverse = inverse_of(sum, most == -INFINITY);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
         const f32x4 x = acc[j] * inverse;
@@ -1067,6 +1075,7 @@ __global__ __launch_bounds__(256) void latent_join_f32_kernel(const float* parti
     if (lane == 0) reduced[wave] = sum;
     __syncthreads();
     sum = (reduced[0] + reduced[1]) + (reduced[2] + reduced[3]);
+    const float inverse = inverse_of(sum, most == -INFINITY);
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -1081,7 +1090,6 @@ __global__ __launch_bounds__(256) void latent_join_f32_kernel(const float* parti
     if (group != 0) return;
 #pragma unroll
     for (int i = 1; i < 16; ++i) acc += sums[i][threadIdx.x];
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     acc *= inverse;
     *reinterpret_cast<f32x4*>(out + row * R + column) = acc;
 }

@@ -416,3 +416,31 @@ def test_every_number_outside_the_pages_is_a_missing_page(dev, dtype, store, nam
     q, qr = _queries(g, 3, 3, 4, 64, 16, dtype)
     got = _check(dev, q, qr, cache, table, positions, store)
     assert torch.isnan(got).all(-1).all(-1).tolist() == [[True, True, True], [False, True, True], [False, True, True]]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("H", [2, 40])
+@pytest.mark.parametrize("B,n,width", [(2, 40, 1), (1, 5000, 80), (20, 1500, 32)])
+def test_scores_of_minus_infinity_alone(dev, dtype, store, H, B, n, width):
+    """Every second head's scores are -2^160 or less, which fp32 holds as -infinity: NaN as of a softmax over nothing but
+    minus infinities, in one piece and in parts; zeros stay with what sees no token. The other heads weigh all tokens alike."""
+    g = torch.Generator().manual_seed(n)
+    pages = B * width
+    cache, table = ref.random_cache(g, pages, 64, 64, 16, store), ref.random_table(g, B, width, pages)
+    if store == E4M3:
+        cache[..., 0] = 254  # -448
+        cache[..., 96:100] = torch.tensor([2.0 ** 92]).view(torch.uint8)
+    else:
+        cache[..., :2] = torch.tensor([-2.0 ** 100], dtype=BF16).view(torch.uint8)
+    positions = torch.tensor([[n - 1, -1]] * B, dtype=torch.int32)
+    q, qr = torch.zeros(B, 2, H, 64), torch.zeros(B, 2, H, 16)
+    q[:, :, ::2, 0] = 2.0 ** 60
+    q, qr = q.to(dtype), qr.to(dtype)
+    got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), 1.0)
+    assert torch.isnan(got[:, 0, ::2]).all() and (got[:, 1] == 0).all() and torch.isfinite(got[:, 0, 1::2]).all()
+    # Past the table it is NaN, in a tree that sees no place zeros.
+    positions[:, 0], positions[:, 1] = 64 * width, 0
+    got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), 1.0,
+                                torch.tensor([[1, 1]] * B).to(dev))
+    assert torch.isnan(got[:, 0]).all() and (got[:, 1] == 0).all()
