@@ -548,7 +548,9 @@ mlk_status mlk_latent_read(const uint8_t* cache, int32_t cache_dtype, int64_t pa
  * every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one past the page
  * table, that sees a token on a page outside [0, pages), or all of whose scores are -infinity in fp32, NaN. What the cache holds where a token does not see it, of any
  * bytes, does not reach it. fp32 queries run with fp32 accuracy, bf16 ones with the softmax weights rounded to bf16 for
- * the product with the latents; theirs hold latents of up to 2^110 in size (larger ones may give an infinity). The workspace is 16-byte aligned and private to the call until it has run. */
+ * the product with the latents. Sums are divided last, and hold n seen tokens with latents of up to 2^126 / n in size; of bf16
+ * queries, whose weights may be 2^16 times as large, 2^110 / n. Larger ones may give an infinity. The workspace is 16-byte
+ * aligned and private to the call until it has run. */
 size_t mlk_latent_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t rank, int64_t rope_dim,
                                             int32_t dtype, int32_t cache_dtype, int64_t page_size, int64_t table_width);
 mlk_status mlk_latent_attention(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,

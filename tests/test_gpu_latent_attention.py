@@ -444,3 +444,30 @@ def test_scores_of_minus_infinity_alone(dev, dtype, store, H, B, n, width):
     got = _c().latent_attention(q.to(dev), qr.to(dev), cache.to(dev), table.to(dev), positions.to(dev), 1.0,
                                 torch.tensor([[1, 1]] * B).to(dev))
     assert torch.isnan(got[:, 0]).all() and (got[:, 1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("store", [E4M3, BF16])
+@pytest.mark.parametrize("H", [2, 40])
+@pytest.mark.parametrize("n", [1, 128, 4096])
+def test_the_largest_latents_that_sums_hold(dev, dtype, store, H, n):
+    """n tokens of +-2^126 / n (bf16: 2^110 / n), the scores of all but the first 64 of them 2^15.87 times theirs, which is less
+    than what a maximum may grow by unnoticed. All latents of a column are alike, and so is their mean: it is off by the
+    softmax's rounding, which attention_bound derives, and by no infinity."""
+    g = torch.Generator().manual_seed(n)
+    width, most = -(-n // 64), 2.0 ** (126 if dtype == F32 else 110) / n
+    table = ref.random_table(g, 1, width, width)
+    sign = torch.where(torch.rand(64, generator=g) < 0.5, -1.0, 1.0)
+    cache = torch.zeros(width, 64, ref.row_bytes(64, 16, store), dtype=torch.uint8)
+    if store == E4M3:
+        cache[..., :64] = (256 * sign).to(E4M3).view(torch.uint8)
+        cache[..., 96:100] = torch.tensor([most / 256]).view(torch.uint8)
+    else:
+        cache[..., :128] = (most * sign).to(BF16).view(torch.uint8)
+    flat = cache[table[0].long()].flatten(0, 1)
+    first = 64 if store == E4M3 else 128
+    flat[64:, first:first + 2] = torch.tensor([1.0], dtype=BF16).view(torch.uint8)
+    cache[table[0].long()] = flat.view(width, 64, -1)
+    q, qr = torch.zeros(1, 1, H, 64, dtype=dtype), torch.zeros(1, 1, H, 16, dtype=dtype)
+    qr[..., 0] = 11.0
+    _check(dev, q, qr, cache, table, torch.tensor([[n - 1]], dtype=torch.int32), store, scale=1.0)
