@@ -196,12 +196,14 @@ class MLAHIP(nn.Module):
 
     def new_state(self, streams: int, max_length: int, dtype: torch.dtype = torch.bfloat16, page_size: int = 64,
                   device=None) -> dict:
-        """An empty cache for ``streams`` sequences of up to ``max_length`` tokens, latents in bfloat16 or, as
-        ``torch.float8_e4m3fn``, in eight bits (kv_lora_rank 64, 128, 256 or 512, rope_dim 16, 32 or 64)."""
+        """An empty cache for ``streams`` sequences of up to ``max_length`` tokens, in pages of ``page_size`` at most, latents in
+        bfloat16 or, as ``torch.float8_e4m3fn``, in eight bits (kv_lora_rank 64, 128, 256 or 512, rope_dim 16, 32 or 64)."""
         if streams <= 0 or max_length <= 0 or page_size <= 0:
             raise ValueError("streams, max_length and page_size must be positive")
         device = device if device is not None else self.o_proj.weight.device
         pages = -(-max_length // page_size)
+        if max_length % pages == 0:
+            page_size = max_length // pages  # the last page ends with the stream, and step has no end to look for
         table = torch.arange(streams * pages, dtype=torch.int32, device=device).view(streams, pages)
         return {"cache": ext().latent_cache(streams * pages, page_size, self.kv_lora_rank, self.rope_dim, dtype, device),
                 "page_table": table, "length": torch.zeros(streams, 1, dtype=torch.int32, device=device),
@@ -211,8 +213,8 @@ class MLAHIP(nn.Module):
     def step(self, u: torch.Tensor, state: dict) -> torch.Tensor:
         """The next token ``u [S, d_model]`` of every stream, or the next ``[S, L, d_model]``; ``state`` advances in place
         and outputs have u's shape. Each token sees what its stream held and the call's tokens up to itself. The result is
-        ``forward``'s over the stream but for the cached latents' and key parts' rounding; tokens past max_length give
-        NaN."""
+        ``forward``'s over the stream but for the rounding of the cached latents and key parts and of the rotation's angles,
+        which are float64 here and float32 there (2^17 positions: 0.008 radians); tokens past max_length give NaN."""
         if u.ndim not in (2, 3) or u.shape[-1] != self.d_model:
             raise ValueError("MLAHIP.step expects [streams, d_model] or [streams, length, d_model]")
         if self.training:
