@@ -542,15 +542,16 @@ mlk_status mlk_latent_read(const uint8_t* cache, int32_t cache_dtype, int64_t pa
                            mlk_stream_t stream);
 
 /* softmax((q_latent . c + q_rope . r) * scale) c over cached tokens, q_latent [batch, length, heads, R], q_rope [.., P],
- * strides {sequence, token, head}; scale finite, of any sign; out [batch, length, heads, R] contiguous, 16-byte aligned. Without `ancestors` a token
- * sees the cached tokens 0 .. its position. With ancestors [batch, length] (int64, length <= 64) the call's tokens are a
- * tree that lies in the cache in the call's order: token i at the place p sees the places below p - i, and p - i + j for
- * every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one past the page
- * table, that sees a token on a page outside [0, pages), or all of whose scores are -infinity in fp32, NaN. What the cache holds where a token does not see it, of any
- * bytes, does not reach it. fp32 queries run with fp32 accuracy, bf16 ones with the softmax weights rounded to bf16 for
- * the product with the latents. Sums are divided last, and hold n seen tokens with latents of up to 2^126 / n in size; of bf16
- * queries, whose weights may be 2^16 times as large, 2^110 / n. Larger ones may give an infinity. The workspace is 16-byte
- * aligned and private to the call until it has run. */
+ * strides {sequence, token, head}; scale finite, of any sign; out [batch, length, heads, R] contiguous, 16-byte aligned.
+ * Without `ancestors` a token sees the cached tokens 0 .. its position. With ancestors [batch, length] (int64, length <= 64)
+ * the call's tokens are a tree that lies in the cache in the call's order: token i at the place p sees the places below p - i,
+ * and p - i + j for every bit j < length that is set. A token at a negative position, or that sees nothing, gives zeros; one
+ * past the page table, that sees a token on a page outside [0, pages), or all of whose scores are -infinity in fp32, NaN.
+ * What the cache holds where a token does not see it, of any bytes, does not reach it. fp32 queries run with fp32 accuracy
+ * (of queries, and of weights times a row's scale, what lies under 2^-133 is lost), bf16 ones with the softmax weights rounded
+ * to bf16 for the product with the latents. Sums are divided last, and hold n seen tokens with latents of up to 2^126 / n in
+ * size; of bf16 queries, whose weights may be 2^16 times as large, 2^110 / n. Larger ones may give an infinity. The workspace
+ * is 16-byte aligned and private to the call until it has run. */
 size_t mlk_latent_attention_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t rank, int64_t rope_dim,
                                             int32_t dtype, int32_t cache_dtype, int64_t page_size, int64_t table_width);
 mlk_status mlk_latent_attention(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,

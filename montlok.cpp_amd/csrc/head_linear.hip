@@ -113,7 +113,8 @@ __device__ __forceinline__ void store_outputs(const HeadArgs& p, const f32x16& a
 //
 // Bound by memory: 512 outputs of 128 inputs make 51 operations a byte. 4096 tokens of 64 heads take 140 us (W dense along its
 // inputs) or 122 with 512 outputs of 128 inputs, 91 with 128 of 512: 2.4, 2.8 and 3.7 TB/s (210 and 275 with each wave reading
-// the tokens by itself, 32 bytes of a row a load).
+// the tokens by itself, 32 bytes of a row a load). The form for more than 256 inputs takes all 256 registers of a lane, and two
+// (W dense along its outputs) or four more in scratch memory.
 template <int KS, int NT, bool IN_DENSE>
 __global__ __launch_bounds__(256, 2) void head_linear_kernel(HeadArgs p, unsigned n_blocks, unsigned chunks, unsigned blocks) {
     constexpr int ROW = KS * 16 + 8, PIECES = 64 * KS, EACH = (PIECES + 255) / 256;

@@ -103,13 +103,14 @@ __device__ __forceinline__ float inverse_of(float sum, bool nothing) { return su
 constexpr float kNoWeight = -FLT_MAX;
 
 // fp32 queries: 16 rows (a row is a token and a query head) of one sequence over every `splits`-th part of its tokens. Queries
-// and weights are three bf16 planes each, which hold every bit of them, so that products with the cache's values are exact.
+// and weights are three bf16 planes each, which hold every bit of them (from 2^-110 on), so that products with the cache's
+// values are exact.
 // Wave i scores tokens 16 i .. of a tile of 64, then takes R / 4 columns of all rows' sums. Every product has the rows as its
 // columns (scores are tokens x rows, sums are columns x rows), so that a lane's numbers all belong to row lane & 15: its
 // maximum, sum and rescaling are one number, its weights of four tokens and its sums of four columns lie side by side.
 //
-// Bound by latency where it is small (480 tokens of 8 heads, R = 64: 6.9 us and 4.2 for the join) and by the products of the
-// planes, three of each, where it is not: 64 sequences of up to 4096 tokens, 64 heads, R = 512, take 255 us, 91 TFLOP/s.
+// Bound by latency where it is small (480 tokens of 8 heads, R = 64: 6.7 us and 3.8 for the join) and by the products of the
+// planes, three of each, where it is not: 64 sequences of up to 4096 tokens, 64 heads, R = 512, take 257 us, 90 TFLOP/s.
 template <int R, int P, bool E4M3>
 __global__ __launch_bounds__(256) void latent_attention_f32_kernel(LatentAttentionArgs p) {
     constexpr int ROW = row_bytes<E4M3>(R, P), PIECES = ROW / 16, COLS = R / 4, CT = COLS / 16, kPlanes = 3;
@@ -383,18 +384,20 @@ constexpr int kIds = 512;  // page numbers that are looked up at a time
 
 // Waves of two kinds, RW groups of 32 rows: a scorer takes the rows' scores of 32 tokens of a tile (KW of them a group) and
 // turns them into weights, a summer adds all tokens' latents to a part of the columns, and sees to the loads. Scorers
-// hold the queries, summers the sums: what either holds leaves room for a wave of the other kind on its SIMD, and the one's
-// exponents and conversions run beside the other's products (both in one wave, which then has a SIMD to itself: 6500 cycles a
-// tile of 64 tokens and 64 rows, of which the matrix cores are busy for 2200).
+// hold the queries, summers the sums. With 64 rows what either holds leaves room for a wave of the other kind on its SIMD, and
+// the one's exponents and conversions run beside the other's products (both in one wave, which then has a SIMD to itself: 6500
+// cycles a tile of 64 tokens and 64 rows, of which the matrix cores are busy for 2200). Up to 32 rows are half of that, two
+// scorers and two summers with a SIMD each; LDS holds one such block, or two where a tile is small.
 //
 // A tile is scored while the one before it is summed, with one barrier between.
 //
-// Measured with R = 512, P = 64 in eight bits: 24 sequences of up to 8000 tokens, 16 heads, 32.6 us; one of 131072 tokens, 32
-// heads, 28.5 us (84 MB); 64 of up to 16384, 64 heads, 125 us (435 MB, 3.5 TB/s, 735 TFLOP/s); two chunks of 256 tokens of 24
-// heads over up to 8000 183 us (900 TFLOP/s). A launch's first 8 us (positions, page numbers, row addresses, a tile, each after
-// the other) and its last 2 are no work on tiles; a tile of 64 rows and 64 tokens then takes 2.0 us where its products alone
-// take 1.1: LDS reads and conversions of the operands share the SIMD with them (a product of 32 cycles takes 47 beside its
-// operand's read, 50 with its conversion too), and the clock is 1.8 to 2.1 GHz under them.
+// Measured with R = 512, P = 64 in eight bits, the kernel alone: 24 sequences of up to 8000 tokens, 16 heads, 32.0 us; one of
+// 131072 tokens, 32 heads, 28.2 us (84 MB); 64 of up to 16384, 64 heads, 126 us (435 MB, 3.5 TB/s, 735 TFLOP/s); two chunks of
+// 256 tokens of 24 heads over up to 8000 173 us (950 TFLOP/s). A launch's first 8 us (positions, page numbers, row addresses, a
+// tile, each after the other) and its last 2 are no work on tiles; a tile of 64 rows and 64 tokens then takes 2.0 us where its
+// products alone take 1.1: LDS reads and conversions of the operands share the SIMD with them (a product of 32 cycles takes 47
+// beside its operand's read, 50 with its conversion too), and the clock is 1.8 to 2.1 GHz under them. That form takes all 256
+// registers of a lane, and one more in scratch memory (its wide one four).
 template <int R, int P, bool E4M3, int RW>
 struct Shape {
     static constexpr int ROW = row_bytes<E4M3>(R, P), KW = 64 * ROW * 3 <= 140 * 1024 ? 2 : 1, KEYS = 32 * KW, BYTES = KEYS * ROW;
@@ -1112,7 +1115,8 @@ Plan plan_of(int64_t batch, int64_t rows, int64_t rank, bool f32, int64_t capaci
         plan.workspace = plan.splits == 1 ? 0 : batch * rows * plan.splits * (rank + 2) * 4;
         return plan;
     }
-    // Shares where there are few units; with more a unit a block balances well enough, and has nothing to join.
+    // Shares where there are few units; with more a unit a block balances well enough where sequences are of like lengths, and
+    // has nothing to join. One long sequence among more than 1024 units is then one block's work a unit.
     if (plan.units <= kMaxUnits && tiles > kLeastShare && plan.units * 2 * tiles < (int64_t{1} << 31)) {
         plan.shares = kChip;
         plan.workspace = plan.shares * 2 * per * (rank + 2) * 4 + (kMaxUnits + 1) * 4;
@@ -1151,7 +1155,9 @@ void launch_attention(const LatentAttentionArgs& p, int64_t rope, bool f32, bool
         if (p.shares == 0) return;
         const int per = static_cast<int>(rows_per_block(p.rows, false));
         // A row of many parts falls to several blocks of 64 columns: 256 parts of each of 32 rows 35.0 us with the attention, by
-        // one wave a row 78.9. Where rows have some ten parts a wave each is faster: 24 units 6.0 us, by 64 columns 9.8.
+        // one wave a row 78.9. Where rows have some ten parts a wave each is faster: 24 units 6.0 us, by 64 columns 9.8. How many
+        // a row has is not known here: units stand for it, and of 17 or more with one long sequence among them that one's rows,
+        // of up to 256 parts, are joined by a wave each.
         if (p.units * 16 <= p.shares) hipLaunchKernelGGL((latent_join_rows_kernel<R>), dim3(static_cast<unsigned>(p.units * per * (R / 64))), dim3(256), 0, s, p, per);
         else hipLaunchKernelGGL((latent_join_few_kernel<R>), dim3(static_cast<unsigned>(p.units * per / (R / 4 < 64 ? 1024 / R : 4))), dim3(256), 0, s, p, per);
         return;

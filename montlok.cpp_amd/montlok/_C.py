@@ -766,9 +766,10 @@ def latent_attention(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: torch.
     One new token a sequence, a chunk of a prompt and padded batches are the same call. With ``ancestors`` [B, L] (int64,
     L <= 64) the tokens of the call are a tree, cached at successive places: token i, at the place p, sees the places below
     p - i, and p - i + j for every bit j < L that is set (its own bit i among them, if it is to see itself). A token at a
-    negative position, or that sees nothing, gives zeros; one past the page table, or that sees a token on a page that the
-    table does not name, NaN; what the cache holds where a token does not see it does not reach it. float32 queries run
-    with float32 accuracy."""
+    negative position, or that sees nothing, gives zeros; one past the table, that sees a token on a page that the table
+    does not name, or all of whose scores are -infinity in float32, NaN; what the cache holds where a token does not see
+    it does not reach it. float32 queries run with float32 accuracy; bfloat16 ones have their softmax weights rounded to
+    bfloat16. Latents of n seen tokens may be up to 2^126 / n in size (bfloat16 queries 2^110 / n)."""
     return (_native or _ops()).latent_attention(q_latent, q_rope, cache, page_table, positions, scale, ancestors)
 
 

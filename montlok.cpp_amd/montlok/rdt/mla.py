@@ -214,7 +214,7 @@ class MLAHIP(nn.Module):
         """The next token ``u [S, d_model]`` of every stream, or the next ``[S, L, d_model]``; ``state`` advances in place
         and outputs have u's shape. Each token sees what its stream held and the call's tokens up to itself. The result is
         ``forward``'s over the stream but for the rounding of the cached latents and key parts and of the rotation's angles,
-        which are float64 here and float32 there (2^17 positions: 0.008 radians); tokens past max_length give NaN."""
+        which are float64 here and float32 there (up to 2^17 positions 0.004 radians); tokens past max_length give NaN."""
         if u.ndim not in (2, 3) or u.shape[-1] != self.d_model:
             raise ValueError("MLAHIP.step expects [streams, d_model] or [streams, length, d_model]")
         if self.training:
