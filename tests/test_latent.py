@@ -200,3 +200,16 @@ def test_frequencies_of_a_context_that_no_pair_turns_in_are_refused():
             _C.rope_frequencies(16, factor=4.0, device="cpu", **bad)
     _C.rope_frequencies(16, factor=4.0, original_length=7, device="cpu")
     assert torch.equal(_C.rope_frequencies(16, original_length=1, device="cpu")[0], _C.rope_frequencies(16, device="cpu")[0])
+
+
+@pytest.mark.parametrize("length,page_size,pages,size", [(480, 64, 8, 60), (512, 64, 8, 64), (20, 16, 2, 10), (33, 7, 5, 7), (5, 64, 1, 5), (1, 1, 1, 1)])
+def test_pages_of_a_stream(length, page_size, pages, size):
+    """Pages of one size that end with the stream where there are such, else of the size asked for."""
+    from types import SimpleNamespace
+
+    from montlok.rdt import MLAHIP
+
+    m = MLAHIP(SimpleNamespace(d_model=64, n_heads=2, head_dim=32, nope_head_dim=16, rope_head_dim=16, kv_lora_rank=64, q_lora_rank=0))
+    state = m.new_state(3, length, torch.float8_e4m3fn, page_size, "cpu")
+    assert state["cache"].shape == (3 * pages, size, 64 + 32 + 16) and state["max_length"] == length
+    assert state["page_table"].flatten().tolist() == list(range(3 * pages)) and state["length"].tolist() == [[0]] * 3
